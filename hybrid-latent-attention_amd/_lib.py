@@ -13,7 +13,7 @@ import torch
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get('HLA_S6_LIBRARY') or os.path.join(HERE, 'libhla_s6.so')   # override: another build
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 OK, EINVAL, EUNSUPPORTED, EWORKSPACE, ELAUNCH, EDEVICE = range(6)
 
@@ -86,6 +86,14 @@ SIGNATURES = {
     'hla_s6_mixed_merge_db': [I32, I32, I32, I32, I32, P, I32, P, P, P, P, I64, I64, I64, I32, P, I64, P, I32, P],
     'hla_s6_rope_rows_forward': [I32, P, P, P, P, I32, I32, I32, I32, P, P, I64, I64, I32, P],
     'hla_s6_rope_rows_backward': [I32, P, P, P, P, I32, I32, I32, I32, P, P, I64, I64, I32, P],
+    'hla_s6_compact_store': [P, I64, P, I64, I32, I32, P, P, I64, I32, I64, P],
+    'hla_s6_compact_load': [P, I32, I64, I32, I64, P, I64, I32, P, P, P, I32, I32, I32, P, I64, I64, P],
+    'hla_s6_compact_history': [P, I32, I32, I32, I64, I64, P, I64, I32, I64, P, I64, I32, I32, P, P, F32, I32, P, I64, P,
+                               I64, P, I64, I64, P, P],
+    'hla_s6_attention_weights': [P, I32, I32, I32, I64, I64, P, I32, I64, I64, I32, I64, P, I64, I32, P, I32, P, P, F32,
+                                 P, I64, I32, I32, I32, P, I64, P],
+    'hla_s6_select_rows': [P, I64, P, I64, P, I32, I32, I32, P, P, P, P, P, P, P, P],
+    'hla_s6_move_rows': [P, I32, I32, I64, I64, I32, I64, P, I64, I32, P, P, I64, I32, I32, P],
 }
 
 RESTYPES = {'hla_s6_last_error': ctypes.c_char_p, 'hla_s6_split_plan_ints': ctypes.c_int64,

@@ -1,0 +1,369 @@
+"""The compact latent cache on MI355X: latent rows in 4 bits per value, attention over them, and eviction.
+
+A compact cache takes the place of a ``[num_blocks, 1, block, 2w]`` bf16 latent cache where HBM capacity or bandwidth is
+what a step waits for: it is a uint8 tensor ``[num_blocks, block / 16, 17 w]`` (``cache_shape``), 4.25 bits per value. Values
+are E2M1 numbers (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) times a power of two shared by 32 columns; the bytes of a
+tile of 16 rows lie in the order in which the matrix instructions read them (``csrc/compact.h``). Block tables, slots and
+lengths are those of the bf16 cache.
+
+``store_rows`` and ``load_rows`` move rows in and out, ``history_attention`` (or ``history_partials`` with
+``s6_ops.split_epilogue``) attends to them; ``s6_layer.attend``, ``write_commit`` and ``store_rows`` take a compact cache where
+they take a bf16 one.
+
+Eviction works on both kinds of cache: ``attention_weights`` adds what a step's attention gave every row to an account,
+``select_rows`` picks the rows that stay, ``move_rows`` brings them together at the front of each request's pages.
+
+Checks, streams and errors are those of ``s6_ops``: tensors on the GPU (``RuntimeError`` otherwise), shapes and types
+refused with ``ValueError`` before any launch, everything enqueued on the current stream of the tensors' device, nothing
+synchronised, every call capturable in a HIP graph.
+"""
+from __future__ import annotations
+
+from collections import namedtuple
+
+import torch
+
+from . import _lib, s6_ops
+
+BF16, F32, I32, I64, U8 = torch.bfloat16, torch.float32, torch.int32, torch.int64, torch.uint8
+WIDTHS = (128, 256, 512, 1024)
+HEADS, TILE = 16, 16
+# tokens per request from which a step's rows are expanded once and read by the bf16 cache's multi-query kernels
+CHUNK_TOKENS = 16
+
+#: What ``select_rows`` returns. ``lengths [R]``: rows per request from now on; ``weights``, ``positions [R, M]``: the account
+#: and positions in the new order (0 and -1 behind the last row); ``source``, ``target [R, M // 2]``: the row moves, ended by -1.
+Eviction = namedtuple('Eviction', 'lengths weights positions source target')
+
+
+def _call(name, device, *args):
+    """One entry point on the current stream of ``device``, whichever device is current."""
+    if device.index == torch.cuda.current_device():
+        _lib.call(name, *args, _lib.stream(device))
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, _lib.stream(device))
+
+
+def _same_device(first, *others):
+    s6_ops._dev(first, *others)
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise RuntimeError(f'tensors on {first.device} and {t.device}')
+
+
+def _width(w):
+    if w not in WIDTHS:
+        raise ValueError(f'latent width {w} not in {WIDTHS}')
+    return w
+
+
+def cache_shape(num_blocks, block_size, width):
+    """Shape of a compact cache (uint8) of ``num_blocks`` pages of ``block_size`` rows of ``2 * width`` values."""
+    if block_size <= 0 or block_size % TILE:
+        raise ValueError(f'block size {block_size} is not a positive multiple of {TILE}')
+    return int(num_blocks), block_size // TILE, 17 * _width(width)
+
+
+def is_compact(cache):
+    """Whether ``cache`` is a compact cache (uint8) rather than a bf16 one."""
+    return cache is not None and cache.dtype == U8
+
+
+def block_size(cache):
+    """Rows per page of a compact cache."""
+    return cache.shape[1] * TILE
+
+
+def _compact(cache, width=None):
+    if cache.dtype != U8:
+        raise ValueError(f'a compact cache is uint8, got {cache.dtype}')
+    if cache.dim() != 3 or cache.shape[2] % 17 or (width is not None and cache.shape[2] != 17 * width):
+        raise ValueError(f'compact cache must be [num_blocks, block / 16, {17 * width if width else "17 w"}], '
+                         f'got {tuple(cache.shape)}')
+    if cache.stride(2) != 1 or (cache.shape[1] > 1 and cache.stride(1) != cache.shape[2]):
+        raise ValueError('the pages of a compact cache must be contiguous')
+    return _width(cache.shape[2] // 17)
+
+
+def _table(block_table, rows):
+    if block_table.dtype != I32 or block_table.dim() != 2 or block_table.stride(-1) != 1:
+        raise ValueError('block_table must be a 2-d int32 tensor with a unit last stride')
+    if block_table.shape[0] < rows:
+        raise ValueError(f'block_table has {block_table.shape[0]} rows, {rows} are needed')
+
+
+def _vector(name, t, n, dtype=I32):
+    if t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f'{name} must have {n} entries, got {tuple(t.shape)}')
+    return s6_ops._int(name, t, dtype)
+
+
+def _rows2d(name, t, dtype, shape=None):
+    if t.dtype != dtype or t.dim() != 2 or t.stride(-1) != 1 or (shape is not None and tuple(t.shape) != shape):
+        want = '' if shape is None else f' {list(shape)}'
+        raise ValueError(f'{name} must be a 2-d {dtype} tensor{want} with a unit last stride, got {t.dtype} {list(t.shape)}')
+
+
+def _query(q, width=None):
+    s6_ops._bf16('q_lat', q)
+    if q.dim() != 3 or q.shape[1] != HEADS:
+        raise ValueError(f'q_lat must be [T, {HEADS}, width], got {tuple(q.shape)}')
+    if width is not None and q.shape[2] != width:
+        raise ValueError(f'q_lat has width {q.shape[2]}, the cache {width}')
+    return q.shape[0], q.shape[2]
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# Rows in and out
+# ----------------------------------------------------------------------------------------------------------------
+
+def store_rows(key, value, slots, cache):
+    """Quantise ``[key | value]`` rows (``[T, w]`` bf16 each, any row stride) into slots (int64 ``[T]``, ``page * block +
+    row``) of a compact cache; slots outside the cache are skipped, and the slots of a call must differ.
+
+    Per 32 columns the scale is the smallest power of two ``s`` with ``max|x| <= 7 s`` (so the largest value goes to its nearest
+    neighbour), exponent -120 to 125; values go to the nearest E2M1 number, ties to the even one. 32 columns with an
+    infinity or NaN among them read as NaN."""
+    _same_device(cache, key, value, slots)
+    s6_ops._bf16('key', key)
+    s6_ops._bf16('value', value)
+    if key.dim() != 2 or key.shape != value.shape:
+        raise ValueError(f'key and value must be [T, w] alike, got {tuple(key.shape)} and {tuple(value.shape)}')
+    T, w = key.shape
+    _compact(cache, w)
+    slots = _vector('slots', slots, T, I64)
+    _call('hla_s6_compact_store', cache.device, _lib.ptr(key), key.stride(0), _lib.ptr(value), value.stride(0), T, w,
+          _lib.ptr(slots), _lib.ptr(cache), cache.stride(0), block_size(cache), cache.shape[0])
+
+
+def load_rows(cache, block_table, lengths, max_rows, out=None):
+    """The rows of requests as bf16: ``[R, max_rows, 2w]`` with rows ``lengths[r]`` (int32 ``[R]``) and on of request ``r``
+    zero. ``block_table`` is per request. ``out`` (any request and row strides) is written if given."""
+    _same_device(cache, block_table, lengths, out)
+    w = _compact(cache)
+    R = lengths.shape[0]
+    lengths = _vector('lengths', lengths, R)
+    _table(block_table, R)
+    max_rows = int(max_rows)
+    if out is None:
+        out = torch.empty(R, max_rows, 2 * w, dtype=BF16, device=cache.device)
+    else:
+        s6_ops._bf16('out', out)
+        if tuple(out.shape) != (R, max_rows, 2 * w):
+            raise ValueError(f'out must be [{R}, {max_rows}, {2 * w}], got {tuple(out.shape)}')
+    _load(cache, w, block_table, lengths, None, None, 0, R, max_rows, out)
+    return out
+
+
+def _load(cache, w, block_table, lengths, query_start_loc, ctx, T, R, max_rows, out):
+    _call('hla_s6_compact_load', cache.device, _lib.ptr(cache), w, cache.stride(0), block_size(cache), cache.shape[0],
+          _lib.ptr(block_table), block_table.stride(0), block_table.shape[1], _lib.ptr(lengths),
+          _lib.ptr(query_start_loc), _lib.ptr(ctx), T, R, max_rows, _lib.ptr(out), out.stride(0), out.stride(1))
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# History attention
+# ----------------------------------------------------------------------------------------------------------------
+
+def kv_splits(max_seq_len, num_tokens, cu_count=256, width=512, small_step_tiles=768):
+    """Split slots per row for ``history_attention`` over a compact cache. A split is a workgroup of four waves that walk
+    128 rows at a time; one per CU is resident at widths 512 and 1024, two below, and like ``s6_ops.mi355x_kv_splits`` this
+    returns twice the count that fills them (the plan cuts rows so that about half of the slots get equal work), at most two
+    per 128 keys of the longest row, or per 64 in small steps; one for rows that a single pass covers. A function of
+    constants and the row count only (graph-stable)."""
+    if max_seq_len <= 128:
+        return 1
+    tokens = max(1, num_tokens)
+    busy = cu_count * (1 if width >= 512 else 2)
+    small = tokens * -(-max_seq_len // TILE) < small_step_tiles
+    by_length = 2 * -(-max_seq_len // (64 if small else 128))
+    return max(2, min(2 * max(1, busy // tokens), by_length, 1024))
+
+
+def _history(q, cache, block_table, ctx, scale, token_requests, splits, workspace, plan, out):
+    """The split kernel, and with ``out`` the reduction; returns ``(lse or None, workspace or None)``."""
+    T, w = q.shape[0], q.shape[2]
+    ws = lse = None
+    if splits > 1 or out is None:
+        need = T * HEADS * splits * (w + 1)
+        ws = (torch.empty(need, dtype=F32, device=q.device) if workspace is None
+              else workspace.attn_logits(T, HEADS, splits, w, q.device))
+    if out is not None:
+        lse = torch.empty(HEADS, T, dtype=F32, device=q.device)
+    _call('hla_s6_compact_history', q.device, _lib.ptr(q), T, HEADS, w, q.stride(0), q.stride(1), _lib.ptr(cache),
+          cache.stride(0), block_size(cache), cache.shape[0], _lib.ptr(block_table), block_table.stride(0),
+          block_table.shape[1], block_table.shape[0], _lib.ptr(token_requests), _lib.ptr(ctx), float(scale), splits,
+          _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.ptr(plan), 0 if plan is None else plan.numel(),
+          _lib.ptr(out), 0 if out is None else out.stride(0), 0 if out is None else out.stride(1), _lib.ptr(lse))
+    return lse, ws
+
+
+def _operands(q, cache, block_table, ctx, token_requests, plan=None):
+    _same_device(cache, q, block_table, ctx, token_requests, plan)
+    T, w = _query(q)
+    _compact(cache, w)
+    ctx = _vector('ctx', ctx, T)
+    _table(block_table, T if token_requests is None else min(T, 1))
+    if token_requests is not None:
+        token_requests = _vector('token_requests', token_requests, T, I64)
+    return T, w, ctx, token_requests
+
+
+def history_attention(q_lat, cache, block_table, ctx, scale, max_seq_len, token_requests=None, query_start_loc=None,
+                      max_query_len=1, num_kv_splits=None, workspace=None, plan=None):
+    """Fully visible attention of ``q_lat [T, 16, w]`` (bf16) over the first ``ctx[t]`` (int32) rows of a compact cache:
+    ``(o [T, 16, w] bf16, lse [16, T] fp32)``; tokens without rows give ``o = 0``, ``lse = -inf``.
+
+    ``block_table`` (int32) is per token, or per request with ``token_requests[t]`` (int64) naming the row of token ``t``. No
+    entry of ``ctx`` may be above ``max_seq_len`` (a host number: it sets the split count). Scores, softmax statistics and
+    sums are fp32; the weights are rounded to bf16 for their product with the rows, as over a bf16 cache.
+
+    With ``query_start_loc`` (int32 ``[R + 1]``), ``token_requests`` and a ``max_query_len`` of ``CHUNK_TOKENS`` or more, the rows
+    of each request are expanded to bf16 once, into scratch of ``R * max_seq_len`` rows, and the multi-query kernels of the bf16
+    cache read them: a chunk's tokens share them. Otherwise every token reads its rows as they are.
+
+    ``num_kv_splits`` defaults to ``kv_splits``; ``workspace`` (an ``S6Workspace``) to a new buffer; ``plan`` is an optional
+    ``s6_ops.split_plan`` for ``(ctx, columns * block, num_kv_splits)``. Calls that share a workspace must not overlap."""
+    T, w, ctx, token_requests = _operands(q_lat, cache, block_table, ctx, token_requests, plan)
+    max_seq_len = int(max_seq_len)
+    if max_query_len >= CHUNK_TOKENS and query_start_loc is not None and token_requests is not None and T > 0 and max_seq_len > 0:
+        return _chunk_attention(q_lat, cache, block_table, ctx, scale, max_seq_len, token_requests, query_start_loc,
+                                num_kv_splits, workspace)
+    splits = kv_splits(max_seq_len, T, _lib.device_cus(q_lat.device.index), w) if num_kv_splits is None else int(num_kv_splits)
+    out = torch.empty(T, HEADS, w, dtype=BF16, device=q_lat.device)
+    lse, _ = _history(q_lat, cache, block_table, ctx, scale, token_requests, splits, workspace, plan, out)
+    return out, lse
+
+
+def _chunk_attention(q, cache, block_table, ctx, scale, max_seq_len, token_requests, query_start_loc, splits, workspace):
+    T, w = q.shape[0], q.shape[2]
+    _same_device(cache, query_start_loc)
+    R = query_start_loc.shape[0] - 1
+    qsl = _vector('query_start_loc', query_start_loc, R + 1)
+    _table(block_table, R)
+    pages = -(-min(max_seq_len, block_table.shape[1] * block_size(cache)) // TILE)
+    rows = torch.empty(R * pages, 1, TILE, 2 * w, dtype=BF16, device=q.device)
+    _load(cache, w, block_table, None, qsl, ctx, T, R, pages * TILE, rows.view(R, pages * TILE, 2 * w))
+    table = torch.arange(R * pages, dtype=I32, device=q.device).view(R, pages)
+    group = 4 if w <= 512 else 2
+    if splits is None:
+        splits = s6_ops.mi355x_kv_splits(max_seq_len, T, _lib.device_cus(q.device.index), w, tokens_per_group=group)
+    if splits > 1 and workspace is None:
+        workspace = s6_ops.S6Workspace(HEADS, w, T * splits)
+    return s6_ops.history_attention_kv(q, rows[..., :w], rows[..., w:], table, ctx, scale, splits, workspace, None, None,
+                                       s6_ops.HIP, bt_rows=token_requests, tokens_per_group=group, shared_rows=True)
+
+
+def history_partials(q_lat, cache, block_table, ctx, scale, num_kv_splits, workspace, token_requests=None, plan=None):
+    """The split kernel of ``history_attention`` alone: its partials in ``workspace``, in the layout that
+    ``s6_ops.history_reduce`` and ``s6_ops.split_epilogue`` read (``[T, 16, splits, w + 1]``, private)."""
+    T, w, ctx, token_requests = _operands(q_lat, cache, block_table, ctx, token_requests, plan)
+    splits = int(num_kv_splits)
+    if workspace is None:
+        raise RuntimeError('history partials need an S6Workspace')
+    _, ws = _history(q_lat, cache, block_table, ctx, scale, token_requests, splits, workspace, plan, None)
+    return ws
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# Eviction
+# ----------------------------------------------------------------------------------------------------------------
+
+def _pages(cache, width=None):
+    """Geometry of either kind of cache: ``(width, compact, page_stride, row_stride, block, num_blocks)``."""
+    if is_compact(cache):
+        return _compact(cache, width), 1, cache.stride(0), 0, block_size(cache), cache.shape[0]
+    s6_ops._bf16('cache', cache)
+    if cache.dim() != 4 or cache.shape[1] != 1 or cache.shape[3] % 2 or (width is not None and cache.shape[3] != 2 * width):
+        raise ValueError(f'latent cache must be [num_blocks, 1, block, {2 * width if width else "2 w"}], got {tuple(cache.shape)}')
+    return _width(cache.shape[3] // 2), 0, cache.stride(0), cache.stride(2), cache.shape[2], cache.shape[0]
+
+
+def attention_weights(q_lat, cache, block_table, query_start_loc, ctx, lse, scale, weights):
+    """Add to ``weights [R, M]`` (fp32, in place, returned) what a step's attention gave every history row:
+
+        weights[r, j] += sum over the tokens t of request r and the heads h of exp(scale * q_lat[t, h] . K[r, j] - lse[h, t])
+
+    for ``j < min(ctx[t], M)``. ``cache`` is compact or bf16, ``block_table`` and ``weights`` are per request, ``query_start_loc``
+    (int32 ``[R + 1]``) says which tokens are whose, ``ctx`` is per token. ``lse [16, T]`` is that of the whole softmax, which
+    may cover more keys than the history (``s6_ops.merge_lse``); an infinite one marks an empty row and adds nothing. Sums are
+    fp32 in a fixed order: the same call gives the same bits. Requests must have rows of ``weights`` of their own."""
+    _same_device(cache, q_lat, block_table, query_start_loc, ctx, lse, weights)
+    T, w = _query(q_lat)
+    _, compact, page_stride, row_stride, block, num_blocks = _pages(cache, w)
+    R = query_start_loc.shape[0] - 1
+    qsl = _vector('query_start_loc', query_start_loc, R + 1)
+    ctx = _vector('ctx', ctx, T)
+    _table(block_table, R)
+    _rows2d('lse', lse, F32, (HEADS, T))
+    _rows2d('weights', weights, F32)
+    if weights.shape[0] != R:
+        raise ValueError(f'weights has {weights.shape[0]} rows for {R} requests')
+    lse = lse.contiguous()
+    rows = min(block_table.shape[1] * block, weights.shape[1])
+    shares, keys = account_shape(T, R, rows, _lib.device_cus(q_lat.device.index), w)
+    ws = torch.empty(shares * R * weights.shape[1], dtype=F32, device=weights.device) if shares > 1 else None
+    _call('hla_s6_attention_weights', q_lat.device, _lib.ptr(q_lat), T, HEADS, w, q_lat.stride(0), q_lat.stride(1),
+          _lib.ptr(cache), compact, page_stride, row_stride, block, num_blocks, _lib.ptr(block_table),
+          block_table.stride(0), block_table.shape[1], _lib.ptr(qsl), R, _lib.ptr(ctx), _lib.ptr(lse), float(scale),
+          _lib.ptr(weights), weights.stride(0), weights.shape[1], keys, shares, _lib.ptr(ws),
+          0 if ws is None else ws.numel())
+    return weights
+
+
+def account_shape(num_tokens, num_reqs, rows, cu_count, width):
+    """How ``attention_weights`` is cut: ``(shares of each request's tokens or 0, rows per workgroup)``. Steps of few
+    tokens per request stream K past their queries (shares 0), longer chunks hold K and stream the queries."""
+    if num_tokens < 4 * num_reqs:
+        per = -(-num_reqs * rows // (4 * cu_count))
+        return 0, max(64, -(-per // 64) * 64)
+    wgs = max(1, num_reqs * -(-rows // (128 if width <= 512 else 64)))
+    return max(1, min(2 * cu_count // wgs, num_tokens // max(1, num_reqs) // 16, 16)), 64
+
+
+def select_rows(weights, positions, lengths, budget, protect_from):
+    """Which rows of each request stay, and how they come together (an ``Eviction``; the inputs are left as they are).
+
+    Of the first ``lengths[r]`` (int32 ``[R]``) rows the best ``budget`` (a number, or int32 ``[R]``) stay: first those whose
+    ``positions[r, j]`` (int32 ``[R, M]``) is at least ``protect_from[r]`` (int32 ``[R]``), then by ``weights[r, j]`` (fp32 ``[R, M]``),
+    descending; equal weights go to the earlier row, NaN ranks below everything. Rows that stay below the new length keep
+    their place, and the i-th row behind it that stays moves to the i-th place left free: order among rows is not kept
+    (attention over latent rows does not depend on it), positions tell it. ``move_rows`` applies the moves to a cache."""
+    _same_device(weights, positions, lengths, protect_from, budget if torch.is_tensor(budget) else None)
+    _rows2d('weights', weights, F32)
+    R, M = weights.shape
+    _rows2d('positions', positions, I32, (R, M))
+    lengths = _vector('lengths', lengths, R)
+    protect_from = _vector('protect_from', protect_from, R)
+    budgets = None
+    if torch.is_tensor(budget):
+        budgets, budget = _vector('budget', budget, R), 0
+    elif int(budget) < 0:
+        raise ValueError(f'budget must not be negative, got {budget}')
+    dev = weights.device
+    e = Eviction(torch.empty(R, dtype=I32, device=dev), torch.empty(R, M, dtype=F32, device=dev),
+                 torch.empty(R, M, dtype=I32, device=dev), torch.empty(R, M // 2, dtype=I32, device=dev),
+                 torch.empty(R, M // 2, dtype=I32, device=dev))
+    _call('hla_s6_select_rows', dev, _lib.ptr(weights), weights.stride(0), _lib.ptr(positions), positions.stride(0),
+          _lib.ptr(lengths), R, M, min(int(budget), 2 ** 31 - 1), _lib.ptr(budgets), _lib.ptr(protect_from),
+          _lib.ptr(e.lengths), _lib.ptr(e.weights), _lib.ptr(e.positions), _lib.ptr(e.source), _lib.ptr(e.target))
+    return e
+
+
+def move_rows(cache, block_table, eviction):
+    """Apply the row moves of ``select_rows`` to a cache (compact or bf16) in place, through the per-request
+    ``block_table``. A request's pages must be its own: a page in two rows of the table would change for both. Moves through
+    page ids outside the cache are skipped."""
+    source, target = eviction.source, eviction.target
+    _same_device(cache, block_table, source, target)
+    w, compact, page_stride, row_stride, block, num_blocks = _pages(cache)
+    _rows2d('source', source, I32)
+    R, count = source.shape
+    _rows2d('target', target, I32, (R, count))
+    if source.stride(0) != target.stride(0):
+        source, target = source.contiguous(), target.contiguous()
+    _table(block_table, R)
+    _call('hla_s6_move_rows', cache.device, _lib.ptr(cache), w, compact, page_stride, row_stride, block, num_blocks,
+          _lib.ptr(block_table), block_table.stride(0), block_table.shape[1], _lib.ptr(source), _lib.ptr(target),
+          source.stride(0), count, R)

@@ -1,0 +1,536 @@
+// The compact latent cache (compact.h): row commit, row load and paged history attention over 4-bit rows.
+#include "compact.h"
+#include "split_plan.h"
+
+namespace hla {
+namespace {
+
+// ---- commit ------------------------------------------------------------------------------------------------------
+// One thread per eight columns of a row, four threads per block of 32. The block's scale exponent is the smallest e with
+// max|x| <= 7 * 2^e: the largest value then takes its nearest representable one (up to 7 * 2^e it is nearer to 6 * 2^e
+// than to 8 * 2^e). Values go to the nearest E2M1 number, ties to the even one (v_cvt_scalef32_pk_fp4_bf16); a block with
+// a value that is not finite gets scale byte 255 and reads as NaN.
+struct StoreParams {
+  const uint16_t* key;
+  const uint16_t* value;
+  int64_t k_st, v_st;
+  const int64_t* slots;
+  uint8_t* cache;
+  int64_t page_stride;
+  int block;
+  int64_t num_slots;
+  int64_t units;  // threads of work: T * 2 W / 8
+};
+
+__device__ __forceinline__ uint32_t abs_max2(uint32_t m, uint32_t pair) {
+  return max(m, max(pair & 0x7fffu, (pair >> 16) & 0x7fffu));
+}
+
+template <int W, bool VEC>
+__global__ __launch_bounds__(256) void compact_store_kernel(StoreParams a) {
+  constexpr int PER = W / 4;  // threads per row
+  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (u >= a.units) return;  // whole rows of threads: PER is a multiple of 4, and 256 of PER or PER of 256
+  const int64_t t = u / PER;
+  const int i = (int)(u % PER);
+  const int64_t slot = a.slots[t];
+  if (slot < 0 || slot >= a.num_slots) return;  // the same for all four threads of a block
+  const bool is_v = i >= PER / 2;
+  const int col = (is_v ? i - PER / 2 : i) * 8;
+  const uint16_t* src = (is_v ? a.value + t * a.v_st : a.key + t * a.k_st) + col;
+  u32x4 x;
+  if (VEC) {
+    x = ld16(src);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = (uint32_t)src[2 * e] | ((uint32_t)src[2 * e + 1] << 16);
+  }
+  uint32_t most = 0;  // bit patterns of non-negative bf16 order as integers
+#pragma unroll
+  for (int e = 0; e < 4; ++e) most = abs_max2(most, x[e]);
+  most = max(most, (uint32_t)__shfl_xor((int)most, 1));
+  most = max(most, (uint32_t)__shfl_xor((int)most, 2));
+  const bool finite = most < 0x7f80u;
+  const int e0 = (int)(most >> 7) - 129 + ((most & 127u) > 96u ? 1 : 0);  // 7 = 1.75 * 4: fraction 96 / 128
+  const int exponent = min(max(e0, kMinExponent), kMaxExponent);
+  const uint32_t byte = finite ? (uint32_t)(exponent + 127) : 255u;
+  const float scale = __uint_as_float((uint32_t)(exponent + 127) << 23);
+  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+  uint32_t code = 0;
+  code = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(code, __builtin_bit_cast(bf16x2_t, (uint32_t)x[0]), scale, 0);
+  code = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(code, __builtin_bit_cast(bf16x2_t, (uint32_t)x[1]), scale, 1);
+  code = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(code, __builtin_bit_cast(bf16x2_t, (uint32_t)x[2]), scale, 2);
+  code = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(code, __builtin_bit_cast(bf16x2_t, (uint32_t)x[3]), scale, 3);
+  if (!finite) code = 0;
+  const int in_page = (int)(slot % a.block), r = in_page & 15, b = col >> 5;
+  uint8_t* tile = a.cache + (slot / a.block) * a.page_stride + (in_page >> 4) * compact_tile_bytes(W);
+  const int at = is_v ? v_code_at(W, r, col >> 1) : k_code_at(r, b) + ((col & 31) >> 1);
+  *reinterpret_cast<uint32_t*>(tile + at) = code;
+  if ((i & 3) == 0) tile[is_v ? v_scale_at(W, r, b) : k_scale_at(W, r, b)] = (uint8_t)byte;
+}
+
+// ---- load --------------------------------------------------------------------------------------------------------
+// out[r, j, :] = row j of request r in bf16 for j < lengths[r], 0 behind it (without lengths: of a step's tokens, and
+// nothing behind it). One thread per eight columns: 4 bytes in, 16 out. HBM-bound by the writes (64 W bytes of every 81 W).
+struct LoadParams {
+  const uint8_t* cache;
+  int64_t page_stride;
+  int block;
+  int64_t num_blocks;
+  const int32_t* bt;
+  int64_t bt_stride;
+  int bt_cols;
+  const int32_t* lengths;  // or null: the largest ctx of the request's tokens
+  const int32_t* qsl;
+  const int32_t* ctx;
+  int T;
+  uint16_t* out;
+  int64_t o_sr, o_sj;  // elements per request and per row
+  int max_rows;
+};
+
+__device__ int most_ctx(const LoadParams& a, int r) {
+  __shared__ int red[4];
+  int most = 0;
+  for (int t = max(a.qsl[r], 0) + (int)threadIdx.x; t < min(a.qsl[r + 1], a.T); t += 256) most = max(most, a.ctx[t]);
+  for (int off = 32; off > 0; off >>= 1) most = max(most, __shfl_xor(most, off));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = most;
+  __syncthreads();
+  return max(max(red[0], red[1]), max(red[2], red[3]));
+}
+
+template <int W>
+__global__ __launch_bounds__(256) void compact_load_kernel(LoadParams a) {
+  constexpr int PER = W / 4;                         // threads per row
+  constexpr int ROWS = PER <= 256 ? 256 / PER : 1;   // rows per pass of the workgroup
+  const int r = blockIdx.y, i = threadIdx.x % PER;
+  const int n = (int)min((int64_t)max(a.lengths ? a.lengths[r] : most_ctx(a, r), 0), (int64_t)a.bt_cols * a.block);
+  const int32_t* btr = a.bt + (int64_t)r * a.bt_stride;
+  const bool is_v = i >= PER / 2;
+  const int col = (is_v ? i - PER / 2 : i) * 8, b = col >> 5;
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const int64_t j = ((int64_t)blockIdx.x * 4 + p) * ROWS + threadIdx.x / PER;
+    if (j >= a.max_rows || (j >= n && !a.lengths)) return;
+    u32x4 x = {0u, 0u, 0u, 0u};
+    if (j < n) {
+      const int64_t page = clamp_page(btr[j / a.block], a.num_blocks);
+      const int in_page = (int)(j % a.block), x16 = in_page & 15;
+      const uint8_t* tile = a.cache + page * a.page_stride + (in_page >> 4) * compact_tile_bytes(W);
+      const int at = is_v ? v_code_at(W, x16, col >> 1) : k_code_at(x16, b) + ((col & 31) >> 1);
+      const uint32_t code = *reinterpret_cast<const uint32_t*>(tile + at);
+      const uint32_t scale = tile[is_v ? v_scale_at(W, x16, b) : k_scale_at(W, x16, b)];
+      x = eight_bf16(code, scale_of(scale, 0));
+    }
+    st16(a.out + (int64_t)r * a.o_sr + j * a.o_sj + (is_v ? W : 0) + col, x);
+  }
+}
+
+// ---- history attention ---------------------------------------------------------------------------------------------
+// One workgroup of four waves per (token, split). Every wave walks its own 32 rows of each 128 (two tiles), alone:
+//   * S^T[32 keys x 16 heads] = K Q^T on v_mfma_f32_16x16x32_bf16. A lane's 16 bytes of K are one block of 32 columns of
+//     one row, four k-steps of eight values; Q^T is read with the same order of columns, so nothing is moved.
+//   * online softmax in the exp2 domain: a lane holds 8 keys of one head, and P^T stays where it is: the order of keys in
+//     the next product's contraction is free, and is taken to be the one the scores come out in.
+//   * O^T[columns x 16 heads] += V^T P^T: a lane loads the same 8 keys' values of W / 16 consecutive columns (one scale
+//     per key and 32 columns); two keys' values of a column are joined by one v_perm_b32 per pair. Product c of a wave
+//     takes column c of every lane's range.
+// No value passes through LDS until the waves' partials are joined at the end. At W = 1024 two waves share 32 keys, each
+// with all of K and half of the columns of V.
+struct CompactParams {
+  const uint16_t* q;
+  int64_t q_st, q_sh;
+  const uint8_t* cache;
+  int64_t page_stride;
+  int block;
+  int64_t num_blocks;
+  const int32_t* bt;
+  int64_t bt_stride;
+  int bt_cols, bt_count;
+  const int64_t* bt_rows;
+  const int32_t* ctx;
+  float scale_log2;
+  int num_splits, T;
+  float* ws_o;    // [T][S][16][W]
+  float* ws_lse;  // [T][S][16]
+  const int32_t* plan;
+  uint16_t* out;  // one split: the final output and lse
+  int64_t o_st, o_sh;
+  float* lse;
+};
+
+template <int W>
+struct VTile {  // one tile of V: rows 4g .. 4g + 3, CPL columns per lane (m, g)
+  Words<CompactGeo<W>::VD> code[4];
+  uint32_t scale;  // of the four rows
+};
+
+template <int W>
+__device__ __forceinline__ void load_v(const uint8_t* tile, int m, int g, int half, VTile<W>& v) {
+  using G = CompactGeo<W>;
+  const int col = half * (W / G::CH) + m * G::CPL;
+  v.scale = *reinterpret_cast<const uint32_t*>(tile + 16 * W + W / 2 + (col / 32) * 16 + 4 * g);
+#pragma unroll
+  for (int r = 0; r < 4; ++r) v.code[r] = load_words<G::VD>(tile + 8 * W + (r * 4 + g) * (W / 2) + col / 2);
+}
+
+// Columns 2 kByte and 2 kByte + 1 of dword d of every lane's range: eight keys each, two products
+template <int W, int kByte>
+__device__ __forceinline__ void pv_pair(const VTile<W> (&v)[2], const float (&f)[8], u32x4 p, int d, floatx4& even,
+                                        floatx4& odd) {
+  uint32_t x[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = two_bf16<kByte>(v[e / 4].code[e % 4].w[d], f[e]);
+  u32x4 lo, hi;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    lo[e] = __builtin_amdgcn_perm(x[2 * e + 1], x[2 * e], 0x05040100u);
+    hi[e] = __builtin_amdgcn_perm(x[2 * e + 1], x[2 * e], 0x07060302u);
+  }
+  even = mfma16x16x32(lo, p, even);
+  odd = mfma16x16x32(hi, p, odd);
+}
+
+template <int W>
+__global__ __launch_bounds__(256, 1) void compact_history_kernel(CompactParams a) {
+  using G = CompactGeo<W>;
+  __shared__ int64_t red_lds[8];
+  __shared__ int item_lds[6];
+  __shared__ float m_lds[4][16], l_lds[4][16];
+  __shared__ floatx4 o_lds[2][G::CH][G::G - 1][G::CPL / 4][64];
+  __shared__ u32x4 q_lds[QOperand<W>::kLds ? G::KC * 4 : 1][64];
+
+  const int tid = threadIdx.x, lane = tid & 63, h = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = wave % G::CH, set = wave / G::CH;
+  const int S = a.num_splits, b = blockIdx.x;
+  const int64_t cap = (int64_t)a.bt_cols * a.block;
+  int t = b, s = 0, chunk = 0;
+  if (S > 1 && a.plan) {
+    const int ni = (int)split_workgroups(a.T, S);
+    chunk = a.plan[0];
+    t = a.plan[1 + a.T + b];
+    s = a.plan[1 + a.T + ni + b];
+  } else if (S > 1) {
+    chunk = split_chunk(a.ctx, a.T, cap, S, red_lds);
+    find_item(a.ctx, a.T, cap, chunk, b, item_lds, item_lds + 4, t, s);
+  }
+  if (S > 1 && b < a.T) {  // slots of row b past its work
+    const int used = a.plan ? a.plan[1 + b] : used_slots(a.ctx[b], cap, chunk);
+    float* l0 = a.ws_lse + ((int64_t)b * S + used) * kHeads;
+    for (int i = tid; i < (S - used) * kHeads; i += 256) l0[i] = -INFINITY;
+  }
+  if (t < 0) return;
+  t = __builtin_amdgcn_readfirstlane(t);
+  s = __builtin_amdgcn_readfirstlane(s);
+  const int n = (int)min((int64_t)max(a.ctx[t], 0), cap);
+  const int tiles = (n + kTile - 1) / kTile;
+  if (S == 1) chunk = tiles;
+  const int j_begin = s * chunk, j_end = min(tiles, j_begin + chunk);
+  const int64_t part = ((int64_t)t * S + s) * kHeads;
+
+  if (j_begin >= j_end) {  // a row without history
+    if (!a.out) {
+      if (tid < kHeads) a.ws_lse[part + tid] = -INFINITY;
+      return;
+    }
+    for (int i = tid; i < kHeads * W / 4; i += 256)
+      *reinterpret_cast<uint2*>(a.out + (int64_t)t * a.o_st + (int64_t)(i / (W / 4)) * a.o_sh + i % (W / 4) * 4) =
+          uint2{0u, 0u};
+    if (tid < kHeads) a.lse[(int64_t)tid * a.T + t] = -INFINITY;
+    return;
+  }
+
+  QOperand<W> q;
+  q.load(a.q + (int64_t)t * a.q_st + (int64_t)h * a.q_sh, g, wave, lane, q_lds);
+  const int64_t table_row = min(max(a.bt_rows ? a.bt_rows[t] : (int64_t)t, (int64_t)0), (int64_t)a.bt_count - 1);
+  const int32_t* btr = a.bt + table_row * a.bt_stride;
+  const int limit = min(n, j_end * kTile);
+  auto tile_at = [&](int j) -> const uint8_t* {
+    const int row = min(j, j_end - 1) * kTile;  // (a tile past the chunk reads its last one, and its keys are masked)
+    const int64_t page = clamp_page(btr[row / a.block], a.num_blocks);
+    return a.cache + page * a.page_stride + (row % a.block) / kTile * compact_tile_bytes(W);
+  };
+
+  floatx4 acc[G::CPL];
+#pragma unroll
+  for (int c = 0; c < G::CPL; ++c) acc[c] = floatx4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  KTile<W> k[2];
+  VTile<W> v[2];
+  int j = j_begin + 2 * set;
+  const uint8_t *t0 = tile_at(j), *t1 = tile_at(j + 1);
+  if (j < j_end) {
+    load_k<W>(t0, h, g, k[0]);
+    load_k<W>(t1, h, g, k[1]);
+    load_v<W>(t0, h, g, half, v[0]);
+    load_v<W>(t1, h, g, half, v[1]);
+  }
+  for (; j < j_end; j += 2 * G::G) {
+    floatx4 s0, s1;
+    scores<W>(k, q, lane, s0, s1);
+    const bool more = j + 2 * G::G < j_end;
+    if (more) {
+      t0 = tile_at(j + 2 * G::G);
+      t1 = tile_at(j + 2 * G::G + 1);
+      load_k<W>(t0, h, g, k[0]);
+      load_k<W>(t1, h, g, k[1]);
+    }
+    float sc[8], f[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      sc[e] = s0[e] * a.scale_log2;
+      sc[4 + e] = s1[e] * a.scale_log2;
+      f[e] = scale_of(v[0].scale, e);
+      f[4 + e] = scale_of(v[1].scale, e);
+    }
+    const int key = j * kTile + 4 * g;
+    if ((j + 2) * kTile > limit) {  // hide the keys past the end, and their scales, which may be those of NaN
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (key + (e / 4) * kTile + e % 4 >= limit) {
+          sc[e] = -INFINITY;
+          f[e] = 0.f;
+        }
+    }
+    float mx = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
+    mx = wave_max16x4(mx);
+    // the running maximum is raised only past 2^8, so most steps leave the accumulators alone
+    const bool raise = mx > m + 8.f;
+    if (__any(raise)) {
+      const float m_new = raise ? mx : m;
+      const float alpha = raise ? fast_exp2(m - m_new) : 1.f;
+      l *= alpha;
+      m = m_new;
+#pragma unroll
+      for (int c = 0; c < G::CPL; ++c) acc[c] = acc[c] * alpha;
+    }
+    const float m_use = m == -INFINITY ? 0.f : m;
+    float p[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] = fast_exp2(sc[e] - m_use);
+    l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+    // P in bf16, as in the bf16 cache's kernels: half a step of 2^-8 per weight, independent from key to key
+    const u32x4 pb = {pack2(p[0], p[1]), pack2(p[2], p[3]), pack2(p[4], p[5]), pack2(p[6], p[7])};
+#pragma unroll
+    for (int d = 0; d < G::VD; ++d) {
+      pv_pair<W, 0>(v, f, pb, d, acc[8 * d + 0], acc[8 * d + 1]);
+      pv_pair<W, 1>(v, f, pb, d, acc[8 * d + 2], acc[8 * d + 3]);
+      pv_pair<W, 2>(v, f, pb, d, acc[8 * d + 4], acc[8 * d + 5]);
+      pv_pair<W, 3>(v, f, pb, d, acc[8 * d + 6], acc[8 * d + 7]);
+    }
+    if (more) {
+      load_v<W>(t0, h, g, half, v[0]);
+      load_v<W>(t1, h, g, half, v[1]);
+    }
+  }
+
+  // Join the sets of keys: every wave at the common maximum, then in four rounds wave (round mod sets) of each column half
+  // adds up accumulator element `round` of all of them and writes it: CPL consecutive columns per lane.
+  l = wave_sum16x4(l);
+  if (g == 0) {
+    m_lds[wave][h] = m;
+    l_lds[wave][h] = l;
+  }
+  __syncthreads();
+  float top = -INFINITY, total = 0.f;
+#pragma unroll
+  for (int x = 0; x < G::G; ++x) top = fmaxf(top, m_lds[x * G::CH][h]);
+#pragma unroll
+  for (int x = 0; x < G::G; ++x) total += l_lds[x * G::CH][h] * fast_exp2(m_lds[x * G::CH][h] - top);
+  const float mine = fast_exp2(m - top);
+  const float inv = 1.0f / total;
+  if (wave == 0 && g == 0) {
+    const float lse = (top + log2f(total)) * kLn2;
+    if (a.out) a.lse[(int64_t)h * a.T + t] = lse;
+    else a.ws_lse[part + h] = lse;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int owner = i % G::G;
+    if (set != owner) {
+      const int at = set < owner ? set : set - 1;
+#pragma unroll
+      for (int c = 0; c < G::CPL / 4; ++c)
+        o_lds[i & 1][half][at][c][lane] = floatx4{acc[4 * c][i], acc[4 * c + 1][i], acc[4 * c + 2][i],
+                                                  acc[4 * c + 3][i]} * mine;
+    }
+    __syncthreads();
+    if (set == owner) {
+      const int col = half * (W / G::CH) + G::CPL * (4 * g + i);
+#pragma unroll
+      for (int c = 0; c < G::CPL / 4; ++c) {
+        floatx4 o = floatx4{acc[4 * c][i], acc[4 * c + 1][i], acc[4 * c + 2][i], acc[4 * c + 3][i]} * mine;
+#pragma unroll
+        for (int x = 0; x < G::G - 1; ++x) o += o_lds[i & 1][half][x][c][lane];
+        o = o * inv;
+        if (a.out)
+          *reinterpret_cast<uint2*>(a.out + (int64_t)t * a.o_st + (int64_t)h * a.o_sh + col + 4 * c) =
+              uint2{pack2(o[0], o[1]), pack2(o[2], o[3])};
+        else
+          *reinterpret_cast<floatx4*>(a.ws_o + (part + h) * W + col + 4 * c) = o;
+      }
+    }
+  }
+}
+
+template <int W>
+void launch_store(const StoreParams& p, bool vec, hipStream_t st) {
+  const dim3 grid((unsigned)((p.units + 255) / 256));
+  if (vec) hipLaunchKernelGGL((compact_store_kernel<W, true>), grid, dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((compact_store_kernel<W, false>), grid, dim3(256), 0, st, p);
+}
+
+template <int W>
+void launch_load(const LoadParams& p, int R, hipStream_t st) {
+  constexpr int rows = 4 * (W / 4 <= 256 ? 256 / (W / 4) : 1);
+  hipLaunchKernelGGL((compact_load_kernel<W>), dim3((unsigned)((p.max_rows + rows - 1) / rows), (unsigned)R), dim3(256), 0,
+                     st, p);
+}
+
+}  // namespace
+}  // namespace hla
+
+extern "C" int hla_s6_compact_store(const void* key, int64_t k_st, const void* value, int64_t v_st, int32_t num_tokens,
+                                    int32_t width, const int64_t* slots, void* cache, int64_t page_stride,
+                                    int32_t block_size, int64_t num_blocks, void* stream) {
+  using namespace hla;
+  HLA_REQUIRE(num_tokens >= 0, HLA_S6_EINVAL, "compact_store: negative token count");
+  int rc = check_cache("compact_store", width, cache, page_stride, block_size, num_blocks);
+  if (rc != HLA_S6_OK || num_tokens == 0) return rc;
+  HLA_REQUIRE(key && value && slots, HLA_S6_EINVAL, "compact_store: null pointer argument");
+  StoreParams p = {};
+  p.key = static_cast<const uint16_t*>(key);
+  p.value = static_cast<const uint16_t*>(value);
+  p.k_st = k_st;
+  p.v_st = v_st;
+  p.slots = slots;
+  p.cache = static_cast<uint8_t*>(cache);
+  p.page_stride = page_stride;
+  p.block = block_size;
+  p.num_slots = num_blocks * block_size;
+  p.units = (int64_t)num_tokens * (width / 4);
+  const bool vec = aligned(key, 16) && aligned(value, 16) && k_st % 8 == 0 && v_st % 8 == 0;
+  const hipStream_t st = as_stream(stream);
+  switch (width) {
+    case 128: launch_store<128>(p, vec, st); break;
+    case 256: launch_store<256>(p, vec, st); break;
+    case 512: launch_store<512>(p, vec, st); break;
+    default: launch_store<1024>(p, vec, st); break;
+  }
+  return check_launch("compact_store");
+}
+
+extern "C" int hla_s6_compact_load(const void* cache, int32_t width, int64_t page_stride, int32_t block_size,
+                                   int64_t num_blocks, const int32_t* block_table, int64_t bt_stride, int32_t bt_cols,
+                                   const int32_t* lengths, const int32_t* query_start_loc, const int32_t* ctx,
+                                   int32_t num_tokens, int32_t num_reqs, int32_t max_rows, void* out, int64_t o_sr,
+                                   int64_t o_sj, void* stream) {
+  using namespace hla;
+  HLA_REQUIRE(num_reqs >= 0 && num_reqs <= 65535 && max_rows >= 0 && bt_cols >= 0, HLA_S6_EINVAL,
+              "compact_load: bad request count (0..65535), row count or table width");
+  int rc = check_cache("compact_load", width, cache, page_stride, block_size, num_blocks);
+  if (rc != HLA_S6_OK || num_reqs == 0 || max_rows == 0) return rc;
+  HLA_REQUIRE((lengths || (query_start_loc && ctx)) && out && (block_table || bt_cols == 0), HLA_S6_EINVAL,
+              "compact_load: null pointer argument");
+  HLA_REQUIRE(aligned(out, 16) && o_sr % 8 == 0 && o_sj % 8 == 0 && o_sj >= 2 * width, HLA_S6_EINVAL,
+              "compact_load: output rows must be 16-byte aligned and apart");
+  LoadParams p = {};
+  p.cache = static_cast<const uint8_t*>(cache);
+  p.page_stride = page_stride;
+  p.block = block_size;
+  p.num_blocks = num_blocks;
+  p.bt = block_table;
+  p.bt_stride = bt_stride;
+  p.bt_cols = bt_cols;
+  p.lengths = lengths;
+  p.qsl = query_start_loc;
+  p.ctx = ctx;
+  p.T = num_tokens;
+  p.out = static_cast<uint16_t*>(out);
+  p.o_sr = o_sr;
+  p.o_sj = o_sj;
+  p.max_rows = max_rows;
+  const hipStream_t st = as_stream(stream);
+  switch (width) {
+    case 128: launch_load<128>(p, num_reqs, st); break;
+    case 256: launch_load<256>(p, num_reqs, st); break;
+    case 512: launch_load<512>(p, num_reqs, st); break;
+    default: launch_load<1024>(p, num_reqs, st); break;
+  }
+  return check_launch("compact_load");
+}
+
+extern "C" int hla_s6_compact_history(const void* q, int32_t num_tokens, int32_t num_heads, int32_t width, int64_t q_st,
+                                      int64_t q_sh, const void* cache, int64_t page_stride, int32_t block_size,
+                                      int64_t num_blocks, const int32_t* block_table, int64_t bt_stride,
+                                      int32_t bt_cols, int32_t bt_count, const int64_t* bt_rows, const int32_t* ctx,
+                                      float scale, int32_t num_splits, float* workspace, int64_t workspace_floats,
+                                      const int32_t* plan, int64_t plan_len, void* out, int64_t o_st, int64_t o_sh,
+                                      float* lse, void* stream) {
+  using namespace hla;
+  HLA_REQUIRE(num_tokens >= 0, HLA_S6_EINVAL, "compact_history: negative token count");
+  HLA_REQUIRE(num_heads == kHeads, HLA_S6_EUNSUPPORTED, "compact_history: %d query heads (the kernel is built for 16)",
+              num_heads);
+  int rc = check_cache("compact_history", width, cache, page_stride, block_size, num_blocks);
+  if (rc != HLA_S6_OK) return rc;
+  HLA_REQUIRE(num_splits >= 1 && num_splits <= kMaxSplits, HLA_S6_EINVAL,
+              "compact_history: num_kv_splits must be in [1, %d]", kMaxSplits);
+  HLA_REQUIRE(bt_cols >= 0, HLA_S6_EINVAL, "compact_history: bad table width");
+  if (num_tokens == 0) return HLA_S6_OK;
+  HLA_REQUIRE(bt_count >= (bt_rows ? 1 : num_tokens), HLA_S6_EINVAL, "compact_history: %d table rows", bt_count);
+  HLA_REQUIRE(q && block_table && ctx && (out == nullptr) == (lse == nullptr), HLA_S6_EINVAL,
+              "compact_history: null pointer argument");
+  HLA_REQUIRE(aligned(q, 16) && q_st % 8 == 0 && q_sh % 8 == 0, HLA_S6_EINVAL,
+              "compact_history: q needs 16-byte aligned rows (unit last stride, strides multiple of 8)");
+  HLA_REQUIRE(aligned(out, 8) && o_st % 4 == 0 && o_sh % 4 == 0, HLA_S6_EINVAL,
+              "compact_history: output rows must be 8-byte aligned");
+  const bool partials = num_splits > 1 || !out;
+  if (partials) {
+    const int64_t need = (int64_t)num_tokens * num_splits * kHeads * (width + 1);
+    HLA_REQUIRE(workspace != nullptr && workspace_floats >= need, HLA_S6_EWORKSPACE,
+                "S6 workspace overflow: need %lld floats, have %lld", (long long)need, (long long)workspace_floats);
+    HLA_REQUIRE(aligned(workspace, 16), HLA_S6_EINVAL, "compact_history: workspace must be 16-byte aligned");
+  }
+  HLA_REQUIRE(!plan || num_splits == 1 || plan_len >= plan_ints(num_tokens, num_splits), HLA_S6_EINVAL,
+              "compact_history: split plan of %lld ints, need %lld", (long long)plan_len,
+              (long long)plan_ints(num_tokens, num_splits));
+  CompactParams p = {};
+  p.q = static_cast<const uint16_t*>(q);
+  p.q_st = q_st;
+  p.q_sh = q_sh;
+  p.cache = static_cast<const uint8_t*>(cache);
+  p.page_stride = page_stride;
+  p.block = block_size;
+  p.num_blocks = num_blocks;
+  p.bt = block_table;
+  p.bt_stride = bt_stride;
+  p.bt_cols = bt_cols;
+  p.bt_count = bt_count;
+  p.bt_rows = bt_rows;
+  p.ctx = ctx;
+  p.scale_log2 = scale * kLog2e;
+  p.num_splits = num_splits;
+  p.T = num_tokens;
+  p.plan = plan;
+  if (partials) {
+    p.ws_o = workspace;
+    p.ws_lse = workspace + (int64_t)num_tokens * num_splits * kHeads * width;
+  } else {
+    p.out = static_cast<uint16_t*>(out);
+    p.o_st = o_st;
+    p.o_sh = o_sh;
+    p.lse = lse;
+  }
+  const dim3 grid(split_workgroups(num_tokens, num_splits)), block(256);
+  const hipStream_t st = as_stream(stream);
+  switch (width) {
+    case 128: hipLaunchKernelGGL((compact_history_kernel<128>), grid, block, 0, st, p); break;
+    case 256: hipLaunchKernelGGL((compact_history_kernel<256>), grid, block, 0, st, p); break;
+    case 512: hipLaunchKernelGGL((compact_history_kernel<512>), grid, block, 0, st, p); break;
+    default: hipLaunchKernelGGL((compact_history_kernel<1024>), grid, block, 0, st, p); break;
+  }
+  rc = check_launch("compact_history");
+  if (rc != HLA_S6_OK || !out || !partials) return rc;
+  return hla_s6_history_reduce(workspace, workspace_floats, num_tokens, num_heads, width, num_splits, out, o_st, o_sh,
+                               lse, stream);
+}

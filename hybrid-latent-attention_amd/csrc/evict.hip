@@ -1,0 +1,695 @@
+// Eviction from a latent cache by accumulated attention weight: the account of a step's attention, the selection of the
+// rows that stay, and the moves that bring them together. On compact pages (compact.h) and on bf16 ones.
+#include "compact.h"
+
+namespace hla {
+namespace {
+
+// ---- account -----------------------------------------------------------------------------------------------------
+// account[r, j] += sum over the tokens t of request r and the 16 heads h of exp(scale q[t, h] K[r, j] - lse[h, t]), for
+// j < ctx[t]. The lse is the caller's: of the whole softmax, which may cover more keys than these. Sums are fp32 and in a
+// fixed order: every row's sum is made by one wave.
+struct AccountParams {
+  const uint16_t* q;
+  int64_t q_st, q_sh;
+  const uint8_t* cache;     // compact: page_stride in bytes
+  const uint16_t* cache16;  // bf16: page_stride and row_stride in elements
+  int64_t page_stride, row_stride;
+  int block;
+  int64_t num_blocks;
+  const int32_t* bt;
+  int64_t bt_stride;
+  int bt_cols;
+  const int32_t* qsl;
+  const int32_t* ctx;
+  const float* lse;  // [16][T]
+  int T;
+  float scale;
+  float* account;
+  int64_t a_st;
+  int cols;      // columns of the account
+  int per_wg;    // keys per workgroup (single tokens)
+  float* partial;  // chunks: [shares][R][cols] sums of the shares of each request's tokens, or null (one share)
+};
+
+// K of one tile as the A operand of S^T = K Q^T, and the columns of its steps. Compact pages: step 4i + j of lane (x, g)
+// holds columns 32 (4i + g) + 8j .. + 8 of row x; bf16 pages: step s holds columns 32s + 8g .. + 8.
+template <int W, bool kCompact>
+struct KeyTile {
+  KTile<W> c;
+  __device__ __forceinline__ void load(const AccountParams& a, const int32_t* btr, int row, int x, int g) {
+    const int64_t page = clamp_page(btr[row / a.block], a.num_blocks);
+    load_k<W>(a.cache + page * a.page_stride + (row % a.block) / kTile * compact_tile_bytes(W), x, g, c);
+  }
+  __device__ __forceinline__ u32x4 operand(int s) const {
+    return eight_bf16(c.code[s / 4][s % 4], scale_of(c.scale[s / 16], s / 4 % 4));
+  }
+  static __device__ __forceinline__ int column(int s, int g) { return 32 * (s / 4 * 4 + g) + 8 * (s % 4); }
+};
+
+template <int W>
+struct KeyTile<W, false> {
+  u32x4 v[W / 32];
+  __device__ __forceinline__ void load(const AccountParams& a, const int32_t* btr, int row, int x, int g) {
+    const int64_t page = clamp_page(btr[row / a.block], a.num_blocks);
+    const uint16_t* p = a.cache16 + page * a.page_stride + (int64_t)(row % a.block + x) * a.row_stride + 8 * g;
+#pragma unroll
+    for (int s = 0; s < W / 32; ++s) v[s] = ld16(p + 32 * s);
+  }
+  __device__ __forceinline__ u32x4 operand(int s) const { return v[s]; }
+  static __device__ __forceinline__ int column(int s, int g) { return 32 * s + 8 * g; }
+};
+
+// sum over the 16 lanes of a row (every lane gets it)
+__device__ __forceinline__ float row_sum16(float v) {
+  v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x128, 0xf, 0xf, false));  // row_ror:8
+  v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x124, 0xf, 0xf, false));
+  v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x122, 0xf, 0xf, false));
+  v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x121, 0xf, 0xf, false));
+  return v;
+}
+
+// weight of a score under its softmax's lse (+inf: an empty row, which weighs nothing)
+__device__ __forceinline__ float weight(float s, float scale, float lse) {
+  return fast_exp2(__builtin_fmaf(s, scale, -lse) * kLog2e);
+}
+__device__ __forceinline__ float row_lse(const AccountParams& a, int t, int h) {
+  const float v = a.lse[(int64_t)h * a.T + t];
+  return v == -INFINITY ? INFINITY : v;
+}
+
+// adds the four keys' weights of a tile, summed over the heads, to the account: lane h < 4 of group g takes key 4g + h
+__device__ __forceinline__ void add_to_account(float* row, int limit, int key0, int h, int g, const float (&w)[4]) {
+  float s[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) s[e] = row_sum16(w[e]);
+  const int key = key0 + 4 * g + h;
+  if (h < 4 && key < limit) row[key] += h == 0 ? s[0] : h == 1 ? s[1] : h == 2 ? s[2] : s[3];
+}
+
+// Single tokens: Q^T stays in registers, K streams by (one pass over K per token).
+template <int W, bool kCompact>
+__global__ __launch_bounds__(256) void account_step_kernel(AccountParams a) {
+  using K = KeyTile<W, kCompact>;
+  const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63, h = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int cap = (int)min((int64_t)a.bt_cols * a.block, (int64_t)a.cols);
+  const int t0 = max(a.qsl[r], 0), t1 = min(a.qsl[r + 1], a.T);
+  const int32_t* btr = a.bt + (int64_t)r * a.bt_stride;
+  float* row = a.account + (int64_t)r * a.a_st;
+  for (int t = t0; t < t1; ++t) {
+    const int n = min(a.ctx[t], cap);
+    const int end = min(n, (int)(blockIdx.x + 1) * a.per_wg);
+    int j = blockIdx.x * a.per_wg + wave * kTile;
+    if (j >= end) continue;
+    const uint16_t* qp = a.q + (int64_t)t * a.q_st + (int64_t)h * a.q_sh;
+    u32x4 q[W / 32];
+#pragma unroll
+    for (int s = 0; s < W / 32; ++s) q[s] = ld16(qp + K::column(s, g));
+    const float lse = row_lse(a, t, h);
+    K k;
+    k.load(a, btr, j, h, g);
+    for (; j < end; j += 4 * kTile) {
+      floatx4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < W / 32; ++i) s = mfma16x16x32(k.operand(i), q[i], s);
+      if (j + 4 * kTile < end) k.load(a, btr, j + 4 * kTile, h, g);
+      float w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = weight(s[e], a.scale, lse);
+      add_to_account(row, end, j, h, g, w);
+    }
+  }
+}
+
+// Prompt chunks: a wave keeps 32 rows of K (16 at W = 1024) as bf16 operands and all of the request's queries stream by,
+// through LDS in operand order, one token ahead. The tokens of a request may be shared out over blockIdx.z.
+template <int W, bool kCompact>
+__global__ __launch_bounds__(256, 1) void account_chunk_kernel(AccountParams a) {
+  using K = KeyTile<W, kCompact>;
+  constexpr int NT = W <= 512 ? 2 : 1, STEPS = W / 32, MINE = STEPS / 4;  // steps of Q that a wave stages
+  __shared__ u32x4 q_lds[2][STEPS][64];
+  __shared__ int n_lds[4];
+  const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63, h = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int cap = (int)min((int64_t)a.bt_cols * a.block, (int64_t)a.cols);
+  int t0 = max(a.qsl[r], 0), t1 = min(a.qsl[r + 1], a.T);
+  const int share = (max(t1 - t0, 0) + gridDim.z - 1) / gridDim.z;
+  t0 += blockIdx.z * share;
+  t1 = min(t1, t0 + share);
+  int most = 0;
+  for (int t = t0 + tid; t < t1; t += 256) most = max(most, a.ctx[t]);
+  for (int off = 32; off > 0; off >>= 1) most = max(most, __shfl_xor(most, off));
+  if (lane == 0) n_lds[wave] = most;
+  __syncthreads();
+  most = min(max(max(n_lds[0], n_lds[1]), max(n_lds[2], n_lds[3])), cap);
+  const int wg0 = blockIdx.x * (4 * NT * kTile), key0 = wg0 + wave * (NT * kTile);
+  float* row = a.partial ? a.partial + ((int64_t)blockIdx.z * gridDim.y + r) * a.cols : a.account + (int64_t)r * a.a_st;
+  float w[NT][4];
+#pragma unroll
+  for (int x = 0; x < NT; ++x)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[x][e] = 0.f;
+  if (wg0 < most) {  // uniform over the workgroup
+    u32x4 k[NT][STEPS];
+    {
+      const int32_t* btr = a.bt + (int64_t)r * a.bt_stride;
+#pragma unroll
+      for (int x = 0; x < NT; ++x) {
+        K tile;
+        tile.load(a, btr, min(key0 + x * kTile, (most - 1) / kTile * kTile), h, g);
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) k[x][s] = tile.operand(s);
+      }
+    }
+    u32x4 next[MINE];
+    auto fetch = [&](int t) {
+      const uint16_t* qp = a.q + (int64_t)t * a.q_st + (int64_t)h * a.q_sh;
+#pragma unroll
+      for (int s = 0; s < MINE; ++s) next[s] = ld16(qp + K::column(wave * MINE + s, g));
+    };
+    fetch(t0);
+    float lse_next = row_lse(a, t0, h);
+    int n_next = a.ctx[t0];
+    for (int t = t0; t < t1; ++t) {
+      const int buf = (t - t0) & 1;
+#pragma unroll
+      for (int s = 0; s < MINE; ++s) q_lds[buf][wave * MINE + s][lane] = next[s];
+      const float lse = lse_next;
+      const int n = n_next;
+      if (t + 1 < t1) {
+        fetch(t + 1);
+        lse_next = row_lse(a, t + 1, h);
+        n_next = a.ctx[t + 1];
+      }
+      // one barrier per token: a wave that writes this buffer again has passed the barrier of the token between, which
+      // every wave reaches only after its reads of this one
+      __syncthreads();
+      floatx4 s[NT];
+#pragma unroll
+      for (int x = 0; x < NT; ++x) s[x] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        const u32x4 q = q_lds[buf][i][lane];
+#pragma unroll
+        for (int x = 0; x < NT; ++x) s[x] = mfma16x16x32(k[x][i], q, s[x]);
+      }
+      const int limit = min(n, cap) - key0 - 4 * g;
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p = weight(s[x][e], a.scale, lse);
+          w[x][e] += x * kTile + e < limit ? p : 0.f;
+        }
+    }
+  }
+  if (a.partial) {
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+      float s[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] = row_sum16(w[x][e]);
+      const int key = key0 + x * kTile + 4 * g + h;
+      if (h < 4 && key < a.cols) row[key] = h == 0 ? s[0] : h == 1 ? s[1] : h == 2 ? s[2] : s[3];
+    }
+  } else {
+#pragma unroll
+    for (int x = 0; x < NT; ++x) add_to_account(row, most, key0 + x * kTile, h, g, w[x]);
+  }
+}
+
+// account += the shares' sums, in their order
+__global__ __launch_bounds__(256) void account_reduce_kernel(const float* partial, int shares, int R, int cols,
+                                                             float* account, int64_t a_st) {
+  const int j = blockIdx.x * 256 + threadIdx.x, r = blockIdx.y;
+  if (j >= cols) return;
+  float s = 0.f;
+  for (int z = 0; z < shares; ++z) s += partial[((int64_t)z * R + r) * cols + j];
+  account[(int64_t)r * a_st + j] += s;
+}
+
+// ---- selection -----------------------------------------------------------------------------------------------------
+// Of a request's n rows the best `budget` stay: first the rows whose position is at least protect_from, then by account,
+// descending, ties to the earlier row (NaN ranks last). One workgroup of 16 waves per request; wave w holds rows
+// [w, w + 1) * 64 * per_wave, lane by lane, so that every rank in row order is a sum of ballots. The threshold (the
+// account of the last row to stay) is found two bits at a time by counting, in registers where the rows fit them.
+struct SelectParams {
+  const float* account;
+  int64_t a_st;
+  const int32_t* positions;
+  int64_t p_st;
+  const int32_t* lengths;
+  int budget;
+  const int32_t* budgets;  // per request, or null
+  const int32_t* protect_from;
+  int cols;
+  int32_t* out_lengths;
+  float* out_account;      // [R][cols]
+  int32_t* out_positions;  // [R][cols]
+  int32_t* source;         // [R][cols / 2]
+  int32_t* target;
+};
+
+constexpr int kSelWaves = 16;
+
+// Order of accounts as an unsigned number above 0: NaN 1, then -inf to +inf, the zeros alike
+__device__ __forceinline__ uint32_t rank_key(float a) {
+  if (a != a) return 1u;
+  const uint32_t u = __float_as_uint(a + 0.f);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+__device__ __forceinline__ int below(uint64_t mask, int lane) {
+  return __popcll(mask & ((1ull << lane) - 1));
+}
+
+// f(i) for the rows i of a lane
+template <int kItems, class F>
+__device__ __forceinline__ void each_row(int items, F f) {
+  if constexpr (kItems > 0) {
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) f(i);
+  } else {
+    for (int i = 0; i < items; ++i) f(i);
+  }
+}
+
+// kItems > 0: the rank keys of kItems rows per lane stay in registers; kLdsKeys: up to kMaxLdsItems in LDS; kReadKeys: any
+// number, made anew in every pass
+constexpr int kLdsKeys = 0, kReadKeys = -1, kMaxLdsItems = 32;
+
+template <int kItems>
+__global__ __launch_bounds__(64 * kSelWaves) void select_rows_kernel(SelectParams a) {
+  __shared__ int sums[2][kSelWaves][4];
+  __shared__ uint32_t keys_lds[kItems == kLdsKeys ? kMaxLdsItems * 64 * kSelWaves : 1];
+  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const float* acc = a.account + (int64_t)r * a.a_st;
+  const int32_t* pos = a.positions + (int64_t)r * a.p_st;
+  const int n = min(max(a.lengths[r], 0), a.cols);
+  const int b = min(n, max(a.budgets ? a.budgets[r] : a.budget, 0));
+  const int first = a.protect_from[r];
+  const int items = kItems > 0 ? kItems : (a.cols + 64 * kSelWaves - 1) / (64 * kSelWaves);
+  const int j0 = wave * items * 64 + lane;
+  const bool all = n == b;  // nothing goes
+
+  int turn = 0;  // `sums` alternates between two buffers: one barrier per total
+  // sums of x, y, z (uniform over a wave) over all waves, and of x and y over the waves before this one
+  auto total = [&](int x, int y, int z, int& before_x, int& before_y) {
+    if (lane == 0) {
+      sums[turn][wave][0] = x;
+      sums[turn][wave][1] = y;
+      sums[turn][wave][2] = z;
+    }
+    __syncthreads();
+    int sx = 0, sy = 0, sz = 0;
+    before_x = before_y = 0;
+#pragma unroll
+    for (int w = 0; w < kSelWaves; ++w) {
+      const int ux = sums[turn][w][0], uy = sums[turn][w][1];
+      before_x += w < wave ? ux : 0;
+      before_y += w < wave ? uy : 0;
+      sx += ux;
+      sy += uy;
+      sz += sums[turn][w][2];
+    }
+    turn ^= 1;
+    return make_int3(sx, sy, sz);
+  };
+  int skip_x, skip_y;
+
+  uint32_t reg[kItems > 0 ? kItems : 1];
+  uint64_t guarded = 0;  // bit i: row i of this lane is protected (not kReadKeys)
+  bool among_protected = false;
+  int need = 0;
+  if (!all) {
+    int here = 0;
+    each_row<kItems>(items, [&](int i) {
+      const int j = j0 + 64 * i;
+      const bool prot = j < n && pos[j] >= first;
+      here += __popcll(__ballot(prot));
+      if constexpr (kItems != kReadKeys) {
+        guarded |= (uint64_t)prot << i;
+        const uint32_t key = j < n ? rank_key(acc[j]) : 0u;
+        if constexpr (kItems > 0) reg[i] = key;
+        else keys_lds[i * (64 * kSelWaves) + tid] = key;
+      }
+    });
+    const int np = total(here, 0, 0, skip_x, skip_y).x;
+    // candidates: the unprotected rows (the protected ones all stay), or the protected ones where these are too many
+    among_protected = np >= b;
+    need = among_protected ? b : b - np;
+    if constexpr (kItems > 0) {
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) reg[i] = (((guarded >> i) & 1) != 0) == among_protected ? reg[i] : 0u;
+    }
+  }
+  // key of row i as a candidate (0: it is none), and whether it stays anyhow
+  auto row_of = [&](int i, bool& anyhow) -> uint32_t {
+    const int j = j0 + 64 * i;
+    if (all) {
+      anyhow = j < n;
+      return 0u;
+    }
+    bool prot;
+    if constexpr (kItems == kReadKeys) prot = j < n && pos[j] >= first;
+    else prot = (guarded >> i) & 1;
+    anyhow = prot && !among_protected;
+    if constexpr (kItems > 0) return reg[i];
+    else if constexpr (kItems == kLdsKeys) return prot == among_protected ? keys_lds[i * (64 * kSelWaves) + tid] : 0u;
+    else return j < n && prot == among_protected ? rank_key(acc[j]) : 0u;
+  };
+
+  uint32_t threshold = 0xffffffffu;  // candidates above it stay, and the first `ties` at it (no key is that high)
+  int ties = 0;
+  if (need > 0) {
+    uint32_t found = 0;
+    int above = 0;  // candidates above every key that still fits `found`
+    bool exact = false;
+    for (int bit = 30; bit >= 0; bit -= 2) {
+      const uint32_t t1 = found | (1u << bit), t2 = found | (2u << bit), t3 = found | (3u << bit);
+      int c1 = 0, c2 = 0, c3 = 0;
+      each_row<kItems>(items, [&](int i) {
+        bool anyhow;
+        const uint32_t key = row_of(i, anyhow);
+        c1 += __popcll(__ballot(key >= t1));
+        c2 += __popcll(__ballot(key >= t2));
+        c3 += __popcll(__ballot(key >= t3));
+      });
+      const int3 c = total(c1, c2, c3, skip_x, skip_y);
+      const int at = c.z >= need ? c.z : c.y >= need ? c.y : c.x >= need ? c.x : -1;
+      above = c.z >= need ? above : c.y >= need ? c.z : c.x >= need ? c.y : c.x;
+      found = c.z >= need ? t3 : c.y >= need ? t2 : c.x >= need ? t1 : found;
+      if (at == need) {  // exactly the candidates at or above `found` stay (uniform over the workgroup)
+        exact = true;
+        break;
+      }
+    }
+    threshold = exact ? found - 1 : found;
+    ties = exact ? 0 : need - above;
+  }
+
+  // ranks in row order: the ties before this wave's rows, then holes (rows below b that go) and extras (rows behind that stay)
+  int ties0 = 0;
+  if (ties > 0) {
+    int here = 0;
+    each_row<kItems>(items, [&](int i) {
+      bool anyhow;
+      here += __popcll(__ballot(row_of(i, anyhow) == threshold));
+    });
+    total(here, 0, 0, ties0, skip_y);
+  }
+  int run;  // ties so far
+  auto stays = [&](int i) {
+    bool anyhow;
+    const uint32_t key = row_of(i, anyhow);
+    const uint64_t at = ties > 0 ? __ballot(key == threshold) : 0;
+    const bool tie = ties > 0 && key == threshold && run + below(at, lane) < ties;
+    run += __popcll(at);
+    return anyhow || key > threshold || tie;
+  };
+  int holes = 0, extras = 0;
+  run = ties0;
+  each_row<kItems>(items, [&](int i) {
+    const int j = j0 + 64 * i;
+    const bool stay = stays(i);
+    holes += __popcll(__ballot(!stay && j < b));
+    extras += __popcll(__ballot(stay && j >= b));
+  });
+  int hole0, extra0;
+  const int moves = total(holes, extras, 0, hole0, extra0).x;
+  const int half = a.cols / 2;
+  int32_t* source = a.source + (int64_t)r * half;
+  int32_t* target = a.target + (int64_t)r * half;
+  run = ties0;
+  holes = hole0;
+  extras = extra0;
+  each_row<kItems>(items, [&](int i) {
+    const int j = j0 + 64 * i;
+    const bool stay = stays(i);
+    const uint64_t hm = __ballot(!stay && j < b), em = __ballot(stay && j >= b);
+    if (!stay && j < b) target[holes + below(hm, lane)] = j;
+    if (stay && j >= b) source[extras + below(em, lane)] = j;
+    holes += __popcll(hm);
+    extras += __popcll(em);
+  });
+  for (int i = moves + tid; i < half; i += 64 * kSelWaves) source[i] = target[i] = -1;
+  if (tid == 0) a.out_lengths[r] = b;
+  __syncthreads();  // the lists are whole
+  run = ties0;
+  holes = hole0;
+  each_row<kItems>(items, [&](int i) {
+    const int j = j0 + 64 * i;
+    const bool stay = stays(i);
+    const uint64_t hm = __ballot(!stay && j < b);
+    if (j < a.cols) {
+      float w = 0.f;
+      int32_t p = -1;
+      if (j < b) {
+        const int from = stay ? j : source[holes + below(hm, lane)];
+        w = acc[from];
+        p = pos[from];
+      }
+      a.out_account[(int64_t)r * a.cols + j] = w;
+      a.out_positions[(int64_t)r * a.cols + j] = p;
+    }
+    holes += __popcll(hm);
+  });
+}
+
+// ---- moves -----------------------------------------------------------------------------------------------------------
+// Row source[r, i] of request r over row target[r, i], for every pair that is not -1. A target lies below the request's new
+// length and a source behind it, so no pair touches another's rows.
+struct MoveParams {
+  uint8_t* cache;
+  int64_t page_stride, row_stride;  // bytes (row_stride: bf16 pages)
+  int block;
+  int64_t num_blocks;
+  const int32_t* bt;
+  int64_t bt_stride;
+  int bt_cols;
+  const int32_t* source;
+  const int32_t* target;
+  int64_t list_st;
+  int count;
+};
+
+constexpr int kMoveRows = 4;  // moves per thread
+
+// pieces of a row: 16 bytes of values, or one scale (compact); 16 bytes (bf16)
+template <int W, bool kCompact>
+struct RowPieces {
+  static constexpr int N = kCompact ? W / 8 : W / 4;
+};
+
+template <int W, bool kCompact>
+__device__ __forceinline__ uint8_t* piece_at(const MoveParams& a, int64_t page, int in_page, int u) {
+  uint8_t* p = a.cache + page * a.page_stride;
+  if constexpr (!kCompact) {
+    return p + in_page * a.row_stride + 16 * u;
+  } else {
+    constexpr int NB = W / 32;
+    const int x = in_page & 15, b = u % NB;
+    p += (in_page >> 4) * compact_tile_bytes(W);
+    return p + (u < NB ? k_code_at(x, b)
+                       : u < 2 * NB ? v_code_at(W, x, 16 * b) : u < 3 * NB ? k_scale_at(W, x, b) : v_scale_at(W, x, b));
+  }
+}
+
+template <int W, bool kCompact>
+__global__ __launch_bounds__(256) void move_rows_kernel(MoveParams a) {
+  constexpr int N = RowPieces<W, kCompact>::N;
+  constexpr int ROWS = N <= 256 ? 256 / N : 1;
+  const int r = blockIdx.y;
+  const int32_t* source = a.source + (int64_t)r * a.list_st;
+  const int32_t* target = a.target + (int64_t)r * a.list_st;
+  const int32_t* btr = a.bt + (int64_t)r * a.bt_stride;
+  const int first = blockIdx.x * (ROWS * kMoveRows) + threadIdx.x / N;
+  u32x4 big[kMoveRows];
+  uint8_t small[kMoveRows];
+  uint8_t* to[kMoveRows];
+  const int u = threadIdx.x % N;
+  const bool scale = kCompact && u >= W / 16;
+#pragma unroll
+  for (int k = 0; k < kMoveRows; ++k) {
+    const int i = first + k * ROWS;
+    to[k] = nullptr;
+    if (i < a.count) {
+      const int s = source[i], t = target[i];
+      const int64_t cap = (int64_t)a.bt_cols * a.block;
+      if (s >= 0 && t >= 0 && s < cap && t < cap) {
+        const int64_t from = btr[s / a.block], dest = btr[t / a.block];
+        if (from >= 0 && from < a.num_blocks && dest >= 0 && dest < a.num_blocks) {
+          const uint8_t* p = piece_at<W, kCompact>(a, from, s % a.block, u);
+          to[k] = piece_at<W, kCompact>(a, dest, t % a.block, u);
+          if (scale) small[k] = *p;
+          else big[k] = ld16(p);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kMoveRows; ++k)
+    if (to[k]) {
+      if (scale) *to[k] = small[k];
+      else st16(to[k], big[k]);
+    }
+}
+
+template <int W, bool kCompact>
+void launch_account(const AccountParams& p, int R, int shares, bool chunks, hipStream_t st) {
+  const int keys = min((int64_t)p.bt_cols * p.block, (int64_t)p.cols);
+  if (!chunks) {
+    hipLaunchKernelGGL((account_step_kernel<W, kCompact>), dim3((unsigned)((keys + p.per_wg - 1) / p.per_wg), (unsigned)R),
+                       dim3(256), 0, st, p);
+    return;
+  }
+  constexpr int per = 4 * (W <= 512 ? 2 : 1) * kTile;
+  hipLaunchKernelGGL((account_chunk_kernel<W, kCompact>),
+                     dim3((unsigned)(((p.partial ? p.cols : keys) + per - 1) / per), (unsigned)R, (unsigned)shares),
+                     dim3(256), 0, st, p);
+  if (p.partial)
+    hipLaunchKernelGGL(account_reduce_kernel, dim3((unsigned)((p.cols + 255) / 256), (unsigned)R), dim3(256), 0, st,
+                       p.partial, shares, R, p.cols, p.account, p.a_st);
+}
+
+template <int W, bool kCompact>
+void launch_move(const MoveParams& p, int R, hipStream_t st) {
+  constexpr int N = RowPieces<W, kCompact>::N, rows = kMoveRows * (N <= 256 ? 256 / N : 1);
+  hipLaunchKernelGGL((move_rows_kernel<W, kCompact>), dim3((unsigned)((p.count + rows - 1) / rows), (unsigned)R),
+                     dim3(256), 0, st, p);
+}
+
+int check_pages16(const char* what, int width, const void* cache, int64_t page_stride, int64_t row_stride, int block,
+                  int64_t num_blocks) {
+  HLA_REQUIRE(known_width(width), HLA_S6_EUNSUPPORTED, "%s: latent width %d not in {128, 256, 512, 1024}", what, width);
+  HLA_REQUIRE(block > 0 && block % kTile == 0, HLA_S6_EUNSUPPORTED, "%s: block size %d is not a positive multiple of 16",
+              what, block);
+  HLA_REQUIRE(num_blocks >= 1, HLA_S6_EINVAL, "%s: empty cache", what);
+  HLA_REQUIRE(cache && aligned(cache, 16) && page_stride % 8 == 0 && row_stride % 8 == 0, HLA_S6_EINVAL,
+              "%s: cache rows must be 16-byte aligned (strides multiple of 8 elements)", what);
+  return HLA_S6_OK;
+}
+
+}  // namespace
+}  // namespace hla
+
+extern "C" int hla_s6_attention_weights(const void* q, int32_t num_tokens, int32_t num_heads, int32_t width, int64_t q_st,
+                                        int64_t q_sh, const void* cache, int32_t compact, int64_t page_stride,
+                                        int64_t row_stride, int32_t block_size, int64_t num_blocks,
+                                        const int32_t* block_table, int64_t bt_stride, int32_t bt_cols,
+                                        const int32_t* query_start_loc, int32_t num_reqs, const int32_t* ctx,
+                                        const float* lse, float scale, float* account, int64_t a_st, int32_t cols,
+                                        int32_t keys_per_wg, int32_t shares, float* workspace, int64_t workspace_floats,
+                                        void* stream) {
+  using namespace hla;
+  HLA_REQUIRE(num_tokens >= 0 && num_reqs >= 0 && num_reqs <= 65535 && bt_cols >= 0 && cols >= 0, HLA_S6_EINVAL,
+              "attention_weights: bad token count, request count (0..65535) or table width");
+  HLA_REQUIRE(num_heads == kHeads, HLA_S6_EUNSUPPORTED, "attention_weights: %d query heads (the kernel is built for 16)",
+              num_heads);
+  int rc = compact ? check_cache("attention_weights", width, cache, page_stride, block_size, num_blocks)
+                   : check_pages16("attention_weights", width, cache, page_stride, row_stride, block_size, num_blocks);
+  if (rc != HLA_S6_OK || num_tokens == 0 || num_reqs == 0 || cols == 0 || bt_cols == 0) return rc;
+  HLA_REQUIRE(q && block_table && query_start_loc && ctx && lse && account, HLA_S6_EINVAL,
+              "attention_weights: null pointer argument");
+  HLA_REQUIRE(aligned(q, 16) && q_st % 8 == 0 && q_sh % 8 == 0, HLA_S6_EINVAL,
+              "attention_weights: q needs 16-byte aligned rows (unit last stride, strides multiple of 8)");
+  HLA_REQUIRE(a_st >= cols, HLA_S6_EINVAL, "attention_weights: account rows overlap");
+  HLA_REQUIRE(shares >= 0 && shares <= 64, HLA_S6_EINVAL, "attention_weights: shares must be in [0, 64]");
+  HLA_REQUIRE(shares > 0 || (keys_per_wg > 0 && keys_per_wg % 64 == 0), HLA_S6_EINVAL,
+              "attention_weights: keys per workgroup must be a positive multiple of 64");
+  if (shares > 1) {
+    const int64_t need = (int64_t)shares * num_reqs * cols;
+    HLA_REQUIRE(workspace && workspace_floats >= need, HLA_S6_EWORKSPACE,
+                "attention_weights: workspace needs %lld floats, has %lld", (long long)need, (long long)workspace_floats);
+  }
+  AccountParams p = {};
+  p.q = static_cast<const uint16_t*>(q);
+  p.q_st = q_st;
+  p.q_sh = q_sh;
+  p.cache = static_cast<const uint8_t*>(cache);
+  p.cache16 = static_cast<const uint16_t*>(cache);
+  p.page_stride = page_stride;
+  p.row_stride = row_stride;
+  p.block = block_size;
+  p.num_blocks = num_blocks;
+  p.bt = block_table;
+  p.bt_stride = bt_stride;
+  p.bt_cols = bt_cols;
+  p.qsl = query_start_loc;
+  p.ctx = ctx;
+  p.lse = lse;
+  p.T = num_tokens;
+  p.scale = scale;
+  p.account = account;
+  p.a_st = a_st;
+  p.cols = cols;
+  p.per_wg = keys_per_wg;
+  p.partial = shares > 1 ? workspace : nullptr;
+  const hipStream_t st = as_stream(stream);
+  const bool chunks = shares > 0;
+#define HLA_ACCOUNT(W)                                                      \
+  compact ? launch_account<W, true>(p, num_reqs, shares, chunks, st)        \
+          : launch_account<W, false>(p, num_reqs, shares, chunks, st)
+  switch (width) {
+    case 128: HLA_ACCOUNT(128); break;
+    case 256: HLA_ACCOUNT(256); break;
+    case 512: HLA_ACCOUNT(512); break;
+    default: HLA_ACCOUNT(1024); break;
+  }
+#undef HLA_ACCOUNT
+  return check_launch("attention_weights");
+}
+
+extern "C" int hla_s6_select_rows(const float* account, int64_t a_st, const int32_t* positions, int64_t p_st,
+                                  const int32_t* lengths, int32_t num_reqs, int32_t cols, int32_t budget,
+                                  const int32_t* budgets, const int32_t* protect_from, int32_t* out_lengths,
+                                  float* out_account, int32_t* out_positions, int32_t* source, int32_t* target,
+                                  void* stream) {
+  using namespace hla;
+  HLA_REQUIRE(num_reqs >= 0 && cols >= 0 && (budgets || budget >= 0), HLA_S6_EINVAL,
+              "select_rows: bad request count, row count or budget");
+  if (num_reqs == 0) return HLA_S6_OK;
+  HLA_REQUIRE(lengths && protect_from && out_lengths, HLA_S6_EINVAL, "select_rows: null pointer argument");
+  HLA_REQUIRE(cols == 0 || (account && positions && out_account && out_positions), HLA_S6_EINVAL,
+              "select_rows: null pointer argument");
+  HLA_REQUIRE(cols < 2 || (source && target), HLA_S6_EINVAL, "select_rows: null list");
+  HLA_REQUIRE(a_st >= cols && p_st >= cols, HLA_S6_EINVAL, "select_rows: rows overlap");
+  SelectParams p = {account, a_st, positions, p_st, lengths, budget, budgets, protect_from, cols,
+                    out_lengths, out_account, out_positions, source, target};
+  const hipStream_t st = as_stream(stream);
+  const dim3 grid((unsigned)num_reqs), block(64 * kSelWaves);
+  const int items = (cols + 64 * kSelWaves - 1) / (64 * kSelWaves);
+  if (items <= 2) hipLaunchKernelGGL(select_rows_kernel<2>, grid, block, 0, st, p);
+  else if (items <= 8) hipLaunchKernelGGL(select_rows_kernel<8>, grid, block, 0, st, p);
+  else if (items <= kMaxLdsItems) hipLaunchKernelGGL(select_rows_kernel<kLdsKeys>, grid, block, 0, st, p);
+  else hipLaunchKernelGGL(select_rows_kernel<kReadKeys>, grid, block, 0, st, p);
+  return check_launch("select_rows");
+}
+
+extern "C" int hla_s6_move_rows(void* cache, int32_t width, int32_t compact, int64_t page_stride, int64_t row_stride,
+                                int32_t block_size, int64_t num_blocks, const int32_t* block_table, int64_t bt_stride,
+                                int32_t bt_cols, const int32_t* source, const int32_t* target, int64_t list_st,
+                                int32_t count, int32_t num_reqs, void* stream) {
+  using namespace hla;
+  HLA_REQUIRE(num_reqs >= 0 && num_reqs <= 65535 && count >= 0 && bt_cols >= 0, HLA_S6_EINVAL,
+              "move_rows: bad request count (0..65535), list length or table width");
+  int rc = compact ? check_cache("move_rows", width, cache, page_stride, block_size, num_blocks)
+                   : check_pages16("move_rows", width, cache, page_stride, row_stride, block_size, num_blocks);
+  if (rc != HLA_S6_OK || num_reqs == 0 || count == 0 || bt_cols == 0) return rc;
+  HLA_REQUIRE(block_table && source && target, HLA_S6_EINVAL, "move_rows: null pointer argument");
+  HLA_REQUIRE(list_st >= count, HLA_S6_EINVAL, "move_rows: lists overlap");
+  MoveParams p = {static_cast<uint8_t*>(cache), compact ? page_stride : 2 * page_stride, 2 * row_stride, block_size,
+                  num_blocks, block_table, bt_stride, bt_cols, source, target, list_st, count};
+  const hipStream_t st = as_stream(stream);
+#define HLA_MOVE(W) compact ? launch_move<W, true>(p, num_reqs, st) : launch_move<W, false>(p, num_reqs, st)
+  switch (width) {
+    case 128: HLA_MOVE(128); break;
+    case 256: HLA_MOVE(256); break;
+    case 512: HLA_MOVE(512); break;
+    default: HLA_MOVE(1024); break;
+  }
+#undef HLA_MOVE
+  return check_launch("move_rows");
+}

@@ -12,7 +12,7 @@ from dataclasses import dataclass
 
 import torch
 
-from . import _lib, s6_ops
+from . import _lib, compact_cache, s6_ops
 
 
 def latent_inv_freq(head_dim, theta):
@@ -201,7 +201,7 @@ class StepContext:
 FUSED_CHUNK_TOKENS = 16
 
 
-def attend(sl, loop, q_lat, q_rope, k_rope, v, cache, block_table, k_scale, v_scale, ctx, window=None):
+def attend(sl, loop, q_lat, q_rope, k_rope, v, cache, block_table, k_scale, v_scale, ctx, window=None, weights=None):
     """One softmax over the paged latent history (fully visible) and the causal current chunk
     (``hla/vllm_latent/s6_layer.py:87-115``).
 
@@ -217,13 +217,19 @@ def attend(sl, loop, q_lat, q_rope, k_rope, v, cache, block_table, k_scale, v_sc
     (``kv_splits > 1``) compute their chunk + window partial as the reference does, then the history kernels' split
     partials, and one epilogue reduces the splits, applies ``B_t`` and merges (the decode step's epilogue). Other
     steps compose the single ops in the reference's order.
+
+    ``cache`` may be a compact one (``compact_cache``, uint8; no reference counterpart): the history then runs on its kernels,
+    split and merged by the same epilogue. ``weights`` (fp32 ``[R, M]``, likewise) is the account of
+    ``compact_cache.attention_weights``: what the joint softmax gives every latent row is added to it, and the step is composed
+    of single ops, whose merge returns the joint lse.
     """
     fused = window is not None and ctx.md_present and (ctx.max_query_len == 1 or
                                                        (ctx.fused_chunks and ctx.max_query_len < FUSED_CHUNK_TOKENS))
     has_history = cache is not None and ctx.md_present and ctx.history_needed
-    if fused and has_history:
+    composed = has_history and (weights is not None or compact_cache.is_compact(cache))
+    if fused and has_history and not composed:
         return _attend_decode(sl, loop, q_lat, q_rope, cache, block_table, ctx, window)
-    if fused:
+    if fused and not (composed and ctx.max_query_len > 1):   # (a chunk of several tokens has its window history in common)
         o_chunk, lse_chunk = s6_ops.window_attention_fa(q_rope, window[0], window[1], ctx.query_start_loc, ctx.seq_lens,
                                                         ctx.window, ctx.scale, ctx.max_seqlen_k, ctx.invalid)
     elif window is not None and has_history:  # the chunk and its exact window history in one softmax
@@ -237,6 +243,8 @@ def attend(sl, loop, q_lat, q_rope, k_rope, v, cache, block_table, k_scale, v_sc
         return o_chunk.masked_fill_(ctx.invalid[:, None, None], 0)
     _, B, _ = sl.readers(loop)
     w = q_lat.shape[-1]
+    if composed:
+        return _attend_composed(q_lat, o_chunk, lse_chunk, B, cache, block_table, ctx, weights)
     if window is not None and ctx.fused_chunks and ctx.history_group > 1 and ctx.kv_splits(w) > 1:
         # multi-query step with split history: the grouped kernels' split partials, then the fused decode step's
         # epilogue (LSE reduction, B_t, merge with the chunk + window partial) in place of history_attention,
@@ -254,6 +262,42 @@ def attend(sl, loop, q_lat, q_rope, k_rope, v, cache, block_table, k_scale, v_sc
                                                    shared_rows=ctx.max_query_len > 1)
     o_hist = absorb_out(o_hist, B)
     return s6_ops.merge_states(o_hist, lse_hist, o_chunk, lse_chunk, ctx.invalid, ctx.backends.merge)
+
+
+def _attend_composed(q_lat, o_chunk, lse_chunk, B, cache, block_table, ctx, weights):
+    """History of a compact cache, or of any cache with an account of its attention weights, merged with the chunk's
+    partial. Steps of short chunks over a compact cache take the split kernel and the fused epilogue; an account needs the
+    merged lse, which only the single ops return."""
+    for kind in ('history', 'merge'):
+        s6_ops._backend(kind, getattr(ctx.backends, kind))
+    w = q_lat.shape[-1]
+    if compact_cache.is_compact(cache):
+        T, rows = q_lat.shape[0], block_table.shape[1] * compact_cache.block_size(cache)
+        longest = min(int(ctx.max_seqlen_k), rows) if ctx.max_seqlen_k else rows
+        splits = compact_cache.kv_splits(longest, T, _lib.device_cus(q_lat.device.index or 0), w)
+        workspace = ctx.workspace
+        if workspace is not None and T * q_lat.shape[1] * splits * (w + 1) > workspace.floats:
+            workspace = None
+        if weights is None and splits > 1 and ctx.max_query_len < compact_cache.CHUNK_TOKENS:
+            if workspace is None:
+                workspace = s6_ops.S6Workspace(q_lat.shape[1], w, T * splits)
+            ws = compact_cache.history_partials(q_lat, cache, block_table, ctx.ctx_latent, ctx.scale, splits, workspace,
+                                                ctx.token_requests, ctx.split_plan(splits, rows))
+            return s6_ops.split_epilogue(ws, B, o_chunk, lse_chunk, ctx.invalid)
+        o_hist, lse_hist = compact_cache.history_attention(
+            q_lat, cache, block_table, ctx.ctx_latent, ctx.scale, longest, ctx.token_requests, ctx.query_start_loc,
+            ctx.max_query_len, workspace=workspace if ctx.max_query_len < compact_cache.CHUNK_TOKENS else None)
+    else:
+        o_hist, lse_hist = s6_ops.history_attention_kv(
+            q_lat, cache[..., :w], cache[..., w:], block_table, ctx.ctx_latent, ctx.scale, ctx.kv_splits(w), ctx.workspace,
+            None, None, ctx.backends.history, bt_rows=ctx.token_requests, tokens_per_group=ctx.history_group,
+            shared_rows=ctx.max_query_len > 1)
+    o_hist = absorb_out(o_hist, B)
+    if weights is None:
+        return s6_ops.merge_states(o_hist, lse_hist, o_chunk, lse_chunk, ctx.invalid, ctx.backends.merge)
+    out, lse = s6_ops.merge_lse(o_hist, lse_hist, o_chunk, lse_chunk)
+    compact_cache.attention_weights(q_lat, cache, block_table, ctx.query_start_loc, ctx.ctx_latent, lse, ctx.scale, weights)
+    return out.masked_fill_(ctx.invalid[:, None, None], 0)
 
 
 def _attend_decode(sl, loop, q_lat, q_rope, cache, block_table, ctx, window):
@@ -378,9 +422,13 @@ def write_commit(sl, loop, h, state, ctx, cache, block_table):
     launch. At loop 0 and the last loop the committed row goes straight from the projection's epilogue into
     ``cache`` (``[num_blocks, 1, block, 2w]``; K half latent-rotated, padding tokens skipped) and the returned state
     holds no row, since nothing reads it again; other loops return the accumulated register as ``write_rows`` does.
-    ``block_table`` is the per-request table of ``cache``."""
+    ``block_table`` is the per-request table of ``cache``. A compact cache takes its rows in the three steps."""
     if loop != 0 and loop != sl.loops - 1:
         return write_rows(sl, loop, h, state)
+    if compact_cache.is_compact(cache):
+        key, value = committed_row(sl, loop, write_rows(sl, loop, h, state), ctx)
+        compact_cache.store_rows(key, value, ctx.slots(block_table, compact_cache.block_size(cache)), cache)
+        return WriterState(None, None)
     weight, width = _writer_weight(sl, loop)
     prev = None if loop == 0 or state is None else state.reg
     slots = ctx.slots(block_table, cache.shape[2])
@@ -413,7 +461,10 @@ def slot_mapping(ctx, block_table, block_size):
 
 def store_rows(key, value, slots, cache):
     """Slot-mapped store of ``[key | value]`` rows into a ``[num_blocks, 1, block, 2w]`` latent cache (negative slots
-    skipped): the ``unified_kv_cache_update`` of ``hla/vllm_latent/ouro_latent.py:127-129``."""
+    skipped): the ``unified_kv_cache_update`` of ``hla/vllm_latent/ouro_latent.py:127-129``. A compact cache (uint8) quantises
+    them (``compact_cache.store_rows``)."""
+    if compact_cache.is_compact(cache):
+        return compact_cache.store_rows(key, value, slots, cache)
     s6_ops._bf16('key', key)
     s6_ops._bf16('value', value)
     s6_ops._bf16('cache', cache)

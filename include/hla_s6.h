@@ -24,7 +24,7 @@
 extern "C" {
 #endif
 
-#define HLA_S6_ABI_VERSION 14
+#define HLA_S6_ABI_VERSION 15
 
 #define HLA_S6_OK 0
 #define HLA_S6_EINVAL 1       /* bad shape, stride or argument            (Python: ValueError)   */
@@ -505,6 +505,76 @@ int hla_s6_rope_rows_backward(int32_t count, const float *const *dy, const int64
                               const int64_t *dx_strides, int32_t batch, int32_t num_heads, int32_t chunk,
                               int32_t head_dim, const void *cos, const void *sin, int64_t c_sb, int64_t c_si,
                               int32_t trig_bf16, void *stream);
+
+/* ---- the compact latent cache ----------------------------------------------------------------------
+ * Rows [K | V] of 2 * width values in 4 bits each, in pages of block_size rows (a multiple of 16) of which every 16 rows are
+ * a tile of 17 * width consecutive bytes: E2M1 values with a power-of-two scale per 32 columns, in the order of
+ * csrc/compact.h. `cache` is 16-byte aligned bytes, page_stride (bytes) a multiple of 16 of at least a page; width in
+ * {128, 256, 512, 1024}. Block tables, slots and lengths are those of the bf16 cache (a4, a10).
+ *
+ * hla_s6_compact_store quantises row t of key / value (bf16 [num_tokens, width], row strides k_st / v_st) into slot slots[t]
+ * (page * block_size + row; outside the cache: skipped; the slots of a call differ). Scale of 32 columns: the smallest
+ * power of two s with max|x| <= 7 s, exponent -120 to 125; values to the nearest, ties to even; an infinity or NaN makes
+ * its 32 columns read as NaN. */
+int hla_s6_compact_store(const void *key, int64_t k_st, const void *value, int64_t v_st, int32_t num_tokens,
+                         int32_t width, const int64_t *slots, void *cache, int64_t page_stride, int32_t block_size,
+                         int64_t num_blocks, void *stream);
+
+/* out[r, j, :] (bf16, strides o_sr, o_sj, 1; 16-byte aligned rows) = row j of request r, for j < max_rows. With `lengths`
+ * [num_reqs], rows at and past lengths[r] are zero. With lengths NULL the length of request r is the largest ctx[t] of its
+ * tokens query_start_loc[r] <= t < query_start_loc[r + 1] (below num_tokens), and rows past it are not written. Page ids
+ * are clamped into the cache. num_reqs <= 65535. */
+int hla_s6_compact_load(const void *cache, int32_t width, int64_t page_stride, int32_t block_size, int64_t num_blocks,
+                        const int32_t *block_table, int64_t bt_stride, int32_t bt_cols, const int32_t *lengths,
+                        const int32_t *query_start_loc, const int32_t *ctx, int32_t num_tokens, int32_t num_reqs,
+                        int32_t max_rows, void *out, int64_t o_sr, int64_t o_sj, void *stream);
+
+/* hla_s6_history_attention over a compact cache: same outputs, splits, workspace and plan (hla_s6_split_plan of (ctx,
+ * bt_cols * block_size, num_splits), nullable). Token t reads row bt_rows ? bt_rows[t] : t of the table, clamped into its
+ * bt_count rows. With out and lse NULL the call ends with the partials in the workspace (num_splits >= 1), in the layout
+ * that hla_s6_history_reduce and hla_s6_split_epilogue read. */
+int hla_s6_compact_history(const void *q, int32_t num_tokens, int32_t num_heads, int32_t width, int64_t q_st,
+                           int64_t q_sh, const void *cache, int64_t page_stride, int32_t block_size,
+                           int64_t num_blocks, const int32_t *block_table, int64_t bt_stride, int32_t bt_cols,
+                           int32_t bt_count, const int64_t *bt_rows, const int32_t *ctx, float scale,
+                           int32_t num_splits, float *workspace, int64_t workspace_floats, const int32_t *plan,
+                           int64_t plan_len, void *out, int64_t o_st, int64_t o_sh, float *lse, void *stream);
+
+/* ---- eviction from a latent cache --------------------------------------------------------------------
+ * On compact caches (compact != 0: page_stride in bytes, row_stride unused) and on bf16 ones (strides in elements, rows
+ * 16-byte aligned, K then V).
+ *
+ * hla_s6_attention_weights: account[r, j] += sum over the tokens t of request r (query_start_loc [num_reqs + 1]) and the 16
+ * heads h of exp(scale * q[t, h] . K[r, j] - lse[h, t]) for j < min(ctx[t], cols, bt_cols * block_size). lse [16, num_tokens]
+ * is contiguous; an infinite one adds nothing. account is fp32 with row stride a_st >= cols. shares 0: K streams past the
+ * queries, keys_per_wg (a multiple of 64) rows per workgroup; shares >= 1 (at most 64): the queries stream past K, each
+ * request's tokens in that many parts, whose sums go through `workspace` (shares * num_reqs * cols floats) when there is
+ * more than one. Sums are in a fixed order. */
+int hla_s6_attention_weights(const void *q, int32_t num_tokens, int32_t num_heads, int32_t width, int64_t q_st,
+                             int64_t q_sh, const void *cache, int32_t compact, int64_t page_stride, int64_t row_stride,
+                             int32_t block_size, int64_t num_blocks, const int32_t *block_table, int64_t bt_stride,
+                             int32_t bt_cols, const int32_t *query_start_loc, int32_t num_reqs, const int32_t *ctx,
+                             const float *lse, float scale, float *account, int64_t a_st, int32_t cols,
+                             int32_t keys_per_wg, int32_t shares, float *workspace, int64_t workspace_floats,
+                             void *stream);
+
+/* Of the first lengths[r] rows of request r the best min(budget, lengths[r]) stay (budgets [num_reqs], when given, in place of
+ * budget): first those with positions[r, j] >= protect_from[r], then by account[r, j], descending, ties to the earlier row,
+ * NaN last. Rows that stay below the new length out_lengths[r] keep their place; the i-th one behind it (source[r, i])
+ * moves to the i-th place left free (target[r, i]); both lists are [num_reqs, cols / 2], -1 behind their end. out_account
+ * and out_positions [num_reqs, cols] hold the new order, 0 and -1 behind the new length. */
+int hla_s6_select_rows(const float *account, int64_t a_st, const int32_t *positions, int64_t p_st,
+                       const int32_t *lengths, int32_t num_reqs, int32_t cols, int32_t budget, const int32_t *budgets,
+                       const int32_t *protect_from, int32_t *out_lengths, float *out_account, int32_t *out_positions,
+                       int32_t *source, int32_t *target, void *stream);
+
+/* Row source[r, i] of request r over row target[r, i], for i < count and every pair without a -1 (lists with row stride
+ * list_st). No source may be another pair's target; pairs through rows or page ids outside the table or cache are
+ * skipped. num_reqs <= 65535. */
+int hla_s6_move_rows(void *cache, int32_t width, int32_t compact, int64_t page_stride, int64_t row_stride,
+                     int32_t block_size, int64_t num_blocks, const int32_t *block_table, int64_t bt_stride,
+                     int32_t bt_cols, const int32_t *source, const int32_t *target, int64_t list_st, int32_t count,
+                     int32_t num_reqs, void *stream);
 
 #ifdef __cplusplus
 }
