@@ -168,20 +168,22 @@ def _load(cache, w, block_table, lengths, query_start_loc, ctx, T, R, max_rows, 
 
 def kv_splits(max_seq_len, num_tokens, cu_count=256, width=512, small_step_tiles=768):
     """Split slots per row for ``history_attention`` over a compact cache. A split is a workgroup of four waves that walk
-    128 rows at a time; one per CU is resident at widths 512 and 1024, two below, and like ``s6_ops.mi355x_kv_splits`` this
-    returns twice the count that fills them (the plan cuts rows so that about half of the slots get equal work), at most two
-    per 128 keys of the longest row, or per 64 in small steps; one for rows that a single pass covers. A function of
-    constants and the row count only (graph-stable)."""
-    if max_seq_len <= 128:
-        return 1
+    128 rows at a time. Like ``s6_ops.mi355x_kv_splits`` this returns twice the count that gives every CU one of them (the
+    plan cuts rows so that about half of the slots get equal work; with two a CU the partials cost more than the waves gain:
+    64 rows of 8160 at width 512 60.6 us with 8 slots, 70.6 with 16), at most two per 128 keys of the longest row, or per 64
+    in small steps. One slot, without a reduction, for rows that a single pass covers and for steps with a row for every
+    other CU (130 rows of 4000: 71.9 us with one slot, 79.9 with two; 200 of 200 to 4000: 65.8 and 79.1; 300 of 1000 to 3900:
+    117.7 and 138.3). A function of constants and the row count only (graph-stable)."""
     tokens = max(1, num_tokens)
-    busy = cu_count * (1 if width >= 512 else 2)
+    busy = cu_count
+    if max_seq_len <= 128 or 2 * tokens >= busy:
+        return 1
     small = tokens * -(-max_seq_len // TILE) < small_step_tiles
     by_length = 2 * -(-max_seq_len // (64 if small else 128))
     return max(2, min(2 * max(1, busy // tokens), by_length, 1024))
 
 
-def _history(q, cache, block_table, ctx, scale, token_requests, splits, workspace, plan, out):
+def _history(q, cache, block_table, ctx, scale, token_requests, splits, workspace, plan, shared_rows, out):
     """The split kernel, and with ``out`` the reduction; returns ``(lse or None, workspace or None)``."""
     T, w = q.shape[0], q.shape[2]
     ws = lse = None
@@ -195,7 +197,7 @@ def _history(q, cache, block_table, ctx, scale, token_requests, splits, workspac
           cache.stride(0), block_size(cache), cache.shape[0], _lib.ptr(block_table), block_table.stride(0),
           block_table.shape[1], block_table.shape[0], _lib.ptr(token_requests), _lib.ptr(ctx), float(scale), splits,
           _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.ptr(plan), 0 if plan is None else plan.numel(),
-          _lib.ptr(out), 0 if out is None else out.stride(0), 0 if out is None else out.stride(1), _lib.ptr(lse))
+          int(bool(shared_rows)), _lib.ptr(out), 0 if out is None else out.stride(0), 0 if out is None else out.stride(1), _lib.ptr(lse))
     return lse, ws
 
 
@@ -232,7 +234,7 @@ def history_attention(q_lat, cache, block_table, ctx, scale, max_seq_len, token_
                                 num_kv_splits, workspace)
     splits = kv_splits(max_seq_len, T, _lib.device_cus(q_lat.device.index), w) if num_kv_splits is None else int(num_kv_splits)
     out = torch.empty(T, HEADS, w, dtype=BF16, device=q_lat.device)
-    lse, _ = _history(q_lat, cache, block_table, ctx, scale, token_requests, splits, workspace, plan, out)
+    lse, _ = _history(q_lat, cache, block_table, ctx, scale, token_requests, splits, workspace, plan, max_query_len > 1, out)
     return out, lse
 
 
@@ -255,14 +257,15 @@ def _chunk_attention(q, cache, block_table, ctx, scale, max_seq_len, token_reque
                                        s6_ops.HIP, bt_rows=token_requests, tokens_per_group=group, shared_rows=True)
 
 
-def history_partials(q_lat, cache, block_table, ctx, scale, num_kv_splits, workspace, token_requests=None, plan=None):
+def history_partials(q_lat, cache, block_table, ctx, scale, num_kv_splits, workspace, token_requests=None, plan=None,
+                     max_query_len=1):
     """The split kernel of ``history_attention`` alone: its partials in ``workspace``, in the layout that
     ``s6_ops.history_reduce`` and ``s6_ops.split_epilogue`` read (``[T, 16, splits, w + 1]``, private)."""
     T, w, ctx, token_requests = _operands(q_lat, cache, block_table, ctx, token_requests, plan)
     splits = int(num_kv_splits)
     if workspace is None:
         raise RuntimeError('history partials need an S6Workspace')
-    _, ws = _history(q_lat, cache, block_table, ctx, scale, token_requests, splits, workspace, plan, None)
+    _, ws = _history(q_lat, cache, block_table, ctx, scale, token_requests, splits, workspace, plan, max_query_len > 1, None)
     return ws
 
 

@@ -54,23 +54,30 @@ __device__ __forceinline__ int64_t clamp_page(int32_t page, int64_t num_blocks) 
   return min(max((int64_t)page, (int64_t)0), num_blocks - 1);
 }
 
-template <int W>
+template <int W, int NW = 4>
 struct CompactGeo {
   static constexpr int KC = W / 128;              // 16-byte K pieces per lane and tile
   static constexpr int CH = W > 512 ? W / 512 : 1;  // waves that share a set of keys
-  static constexpr int G = 4 / CH;                // sets of keys per workgroup
+  static constexpr int G = NW / CH;               // sets of keys per workgroup of NW waves
   static constexpr int CPL = W / CH / 16;         // V columns per lane
   static constexpr int VD = CPL / 8;              // dwords of V per lane and row
 };
 
+// 16 bytes, past the caches where nothing reads them again
+template <bool kOnce>
+__device__ __forceinline__ u32x4 ld_row(const void* p) {
+  if constexpr (kOnce) return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+  else return ld16(p);
+}
+
 template <int N> struct Words { uint32_t w[N]; };
 
 // N dwords from p (N * 4 bytes aligned)
-template <int N>
+template <int N, bool kOnce>
 __device__ __forceinline__ Words<N> load_words(const uint8_t* p) {
   Words<N> r;
   if constexpr (N == 4) {
-    const u32x4 v = ld16(p);
+    const u32x4 v = ld_row<kOnce>(p);
     r.w[0] = v[0]; r.w[1] = v[1]; r.w[2] = v[2]; r.w[3] = v[3];
   } else if constexpr (N == 2) {
     const u32x2 v = *reinterpret_cast<const u32x2*>(p);
@@ -87,7 +94,7 @@ struct KTile {  // one tile of K: block 4i + g of row x per lane (x, g)
   uint32_t scale[(CompactGeo<W>::KC + 3) / 4];
 };
 
-template <int W>
+template <int W, bool kOnce>
 __device__ __forceinline__ void load_k(const uint8_t* tile, int x, int g, KTile<W>& k) {
   constexpr int KC = CompactGeo<W>::KC;
   const uint8_t* sp = tile + 16 * W + x * (W / 32) + g * KC;
@@ -98,29 +105,35 @@ __device__ __forceinline__ void load_k(const uint8_t* tile, int x, int g, KTile<
     for (int i = 0; i < KC / 4; ++i) k.scale[i] = reinterpret_cast<const uint32_t*>(sp)[i];
   }
 #pragma unroll
-  for (int i = 0; i < KC; ++i) k.code[i] = ld16(tile + i * 1024 + x * 64 + g * 16);
+  for (int i = 0; i < KC; ++i) k.code[i] = ld_row<kOnce>(tile + i * 1024 + x * 64 + g * 16);
 }
 
 // Q^T as the B operand in the column order of the K pieces: step 4i + j of lane (h, g) takes columns 32 (4i + g) + 8j
-// .. + 8. In registers, or, at W = 1024 where these would be 128 of them, in LDS (every wave of a workgroup reads the same).
+// .. + 8. In registers, or, from W = 512 on, where these would be 64 and more, in LDS (every wave of a workgroup reads the
+// same; at 512 the history kernel then fits 256 registers and two workgroups a CU).
 template <int W>
 struct QOperand {
   static constexpr int N = CompactGeo<W>::KC * 4;
-  static constexpr bool kLds = W > 512;
-  u32x4 r[kLds ? 1 : N];
+  static constexpr bool kLds = W >= 512;
+  u32x4 r[kLds ? N / 4 : N];
   const u32x4 (*lds)[64];
-  __device__ __forceinline__ void load(const uint16_t* q, int g, int wave, int lane, u32x4 (*buf)[64]) {
+  // the loads, before those of the first rows; with kLds each of the NW waves its share
+  template <int NW>
+  __device__ __forceinline__ void fetch(const uint16_t* q, int g, int wave) {
+#pragma unroll
+    for (int s = 0; s < (kLds ? N / NW : N); ++s) {
+      const int x = kLds ? wave * (N / NW) + s : s;
+      r[s] = ld16(q + 32 * (x / 4 * 4 + g) + 8 * (x % 4));
+    }
+  }
+  // kLds: puts the shares together
+  template <int NW>
+  __device__ __forceinline__ void share(int wave, int lane, u32x4 (*buf)[64]) {
     if constexpr (kLds) {
 #pragma unroll
-      for (int s = 0; s < N / 4; ++s) {
-        const int x = wave * (N / 4) + s;
-        buf[x][lane] = ld16(q + 32 * (x / 4 * 4 + g) + 8 * (x % 4));
-      }
+      for (int s = 0; s < N / NW; ++s) buf[wave * (N / NW) + s][lane] = r[s];
       __syncthreads();
       lds = buf;
-    } else {
-#pragma unroll
-      for (int s = 0; s < N; ++s) r[s] = ld16(q + 32 * (s / 4 * 4 + g) + 8 * (s % 4));
     }
   }
   __device__ __forceinline__ u32x4 at(int s, int lane) const {
@@ -143,7 +156,7 @@ __device__ __forceinline__ void scores(const KTile<W> (&k)[2], const QOperand<W>
       s0 = mfma16x16x32(eight_bf16(k[0].code[i][j], f0), qj, s0);
       s1 = mfma16x16x32(eight_bf16(k[1].code[i][j], f1), qj, s1);
     }
-    // (W = 1024: no conversions ahead of their products, whose operands would not fit the registers)
+    // (no conversions ahead of their products, whose operands would not fit the registers)
     if constexpr (QOperand<W>::kLds) __builtin_amdgcn_sched_barrier(0);
   }
 }

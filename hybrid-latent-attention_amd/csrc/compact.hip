@@ -165,13 +165,13 @@ struct VTile {  // one tile of V: rows 4g .. 4g + 3, CPL columns per lane (m, g)
   uint32_t scale;  // of the four rows
 };
 
-template <int W>
+template <int W, bool kOnce>
 __device__ __forceinline__ void load_v(const uint8_t* tile, int m, int g, int half, VTile<W>& v) {
   using G = CompactGeo<W>;
   const int col = half * (W / G::CH) + m * G::CPL;
   v.scale = *reinterpret_cast<const uint32_t*>(tile + 16 * W + W / 2 + (col / 32) * 16 + 4 * g);
 #pragma unroll
-  for (int r = 0; r < 4; ++r) v.code[r] = load_words<G::VD>(tile + 8 * W + (r * 4 + g) * (W / 2) + col / 2);
+  for (int r = 0; r < 4; ++r) v.code[r] = load_words<G::VD, kOnce>(tile + 8 * W + (r * 4 + g) * (W / 2) + col / 2);
 }
 
 // Columns 2 kByte and 2 kByte + 1 of dword d of every lane's range: eight keys each, two products
@@ -191,11 +191,81 @@ __device__ __forceinline__ void pv_pair(const VTile<W> (&v)[2], const float (&f)
   odd = mfma16x16x32(hi, p, odd);
 }
 
-template <int W>
-__global__ __launch_bounds__(256, 1) void compact_history_kernel(CompactParams a) {
+// Inclusive sums and the maximum over a wave's lanes on DPP moves (within rows of 16, then row to row): no LDS round trip
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int dpp_from(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, kCtrl, kRows, 0xf, false);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+  v += dpp_from<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+  v += dpp_from<0x112, 0xf>(v);
+  v += dpp_from<0x114, 0xf>(v);
+  v += dpp_from<0x118, 0xf>(v);
+  v += dpp_from<0x142, 0xa>(v);  // row_bcast 15 into rows 1 and 3
+  v += dpp_from<0x143, 0xc>(v);  // row_bcast 31 into rows 2 and 3
+  return v;
+}
+__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
+__device__ __forceinline__ int wave_max(int v) {  // of values that are not negative
+  v = max(v, dpp_from<0x111, 0xf>(v));
+  v = max(v, dpp_from<0x112, 0xf>(v));
+  v = max(v, dpp_from<0x114, 0xf>(v));
+  v = max(v, dpp_from<0x118, 0xf>(v));
+  v = max(v, dpp_from<0x142, 0xa>(v));
+  v = max(v, dpp_from<0x143, 0xc>(v));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
+// The workgroup's item of the step's work list, without a plan, worked out by every wave for itself (no barrier): rows are
+// cut in chunks of max(ceil(longest / S), ceil(2 total / (T S))) tiles, at least kMinChunk (kMinChunkSmall in small steps):
+// split_chunk's first value, which fits every row in its S slots, and then grow in a few larger steps where that function
+// takes single tiles. Lane l looks after rows [l, l + 1) * ceil(T / 64). (With split_chunk and find_item, six barriers, a
+// call of 992 rows took 1.2 us longer, one of 32 ragged rows in two slots each 133 us longer.)
+__device__ __forceinline__ void wave_item(const int32_t* ctx, int T, int64_t cap, int S, int b, int lane, int& chunk,
+                                          int& t, int& s) {
+  const int seg = (T + 63) / 64, r0 = min(T, lane * seg), r1 = min(T, r0 + seg);
+  const int one = r0 < r1 ? row_tiles(ctx[r0], cap) : 0;  // the only one where T <= 64
+  int longest = one;
+  int64_t sum = one;
+  for (int r = r0 + 1; r < r1; ++r) {
+    const int tiles = row_tiles(ctx[r], cap);
+    longest = max(longest, tiles);
+    sum += tiles;
+  }
+  longest = wave_max(longest);
+  sum = ((int64_t)wave_total((int)(sum >> 12)) << 12) + wave_total((int)(sum & 4095));
+  const int64_t slots = (int64_t)T * S;
+  const int least = min(longest, sum < kSmallStepTiles ? kMinChunkSmall : kMinChunk);
+  chunk = (int)max((int64_t)max(1, least), max((int64_t)(longest + S - 1) / S, (2 * sum + slots - 1) / slots));
+  int mine, upto;
+  for (int turn = 0;; ++turn) {  // the tails of ragged rows: larger chunks until at most T S / 2 items are left
+    mine = (one + chunk - 1) / chunk;
+    for (int r = r0 + 1; r < r1; ++r) mine += (row_tiles(ctx[r], cap) + chunk - 1) / chunk;
+    upto = wave_scan(mine);
+    const int items = __builtin_amdgcn_readlane(upto, 63);
+    if (items <= slots / 2 || turn == 6 || chunk >= longest) break;
+    chunk = min(longest, max(chunk + 1, (int)((int64_t)chunk * items / (slots / 2))));
+  }
+  const uint64_t owner = __ballot(b >= upto - mine && b < upto);
+  if (owner == 0) {  // past the end of the list
+    t = -1;
+    return;
+  }
+  int row = r0, slot = b - (upto - mine);
+  for (int r = r0; r < r1; ++r) {  // (lanes that do not own the item run on, to no effect)
+    const int used = (row_tiles(ctx[r], cap) + chunk - 1) / chunk;
+    if (slot < used) break;
+    slot -= used;
+    row = r + 1;
+  }
+  const int src = __ffsll((unsigned long long)owner) - 1;
+  t = __builtin_amdgcn_readlane(row, src);
+  s = __builtin_amdgcn_readlane(slot, src);
+}
+
+template <int W, bool kOnce>
+__global__ __launch_bounds__(256, W <= 512 ? 2 : 1) void compact_history_kernel(CompactParams a) {
   using G = CompactGeo<W>;
-  __shared__ int64_t red_lds[8];
-  __shared__ int item_lds[6];
   __shared__ float m_lds[4][16], l_lds[4][16];
   __shared__ floatx4 o_lds[2][G::CH][G::G - 1][G::CPL / 4][64];
   __shared__ u32x4 q_lds[QOperand<W>::kLds ? G::KC * 4 : 1][64];
@@ -205,19 +275,19 @@ __global__ __launch_bounds__(256, 1) void compact_history_kernel(CompactParams a
   const int S = a.num_splits, b = blockIdx.x;
   const int64_t cap = (int64_t)a.bt_cols * a.block;
   int t = b, s = 0, chunk = 0;
-  if (S > 1 && a.plan) {
-    const int ni = (int)split_workgroups(a.T, S);
-    chunk = a.plan[0];
-    t = a.plan[1 + a.T + b];
-    s = a.plan[1 + a.T + ni + b];
-  } else if (S > 1) {
-    chunk = split_chunk(a.ctx, a.T, cap, S, red_lds);
-    find_item(a.ctx, a.T, cap, chunk, b, item_lds, item_lds + 4, t, s);
-  }
-  if (S > 1 && b < a.T) {  // slots of row b past its work
-    const int used = a.plan ? a.plan[1 + b] : used_slots(a.ctx[b], cap, chunk);
-    float* l0 = a.ws_lse + ((int64_t)b * S + used) * kHeads;
-    for (int i = tid; i < (S - used) * kHeads; i += 256) l0[i] = -INFINITY;
+  if (S > 1) {
+    if (a.plan) {
+      chunk = a.plan[0];
+      t = a.plan[1 + a.T + b];
+      s = a.plan[1 + a.T + (int)split_workgroups(a.T, S) + b];
+    } else {
+      wave_item(a.ctx, a.T, cap, S, b, lane, chunk, t, s);
+    }
+    if (b < a.T) {  // slots of row b past its work
+      const int used = a.plan ? a.plan[1 + b] : used_slots(a.ctx[b], cap, chunk);
+      float* l0 = a.ws_lse + ((int64_t)b * S + used) * kHeads;
+      for (int i = tid; i < (S - used) * kHeads; i += 256) l0[i] = -INFINITY;
+    }
   }
   if (t < 0) return;
   t = __builtin_amdgcn_readfirstlane(t);
@@ -240,15 +310,23 @@ __global__ __launch_bounds__(256, 1) void compact_history_kernel(CompactParams a
     return;
   }
 
-  QOperand<W> q;
-  q.load(a.q + (int64_t)t * a.q_st + (int64_t)h * a.q_sh, g, wave, lane, q_lds);
   const int64_t table_row = min(max(a.bt_rows ? a.bt_rows[t] : (int64_t)t, (int64_t)0), (int64_t)a.bt_count - 1);
   const int32_t* btr = a.bt + table_row * a.bt_stride;
   const int limit = min(n, j_end * kTile);
-  auto tile_at = [&](int j) -> const uint8_t* {
-    const int row = min(j, j_end - 1) * kTile;  // (a tile past the chunk reads its last one, and its keys are masked)
+  // Tile addresses of the wave's next 32 steps, worked out by its lanes together: lane 2i + e holds the byte offset of tile e
+  // of step i. (A page id read by the scalar unit in every step put its latency, a trip to L2 or HBM, into each of them.)
+  const int stride = 2 * G::G;
+  uint32_t off_lo, off_hi;
+  auto look_up = [&](int j0) {
+    const int row = min(j0 + (lane >> 1) * stride + (lane & 1), j_end - 1) * kTile;  // (past the chunk: its last tile, masked)
     const int64_t page = clamp_page(btr[row / a.block], a.num_blocks);
-    return a.cache + page * a.page_stride + (row % a.block) / kTile * compact_tile_bytes(W);
+    const int64_t off = page * a.page_stride + (row % a.block) / kTile * compact_tile_bytes(W);
+    off_lo = (uint32_t)off;
+    off_hi = (uint32_t)((uint64_t)off >> 32);
+  };
+  auto tile_at = [&](int i) {
+    const uint32_t lo = __builtin_amdgcn_readlane(off_lo, i), hi = __builtin_amdgcn_readlane(off_hi, i);
+    return a.cache + (int64_t)(((uint64_t)hi << 32) | lo);
   };
 
   floatx4 acc[G::CPL];
@@ -257,24 +335,29 @@ __global__ __launch_bounds__(256, 1) void compact_history_kernel(CompactParams a
   float m = -INFINITY, l = 0.f;
   KTile<W> k[2];
   VTile<W> v[2];
+  // page ids, then the query, then the first rows, each on its way while the one before is waited for
   int j = j_begin + 2 * set;
-  const uint8_t *t0 = tile_at(j), *t1 = tile_at(j + 1);
+  look_up(j);
+  QOperand<W> q;
+  q.template fetch<4>(a.q + (int64_t)t * a.q_st + (int64_t)h * a.q_sh, g, wave);
+  const uint8_t *t0 = tile_at(0), *t1 = tile_at(1);
   if (j < j_end) {
-    load_k<W>(t0, h, g, k[0]);
-    load_k<W>(t1, h, g, k[1]);
-    load_v<W>(t0, h, g, half, v[0]);
-    load_v<W>(t1, h, g, half, v[1]);
+    load_k<W, kOnce>(t0, h, g, k[0]);
+    load_k<W, kOnce>(t1, h, g, k[1]);
+    load_v<W, kOnce>(t0, h, g, half, v[0]);
+    load_v<W, kOnce>(t1, h, g, half, v[1]);
   }
-  for (; j < j_end; j += 2 * G::G) {
+  q.template share<4>(wave, lane, q_lds);
+  for (int step = 1; j < j_end; j += stride, ++step) {
     floatx4 s0, s1;
     scores<W>(k, q, lane, s0, s1);
-    const bool more = j + 2 * G::G < j_end;
-    if (more) {
-      t0 = tile_at(j + 2 * G::G);
-      t1 = tile_at(j + 2 * G::G + 1);
-      load_k<W>(t0, h, g, k[0]);
-      load_k<W>(t1, h, g, k[1]);
-    }
+    // (loads without a condition, the last step's from its own tile again: behind a branch that may have skipped loads the
+    // compiler can only wait for all of them, K of the next step with V of this one: 64 rows of 8160, 77 us and 3.7 TB/s)
+    if ((step & 31) == 0) look_up(j + stride);
+    t0 = tile_at(2 * (step & 31));
+    t1 = tile_at(2 * (step & 31) + 1);
+    load_k<W, kOnce>(t0, h, g, k[0]);
+    load_k<W, kOnce>(t1, h, g, k[1]);
     float sc[8], f[8];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -318,10 +401,8 @@ __global__ __launch_bounds__(256, 1) void compact_history_kernel(CompactParams a
       pv_pair<W, 2>(v, f, pb, d, acc[8 * d + 4], acc[8 * d + 5]);
       pv_pair<W, 3>(v, f, pb, d, acc[8 * d + 6], acc[8 * d + 7]);
     }
-    if (more) {
-      load_v<W>(t0, h, g, half, v[0]);
-      load_v<W>(t1, h, g, half, v[1]);
-    }
+    load_v<W, kOnce>(t0, h, g, half, v[0]);
+    load_v<W, kOnce>(t1, h, g, half, v[1]);
   }
 
   // Join the sets of keys: every wave at the common maximum, then in four rounds wave (round mod sets) of each column half
@@ -371,6 +452,18 @@ __global__ __launch_bounds__(256, 1) void compact_history_kernel(CompactParams a
       }
     }
   }
+}
+
+template <int W>
+void launch_history(const CompactParams& p, bool shared_rows, hipStream_t st) {
+  const dim3 grid(split_workgroups(p.T, p.num_splits));
+  // rows that one token reads stream past the caches from W = 512 on (64 rows of 8160: 68.8 -> 60.6 us, 8 of 32736: 41.8 ->
+  // 37.6); at 256 and below, where a lane's V pieces are shorter than a cached line's share, not (32 rows of up to 8160 at
+  // 256: 20.0 -> 20.6)
+  if (W >= 512 && !shared_rows)
+    hipLaunchKernelGGL((compact_history_kernel<W, (W >= 512)>), grid, dim3(256), 0, st, p);
+  else
+    hipLaunchKernelGGL((compact_history_kernel<W, false>), grid, dim3(256), 0, st, p);
 }
 
 template <int W>
@@ -465,8 +558,8 @@ extern "C" int hla_s6_compact_history(const void* q, int32_t num_tokens, int32_t
                                       int64_t num_blocks, const int32_t* block_table, int64_t bt_stride,
                                       int32_t bt_cols, int32_t bt_count, const int64_t* bt_rows, const int32_t* ctx,
                                       float scale, int32_t num_splits, float* workspace, int64_t workspace_floats,
-                                      const int32_t* plan, int64_t plan_len, void* out, int64_t o_st, int64_t o_sh,
-                                      float* lse, void* stream) {
+                                      const int32_t* plan, int64_t plan_len, int32_t shared_rows, void* out,
+                                      int64_t o_st, int64_t o_sh, float* lse, void* stream) {
   using namespace hla;
   HLA_REQUIRE(num_tokens >= 0, HLA_S6_EINVAL, "compact_history: negative token count");
   HLA_REQUIRE(num_heads == kHeads, HLA_S6_EUNSUPPORTED, "compact_history: %d query heads (the kernel is built for 16)",
@@ -521,13 +614,12 @@ extern "C" int hla_s6_compact_history(const void* q, int32_t num_tokens, int32_t
     p.o_sh = o_sh;
     p.lse = lse;
   }
-  const dim3 grid(split_workgroups(num_tokens, num_splits)), block(256);
   const hipStream_t st = as_stream(stream);
   switch (width) {
-    case 128: hipLaunchKernelGGL((compact_history_kernel<128>), grid, block, 0, st, p); break;
-    case 256: hipLaunchKernelGGL((compact_history_kernel<256>), grid, block, 0, st, p); break;
-    case 512: hipLaunchKernelGGL((compact_history_kernel<512>), grid, block, 0, st, p); break;
-    default: hipLaunchKernelGGL((compact_history_kernel<1024>), grid, block, 0, st, p); break;
+    case 128: launch_history<128>(p, shared_rows != 0, st); break;
+    case 256: launch_history<256>(p, shared_rows != 0, st); break;
+    case 512: launch_history<512>(p, shared_rows != 0, st); break;
+    default: launch_history<1024>(p, shared_rows != 0, st); break;
   }
   rc = check_launch("compact_history");
   if (rc != HLA_S6_OK || !out || !partials) return rc;

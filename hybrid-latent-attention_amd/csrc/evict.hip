@@ -37,9 +37,13 @@ struct AccountParams {
 template <int W, bool kCompact>
 struct KeyTile {
   KTile<W> c;
-  __device__ __forceinline__ void load(const AccountParams& a, const int32_t* btr, int row, int x, int g) {
+  // where the tile of row `row` begins, in bytes (compact) or elements (bf16)
+  static __device__ __forceinline__ int64_t place(const AccountParams& a, const int32_t* btr, int row) {
     const int64_t page = clamp_page(btr[row / a.block], a.num_blocks);
-    load_k<W>(a.cache + page * a.page_stride + (row % a.block) / kTile * compact_tile_bytes(W), x, g, c);
+    return page * a.page_stride + (row % a.block) / kTile * compact_tile_bytes(W);
+  }
+  __device__ __forceinline__ void load(const AccountParams& a, int64_t at, int x, int g) {
+    load_k<W, false>(a.cache + at, x, g, c);
   }
   __device__ __forceinline__ u32x4 operand(int s) const {
     return eight_bf16(c.code[s / 4][s % 4], scale_of(c.scale[s / 16], s / 4 % 4));
@@ -50,9 +54,12 @@ struct KeyTile {
 template <int W>
 struct KeyTile<W, false> {
   u32x4 v[W / 32];
-  __device__ __forceinline__ void load(const AccountParams& a, const int32_t* btr, int row, int x, int g) {
+  static __device__ __forceinline__ int64_t place(const AccountParams& a, const int32_t* btr, int row) {
     const int64_t page = clamp_page(btr[row / a.block], a.num_blocks);
-    const uint16_t* p = a.cache16 + page * a.page_stride + (int64_t)(row % a.block + x) * a.row_stride + 8 * g;
+    return page * a.page_stride + (int64_t)(row % a.block / kTile * kTile) * a.row_stride;
+  }
+  __device__ __forceinline__ void load(const AccountParams& a, int64_t at, int x, int g) {
+    const uint16_t* p = a.cache16 + at + (int64_t)x * a.row_stride + 8 * g;
 #pragma unroll
     for (int s = 0; s < W / 32; ++s) v[s] = ld16(p + 32 * s);
   }
@@ -107,13 +114,27 @@ __global__ __launch_bounds__(256) void account_step_kernel(AccountParams a) {
 #pragma unroll
     for (int s = 0; s < W / 32; ++s) q[s] = ld16(qp + K::column(s, g));
     const float lse = row_lse(a, t, h);
+    // places of the wave's next 64 tiles, one per lane (see compact_history_kernel); the last tile is loaded once more
+    // rather than under a condition
+    uint32_t at_lo, at_hi;
+    auto look_up = [&](int j0) {
+      const int64_t at = K::place(a, btr, min(j0 + lane * 4 * kTile, (end - 1) / kTile * kTile));
+      at_lo = (uint32_t)at;
+      at_hi = (uint32_t)((uint64_t)at >> 32);
+    };
+    auto tile = [&](int i) {
+      const uint32_t lo = __builtin_amdgcn_readlane(at_lo, i), hi = __builtin_amdgcn_readlane(at_hi, i);
+      return (int64_t)(((uint64_t)hi << 32) | lo);
+    };
+    look_up(j);
     K k;
-    k.load(a, btr, j, h, g);
-    for (; j < end; j += 4 * kTile) {
+    k.load(a, tile(0), h, g);
+    for (int step = 1; j < end; j += 4 * kTile, ++step) {
       floatx4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < W / 32; ++i) s = mfma16x16x32(k.operand(i), q[i], s);
-      if (j + 4 * kTile < end) k.load(a, btr, j + 4 * kTile, h, g);
+      if ((step & 63) == 0) look_up(j + 4 * kTile);
+      k.load(a, tile(step & 63), h, g);
       float w[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) w[e] = weight(s[e], a.scale, lse);
@@ -157,7 +178,7 @@ __global__ __launch_bounds__(256, 1) void account_chunk_kernel(AccountParams a) 
 #pragma unroll
       for (int x = 0; x < NT; ++x) {
         K tile;
-        tile.load(a, btr, min(key0 + x * kTile, (most - 1) / kTile * kTile), h, g);
+        tile.load(a, K::place(a, btr, min(key0 + x * kTile, (most - 1) / kTile * kTile)), h, g);
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) k[x][s] = tile.operand(s);
       }

@@ -282,7 +282,8 @@ def _attend_composed(q_lat, o_chunk, lse_chunk, B, cache, block_table, ctx, weig
             if workspace is None:
                 workspace = s6_ops.S6Workspace(q_lat.shape[1], w, T * splits)
             ws = compact_cache.history_partials(q_lat, cache, block_table, ctx.ctx_latent, ctx.scale, splits, workspace,
-                                                ctx.token_requests, ctx.split_plan(splits, rows))
+                                                ctx.token_requests, ctx.split_plan(splits, rows),
+                                                ctx.max_query_len)
             return s6_ops.split_epilogue(ws, B, o_chunk, lse_chunk, ctx.invalid)
         o_hist, lse_hist = compact_cache.history_attention(
             q_lat, cache, block_table, ctx.ctx_latent, ctx.scale, longest, ctx.token_requests, ctx.query_start_loc,

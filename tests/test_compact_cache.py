@@ -54,12 +54,12 @@ def test_selection_by_hand():
 
 
 def test_split_counts(cc):
-    assert cc.kv_splits(8160, 64, 256, 512) == 8 and cc.kv_splits(8160, 64, 256, 256) == 16
+    assert cc.kv_splits(8160, 64, 256, 512) == 8 and cc.kv_splits(8160, 64, 256, 256) == 8
     assert cc.kv_splits(32736, 8, 256, 512) == 64
     assert cc.kv_splits(128, 64, 256, 512) == 1
     assert cc.kv_splits(992, 1, 256, 512) == 32             # a small step: two slots per 64 keys
-    assert cc.kv_splits(10 ** 6, 1, 256, 256) == 1024
-    assert cc.kv_splits(8160, 4096, 256, 512) == 2
+    assert cc.kv_splits(10 ** 6, 1, 256, 256) == 512
+    assert cc.kv_splits(8160, 4096, 256, 512) == 1 and cc.kv_splits(8160, 100, 256, 512) == 4
 
 
 def test_cache_shape(cc):
@@ -102,9 +102,9 @@ def test_entry_points_check_before_they_launch(pkg):
                           (dict(_8=16, _14=16, _5=16, _15=8, _16=8), 'apart'), (dict(_8=16, _14=8, _5=16, _16=256), 'aligned')):
         with pytest.raises(ValueError, match=match):
             call('hla_s6_compact_load', **{**load, **change})
-    history = dict(_0=16, _1=1, _2=16, _3=128, _6=16, _7=page, _8=16, _9=2, _10=16, _12=1, _13=1, _15=16, _17=1, _22=16, _25=16)
+    history = dict(_0=16, _1=1, _2=16, _3=128, _6=16, _7=page, _8=16, _9=2, _10=16, _12=1, _13=1, _15=16, _17=1, _23=16, _26=16)
     for change, match in ((dict(_2=8), 'heads'), (dict(_3=64), 'width'), (dict(_17=0), 'num_kv_splits'), (dict(_17=1025), 'num_kv_splits'),
-                          (dict(_13=0), 'table rows'), (dict(_0=None), 'null pointer'), (dict(_25=None), 'null pointer'), (dict(_4=4), 'aligned'),
+                          (dict(_13=0), 'table rows'), (dict(_0=None), 'null pointer'), (dict(_26=None), 'null pointer'), (dict(_4=4), 'aligned'),
                           (dict(_17=2, _18=16, _19=10 ** 6, _20=16, _21=3), 'split plan')):
         with pytest.raises(ValueError, match=match):
             call('hla_s6_compact_history', **{**history, **change})
