@@ -49,6 +49,31 @@ __device__ __forceinline__ u32x4 eight_bf16(uint32_t word, float scale) {
                two_bf16<3>(word, scale)};
 }
 
+// Inclusive sums and the maximum over a wave's lanes on DPP moves (within rows of 16, then row to row): no LDS round trip
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int dpp_from(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, kCtrl, kRows, 0xf, false);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+  v += dpp_from<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+  v += dpp_from<0x112, 0xf>(v);
+  v += dpp_from<0x114, 0xf>(v);
+  v += dpp_from<0x118, 0xf>(v);
+  v += dpp_from<0x142, 0xa>(v);  // row_bcast 15 into rows 1 and 3
+  v += dpp_from<0x143, 0xc>(v);  // row_bcast 31 into rows 2 and 3
+  return v;
+}
+__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
+__device__ __forceinline__ int wave_max(int v) {  // of values that are not negative
+  v = max(v, dpp_from<0x111, 0xf>(v));
+  v = max(v, dpp_from<0x112, 0xf>(v));
+  v = max(v, dpp_from<0x114, 0xf>(v));
+  v = max(v, dpp_from<0x118, 0xf>(v));
+  v = max(v, dpp_from<0x142, 0xa>(v));
+  v = max(v, dpp_from<0x143, 0xc>(v));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
 // page id of a table entry, in the cache whatever the entry holds
 __device__ __forceinline__ int64_t clamp_page(int32_t page, int64_t num_blocks) {
   return min(max((int64_t)page, (int64_t)0), num_blocks - 1);

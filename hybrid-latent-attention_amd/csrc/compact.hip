@@ -191,31 +191,6 @@ __device__ __forceinline__ void pv_pair(const VTile<W> (&v)[2], const float (&f)
   odd = mfma16x16x32(hi, p, odd);
 }
 
-// Inclusive sums and the maximum over a wave's lanes on DPP moves (within rows of 16, then row to row): no LDS round trip
-template <int kCtrl, int kRows>
-__device__ __forceinline__ int dpp_from(int v) {
-  return __builtin_amdgcn_update_dpp(0, v, kCtrl, kRows, 0xf, false);
-}
-__device__ __forceinline__ int wave_scan(int v) {
-  v += dpp_from<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
-  v += dpp_from<0x112, 0xf>(v);
-  v += dpp_from<0x114, 0xf>(v);
-  v += dpp_from<0x118, 0xf>(v);
-  v += dpp_from<0x142, 0xa>(v);  // row_bcast 15 into rows 1 and 3
-  v += dpp_from<0x143, 0xc>(v);  // row_bcast 31 into rows 2 and 3
-  return v;
-}
-__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
-__device__ __forceinline__ int wave_max(int v) {  // of values that are not negative
-  v = max(v, dpp_from<0x111, 0xf>(v));
-  v = max(v, dpp_from<0x112, 0xf>(v));
-  v = max(v, dpp_from<0x114, 0xf>(v));
-  v = max(v, dpp_from<0x118, 0xf>(v));
-  v = max(v, dpp_from<0x142, 0xa>(v));
-  v = max(v, dpp_from<0x143, 0xc>(v));
-  return __builtin_amdgcn_readlane(v, 63);
-}
-
 // The workgroup's item of the step's work list, without a plan, worked out by every wave for itself (no barrier): rows are
 // cut in chunks of max(ceil(longest / S), ceil(2 total / (T S))) tiles, at least kMinChunk (kMinChunkSmall in small steps):
 // split_chunk's first value, which fits every row in its S slots, and then grow in a few larger steps where that function
