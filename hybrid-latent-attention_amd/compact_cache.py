@@ -316,13 +316,18 @@ def attention_weights(q_lat, cache, block_table, query_start_loc, ctx, lse, scal
 
 
 def account_shape(num_tokens, num_reqs, rows, cu_count, width):
-    """How ``attention_weights`` is cut: ``(shares of each request's tokens or 0, rows per workgroup)``. Steps of few
-    tokens per request stream K past their queries (shares 0), longer chunks hold K and stream the queries."""
-    if num_tokens < 4 * num_reqs:
-        per = -(-num_reqs * rows // (4 * cu_count))
-        return 0, max(64, -(-per // 64) * 64)
-    wgs = max(1, num_reqs * -(-rows // (128 if width <= 512 else 64)))
-    return max(1, min(2 * cu_count // wgs, num_tokens // max(1, num_reqs) // 16, 16)), 64
+    """How ``attention_weights`` is cut: ``(shares of each request's tokens or 0, rows per workgroup)``. Steps of single
+    tokens stream K past the queries (shares 0) in two workgroups a CU; longer ones hold K and stream the queries, the
+    tokens shared out so that the last round of workgroups is a full one."""
+    if num_tokens < 2 * num_reqs:
+        per = -(-num_reqs * rows // (2 * cu_count))
+        return 0, min(4096, max(128, -(-per // 128) * 128))
+    groups = max(1, num_reqs * -(-rows // (256 if width <= 512 else 128)))
+    slots, tokens = cu_count * (1 if width >= 512 else 2), num_tokens // max(1, num_reqs)
+    # rounds of workgroups, each as long as a share's tokens and its rows' expansion (about 4 tokens' time); a reduction of
+    # the shares costs about 4 as well
+    cost = lambda z: -(-groups * z // slots) * (-(-tokens // z) + 4) + (4 if z > 1 else 0)
+    return min(range(1, max(1, min(16, tokens // 4)) + 1), key=cost), 64
 
 
 def select_rows(weights, positions, lengths, budget, protect_from):

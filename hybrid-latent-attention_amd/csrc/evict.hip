@@ -42,8 +42,9 @@ struct KeyTile {
     const int64_t page = clamp_page(btr[row / a.block], a.num_blocks);
     return page * a.page_stride + (row % a.block) / kTile * compact_tile_bytes(W);
   }
+  template <bool kOnce>
   __device__ __forceinline__ void load(const AccountParams& a, int64_t at, int x, int g) {
-    load_k<W, false>(a.cache + at, x, g, c);
+    load_k<W, kOnce>(a.cache + at, x, g, c);
   }
   __device__ __forceinline__ u32x4 operand(int s) const {
     return eight_bf16(c.code[s / 4][s % 4], scale_of(c.scale[s / 16], s / 4 % 4));
@@ -58,10 +59,11 @@ struct KeyTile<W, false> {
     const int64_t page = clamp_page(btr[row / a.block], a.num_blocks);
     return page * a.page_stride + (int64_t)(row % a.block / kTile * kTile) * a.row_stride;
   }
+  template <bool kOnce>
   __device__ __forceinline__ void load(const AccountParams& a, int64_t at, int x, int g) {
     const uint16_t* p = a.cache16 + at + (int64_t)x * a.row_stride + 8 * g;
 #pragma unroll
-    for (int s = 0; s < W / 32; ++s) v[s] = ld16(p + 32 * s);
+    for (int s = 0; s < W / 32; ++s) v[s] = ld_row<kOnce>(p + 32 * s);
   }
   __device__ __forceinline__ u32x4 operand(int s) const { return v[s]; }
   static __device__ __forceinline__ int column(int s, int g) { return 32 * s + 8 * g; }
@@ -85,40 +87,43 @@ __device__ __forceinline__ float row_lse(const AccountParams& a, int t, int h) {
   return v == -INFINITY ? INFINITY : v;
 }
 
-// adds the four keys' weights of a tile, summed over the heads, to the account: lane h < 4 of group g takes key 4g + h
-__device__ __forceinline__ void add_to_account(float* row, int limit, int key0, int h, int g, const float (&w)[4]) {
+// the four keys' weights of a tile summed over the heads: lane h < 4 of group g gets that of key 4g + h
+__device__ __forceinline__ float head_sums(int h, const float (&w)[4]) {
   float s[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) s[e] = row_sum16(w[e]);
-  const int key = key0 + 4 * g + h;
-  if (h < 4 && key < limit) row[key] += h == 0 ? s[0] : h == 1 ? s[1] : h == 2 ? s[2] : s[3];
+  return h == 0 ? s[0] : h == 1 ? s[1] : h == 2 ? s[2] : s[3];
 }
 
-// Single tokens: Q^T stays in registers, K streams by (one pass over K per token).
+// Single tokens: Q^T lies in LDS, K streams by, two tiles a step and wave (one where they are large). The sums of the
+// workgroup's keys gather in LDS and go to the account at the end: an account read in each step stood behind the loads of the
+// next one's rows, and waited for them.
+constexpr int kMaxStepKeys = 4096;  // per workgroup
+
 template <int W, bool kCompact>
 __global__ __launch_bounds__(256) void account_step_kernel(AccountParams a) {
   using K = KeyTile<W, kCompact>;
+  constexpr int STEPS = W / 32, NT = kCompact ? (W <= 512 ? 2 : 1) : (W <= 256 ? 2 : 1), SPAN = 4 * NT * kTile;
+  // past the caches as in compact_history_kernel (64 rows of 8160: 33.2 -> 28.1 us; bf16 rows, and narrow ones, gain nothing)
+  constexpr bool kOnce = kCompact && W >= 512;
+  __shared__ u32x4 q_lds[STEPS][64];
+  __shared__ float sum_lds[kMaxStepKeys];
   const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63, h = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int cap = (int)min((int64_t)a.bt_cols * a.block, (int64_t)a.cols);
   const int t0 = max(a.qsl[r], 0), t1 = min(a.qsl[r + 1], a.T);
+  const int begin = blockIdx.x * a.per_wg;
   const int32_t* btr = a.bt + (int64_t)r * a.bt_stride;
-  float* row = a.account + (int64_t)r * a.a_st;
+  for (int i = tid; i < a.per_wg; i += 256) sum_lds[i] = 0.f;
   for (int t = t0; t < t1; ++t) {
-    const int n = min(a.ctx[t], cap);
-    const int end = min(n, (int)(blockIdx.x + 1) * a.per_wg);
-    int j = blockIdx.x * a.per_wg + wave * kTile;
-    if (j >= end) continue;
-    const uint16_t* qp = a.q + (int64_t)t * a.q_st + (int64_t)h * a.q_sh;
-    u32x4 q[W / 32];
-#pragma unroll
-    for (int s = 0; s < W / 32; ++s) q[s] = ld16(qp + K::column(s, g));
-    const float lse = row_lse(a, t, h);
-    // places of the wave's next 64 tiles, one per lane (see compact_history_kernel); the last tile is loaded once more
-    // rather than under a condition
+    const int end = min(min(a.ctx[t], cap), begin + a.per_wg);
+    if (begin >= end) continue;  // uniform over the workgroup
+    int j = begin + wave * NT * kTile;
+    // places of the wave's next 64 / NT steps' tiles, one per lane (see compact_history_kernel); past the end the last tile is
+    // loaded again rather than under a condition
     uint32_t at_lo, at_hi;
     auto look_up = [&](int j0) {
-      const int64_t at = K::place(a, btr, min(j0 + lane * 4 * kTile, (end - 1) / kTile * kTile));
+      const int64_t at = K::place(a, btr, min(j0 + lane / NT * SPAN + lane % NT * kTile, (end - 1) / kTile * kTile));
       at_lo = (uint32_t)at;
       at_hi = (uint32_t)((uint64_t)at >> 32);
     };
@@ -127,29 +132,64 @@ __global__ __launch_bounds__(256) void account_step_kernel(AccountParams a) {
       return (int64_t)(((uint64_t)hi << 32) | lo);
     };
     look_up(j);
-    K k;
-    k.load(a, tile(0), h, g);
-    for (int step = 1; j < end; j += 4 * kTile, ++step) {
-      floatx4 s = {0.f, 0.f, 0.f, 0.f};
+    u32x4 q[STEPS / 4];
+    const uint16_t* qp = a.q + (int64_t)t * a.q_st + (int64_t)h * a.q_sh;
 #pragma unroll
-      for (int i = 0; i < W / 32; ++i) s = mfma16x16x32(k.operand(i), q[i], s);
-      if ((step & 63) == 0) look_up(j + 4 * kTile);
-      k.load(a, tile(step & 63), h, g);
-      float w[4];
+    for (int s = 0; s < STEPS / 4; ++s) q[s] = ld16(qp + K::column(wave * (STEPS / 4) + s, g));
+    const float lse = row_lse(a, t, h);
+    K k[NT];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = weight(s[e], a.scale, lse);
-      add_to_account(row, end, j, h, g, w);
+    for (int x = 0; x < NT; ++x) k[x].template load<kOnce>(a, tile(x), h, g);
+    __syncthreads();  // (the reads of the token before)
+#pragma unroll
+    for (int s = 0; s < STEPS / 4; ++s) q_lds[wave * (STEPS / 4) + s][lane] = q[s];
+    __syncthreads();
+    for (int step = 1; j < end; j += SPAN, ++step) {
+      floatx4 s[NT];
+#pragma unroll
+      for (int x = 0; x < NT; ++x) s[x] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        const u32x4 qi = q_lds[i][lane];
+#pragma unroll
+        for (int x = 0; x < NT; ++x) s[x] = mfma16x16x32(k[x].operand(i), qi, s[x]);
+      }
+      const int i0 = step % (64 / NT) * NT;
+      if (i0 == 0) look_up(j + SPAN);
+#pragma unroll
+      for (int x = 0; x < NT; ++x) k[x].template load<kOnce>(a, tile(i0 + x), h, g);
+#pragma unroll
+      for (int x = 0; x < NT; ++x) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = weight(s[x][e], a.scale, lse);
+        const float sum = head_sums(h, w);
+        const int key = j + x * kTile + 4 * g + h;
+        if (h < 4 && key < end) sum_lds[key - begin] += sum;  // (the same lane for every token)
+      }
     }
   }
+  __syncthreads();
+  float* row = a.account + (int64_t)r * a.a_st;
+  for (int i = tid; i < a.per_wg && begin + i < cap; i += 256)
+    if (sum_lds[i] != 0.f) row[begin + i] += sum_lds[i];  // (rows behind the request stay untouched; NaN passes)
 }
 
-// Prompt chunks: a wave keeps 32 rows of K (16 at W = 1024) as bf16 operands and all of the request's queries stream by,
-// through LDS in operand order, one token ahead. The tokens of a request may be shared out over blockIdx.z.
+// Prompt chunks: a product of all rows with all queries of the request, whose epilogue takes the weights and sums them over the
+// tokens in registers. A wave keeps 64 rows of K (32 at W = 1024) as bf16 operands; the queries stream by through LDS in
+// operand order, two tokens ahead, so that a KB of LDS feeds four products. Reads from LDS go four steps ahead of their
+// products (the next token's first ones ahead of this one's last), and a token's weights are worked out in the shadow of the
+// next one's products. 4 x 512 tokens over 8160 rows at width 512: 392 us with 32 rows a wave (LDS at its full rate), 343
+// with 64 (every read waited for), 269 with reads ahead, 260 with the next token's, 231 with the weights between the products:
+// 1.19 PFLOP/s, what a large library product reaches. One tile in four of K lies in accumulation registers: all of it
+// and its neighbours do not fit the 256 others.
+// The tokens of a request may be shared out over blockIdx.z.
 template <int W, bool kCompact>
-__global__ __launch_bounds__(256, 1) void account_chunk_kernel(AccountParams a) {
+__global__ __launch_bounds__(256, W <= 256 ? 2 : 1) void account_chunk_kernel(AccountParams a) {
   using K = KeyTile<W, kCompact>;
-  constexpr int NT = W <= 512 ? 2 : 1, STEPS = W / 32, MINE = STEPS / 4;  // steps of Q that a wave stages
-  __shared__ u32x4 q_lds[2][STEPS][64];
+  constexpr int NT = W <= 512 ? 4 : 2, STEPS = W / 32, MINE = STEPS / 4;  // steps of Q that a wave stages
+  constexpr int GROUP = STEPS >= 16 ? 4 : 2, PARTS = STEPS / GROUP;
+  __shared__ u32x4 q_lds[3][STEPS][64];
   __shared__ int n_lds[4];
   const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63, h = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -160,7 +200,7 @@ __global__ __launch_bounds__(256, 1) void account_chunk_kernel(AccountParams a) 
   t1 = min(t1, t0 + share);
   int most = 0;
   for (int t = t0 + tid; t < t1; t += 256) most = max(most, a.ctx[t]);
-  for (int off = 32; off > 0; off >>= 1) most = max(most, __shfl_xor(most, off));
+  most = wave_max(most);
   if (lane == 0) n_lds[wave] = most;
   __syncthreads();
   most = min(max(max(n_lds[0], n_lds[1]), max(n_lds[2], n_lds[3])), cap);
@@ -175,68 +215,117 @@ __global__ __launch_bounds__(256, 1) void account_chunk_kernel(AccountParams a) 
     u32x4 k[NT][STEPS];
     {
       const int32_t* btr = a.bt + (int64_t)r * a.bt_stride;
+      K tile[NT];
 #pragma unroll
-      for (int x = 0; x < NT; ++x) {
-        K tile;
-        tile.load(a, K::place(a, btr, min(key0 + x * kTile, (most - 1) / kTile * kTile)), h, g);
+      for (int x = 0; x < NT; ++x)
+        tile[x].template load<false>(a, K::place(a, btr, min(key0 + x * kTile, (most - 1) / kTile * kTile)), h, g);
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) k[x][s] = tile.operand(s);
-      }
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+          k[x][s] = tile[x].operand(s);
+          if (W == 512 && x == 3) asm("" : "+a"(k[x][s]));  // (the products read them there)
+        }
     }
-    u32x4 next[MINE];
-    auto fetch = [&](int t) {
-      const uint16_t* qp = a.q + (int64_t)t * a.q_st + (int64_t)h * a.q_sh;
+    floatx4 last[NT];  // scores of the token before
 #pragma unroll
-      for (int s = 0; s < MINE; ++s) next[s] = ld16(qp + K::column(wave * MINE + s, g));
-    };
-    fetch(t0);
-    float lse_next = row_lse(a, t0, h);
-    int n_next = a.ctx[t0];
-    for (int t = t0; t < t1; ++t) {
-      const int buf = (t - t0) & 1;
-#pragma unroll
-      for (int s = 0; s < MINE; ++s) q_lds[buf][wave * MINE + s][lane] = next[s];
-      const float lse = lse_next;
-      const int n = n_next;
-      if (t + 1 < t1) {
-        fetch(t + 1);
-        lse_next = row_lse(a, t + 1, h);
-        n_next = a.ctx[t + 1];
-      }
-      // one barrier per token: a wave that writes this buffer again has passed the barrier of the token between, which
-      // every wave reaches only after its reads of this one
-      __syncthreads();
-      floatx4 s[NT];
-#pragma unroll
-      for (int x = 0; x < NT; ++x) s[x] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
-        const u32x4 q = q_lds[buf][i][lane];
-#pragma unroll
-        for (int x = 0; x < NT; ++x) s[x] = mfma16x16x32(k[x][i], q, s[x]);
-      }
-      const int limit = min(n, cap) - key0 - 4 * g;
+    for (int x = 0; x < NT; ++x) last[x] = floatx4{0.f, 0.f, 0.f, 0.f};
+    float lse = INFINITY;  // (before the first token: weights of 0)
+    int limit = 0;
+    auto take = [&](int part) {  // the weights of the token before, one share of them
 #pragma unroll
       for (int x = 0; x < NT; ++x)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p = weight(s[x][e], a.scale, lse);
+          if ((x * 4 + e) * PARTS / (NT * 4) != part) continue;
+          const float p = weight(last[x][e], a.scale, lse);
           w[x][e] += x * kTile + e < limit ? p : 0.f;
         }
+    };
+    auto hold = [&](int part) {  // keeps the share of `take` behind this place
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if ((x * 4 + e) * PARTS / (NT * 4) == part) {
+            float v = last[x][e];
+            asm volatile("" : "+v"(v));
+            last[x][e] = v;
+          }
+    };
+    auto copy = [&](int t, int slot) {  // this wave's steps of token t's queries
+      const uint16_t* qp = a.q + (int64_t)t * a.q_st + (int64_t)h * a.q_sh;
+#pragma unroll
+      for (int s = 0; s < MINE; ++s) copy16_to_lds_v(qp + K::column(wave * MINE + s, g), q_lds[slot][wave * MINE + s]);
+    };
+    // Wait for this wave's copies (nothing else is long on its way here), then for everybody's.
+    auto arrive = [&]() {
+      __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 0));
+      plain_barrier();
+    };
+    copy(t0, 0);
+    arrive();
+    copy(min(t0 + 1, t1 - 1), 1);
+    u32x4 qa[GROUP], qb[GROUP];
+#pragma unroll
+    for (int i = 0; i < GROUP; ++i) qa[i] = q_lds[0][i][lane];
+    int slot = 0;
+    for (int t = t0; t < t1; ++t) {
+      const int slot1 = slot == 2 ? 0 : slot + 1;
+      const float lse_now = row_lse(a, t, h);
+      const int n_now = a.ctx[t];
+      floatx4 s[NT];
+#pragma unroll
+      for (int x = 0; x < NT; ++x) s[x] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int part = 0; part < PARTS; ++part) {
+        if (part + 1 < PARTS) {
+#pragma unroll
+          for (int i = 0; i < GROUP; ++i) qb[i] = q_lds[slot][(part + 1) * GROUP + i][lane];
+        } else {
+          // The next token's queries, ahead of this one's last products: behind the barrier they are whole, and every wave
+          // has read the token before this one, whose place the one after the next takes.
+          arrive();
+          copy(min(t + 2, t1 - 1), slot1 == 2 ? 0 : slot1 + 1);  // (past the end the last one again: no branch here)
+#pragma unroll
+          for (int i = 0; i < GROUP; ++i) qb[i] = q_lds[slot1][i][lane];  // (behind the last token: unused)
+        }
+        // The reads, then the products with the last token's weights in their shadow: a product keeps the matrix unit for the
+        // time of four vector instructions. The scheduler would put all of the weights ahead of the products otherwise.
+        __builtin_amdgcn_sched_barrier(0);
+        hold(part);
+#pragma unroll
+        for (int i = 0; i < GROUP; ++i)
+#pragma unroll
+          for (int x = 0; x < NT; ++x) s[x] = mfma16x16x32(k[x][part * GROUP + i], qa[i], s[x]);
+        take(part);
+#pragma unroll
+        for (int i = 0; i < GROUP * NT; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // one product,
+          __builtin_amdgcn_sched_group_barrier(0x402, 2, 0);  // two vector instructions
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < GROUP; ++i) qa[i] = qb[i];
+      }
+      lse = lse_now;
+      limit = min(n_now, cap) - key0 - 4 * g;
+#pragma unroll
+      for (int x = 0; x < NT; ++x) last[x] = s[x];
+      slot = slot1;
     }
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part) take(part);
+    __builtin_amdgcn_s_waitcnt(waitcnt_imm(0, 15));  // no copy into LDS outlives the workgroup
   }
-  if (a.partial) {
 #pragma unroll
-    for (int x = 0; x < NT; ++x) {
-      float s[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[e] = row_sum16(w[x][e]);
-      const int key = key0 + x * kTile + 4 * g + h;
-      if (h < 4 && key < a.cols) row[key] = h == 0 ? s[0] : h == 1 ? s[1] : h == 2 ? s[2] : s[3];
+  for (int x = 0; x < NT; ++x) {
+    const float sum = head_sums(h, w[x]);
+    const int key = key0 + x * kTile + 4 * g + h;
+    if (h < 4 && key < (a.partial ? a.cols : most)) {
+      if (a.partial) row[key] = sum;
+      else row[key] += sum;
     }
-  } else {
-#pragma unroll
-    for (int x = 0; x < NT; ++x) add_to_account(row, most, key0 + x * kTile, h, g, w[x]);
   }
 }
 
@@ -676,7 +765,7 @@ void launch_account(const AccountParams& p, int R, int shares, bool chunks, hipS
                        dim3(256), 0, st, p);
     return;
   }
-  constexpr int per = 4 * (W <= 512 ? 2 : 1) * kTile;
+  constexpr int per = 4 * (W <= 512 ? 4 : 2) * kTile;
   hipLaunchKernelGGL((account_chunk_kernel<W, kCompact>),
                      dim3((unsigned)(((p.partial ? p.cols : keys) + per - 1) / per), (unsigned)R, (unsigned)shares),
                      dim3(256), 0, st, p);
@@ -728,8 +817,8 @@ extern "C" int hla_s6_attention_weights(const void* q, int32_t num_tokens, int32
               "attention_weights: q needs 16-byte aligned rows (unit last stride, strides multiple of 8)");
   HLA_REQUIRE(a_st >= cols, HLA_S6_EINVAL, "attention_weights: account rows overlap");
   HLA_REQUIRE(shares >= 0 && shares <= 64, HLA_S6_EINVAL, "attention_weights: shares must be in [0, 64]");
-  HLA_REQUIRE(shares > 0 || (keys_per_wg > 0 && keys_per_wg % 64 == 0), HLA_S6_EINVAL,
-              "attention_weights: keys per workgroup must be a positive multiple of 64");
+  HLA_REQUIRE(shares > 0 || (keys_per_wg > 0 && keys_per_wg % 64 == 0 && keys_per_wg <= kMaxStepKeys), HLA_S6_EINVAL,
+              "attention_weights: keys per workgroup must be a positive multiple of 64, at most %d", kMaxStepKeys);
   if (shares > 1) {
     const int64_t need = (int64_t)shares * num_reqs * cols;
     HLA_REQUIRE(workspace && workspace_floats >= need, HLA_S6_EWORKSPACE,
