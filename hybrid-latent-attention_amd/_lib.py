@@ -89,7 +89,7 @@ SIGNATURES = {
     'hla_s6_compact_store': [P, I64, P, I64, I32, I32, P, P, I64, I32, I64, P],
     'hla_s6_compact_load': [P, I32, I64, I32, I64, P, I64, I32, P, P, P, I32, I32, I32, P, I64, I64, P],
     'hla_s6_compact_history': [P, I32, I32, I32, I64, I64, P, I64, I32, I64, P, I64, I32, I32, P, P, F32, I32, P, I64, P,
-                               I64, I32, P, I64, I64, P, P],
+                               I64, I32, I32, P, I64, I64, P, P],
     'hla_s6_attention_weights': [P, I32, I32, I32, I64, I64, P, I32, I64, I64, I32, I64, P, I64, I32, P, I32, P, P, F32,
                                  P, I64, I32, I32, I32, P, I64, P],
     'hla_s6_select_rows': [P, I64, P, I64, P, I32, I32, I32, P, P, P, P, P, P, P, P],

@@ -28,8 +28,8 @@ from . import _lib, s6_ops
 BF16, F32, I32, I64, U8 = torch.bfloat16, torch.float32, torch.int32, torch.int64, torch.uint8
 WIDTHS = (128, 256, 512, 1024)
 HEADS, TILE = 16, 16
-# tokens per request from which a step's rows are expanded once and read by the bf16 cache's multi-query kernels
-CHUNK_TOKENS = 16
+# rows from which a history is long enough to be cut between workgroups in steps that could do without
+LONG_ROWS = 4096
 
 #: What ``select_rows`` returns. ``lengths [R]``: rows per request from now on; ``weights``, ``positions [R, M]``: the account
 #: and positions in the new order (0 and -1 behind the last row); ``source``, ``target [R, M // 2]``: the row moves, ended by -1.
@@ -167,23 +167,53 @@ def _load(cache, w, block_table, lengths, query_start_loc, ctx, T, R, max_rows, 
 # ----------------------------------------------------------------------------------------------------------------
 
 def kv_splits(max_seq_len, num_tokens, cu_count=256, width=512, small_step_tiles=768):
-    """Split slots per row for ``history_attention`` over a compact cache. A split is a workgroup of four waves that walk
-    128 rows at a time. Like ``s6_ops.mi355x_kv_splits`` this returns twice the count that gives every CU one of them (the
-    plan cuts rows so that about half of the slots get equal work; with two a CU the partials cost more than the waves gain:
-    64 rows of 8160 at width 512 60.6 us with 8 slots, 70.6 with 16), at most two per 128 keys of the longest row, or per 64
-    in small steps. One slot, without a reduction, for rows that a single pass covers and for steps with a row for every
-    other CU (130 rows of 4000: 71.9 us with one slot, 79.9 with two; 200 of 200 to 4000: 65.8 and 79.1; 300 of 1000 to 3900:
-    117.7 and 138.3). A function of constants and the row count only (graph-stable)."""
+    """Split slots per row for ``history_attention`` over a compact cache, one token a workgroup. A split is a workgroup of
+    four waves that walk 128 rows at a time. Like ``s6_ops.mi355x_kv_splits`` this returns twice the count that gives every CU
+    one of them (the plan cuts rows so that about half of the slots get equal work; with two a CU the partials cost more than
+    the waves gain: 64 rows of 8160 at width 512 60.6 us with 8 slots, 70.6 with 16), at most two per 128 keys of the longest
+    row, or per 64 in small steps. One slot, without a reduction, for rows that a single pass covers and for steps with a row
+    for every other CU (130 rows of 4000: 71.9 us with one slot, 79.9 with two; 200 of 200 to 4000: 65.8 and 79.1; 128 of
+    2000: 39.4, with four 42.4; exactly so many rows of 4096 and more still take four: 128 of 8160 136.7 us with one, 123.6
+    with four). A function of constants and the row count only (graph-stable)."""
     tokens = max(1, num_tokens)
-    busy = cu_count
-    if max_seq_len <= 128 or 2 * tokens >= busy:
+    if max_seq_len <= 128 or 2 * tokens >= cu_count + (max_seq_len >= LONG_ROWS):
         return 1
     small = tokens * -(-max_seq_len // TILE) < small_step_tiles
     by_length = 2 * -(-max_seq_len // (64 if small else 128))
-    return max(2, min(2 * max(1, busy // tokens), by_length, 1024))
+    return max(2, min(2 * max(1, cu_count // tokens), by_length, 1024))
 
 
-def _history(q, cache, block_table, ctx, scale, token_requests, splits, workspace, plan, shared_rows, out):
+def history_shape(max_seq_len, num_tokens, num_reqs, cu_count=256, width=512):
+    """How ``history_attention`` runs a step: ``(kind, split slots)`` with ``kind`` 1 for a token per workgroup, 2 for two
+    tokens that share the conversion of their rows (uniform splits, no plan), 3 for rows expanded to bf16 once per request and
+    the multi-query kernels of the bf16 cache over them. In us at 1 / 2 / 3, best split counts:
+
+        tokens x rows          w 256             w 512             w 1024
+        4 x 512 on 8160        447 / 318 / 372   776 / 674 / 577   2614 / 1996 / 4673
+        4 x 512 on 1000        78 / 55 / 71      132 / 115 / 106   410 / 302 / 613
+        16 x 128 on 4000       238 / 171 / 214   403 / 351 / 353   1329 / 1019 / 2519
+        1 x 512 on 8160        123 / 96 / 132    211 / 201 / 217   688 / 505 / 1320
+        1 x 512 on 300         14 / 12           21 / 20           51 / 39
+        1 x 256 on 2000        23 / 27           37 / 50           97 / 110
+        2 x 64 on 8160         44 / 36           71 / 69           202 / 167
+        4 x 8 on 8160          23 / 21           34 / 33           68 / 62
+        4 x 3 on 8160          18 / 24           26 / 34           45 / 59
+        2 x 64 on 2000         22 / 23           36 / 37           80 / 70
+
+    At width 128 a token per workgroup is fastest throughout (4 x 512 on 8160: 273, expanded 437). So two tokens from 2 per CU on, and on long rows from one
+    per 8 CUs on; expansion at width 512 alone, from 8 tokens per CU in chunks of 256 and more on average."""
+    per_request = num_tokens / max(1, num_reqs)
+    if width == 512 and num_tokens >= 8 * cu_count and per_request >= 256:
+        return 3, 1
+    if width >= 256 and per_request >= 4:
+        if num_tokens >= 2 * cu_count:
+            return 2, 1
+        if max_seq_len >= LONG_ROWS and 8 * num_tokens >= cu_count:
+            return 2, max(4, 2 * cu_count // num_tokens)
+    return 1, kv_splits(max_seq_len, num_tokens, cu_count, width)
+
+
+def _history(q, cache, block_table, ctx, scale, token_requests, splits, workspace, plan, tokens_per_group, shared_rows, out):
     """The split kernel, and with ``out`` the reduction; returns ``(lse or None, workspace or None)``."""
     T, w = q.shape[0], q.shape[2]
     ws = lse = None
@@ -197,7 +227,7 @@ def _history(q, cache, block_table, ctx, scale, token_requests, splits, workspac
           cache.stride(0), block_size(cache), cache.shape[0], _lib.ptr(block_table), block_table.stride(0),
           block_table.shape[1], block_table.shape[0], _lib.ptr(token_requests), _lib.ptr(ctx), float(scale), splits,
           _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.ptr(plan), 0 if plan is None else plan.numel(),
-          int(bool(shared_rows)), _lib.ptr(out), 0 if out is None else out.stride(0), 0 if out is None else out.stride(1), _lib.ptr(lse))
+          tokens_per_group, int(shared_rows), _lib.ptr(out), 0 if out is None else out.stride(0), 0 if out is None else out.stride(1), _lib.ptr(lse))
     return lse, ws
 
 
@@ -221,24 +251,36 @@ def history_attention(q_lat, cache, block_table, ctx, scale, max_seq_len, token_
     entry of ``ctx`` may be above ``max_seq_len`` (a host number: it sets the split count). Scores, softmax statistics and
     sums are fp32; the weights are rounded to bf16 for their product with the rows, as over a bf16 cache.
 
-    With ``query_start_loc`` (int32 ``[R + 1]``), ``token_requests`` and a ``max_query_len`` of ``CHUNK_TOKENS`` or more, the rows
-    of each request are expanded to bf16 once, into scratch of ``R * max_seq_len`` rows, and the multi-query kernels of the bf16
-    cache read them: a chunk's tokens share them. Otherwise every token reads its rows as they are.
+    Requests of several tokens (``max_query_len`` above 1, a host number) share their rows: with ``token_requests`` two tokens
+    may go through a row together, and with ``query_start_loc`` (int32 ``[R + 1]``) too the rows of large chunks may be
+    expanded to bf16 once, into scratch of ``R * max_seq_len`` rows (``history_shape`` says when).
 
-    ``num_kv_splits`` defaults to ``kv_splits``; ``workspace`` (an ``S6Workspace``) to a new buffer; ``plan`` is an optional
-    ``s6_ops.split_plan`` for ``(ctx, columns * block, num_kv_splits)``. Calls that share a workspace must not overlap."""
+    ``num_kv_splits`` defaults to the count of ``history_shape``; ``workspace`` (an ``S6Workspace``) to a new buffer; ``plan`` is
+    an optional ``s6_ops.split_plan`` for ``(ctx, columns * block, num_kv_splits)``, for a token per workgroup. Calls that share
+    a workspace must not overlap."""
     T, w, ctx, token_requests = _operands(q_lat, cache, block_table, ctx, token_requests, plan)
     max_seq_len = int(max_seq_len)
-    if max_query_len >= CHUNK_TOKENS and query_start_loc is not None and token_requests is not None and T > 0 and max_seq_len > 0:
-        return _chunk_attention(q_lat, cache, block_table, ctx, scale, max_seq_len, token_requests, query_start_loc,
-                                num_kv_splits, workspace)
-    splits = kv_splits(max_seq_len, T, _lib.device_cus(q_lat.device.index), w) if num_kv_splits is None else int(num_kv_splits)
+    kind, splits = _shape(q_lat, block_table, max_seq_len, token_requests, query_start_loc, max_query_len, plan)
+    if num_kv_splits is not None:
+        splits = int(num_kv_splits)
+    if kind == 3 and splits == 1 and query_start_loc is not None and max_seq_len > 0:
+        return _expanded_attention(q_lat, cache, block_table, ctx, scale, max_seq_len, token_requests, query_start_loc)
     out = torch.empty(T, HEADS, w, dtype=BF16, device=q_lat.device)
-    lse, _ = _history(q_lat, cache, block_table, ctx, scale, token_requests, splits, workspace, plan, max_query_len > 1, out)
+    lse, _ = _history(q_lat, cache, block_table, ctx, scale, token_requests, splits, workspace, plan, min(kind, 2),
+                      max_query_len > 1, out)
     return out, lse
 
 
-def _chunk_attention(q, cache, block_table, ctx, scale, max_seq_len, token_requests, query_start_loc, splits, workspace):
+def _shape(q, block_table, max_seq_len, token_requests, query_start_loc, max_query_len, plan):
+    T, w = q.shape[0], q.shape[2]
+    cus = _lib.device_cus(q.device.index)
+    if max_query_len == 1 or token_requests is None or plan is not None:
+        return 1, kv_splits(max_seq_len, T, cus, w)
+    R = block_table.shape[0] if query_start_loc is None else query_start_loc.shape[0] - 1
+    return history_shape(max_seq_len, T, R, cus, w)
+
+
+def _expanded_attention(q, cache, block_table, ctx, scale, max_seq_len, token_requests, query_start_loc):
     T, w = q.shape[0], q.shape[2]
     _same_device(cache, query_start_loc)
     R = query_start_loc.shape[0] - 1
@@ -248,24 +290,21 @@ def _chunk_attention(q, cache, block_table, ctx, scale, max_seq_len, token_reque
     rows = torch.empty(R * pages, 1, TILE, 2 * w, dtype=BF16, device=q.device)
     _load(cache, w, block_table, None, qsl, ctx, T, R, pages * TILE, rows.view(R, pages * TILE, 2 * w))
     table = torch.arange(R * pages, dtype=I32, device=q.device).view(R, pages)
-    group = 4 if w <= 512 else 2
-    if splits is None:
-        splits = s6_ops.mi355x_kv_splits(max_seq_len, T, _lib.device_cus(q.device.index), w, tokens_per_group=group)
-    if splits > 1 and workspace is None:
-        workspace = s6_ops.S6Workspace(HEADS, w, T * splits)
-    return s6_ops.history_attention_kv(q, rows[..., :w], rows[..., w:], table, ctx, scale, splits, workspace, None, None,
-                                       s6_ops.HIP, bt_rows=token_requests, tokens_per_group=group, shared_rows=True)
+    return s6_ops.history_attention_kv(q, rows[..., :w], rows[..., w:], table, ctx, scale, 1, None, None, None, s6_ops.HIP,
+                                       bt_rows=token_requests, tokens_per_group=4, shared_rows=True)
 
 
 def history_partials(q_lat, cache, block_table, ctx, scale, num_kv_splits, workspace, token_requests=None, plan=None,
-                     max_query_len=1):
+                     query_start_loc=None, max_query_len=1):
     """The split kernel of ``history_attention`` alone: its partials in ``workspace``, in the layout that
     ``s6_ops.history_reduce`` and ``s6_ops.split_epilogue`` read (``[T, 16, splits, w + 1]``, private)."""
     T, w, ctx, token_requests = _operands(q_lat, cache, block_table, ctx, token_requests, plan)
-    splits = int(num_kv_splits)
     if workspace is None:
         raise RuntimeError('history partials need an S6Workspace')
-    _, ws = _history(q_lat, cache, block_table, ctx, scale, token_requests, splits, workspace, plan, max_query_len > 1, None)
+    kind, _ = _shape(q_lat, block_table, block_table.shape[1] * block_size(cache), token_requests, query_start_loc,
+                     max_query_len, plan)
+    _, ws = _history(q_lat, cache, block_table, ctx, scale, token_requests, int(num_kv_splits), workspace, plan, min(kind, 2),
+                     max_query_len > 1, None)
     return ws
 
 

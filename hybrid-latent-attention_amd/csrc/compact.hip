@@ -238,6 +238,10 @@ __device__ __forceinline__ void wave_item(const int32_t* ctx, int T, int64_t cap
   s = __builtin_amdgcn_readlane(slot, src);
 }
 
+// The log-sum-exp of a slot: NaN goes in as infinity, which makes the row NaN in the reductions over slots. (They take the
+// largest of a row's first, past NaN, and would find a row empty whose every slot is NaN.)
+__device__ __forceinline__ float slot_lse(float lse) { return lse != lse ? INFINITY : lse; }
+
 template <int W, bool kOnce>
 __global__ __launch_bounds__(256, W <= 512 ? 2 : 1) void compact_history_kernel(CompactParams a) {
   using G = CompactGeo<W>;
@@ -398,7 +402,7 @@ __global__ __launch_bounds__(256, W <= 512 ? 2 : 1) void compact_history_kernel(
   if (wave == 0 && g == 0) {
     const float lse = (top + log2f(total)) * kLn2;
     if (a.out) a.lse[(int64_t)h * a.T + t] = lse;
-    else a.ws_lse[part + h] = lse;
+    else a.ws_lse[part + h] = slot_lse(lse);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -429,8 +433,268 @@ __global__ __launch_bounds__(256, W <= 512 ? 2 : 1) void compact_history_kernel(
   }
 }
 
+// Two tokens of one request, same rows: the conversion of a row to bf16, which is what bounds the kernel above where rows
+// come out of L2 (8 clocks per pair of values, as long as the two 16 x 16 products that a token has for them), serves both.
+// One workgroup of four waves per (pair of tokens, split); 32 columns of the products are the pair's 2 x 16 heads, so S^T and
+// O^T come from v_mfma_f32_32x32x16_bf16. A wave takes 256 columns of 32 rows: W / 256 waves share a set of rows, add their
+// parts of the scores through LDS (one barrier a step, the parts in two buffers), and go on with the softmax each for itself.
+// The queries lie in LDS. O^T needs 128 accumulators a lane at every width. Tokens of a pair that differ in request or
+// length go through their rows one after the other: a product spreads a NaN in one's rows to the other's sums.
+// 4 x 512 tokens on 8160 rows: w = 512 674 us (760 TFLOP/s; a token per workgroup 776), w = 256 318 (447), w = 1024 1996 (2614).
+// Four tokens per workgroup convert half as often, but need registers that spill (w = 512: twice as long).
 template <int W>
-void launch_history(const CompactParams& p, bool shared_rows, hipStream_t st) {
+struct PairGeo {
+  static constexpr int CH = W / 256;     // waves per set of rows
+  static constexpr int G = 4 / CH;       // sets
+  static constexpr int FRAGS = W / 16;   // steps of Q, 16 columns each
+};
+struct PairRows {  // what a lane holds of 32 rows
+  u32x4 k[4];
+  uint32_t k_scale[2];
+  uint32_t v[2][8];
+  uint32_t v_scale[2][2];
+};
+template <int W>
+__device__ __forceinline__ void pair_load_k(const uint8_t* t0, const uint8_t* t1, int n, int f, int slice, PairRows& r) {
+  const uint8_t* tile = n < 16 ? t0 : t1;
+  const int x = n & 15;
+  // scales of blocks b = 8 slice + 2i + f: [b % 4][b / 4], two pairs of neighbours
+  const uint8_t* sp = tile + 16 * W + x * (W / 32) + 2 * slice;
+  r.k_scale[0] = *reinterpret_cast<const uint16_t*>(sp + f * (W / 128));
+  r.k_scale[1] = *reinterpret_cast<const uint16_t*>(sp + (2 + f) * (W / 128));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.k[i] = ld16(tile + k_code_at(x, 8 * slice + 2 * i + f));
+}
+template <int W>
+__device__ __forceinline__ void pair_load_v(const uint8_t* t0, const uint8_t* t1, int n, int f, int slice, PairRows& r) {
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    const uint8_t* tile = m ? t1 : t0;
+    const uint8_t* sp = tile + 16 * W + W / 2 + (8 * slice + n / 4) * 16 + 4 * f;
+    r.v_scale[m][0] = *reinterpret_cast<const uint32_t*>(sp);
+    r.v_scale[m][1] = *reinterpret_cast<const uint32_t*>(sp + 8);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)  // rows 4f + e, then 8 + 4f + e - 4
+      r.v[m][e] = *reinterpret_cast<const uint32_t*>(tile + 8 * W + (4 * (e & 3) + 2 * (e >> 2) + f) * (W / 2) + 128 * slice + 4 * n);
+  }
+}
+// columns 2 kByte and 2 kByte + 1 of the lane's eight for the 16 keys of tile m
+template <int kByte>
+__device__ __forceinline__ void pair_pv(const PairRows& r, int m, const float (&f)[8], u32x4 p, floatx16& even, floatx16& odd) {
+  uint32_t x[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = two_bf16<kByte>(r.v[m][e], f[e]);
+  u32x4 lo, hi;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    lo[e] = __builtin_amdgcn_perm(x[2 * e + 1], x[2 * e], 0x05040100u);
+    hi[e] = __builtin_amdgcn_perm(x[2 * e + 1], x[2 * e], 0x07060302u);
+  }
+  even = mfma32x32x16(lo, p, even);
+  odd = mfma32x32x16(hi, p, odd);
+}
+template <int W>
+__global__ __launch_bounds__(256, W <= 512 ? 2 : 1) void compact_pair_kernel(CompactParams a) {
+  using P = PairGeo<W>;
+  constexpr int JOIN = P::G > 1 ? 2 * P::CH * 4 * (P::G - 1) * 2 : 0, SUMS = P::CH > 1 ? 2 * 4 * 4 : 0;
+  __shared__ u32x4 q_lds[P::FRAGS][64];
+  __shared__ floatx4 x_lds[JOIN > SUMS ? JOIN : SUMS][64];  // parts of the scores; then of the outputs
+  __shared__ float m_lds[4][32], l_lds[4][32];
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, f = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), slice = wave % P::CH, set = wave / P::CH;
+  const int S = a.num_splits, s = blockIdx.y;
+  const int ta = 2 * blockIdx.x, tb = min(ta + 1, a.T - 1);
+  const int64_t cap = (int64_t)a.bt_cols * a.block;
+  const int mine = n < 16 ? ta : tb, h = n & 15;
+#pragma unroll
+  for (int i = 0; i < P::FRAGS / 4; ++i) {
+    const int x = wave * (P::FRAGS / 4) + i;
+    q_lds[x][lane] = ld16(a.q + (int64_t)mine * a.q_st + (int64_t)h * a.q_sh + 32 * (x / 4 * 2 + f) + 8 * (x % 4));
+  }
+  __syncthreads();
+  const int64_t ra = a.bt_rows ? a.bt_rows[ta] : ta, rb = a.bt_rows ? a.bt_rows[tb] : tb;
+  const int na = a.ctx[ta], nb = a.ctx[tb];
+  const bool both = ra == rb && na == nb;
+#pragma unroll 1
+  for (int pass = 0; pass < (both ? 1 : 2); ++pass) {  // (uniform over the workgroup, all but in_pass and what hangs on it)
+    const int rows = (int)min((int64_t)max(pass ? nb : na, 0), cap);
+    const int tiles = (rows + kTile - 1) / kTile, chunk = (tiles + S - 1) / S;
+    const int j_begin = s * chunk, j_end = min(tiles, j_begin + chunk);
+    const int limit = min(rows, j_end * kTile);
+    const bool in_pass = both || (n < 16) == (pass == 0);
+    floatx16 acc[8];
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[t][e] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    if (j_begin < j_end) {
+      const int64_t table_row = min(max(pass ? rb : ra, (int64_t)0), (int64_t)a.bt_count - 1);
+      const int32_t* btr = a.bt + table_row * a.bt_stride;
+      constexpr int stride = 2 * P::G;
+      uint32_t off_lo, off_hi;
+      auto look_up = [&](int j0) {  // as in compact_history_kernel
+        const int row = min(j0 + (lane >> 1) * stride + (lane & 1), j_end - 1) * kTile;
+        const int64_t page = clamp_page(btr[row / a.block], a.num_blocks);
+        const int64_t off = page * a.page_stride + (row % a.block) / kTile * compact_tile_bytes(W);
+        off_lo = (uint32_t)off;
+        off_hi = (uint32_t)((uint64_t)off >> 32);
+      };
+      auto tile_at = [&](int i) {
+        const uint32_t lo = __builtin_amdgcn_readlane(off_lo, i), hi = __builtin_amdgcn_readlane(off_hi, i);
+        return a.cache + (int64_t)(((uint64_t)hi << 32) | lo);
+      };
+      int j = j_begin + 2 * set;  // past the end in the last step of some sets: rows loaded again, and hidden
+      look_up(j);
+      PairRows r;
+      const uint8_t *t0 = tile_at(0), *t1 = tile_at(1);
+      pair_load_k<W>(t0, t1, n, f, slice, r);
+      pair_load_v<W>(t0, t1, n, f, slice, r);
+      for (int step = 1; j_begin + (step - 1) * stride < j_end; j += stride, ++step) {
+        floatx16 sc;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float scale = scale_of(r.k_scale[i & 1], i >> 1);
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            sc = mfma32x32x16(eight_bf16(r.k[i][c], scale), q_lds[16 * slice + 4 * i + c][lane], sc);
+        }
+        if ((step & 31) == 0) look_up(j + stride);
+        t0 = tile_at(2 * (step & 31));
+        t1 = tile_at(2 * (step & 31) + 1);
+        pair_load_k<W>(t0, t1, n, f, slice, r);
+        if constexpr (P::CH > 1) {
+          floatx4(*to)[64] = x_lds + ((step & 1) * 4 + wave) * 4;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) to[e][lane] = floatx4{sc[4 * e], sc[4 * e + 1], sc[4 * e + 2], sc[4 * e + 3]};
+          __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, 0));  // LDS alone: the rows on their way stay on it
+          plain_barrier();
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {  // every wave of the set adds in the same order
+            const floatx4(*from)[64] = x_lds + ((step & 1) * 4 + set * P::CH) * 4;
+            floatx4 v = from[e][lane];
+#pragma unroll
+            for (int c = 1; c < P::CH; ++c) v += from[4 * c + e][lane];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[4 * e + i] = v[i];
+          }
+        }
+        float vf[2][8];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          sc[e] *= a.scale_log2;
+          vf[e / 8][e % 8] = scale_of(r.v_scale[e / 8][e / 4 % 2], e % 4);
+        }
+        if ((j + 2) * kTile > limit || !both) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const bool seen = j * kTile + e / 4 * 8 + 4 * f + e % 4 < limit;
+            if (!seen) vf[e / 8][e % 8] = 0.f;
+            if (!seen || !in_pass) sc[e] = -INFINITY;
+          }
+        }
+        float mx = sc[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) mx = fmaxf(mx, sc[e]);
+        mx = xor32_max(mx);
+        const bool raise = mx > m + 8.f;
+        if (__any(raise)) {
+          const float m_new = raise ? mx : m;
+          const float alpha = raise ? fast_exp2(m - m_new) : 1.f;
+          l *= alpha;
+          m = m_new;
+#pragma unroll
+          for (int t = 0; t < 8; ++t) acc[t] = acc[t] * alpha;
+        }
+        const float m_use = m == -INFINITY ? 0.f : m;
+        float p[16], sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) p[e] = fast_exp2(sc[e] - m_use);
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) sum += (p[e] + p[e + 1]) + (p[e + 2] + p[e + 3]);
+        l += sum;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const u32x4 pb = {pack2(p[8 * x], p[8 * x + 1]), pack2(p[8 * x + 2], p[8 * x + 3]),
+                            pack2(p[8 * x + 4], p[8 * x + 5]), pack2(p[8 * x + 6], p[8 * x + 7])};
+          pair_pv<0>(r, x, vf[x], pb, acc[0], acc[1]);
+          pair_pv<1>(r, x, vf[x], pb, acc[2], acc[3]);
+          __builtin_amdgcn_sched_barrier(0);
+          pair_pv<2>(r, x, vf[x], pb, acc[4], acc[5]);
+          pair_pv<3>(r, x, vf[x], pb, acc[6], acc[7]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        pair_load_v<W>(t0, t1, n, f, slice, r);
+      }
+    }
+    // Join the sets. Element 4j + i of accumulator t is column 256 slice + 8 m' + t with m' = 8j + 4f + i; set i % G writes it.
+    {
+      const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+      l = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+    }
+    if (f == 0) { m_lds[wave][n] = m; l_lds[wave][n] = l; }
+    __syncthreads();
+    float top = -INFINITY, total = 0.f;
+#pragma unroll
+    for (int x = 0; x < P::G; ++x) top = fmaxf(top, m_lds[x * P::CH][n]);
+    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int x = 0; x < P::G; ++x) total += l_lds[x * P::CH][n] * fast_exp2(m_lds[x * P::CH][n] - base);
+    const float own = fast_exp2(m - base), inv = total == 0.f ? 0.f : 1.0f / total;
+    const bool store = in_pass && (n < 16 || ta + 1 < a.T);
+    const int64_t part = ((int64_t)mine * S + s) * kHeads + h;
+    if (wave == 0 && f == 0 && store) {
+      const float lse = total == 0.f ? -INFINITY : (top + log2f(total)) * kLn2;
+      if (a.out) a.lse[(int64_t)h * a.T + mine] = lse;
+      else a.ws_lse[part] = slot_lse(lse);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (P::G > 1) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (set != i % P::G) {
+            const int at = set < i % P::G ? set : set - 1;
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+              x_lds[((((j & 1) * P::CH + slice) * 4 + i) * (P::G - 1) + at) * 2 + c][lane] =
+                  floatx4{acc[4 * c][4 * j + i], acc[4 * c + 1][4 * j + i], acc[4 * c + 2][4 * j + i], acc[4 * c + 3][4 * j + i]} * own;
+          }
+        __syncthreads();
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (set != i % P::G) continue;
+        const int col = 256 * slice + 8 * (8 * j + 4 * f + i);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          floatx4 o = floatx4{acc[4 * c][4 * j + i], acc[4 * c + 1][4 * j + i], acc[4 * c + 2][4 * j + i], acc[4 * c + 3][4 * j + i]} * own;
+#pragma unroll
+          for (int x = 0; x < P::G - 1; ++x) o += x_lds[((((j & 1) * P::CH + slice) * 4 + i) * (P::G - 1) + x) * 2 + c][lane];
+          o = o * inv;
+          if (!store) continue;
+          if (a.out)
+            *reinterpret_cast<uint2*>(a.out + (int64_t)mine * a.o_st + (int64_t)h * a.o_sh + col + 4 * c) = uint2{pack2(o[0], o[1]), pack2(o[2], o[3])};
+          else
+            *reinterpret_cast<floatx4*>(a.ws_o + part * W + col + 4 * c) = o;
+        }
+      }
+    }
+    if (pass == 0 && !both) __syncthreads();  // (the next pass writes what this one may still read)
+  }
+}
+
+template <int W>
+void launch_history(const CompactParams& p, int tokens_per_group, bool shared_rows, hipStream_t st) {
+  if constexpr (W >= 256) {
+    if (tokens_per_group == 2) {
+      hipLaunchKernelGGL((compact_pair_kernel<W>), dim3((unsigned)((p.T + 1) / 2), (unsigned)p.num_splits), dim3(256), 0, st,
+                         p);
+      return;
+    }
+  }
   const dim3 grid(split_workgroups(p.T, p.num_splits));
   // rows that one token reads stream past the caches from W = 512 on (64 rows of 8160: 68.8 -> 60.6 us, 8 of 32736: 41.8 ->
   // 37.6); at 256 and below, where a lane's V pieces are shorter than a cached line's share, not (32 rows of up to 8160 at
@@ -533,7 +797,7 @@ extern "C" int hla_s6_compact_history(const void* q, int32_t num_tokens, int32_t
                                       int64_t num_blocks, const int32_t* block_table, int64_t bt_stride,
                                       int32_t bt_cols, int32_t bt_count, const int64_t* bt_rows, const int32_t* ctx,
                                       float scale, int32_t num_splits, float* workspace, int64_t workspace_floats,
-                                      const int32_t* plan, int64_t plan_len, int32_t shared_rows, void* out,
+                                      const int32_t* plan, int64_t plan_len, int32_t tokens_per_group, int32_t shared_rows, void* out,
                                       int64_t o_st, int64_t o_sh, float* lse, void* stream) {
   using namespace hla;
   HLA_REQUIRE(num_tokens >= 0, HLA_S6_EINVAL, "compact_history: negative token count");
@@ -544,6 +808,8 @@ extern "C" int hla_s6_compact_history(const void* q, int32_t num_tokens, int32_t
   HLA_REQUIRE(num_splits >= 1 && num_splits <= kMaxSplits, HLA_S6_EINVAL,
               "compact_history: num_kv_splits must be in [1, %d]", kMaxSplits);
   HLA_REQUIRE(bt_cols >= 0, HLA_S6_EINVAL, "compact_history: bad table width");
+  HLA_REQUIRE(tokens_per_group == 1 || (tokens_per_group == 2 && width >= 256), HLA_S6_EINVAL,
+              "compact_history: %d tokens per group at width %d", tokens_per_group, width);
   if (num_tokens == 0) return HLA_S6_OK;
   HLA_REQUIRE(bt_count >= (bt_rows ? 1 : num_tokens), HLA_S6_EINVAL, "compact_history: %d table rows", bt_count);
   HLA_REQUIRE(q && block_table && ctx && (out == nullptr) == (lse == nullptr), HLA_S6_EINVAL,
@@ -591,10 +857,10 @@ extern "C" int hla_s6_compact_history(const void* q, int32_t num_tokens, int32_t
   }
   const hipStream_t st = as_stream(stream);
   switch (width) {
-    case 128: launch_history<128>(p, shared_rows != 0, st); break;
-    case 256: launch_history<256>(p, shared_rows != 0, st); break;
-    case 512: launch_history<512>(p, shared_rows != 0, st); break;
-    default: launch_history<1024>(p, shared_rows != 0, st); break;
+    case 128: launch_history<128>(p, tokens_per_group, shared_rows != 0, st); break;
+    case 256: launch_history<256>(p, tokens_per_group, shared_rows != 0, st); break;
+    case 512: launch_history<512>(p, tokens_per_group, shared_rows != 0, st); break;
+    default: launch_history<1024>(p, tokens_per_group, shared_rows != 0, st); break;
   }
   rc = check_launch("compact_history");
   if (rc != HLA_S6_OK || !out || !partials) return rc;

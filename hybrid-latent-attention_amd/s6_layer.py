@@ -268,26 +268,27 @@ def _attend_composed(q_lat, o_chunk, lse_chunk, B, cache, block_table, ctx, weig
     """History of a compact cache, or of any cache with an account of its attention weights, merged with the chunk's
     partial. Steps of short chunks over a compact cache take the split kernel and the fused epilogue; an account needs the
     merged lse, which only the single ops return."""
-    for kind in ('history', 'merge'):
-        s6_ops._backend(kind, getattr(ctx.backends, kind))
+    for op in ('history', 'merge'):
+        s6_ops._backend(op, getattr(ctx.backends, op))
     w = q_lat.shape[-1]
     if compact_cache.is_compact(cache):
         T, rows = q_lat.shape[0], block_table.shape[1] * compact_cache.block_size(cache)
         longest = min(int(ctx.max_seqlen_k), rows) if ctx.max_seqlen_k else rows
-        splits = compact_cache.kv_splits(longest, T, _lib.device_cus(q_lat.device.index or 0), w)
+        requests = T if ctx.max_query_len == 1 else ctx.query_start_loc.shape[0] - 1
+        kind, splits = compact_cache.history_shape(longest, T, requests, _lib.device_cus(q_lat.device.index or 0), w)
         workspace = ctx.workspace
         if workspace is not None and T * q_lat.shape[1] * splits * (w + 1) > workspace.floats:
             workspace = None
-        if weights is None and splits > 1 and ctx.max_query_len < compact_cache.CHUNK_TOKENS:
+        if weights is None and splits > 1:
             if workspace is None:
                 workspace = s6_ops.S6Workspace(q_lat.shape[1], w, T * splits)
             ws = compact_cache.history_partials(q_lat, cache, block_table, ctx.ctx_latent, ctx.scale, splits, workspace,
-                                                ctx.token_requests, ctx.split_plan(splits, rows),
-                                                ctx.max_query_len)
+                                                ctx.token_requests, ctx.split_plan(splits, rows) if kind == 1 else None,
+                                                ctx.query_start_loc, ctx.max_query_len)
             return s6_ops.split_epilogue(ws, B, o_chunk, lse_chunk, ctx.invalid)
         o_hist, lse_hist = compact_cache.history_attention(
             q_lat, cache, block_table, ctx.ctx_latent, ctx.scale, longest, ctx.token_requests, ctx.query_start_loc,
-            ctx.max_query_len, workspace=workspace if ctx.max_query_len < compact_cache.CHUNK_TOKENS else None)
+            ctx.max_query_len, workspace=workspace)
     else:
         o_hist, lse_hist = s6_ops.history_attention_kv(
             q_lat, cache[..., :w], cache[..., w:], block_table, ctx.ctx_latent, ctx.scale, ctx.kv_splits(w), ctx.workspace,

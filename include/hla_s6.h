@@ -531,14 +531,16 @@ int hla_s6_compact_load(const void *cache, int32_t width, int64_t page_stride, i
 
 /* hla_s6_history_attention over a compact cache: same outputs, splits, workspace and plan (hla_s6_split_plan of (ctx,
  * bt_cols * block_size, num_splits), nullable). Token t reads row bt_rows ? bt_rows[t] : t of the table, clamped into its
- * bt_count rows. shared_rows != 0: several tokens read the same rows (else they stream past the caches). With out and lse NULL the call ends with the partials in the workspace (num_splits >= 1), in the layout
- * that hla_s6_history_reduce and hla_s6_split_epilogue read. */
+ * bt_count rows. tokens_per_group 2 (width 256 and up): a workgroup takes tokens 2i and 2i + 1 together where they read the
+ * same rows, cuts every row in num_splits equal parts and reads no plan; 1: a token per workgroup. shared_rows != 0: several
+ * tokens read the same rows (else they stream past the caches). With out and lse NULL the call ends with the partials in the
+ * workspace (num_splits >= 1), in the layout that hla_s6_history_reduce and hla_s6_split_epilogue read. */
 int hla_s6_compact_history(const void *q, int32_t num_tokens, int32_t num_heads, int32_t width, int64_t q_st,
                            int64_t q_sh, const void *cache, int64_t page_stride, int32_t block_size,
                            int64_t num_blocks, const int32_t *block_table, int64_t bt_stride, int32_t bt_cols,
                            int32_t bt_count, const int64_t *bt_rows, const int32_t *ctx, float scale,
                            int32_t num_splits, float *workspace, int64_t workspace_floats, const int32_t *plan,
-                           int64_t plan_len, int32_t shared_rows, void *out, int64_t o_st, int64_t o_sh, float *lse,
+                           int64_t plan_len, int32_t tokens_per_group, int32_t shared_rows, void *out, int64_t o_st, int64_t o_sh, float *lse,
                            void *stream);
 
 /* ---- eviction from a latent cache --------------------------------------------------------------------

@@ -62,6 +62,16 @@ def test_split_counts(cc):
     assert cc.kv_splits(8160, 4096, 256, 512) == 1 and cc.kv_splits(8160, 100, 256, 512) == 4
 
 
+def test_how_steps_run(cc):
+    assert cc.history_shape(8160, 64, 64, 256, 512) == (1, 8)            # single tokens
+    assert cc.history_shape(8160, 2048, 4, 256, 512) == (3, 1)           # large chunks
+    assert cc.history_shape(8160, 2048, 4, 256, 256) == (2, 1) and cc.history_shape(8160, 2048, 4, 256, 1024) == (2, 1)
+    assert cc.history_shape(8160, 2048, 32, 256, 512) == (2, 1)
+    assert cc.history_shape(8160, 64, 4, 256, 512) == (2, 8) and cc.history_shape(8160, 255, 4, 256, 512) == (2, 4)
+    assert cc.history_shape(2000, 64, 4, 256, 512)[0] == 1 and cc.history_shape(8160, 2048, 4, 256, 128) == (1, 1)
+    assert cc.history_shape(8160, 0, 0, 256, 512)[0] == 1
+
+
 def test_cache_shape(cc):
     assert cc.cache_shape(10, 32, 512) == (10, 2, 17 * 512)
     for args in ((10, 24, 512), (10, 0, 512), (10, 16, 384)):
@@ -102,9 +112,10 @@ def test_entry_points_check_before_they_launch(pkg):
                           (dict(_8=16, _14=16, _5=16, _15=8, _16=8), 'apart'), (dict(_8=16, _14=8, _5=16, _16=256), 'aligned')):
         with pytest.raises(ValueError, match=match):
             call('hla_s6_compact_load', **{**load, **change})
-    history = dict(_0=16, _1=1, _2=16, _3=128, _6=16, _7=page, _8=16, _9=2, _10=16, _12=1, _13=1, _15=16, _17=1, _23=16, _26=16)
+    history = dict(_0=16, _1=1, _2=16, _3=128, _6=16, _7=page, _8=16, _9=2, _10=16, _12=1, _13=1, _15=16, _17=1, _22=1, _24=16, _27=16)
     for change, match in ((dict(_2=8), 'heads'), (dict(_3=64), 'width'), (dict(_17=0), 'num_kv_splits'), (dict(_17=1025), 'num_kv_splits'),
-                          (dict(_13=0), 'table rows'), (dict(_0=None), 'null pointer'), (dict(_26=None), 'null pointer'), (dict(_4=4), 'aligned'),
+                          (dict(_13=0), 'table rows'), (dict(_0=None), 'null pointer'), (dict(_27=None), 'null pointer'), (dict(_4=4), 'aligned'),
+                          (dict(_22=2), 'tokens per group'), (dict(_3=256, _7=2 * page, _22=3), 'tokens per group'),
                           (dict(_17=2, _18=16, _19=10 ** 6, _20=16, _21=3), 'split plan')):
         with pytest.raises(ValueError, match=match):
             call('hla_s6_compact_history', **{**history, **change})

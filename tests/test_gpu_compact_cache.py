@@ -166,6 +166,20 @@ def test_history_attention(cc, width, block, splits):
     check_attention(host_f32(o), host_f32(lse), bf16.to_f32(q), p.rows, ctx)
 
 
+@pytest.mark.parametrize('splits', [1, 4])
+def test_rows_that_read_as_nan(cc, splits):
+    """A NaN among a request's rows makes its output and lse NaN, in one slot or in every one, and no other request's."""
+    rng = np.random.default_rng(21)
+    p = Pool(rng, [500, 500, 500], 256, 16)
+    for r, rows in ((0, [499]), (1, np.arange(500))):
+        bad = np.full((len(rows), 256), np.nan)
+        C.store(p.cache, bad, bad, C.slots_of(p.table[r], 16, 500)[rows])
+    q = random_bits(rng, (3, 16, 256))
+    o, lse = cc.history_attention(dev_bf16(q), dev_u8(p.cache), dev_i32(p.table), dev_i32([500] * 3), SCALE, 500, num_kv_splits=splits)
+    assert torch.isnan(o[:2]).all() and torch.isnan(lse[:, :2]).all()
+    check_attention(host_f32(o)[2:], host_f32(lse)[:, 2:], bf16.to_f32(q)[2:], lambda t: p.rows(2), [500])
+
+
 def test_history_of_one_request_and_of_many(cc):
     rng = np.random.default_rng(8)
     for ctx in ([1500], [5] * 70, [300] * 40 + [0] * 3):
@@ -211,6 +225,67 @@ def test_prompt_chunks(cc, width):
     o, lse = cc.history_attention(dev_bf16(q), dev_u8(p.cache), dev_i32(p.table), dev_i32(ctx), SCALE, 210,
                                   token_requests=dev_i64(req), query_start_loc=dev_i32(start), max_query_len=30)
     check_attention(host_f32(o), host_f32(lse), bf16.to_f32(q), lambda t: p.rows(req[t]), ctx)
+
+
+@pytest.mark.parametrize('splits', [1, 3])
+@pytest.mark.parametrize('width,block', [(256, 48), (512, 16), (1024, 32)])
+def test_two_tokens_together(cc, monkeypatch, width, block, splits):
+    """Pairs of one request, pairs that differ in request or length, an odd token at the end, rows of NaN in one request that
+    the other token of its pair must not see, rows longer than the pages a wave looks up at a time."""
+    monkeypatch.setattr(cc, 'history_shape', lambda *a: (2, splits))
+    rng = np.random.default_rng(width + splits)
+    n, chunk = [1100 if width == 256 else 530, 49, 20, 0, 64], [5, 3, 1, 2, 4]
+    p = Pool(rng, n, width, block)
+    C.store(p.cache, np.full((3, width), np.nan), np.full((3, width), np.nan), C.slots_of(p.table[1], block, 49)[[0, 17, 48]])
+    req = np.repeat(np.arange(5), chunk)
+    ctx = np.array(n)[req]
+    ctx[[1, 13]] = 33, 0
+    q = random_bits(rng, (len(req), 16, width), 1.4 * math.sqrt(128 / width))
+    args = (dev_bf16(q), dev_u8(p.cache), dev_i32(p.table), dev_i32(ctx), SCALE)
+    o, lse = cc.history_attention(*args, max(n), token_requests=dev_i64(req), max_query_len=5)
+    bad = req == 1
+    assert torch.isnan(o[torch.from_numpy(bad)]).all() and torch.isnan(lse[:, torch.from_numpy(bad)]).all()
+    keep = np.flatnonzero(~bad)
+    check_attention(host_f32(o)[keep], host_f32(lse)[:, keep], bf16.to_f32(q)[keep], lambda t: p.rows(req[keep[t]]), ctx[keep])
+    again = cc.history_attention(*args, max(n), token_requests=dev_i64(req), max_query_len=5)
+    assert torch.equal(o[keep], again[0][keep])
+
+
+def test_rows_expanded_once(cc, monkeypatch):
+    """The rows of chunks through one expansion to bf16: ragged chunks, an empty request, padding tokens, NaN behind the rows."""
+    monkeypatch.setattr(cc, 'history_shape', lambda *a: (3, 1))
+    rng = np.random.default_rng(11)
+    n, chunk, width = [210, 0, 33, 97], [20, 17, 1, 30], 512
+    p = Pool(rng, n, width, 16)
+    start = np.concatenate(([0], np.cumsum(chunk)))
+    req = np.concatenate((np.repeat(np.arange(4), chunk), [3, 3]))
+    ctx = np.concatenate((np.repeat(n, chunk), [0, 0]))
+    q = random_bits(rng, (len(req), 16, width), 0.5)
+    o, lse = cc.history_attention(dev_bf16(q), dev_u8(p.cache), dev_i32(p.table), dev_i32(ctx), SCALE, 210,
+                                  token_requests=dev_i64(req), query_start_loc=dev_i32(start), max_query_len=30)
+    check_attention(host_f32(o), host_f32(lse), bf16.to_f32(q), lambda t: p.rows(req[t]), ctx)
+
+
+@pytest.mark.parametrize('width,n', [(256, 60), (512, 4200), (1024, 40)])
+def test_steps_of_many_tokens(cc, width, n):
+    """Steps that take two tokens a workgroup by their own size (and, with long rows, few tokens), beside the kernel for one."""
+    rng = np.random.default_rng(width)
+    T = 600 if n < 4096 else 40
+    p = Pool(rng, [n, n // 2], width, 16)
+    req = np.arange(T) // (T // 2 + 1)
+    ctx = np.array([n, n // 2])[req]
+    q = dev_bf16(random_bits(rng, (T, 16, width), 1.4 * math.sqrt(128 / width)))
+    assert cc.history_shape(n, T, 2, 256, width)[0] == 2
+    call = lambda length: cc.history_attention(q, dev_u8(p.cache), dev_i32(p.table), dev_i32(ctx), SCALE, n,
+                                               token_requests=dev_i64(req), max_query_len=length)
+    o, lse = call(T // 2 + 1)
+    o1, lse1 = call(1)
+    some = [0, 1, T // 2, T // 2 + 1, T - 1]
+    rows = {t: p.rows(req[t]) for t in some}
+    for a, b in ((o, lse), (o1, lse1)):
+        check_attention(host_f32(a[some]), host_f32(b[:, some]), host_f32(q[some]), lambda i: rows[some[i]], ctx[some])
+    assert (o.float() - o1.float()).norm() <= 2 * HALF * o.float().norm()   # each output of the two is off by 2^-8 twice
+    assert (lse - lse1).abs().max() <= 1e-4
 
 
 def test_rows_past_four_gigabytes(cc):
