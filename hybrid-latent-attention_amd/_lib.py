@@ -132,7 +132,9 @@ def check(rc: int) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(load(), name)(*args))
+    rc = getattr(_LIB or load(), name)(*args)
+    if rc != OK:
+        check(rc)
 
 
 def ptr(t) -> int | None:
@@ -142,6 +144,9 @@ def ptr(t) -> int | None:
 
 def stream(device=None) -> int:
     """Raw hipStream_t of torch's current stream on ``device``."""
+    index = getattr(device, 'index', device)
+    if isinstance(index, int):   # (without a Stream object around it: 1.5 us of a call)
+        return torch._C._cuda_getCurrentRawStream(index)
     return torch.cuda.current_stream(device).cuda_stream
 
 

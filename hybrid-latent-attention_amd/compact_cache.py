@@ -46,6 +46,13 @@ def _call(name, device, *args):
 
 
 def _same_device(first, *others):
+    at = first.get_device()   # below 0 on the host
+    for t in others:
+        if t is not None and t.get_device() != at:
+            break
+    else:
+        if at >= 0:
+            return
     s6_ops._dev(first, *others)
     for t in others:
         if t is not None and t.device != first.device:
