@@ -529,7 +529,8 @@ __global__ __launch_bounds__(kSelThreads) void select_rows_kernel(SelectParams a
       found = (found << 8) | (uint32_t)__builtin_amdgcn_readlane(bin, owner);
       if (__builtin_amdgcn_readlane(size, owner) == left) {  // all of them stay
         exact = true;
-        threshold = (found << shift) - 1;  // (found is above 0: no candidate's key is 0)
+        // every candidate from this bin on; the lowest one holds NaN and -inf, and no candidate's key is 0
+        threshold = max(found << shift, 1u) - 1;
       }
     }
     if (!exact) {

@@ -434,6 +434,23 @@ def test_select_rows_of_long_histories(cc):
         assert (got.cpu().numpy() == w).all()
 
 
+@pytest.mark.parametrize('M', [100, 3000, 9000, 33000])
+def test_select_keeps_protected_rows_of_any_weight(cc, M):
+    """As many protected rows as the budget, NaN and -inf among them, or all of them: each of them stays."""
+    rng = np.random.default_rng(M)
+    R, b = 4, M // 3
+    weights = rng.standard_normal((R, M)).astype(np.float32)
+    positions = np.stack([rng.permutation(M) for _ in range(R)]).astype(np.int32)
+    kept = positions >= M - b
+    weights[0, np.flatnonzero(kept[0])[:3]] = np.nan, -np.inf, -3.3e38
+    weights[1, kept[1]] = np.nan
+    weights[2, kept[2]] = -np.inf
+    weights[3] = np.nan
+    n = np.full(R, M, np.int32)
+    e = run_select(cc, weights, positions, n, b, np.full(R, M - b))
+    assert (np.sort(e.positions.cpu().numpy()[:, :b], 1) == np.arange(M - b, M)).all()
+
+
 @pytest.mark.parametrize('width,block', [(128, 16), (256, 32), (512, 16), (1024, 48)])
 def test_move_rows(cc, width, block):
     """Moved rows byte for byte, everything else untouched, on compact pages and on bf16 ones."""
