@@ -270,8 +270,10 @@ def history_attention(q_lat, cache, block_table, ctx, scale, max_seq_len, token_
     kind, splits = _shape(q_lat, block_table, max_seq_len, token_requests, query_start_loc, max_query_len, plan)
     if num_kv_splits is not None:
         splits = int(num_kv_splits)
-    if kind == 3 and splits == 1 and query_start_loc is not None and max_seq_len > 0:
-        return _expanded_attention(q_lat, cache, block_table, ctx, scale, max_seq_len, token_requests, query_start_loc)
+    longest = min(max_seq_len, block_table.shape[1] * block_size(cache))
+    if kind == 3 and splits == 1 and query_start_loc is not None and longest > 0:
+        with torch.cuda.device(q_lat.device):
+            return _expanded_attention(q_lat, cache, block_table, ctx, scale, longest, token_requests, query_start_loc)
     out = torch.empty(T, HEADS, w, dtype=BF16, device=q_lat.device)
     lse, _ = _history(q_lat, cache, block_table, ctx, scale, token_requests, splits, workspace, plan, min(kind, 2),
                       max_query_len > 1, out)
@@ -287,13 +289,13 @@ def _shape(q, block_table, max_seq_len, token_requests, query_start_loc, max_que
     return history_shape(max_seq_len, T, R, cus, w)
 
 
-def _expanded_attention(q, cache, block_table, ctx, scale, max_seq_len, token_requests, query_start_loc):
+def _expanded_attention(q, cache, block_table, ctx, scale, longest, token_requests, query_start_loc):
     T, w = q.shape[0], q.shape[2]
     _same_device(cache, query_start_loc)
     R = query_start_loc.shape[0] - 1
     qsl = _vector('query_start_loc', query_start_loc, R + 1)
     _table(block_table, R)
-    pages = -(-min(max_seq_len, block_table.shape[1] * block_size(cache)) // TILE)
+    pages = -(-longest // TILE)
     rows = torch.empty(R * pages, 1, TILE, 2 * w, dtype=BF16, device=q.device)
     _load(cache, w, block_table, None, qsl, ctx, T, R, pages * TILE, rows.view(R, pages * TILE, 2 * w))
     table = torch.arange(R * pages, dtype=I32, device=q.device).view(R, pages)

@@ -263,12 +263,12 @@ __global__ __launch_bounds__(256, W <= 512 ? 2 : 1) void compact_history_kernel(
       wave_item(a.ctx, a.T, cap, S, b, lane, chunk, t, s);
     }
     if (b < a.T) {  // slots of row b past its work
-      const int used = a.plan ? a.plan[1 + b] : used_slots(a.ctx[b], cap, chunk);
+      const int used = a.plan ? min(max(a.plan[1 + b], 0), S) : used_slots(a.ctx[b], cap, chunk);
       float* l0 = a.ws_lse + ((int64_t)b * S + used) * kHeads;
       for (int i = tid; i < (S - used) * kHeads; i += 256) l0[i] = -INFINITY;
     }
   }
-  if (t < 0) return;
+  if (t < 0 || t >= a.T || s < 0 || s >= S) return;  // (past the end of the list; or no plan of this step's)
   t = __builtin_amdgcn_readfirstlane(t);
   s = __builtin_amdgcn_readfirstlane(s);
   const int n = (int)min((int64_t)max(a.ctx[t], 0), cap);
@@ -797,8 +797,9 @@ extern "C" int hla_s6_compact_history(const void* q, int32_t num_tokens, int32_t
                                       int64_t num_blocks, const int32_t* block_table, int64_t bt_stride,
                                       int32_t bt_cols, int32_t bt_count, const int64_t* bt_rows, const int32_t* ctx,
                                       float scale, int32_t num_splits, float* workspace, int64_t workspace_floats,
-                                      const int32_t* plan, int64_t plan_len, int32_t tokens_per_group, int32_t shared_rows, void* out,
-                                      int64_t o_st, int64_t o_sh, float* lse, void* stream) {
+                                      const int32_t* plan, int64_t plan_len, int32_t tokens_per_group,
+                                      int32_t shared_rows, void* out, int64_t o_st, int64_t o_sh, float* lse,
+                                      void* stream) {
   using namespace hla;
   HLA_REQUIRE(num_tokens >= 0, HLA_S6_EINVAL, "compact_history: negative token count");
   HLA_REQUIRE(num_heads == kHeads, HLA_S6_EUNSUPPORTED, "compact_history: %d query heads (the kernel is built for 16)",
@@ -812,7 +813,7 @@ extern "C" int hla_s6_compact_history(const void* q, int32_t num_tokens, int32_t
               "compact_history: %d tokens per group at width %d", tokens_per_group, width);
   if (num_tokens == 0) return HLA_S6_OK;
   HLA_REQUIRE(bt_count >= (bt_rows ? 1 : num_tokens), HLA_S6_EINVAL, "compact_history: %d table rows", bt_count);
-  HLA_REQUIRE(q && block_table && ctx && (out == nullptr) == (lse == nullptr), HLA_S6_EINVAL,
+  HLA_REQUIRE(q && (block_table || bt_cols == 0) && ctx && (out == nullptr) == (lse == nullptr), HLA_S6_EINVAL,
               "compact_history: null pointer argument");
   HLA_REQUIRE(aligned(q, 16) && q_st % 8 == 0 && q_sh % 8 == 0, HLA_S6_EINVAL,
               "compact_history: q needs 16-byte aligned rows (unit last stride, strides multiple of 8)");

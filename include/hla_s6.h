@@ -540,8 +540,8 @@ int hla_s6_compact_history(const void *q, int32_t num_tokens, int32_t num_heads,
                            int64_t num_blocks, const int32_t *block_table, int64_t bt_stride, int32_t bt_cols,
                            int32_t bt_count, const int64_t *bt_rows, const int32_t *ctx, float scale,
                            int32_t num_splits, float *workspace, int64_t workspace_floats, const int32_t *plan,
-                           int64_t plan_len, int32_t tokens_per_group, int32_t shared_rows, void *out, int64_t o_st, int64_t o_sh, float *lse,
-                           void *stream);
+                           int64_t plan_len, int32_t tokens_per_group, int32_t shared_rows, void *out, int64_t o_st,
+                           int64_t o_sh, float *lse, void *stream);
 
 /* ---- eviction from a latent cache --------------------------------------------------------------------
  * On compact caches (compact != 0: page_stride in bytes, row_stride unused) and on bf16 ones (strides in elements, rows
