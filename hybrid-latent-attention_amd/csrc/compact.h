@@ -79,6 +79,12 @@ __device__ __forceinline__ int64_t clamp_page(int32_t page, int64_t num_blocks) 
   return min(max((int64_t)page, (int64_t)0), num_blocks - 1);
 }
 
+// A barrier that waits for this wave's accesses to LDS, and for none to memory
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_s_waitcnt(waitcnt_imm(63, 0));
+  plain_barrier();
+}
+
 template <int W, int NW = 4>
 struct CompactGeo {
   static constexpr int KC = W / 128;              // 16-byte K pieces per lane and tile

@@ -1,4 +1,6 @@
 // The compact latent cache (compact.h): row commit, row load and paged history attention over 4-bit rows.
+#include <type_traits>
+
 #include "compact.h"
 #include "split_plan.h"
 
@@ -246,7 +248,8 @@ template <int W, bool kOnce>
 __global__ __launch_bounds__(256, W <= 512 ? 2 : 1) void compact_history_kernel(CompactParams a) {
   using G = CompactGeo<W>;
   __shared__ float m_lds[4][16], l_lds[4][16];
-  __shared__ floatx4 o_lds[2][G::CH][G::G - 1][G::CPL / 4][64];
+  constexpr int C2 = G::CPL / 8;  // half of a lane's columns, in fours
+  __shared__ floatx4 o_lds[4][G::CH][G::G - 1][C2][64];
   __shared__ u32x4 q_lds[QOperand<W>::kLds ? G::KC * 4 : 1][64];
 
   const int tid = threadIdx.x, lane = tid & 63, h = lane & 15, g = lane >> 4;
@@ -254,6 +257,13 @@ __global__ __launch_bounds__(256, W <= 512 ? 2 : 1) void compact_history_kernel(
   const int S = a.num_splits, b = blockIdx.x;
   const int64_t cap = (int64_t)a.bt_cols * a.block;
   int t = b, s = 0, chunk = 0;
+  int ctx_of_lane = 0;  // of row `lane`, and its table row: on their way with the work list, in steps of up to 64 rows
+  int64_t row_of_lane = 0;
+  const bool from_lanes = S > 1 && !a.plan && a.T <= 64;
+  if (from_lanes && lane < a.T) {
+    ctx_of_lane = a.ctx[lane];
+    row_of_lane = a.bt_rows ? a.bt_rows[lane] : lane;
+  }
   if (S > 1) {
     if (a.plan) {
       chunk = a.plan[0];
@@ -271,15 +281,15 @@ __global__ __launch_bounds__(256, W <= 512 ? 2 : 1) void compact_history_kernel(
   if (t < 0 || t >= a.T || s < 0 || s >= S) return;  // (past the end of the list; or no plan of this step's)
   t = __builtin_amdgcn_readfirstlane(t);
   s = __builtin_amdgcn_readfirstlane(s);
-  const int n = (int)min((int64_t)max(a.ctx[t], 0), cap);
+  const int n = (int)min((int64_t)max(from_lanes ? __builtin_amdgcn_readlane(ctx_of_lane, t) : a.ctx[t], 0), cap);
   const int tiles = (n + kTile - 1) / kTile;
   if (S == 1) chunk = tiles;
   const int j_begin = s * chunk, j_end = min(tiles, j_begin + chunk);
-  const int64_t part = ((int64_t)t * S + s) * kHeads;
+  const int64_t part_row = ((int64_t)t * S + s) * kHeads;
 
   if (j_begin >= j_end) {  // a row without history
     if (!a.out) {
-      if (tid < kHeads) a.ws_lse[part + tid] = -INFINITY;
+      if (tid < kHeads) a.ws_lse[part_row + tid] = -INFINITY;
       return;
     }
     for (int i = tid; i < kHeads * W / 4; i += 256)
@@ -289,7 +299,10 @@ __global__ __launch_bounds__(256, W <= 512 ? 2 : 1) void compact_history_kernel(
     return;
   }
 
-  const int64_t table_row = min(max(a.bt_rows ? a.bt_rows[t] : (int64_t)t, (int64_t)0), (int64_t)a.bt_count - 1);
+  const int64_t named = from_lanes ? (int64_t)(((uint64_t)__builtin_amdgcn_readlane((uint32_t)((uint64_t)row_of_lane >> 32), t) << 32) |
+                                               (uint32_t)__builtin_amdgcn_readlane((uint32_t)row_of_lane, t))
+                                   : a.bt_rows ? a.bt_rows[t] : (int64_t)t;
+  const int64_t table_row = min(max(named, (int64_t)0), (int64_t)a.bt_count - 1);
   const int32_t* btr = a.bt + table_row * a.bt_stride;
   const int limit = min(n, j_end * kTile);
   // Tile addresses of the wave's next 32 steps, worked out by its lanes together: lane 2i + e holds the byte offset of tile e
@@ -327,16 +340,20 @@ __global__ __launch_bounds__(256, W <= 512 ? 2 : 1) void compact_history_kernel(
     load_v<W, kOnce>(t1, h, g, half, v[1]);
   }
   q.template share<4>(wave, lane, q_lds);
-  for (int step = 1; j < j_end; j += stride, ++step) {
+  // (the last step by itself: behind a branch that may have skipped the next one's loads the compiler can only wait for all of
+  // them, K of the next step with V of this one: 64 rows of 8160, 77 us and 3.7 TB/s; loads of the last tiles over again in
+  // its place hold up the end)
+  int step = 1;
+  auto one_step = [&](auto last) {
     floatx4 s0, s1;
     scores<W>(k, q, lane, s0, s1);
-    // (loads without a condition, the last step's from its own tile again: behind a branch that may have skipped loads the
-    // compiler can only wait for all of them, K of the next step with V of this one: 64 rows of 8160, 77 us and 3.7 TB/s)
-    if ((step & 31) == 0) look_up(j + stride);
-    t0 = tile_at(2 * (step & 31));
-    t1 = tile_at(2 * (step & 31) + 1);
-    load_k<W, kOnce>(t0, h, g, k[0]);
-    load_k<W, kOnce>(t1, h, g, k[1]);
+    if constexpr (!last.value || W < 256) {
+      if ((step & 31) == 0) look_up(j + stride);
+      t0 = tile_at(2 * (step & 31));
+      t1 = tile_at(2 * (step & 31) + 1);
+      load_k<W, kOnce>(t0, h, g, k[0]);
+      load_k<W, kOnce>(t1, h, g, k[1]);
+    }
     float sc[8], f[8];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -380,12 +397,20 @@ __global__ __launch_bounds__(256, W <= 512 ? 2 : 1) void compact_history_kernel(
       pv_pair<W, 2>(v, f, pb, d, acc[8 * d + 4], acc[8 * d + 5]);
       pv_pair<W, 3>(v, f, pb, d, acc[8 * d + 6], acc[8 * d + 7]);
     }
-    load_v<W, kOnce>(t0, h, g, half, v[0]);
-    load_v<W, kOnce>(t1, h, g, half, v[1]);
+    if constexpr (!last.value || W < 256) {
+      load_v<W, kOnce>(t0, h, g, half, v[0]);
+      load_v<W, kOnce>(t1, h, g, half, v[1]);
+    }
+  };
+  if constexpr (W >= 256) {  // (at 128, where four waves a SIMD hide it, the second body costs more: 64 rows of 8160 27 us, 33)
+    for (; j + stride < j_end; j += stride, ++step) one_step(std::false_type{});
+    if (j < j_end) one_step(std::true_type{});
+  } else {
+    for (; j < j_end; j += stride, ++step) one_step(std::false_type{});
   }
 
-  // Join the sets of keys: every wave at the common maximum, then in four rounds wave (round mod sets) of each column half
-  // adds up accumulator element `round` of all of them and writes it: CPL consecutive columns per lane.
+  // Join the sets of keys: every wave at the common maximum, then, half of each lane's columns at a time, set i mod G adds up
+  // accumulator element i of all of them and writes it.
   l = wave_sum16x4(l);
   if (g == 0) {
     m_lds[wave][h] = m;
@@ -402,32 +427,46 @@ __global__ __launch_bounds__(256, W <= 512 ? 2 : 1) void compact_history_kernel(
   if (wave == 0 && g == 0) {
     const float lse = (top + log2f(total)) * kLn2;
     if (a.out) a.lse[(int64_t)h * a.T + t] = lse;
-    else a.ws_lse[part + h] = slot_lse(lse);
+    else a.ws_lse[part_row + h] = slot_lse(lse);
   }
+  // (all sets at work in each part, the reads of a part on their way together, and no barrier that waits for the stores: with
+  // one set after the other this took 3.2 us at W = 512)
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int owner = i % G::G;
-    if (set != owner) {
+  for (int part = 0; part < 2; ++part) {
+    if (part > 0) lds_barrier();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int owner = i % G::G;
+      if (set == owner) continue;
       const int at = set < owner ? set : set - 1;
 #pragma unroll
-      for (int c = 0; c < G::CPL / 4; ++c)
-        o_lds[i & 1][half][at][c][lane] = floatx4{acc[4 * c][i], acc[4 * c + 1][i], acc[4 * c + 2][i],
-                                                  acc[4 * c + 3][i]} * mine;
+      for (int c = 0; c < C2; ++c) {
+        const int b = 4 * (part * C2 + c);
+        o_lds[i][half][at][c][lane] = floatx4{acc[b][i], acc[b + 1][i], acc[b + 2][i], acc[b + 3][i]} * mine;
+      }
     }
-    __syncthreads();
-    if (set == owner) {
-      const int col = half * (W / G::CH) + G::CPL * (4 * g + i);
+    lds_barrier();
 #pragma unroll
-      for (int c = 0; c < G::CPL / 4; ++c) {
-        floatx4 o = floatx4{acc[4 * c][i], acc[4 * c + 1][i], acc[4 * c + 2][i], acc[4 * c + 3][i]} * mine;
+    for (int i = 0; i < 4; ++i) {
+      if (set != i % G::G) continue;
+      floatx4 o[C2];
 #pragma unroll
-        for (int x = 0; x < G::G - 1; ++x) o += o_lds[i & 1][half][x][c][lane];
-        o = o * inv;
-        if (a.out)
+      for (int c = 0; c < C2; ++c) {
+        const int b = 4 * (part * C2 + c);
+        o[c] = floatx4{acc[b][i], acc[b + 1][i], acc[b + 2][i], acc[b + 3][i]} * mine;
+#pragma unroll
+        for (int x = 0; x < G::G - 1; ++x) o[c] += o_lds[i][half][x][c][lane];
+        o[c] = o[c] * inv;
+      }
+      const int col = half * (W / G::CH) + G::CPL * (4 * g + i) + 4 * part * C2;
+      if (a.out) {
+#pragma unroll
+        for (int c = 0; c < C2; ++c)
           *reinterpret_cast<uint2*>(a.out + (int64_t)t * a.o_st + (int64_t)h * a.o_sh + col + 4 * c) =
-              uint2{pack2(o[0], o[1]), pack2(o[2], o[3])};
-        else
-          *reinterpret_cast<floatx4*>(a.ws_o + (part + h) * W + col + 4 * c) = o;
+              uint2{pack2(o[c][0], o[c][1]), pack2(o[c][2], o[c][3])};
+      } else {
+#pragma unroll
+        for (int c = 0; c < C2; ++c) *reinterpret_cast<floatx4*>(a.ws_o + (part_row + h) * W + col + 4 * c) = o[c];
       }
     }
   }
