@@ -1,5 +1,7 @@
 // Eviction from a latent cache by accumulated attention weight: the account of a step's attention, the selection of the
 // rows that stay, and the moves that bring them together. On compact pages (compact.h) and on bf16 ones.
+#include <type_traits>
+
 #include "compact.h"
 
 namespace hla {
@@ -119,8 +121,7 @@ __global__ __launch_bounds__(256) void account_step_kernel(AccountParams a) {
     const int end = min(min(a.ctx[t], cap), begin + a.per_wg);
     if (begin >= end) continue;  // uniform over the workgroup
     int j = begin + wave * NT * kTile;
-    // places of the wave's next 64 / NT steps' tiles, one per lane (see compact_history_kernel); past the end the last tile is
-    // loaded again rather than under a condition
+    // places of the wave's next 64 / NT steps' tiles, one per lane; the last step loads nothing (see compact_history_kernel)
     uint32_t at_lo, at_hi;
     auto look_up = [&](int j0) {
       const int64_t at = K::place(a, btr, min(j0 + lane / NT * SPAN + lane % NT * kTile, (end - 1) / kTile * kTile));
@@ -144,7 +145,8 @@ __global__ __launch_bounds__(256) void account_step_kernel(AccountParams a) {
 #pragma unroll
     for (int s = 0; s < STEPS / 4; ++s) q_lds[wave * (STEPS / 4) + s][lane] = q[s];
     __syncthreads();
-    for (int step = 1; j < end; j += SPAN, ++step) {
+    int step = 1;
+    auto one_step = [&](auto last) {
       floatx4 s[NT];
 #pragma unroll
       for (int x = 0; x < NT; ++x) s[x] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -154,10 +156,12 @@ __global__ __launch_bounds__(256) void account_step_kernel(AccountParams a) {
 #pragma unroll
         for (int x = 0; x < NT; ++x) s[x] = mfma16x16x32(k[x].operand(i), qi, s[x]);
       }
-      const int i0 = step % (64 / NT) * NT;
-      if (i0 == 0) look_up(j + SPAN);
+      if constexpr (!last.value) {
+        const int i0 = step % (64 / NT) * NT;
+        if (i0 == 0) look_up(j + SPAN);
 #pragma unroll
-      for (int x = 0; x < NT; ++x) k[x].template load<kOnce>(a, tile(i0 + x), h, g);
+        for (int x = 0; x < NT; ++x) k[x].template load<kOnce>(a, tile(i0 + x), h, g);
+      }
 #pragma unroll
       for (int x = 0; x < NT; ++x) {
         float w[4];
@@ -167,7 +171,9 @@ __global__ __launch_bounds__(256) void account_step_kernel(AccountParams a) {
         const int key = j + x * kTile + 4 * g + h;
         if (h < 4 && key < end) sum_lds[key - begin] += sum;  // (the same lane for every token)
       }
-    }
+    };
+    for (; j + SPAN < end; j += SPAN, ++step) one_step(std::false_type{});
+    if (j < end) one_step(std::true_type{});
   }
   __syncthreads();
   float* row = a.account + (int64_t)r * a.a_st;
