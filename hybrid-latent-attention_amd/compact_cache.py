@@ -83,42 +83,54 @@ def block_size(cache):
 
 
 def _compact(cache, width=None):
+    """``(width, page stride, block, pages)`` of a compact cache, checked."""
     if cache.dtype != U8:
         raise ValueError(f'a compact cache is uint8, got {cache.dtype}')
-    if cache.dim() != 3 or cache.shape[2] % 17 or (width is not None and cache.shape[2] != 17 * width):
+    shape, stride = cache.shape, cache.stride()
+    if len(shape) != 3 or shape[2] % 17 or (width is not None and shape[2] != 17 * width):
         raise ValueError(f'compact cache must be [num_blocks, block / 16, {17 * width if width else "17 w"}], '
-                         f'got {tuple(cache.shape)}')
-    if cache.stride(2) != 1 or (cache.shape[1] > 1 and cache.stride(1) != cache.shape[2]):
+                         f'got {tuple(shape)}')
+    if stride[2] != 1 or (shape[1] > 1 and stride[1] != shape[2]):
         raise ValueError('the pages of a compact cache must be contiguous')
-    return _width(cache.shape[2] // 17)
+    return _width(shape[2] // 17), stride[0], shape[1] * TILE, shape[0]
 
 
 def _table(block_table, rows):
-    if block_table.dtype != I32 or block_table.dim() != 2 or block_table.stride(-1) != 1:
+    """``(row stride, columns, rows)`` of a block table of at least ``rows`` rows, checked."""
+    stride = block_table.stride()
+    if block_table.dtype != I32 or len(stride) != 2 or stride[1] != 1:
         raise ValueError('block_table must be a 2-d int32 tensor with a unit last stride')
-    if block_table.shape[0] < rows:
-        raise ValueError(f'block_table has {block_table.shape[0]} rows, {rows} are needed')
+    count, cols = block_table.shape
+    if count < rows:
+        raise ValueError(f'block_table has {count} rows, {rows} are needed')
+    return stride[0], cols, count
 
 
 def _vector(name, t, n, dtype=I32):
-    if t.dim() != 1 or t.shape[0] != n:
+    if t.shape != (n,):
         raise ValueError(f'{name} must have {n} entries, got {tuple(t.shape)}')
-    return s6_ops._int(name, t, dtype)
+    if t.dtype != dtype:
+        raise ValueError(f'{name} must be {dtype}, got {t.dtype}')
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _rows2d(name, t, dtype, shape=None):
-    if t.dtype != dtype or t.dim() != 2 or t.stride(-1) != 1 or (shape is not None and tuple(t.shape) != shape):
+    """``(row stride, columns)`` of a 2-d tensor, checked."""
+    stride = t.stride()
+    if t.dtype != dtype or len(stride) != 2 or stride[1] != 1 or (shape is not None and t.shape != shape):
         want = '' if shape is None else f' {list(shape)}'
         raise ValueError(f'{name} must be a 2-d {dtype} tensor{want} with a unit last stride, got {t.dtype} {list(t.shape)}')
+    return stride[0], t.shape[1]
 
 
 def _query(q, width=None):
     s6_ops._bf16('q_lat', q)
-    if q.dim() != 3 or q.shape[1] != HEADS:
-        raise ValueError(f'q_lat must be [T, {HEADS}, width], got {tuple(q.shape)}')
-    if width is not None and q.shape[2] != width:
-        raise ValueError(f'q_lat has width {q.shape[2]}, the cache {width}')
-    return q.shape[0], q.shape[2]
+    shape = q.shape
+    if len(shape) != 3 or shape[1] != HEADS:
+        raise ValueError(f'q_lat must be [T, {HEADS}, width], got {tuple(shape)}')
+    if width is not None and shape[2] != width:
+        raise ValueError(f'q_lat has width {shape[2]}, the cache {width}')
+    return shape[0], shape[2]
 
 
 # ----------------------------------------------------------------------------------------------------------------
@@ -138,20 +150,19 @@ def store_rows(key, value, slots, cache):
     if key.dim() != 2 or key.shape != value.shape:
         raise ValueError(f'key and value must be [T, w] alike, got {tuple(key.shape)} and {tuple(value.shape)}')
     T, w = key.shape
-    _compact(cache, w)
+    _, page_stride, block, pages = _compact(cache, w)
     slots = _vector('slots', slots, T, I64)
-    _call('hla_s6_compact_store', cache.device, _lib.ptr(key), key.stride(0), _lib.ptr(value), value.stride(0), T, w,
-          _lib.ptr(slots), _lib.ptr(cache), cache.stride(0), block_size(cache), cache.shape[0])
+    _call('hla_s6_compact_store', cache.device, key.data_ptr(), key.stride(0), value.data_ptr(), value.stride(0), T, w,
+          slots.data_ptr(), cache.data_ptr(), page_stride, block, pages)
 
 
 def load_rows(cache, block_table, lengths, max_rows, out=None):
     """The rows of requests as bf16: ``[R, max_rows, 2w]`` with rows ``lengths[r]`` (int32 ``[R]``) and on of request ``r``
     zero. ``block_table`` is per request. ``out`` (any request and row strides) is written if given."""
     _same_device(cache, block_table, lengths, out)
-    w = _compact(cache)
-    R = lengths.shape[0]
+    geometry = _compact(cache)
+    w, R = geometry[0], lengths.shape[0]
     lengths = _vector('lengths', lengths, R)
-    _table(block_table, R)
     max_rows = int(max_rows)
     if out is None:
         out = torch.empty(R, max_rows, 2 * w, dtype=BF16, device=cache.device)
@@ -159,14 +170,17 @@ def load_rows(cache, block_table, lengths, max_rows, out=None):
         s6_ops._bf16('out', out)
         if tuple(out.shape) != (R, max_rows, 2 * w):
             raise ValueError(f'out must be [{R}, {max_rows}, {2 * w}], got {tuple(out.shape)}')
-    _load(cache, w, block_table, lengths, None, None, 0, R, max_rows, out)
+    _load(cache, geometry, block_table, lengths, None, None, 0, R, max_rows, out)
     return out
 
 
-def _load(cache, w, block_table, lengths, query_start_loc, ctx, T, R, max_rows, out):
-    _call('hla_s6_compact_load', cache.device, _lib.ptr(cache), w, cache.stride(0), block_size(cache), cache.shape[0],
-          _lib.ptr(block_table), block_table.stride(0), block_table.shape[1], _lib.ptr(lengths),
-          _lib.ptr(query_start_loc), _lib.ptr(ctx), T, R, max_rows, _lib.ptr(out), out.stride(0), out.stride(1))
+def _load(cache, geometry, block_table, lengths, query_start_loc, ctx, T, R, max_rows, out):
+    w, page_stride, block, pages = geometry
+    table_stride, cols, _ = _table(block_table, R)
+    request_stride, row_stride, _ = out.stride()
+    _call('hla_s6_compact_load', cache.device, cache.data_ptr(), w, page_stride, block, pages, block_table.data_ptr(),
+          table_stride, cols, _lib.ptr(lengths), _lib.ptr(query_start_loc), _lib.ptr(ctx), T, R, max_rows, out.data_ptr(),
+          request_stride, row_stride)
 
 
 # ----------------------------------------------------------------------------------------------------------------
@@ -220,33 +234,37 @@ def history_shape(max_seq_len, num_tokens, num_reqs, cu_count=256, width=512):
     return 1, kv_splits(max_seq_len, num_tokens, cu_count, width)
 
 
-def _history(q, cache, block_table, ctx, scale, token_requests, splits, workspace, plan, tokens_per_group, shared_rows, out):
+def _history(q, cache, geometry, block_table, table, ctx, scale, token_requests, splits, workspace, plan, tokens_per_group,
+             shared_rows, out):
     """The split kernel, and with ``out`` the reduction; returns ``(lse or None, workspace or None)``."""
-    T, w = q.shape[0], q.shape[2]
+    T, _, w = q.shape
+    _, page_stride, block, pages = geometry
+    token_stride, head_stride, _ = q.stride()
+    table_stride, cols, count = table
+    dev = q.device
     ws = lse = None
     if splits > 1 or out is None:
         need = T * HEADS * splits * (w + 1)
-        ws = (torch.empty(need, dtype=F32, device=q.device) if workspace is None
-              else workspace.attn_logits(T, HEADS, splits, w, q.device))
+        ws = (torch.empty(need, dtype=F32, device=dev) if workspace is None
+              else workspace.attn_logits(T, HEADS, splits, w, dev))
     if out is not None:
-        lse = torch.empty(HEADS, T, dtype=F32, device=q.device)
-    _call('hla_s6_compact_history', q.device, _lib.ptr(q), T, HEADS, w, q.stride(0), q.stride(1), _lib.ptr(cache),
-          cache.stride(0), block_size(cache), cache.shape[0], _lib.ptr(block_table), block_table.stride(0),
-          block_table.shape[1], block_table.shape[0], _lib.ptr(token_requests), _lib.ptr(ctx), float(scale), splits,
-          _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.ptr(plan), 0 if plan is None else plan.numel(),
-          tokens_per_group, int(shared_rows), _lib.ptr(out), 0 if out is None else out.stride(0), 0 if out is None else out.stride(1), _lib.ptr(lse))
+        lse = torch.empty(HEADS, T, dtype=F32, device=dev)
+    _call('hla_s6_compact_history', dev, q.data_ptr(), T, HEADS, w, token_stride, head_stride, cache.data_ptr(), page_stride,
+          block, pages, block_table.data_ptr(), table_stride, cols, count, _lib.ptr(token_requests), ctx.data_ptr(),
+          float(scale), splits, _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.ptr(plan),
+          0 if plan is None else plan.numel(), tokens_per_group, int(shared_rows), _lib.ptr(out), HEADS * w, w, _lib.ptr(lse))
     return lse, ws
 
 
 def _operands(q, cache, block_table, ctx, token_requests, plan=None):
     _same_device(cache, q, block_table, ctx, token_requests, plan)
     T, w = _query(q)
-    _compact(cache, w)
+    geometry = _compact(cache, w)
     ctx = _vector('ctx', ctx, T)
-    _table(block_table, T if token_requests is None else min(T, 1))
+    table = _table(block_table, T if token_requests is None else min(T, 1))
     if token_requests is not None:
         token_requests = _vector('token_requests', token_requests, T, I64)
-    return T, w, ctx, token_requests
+    return T, w, geometry, table, ctx, token_requests
 
 
 def history_attention(q_lat, cache, block_table, ctx, scale, max_seq_len, token_requests=None, query_start_loc=None,
@@ -265,39 +283,39 @@ def history_attention(q_lat, cache, block_table, ctx, scale, max_seq_len, token_
     ``num_kv_splits`` defaults to the count of ``history_shape``; ``workspace`` (an ``S6Workspace``) to a new buffer; ``plan`` is
     an optional ``s6_ops.split_plan`` for ``(ctx, columns * block, num_kv_splits)``, for a token per workgroup. Calls that share
     a workspace must not overlap."""
-    T, w, ctx, token_requests = _operands(q_lat, cache, block_table, ctx, token_requests, plan)
+    T, w, geometry, table, ctx, token_requests = _operands(q_lat, cache, block_table, ctx, token_requests, plan)
     max_seq_len = int(max_seq_len)
-    kind, splits = _shape(q_lat, block_table, max_seq_len, token_requests, query_start_loc, max_query_len, plan)
+    kind, splits = _shape(q_lat, table, max_seq_len, token_requests, query_start_loc, max_query_len, plan)
     if num_kv_splits is not None:
         splits = int(num_kv_splits)
-    longest = min(max_seq_len, block_table.shape[1] * block_size(cache))
+    longest = min(max_seq_len, table[1] * geometry[2])
     if kind == 3 and splits == 1 and query_start_loc is not None and longest > 0:
         with torch.cuda.device(q_lat.device):
-            return _expanded_attention(q_lat, cache, block_table, ctx, scale, longest, token_requests, query_start_loc)
+            return _expanded_attention(q_lat, cache, geometry, block_table, ctx, scale, longest, token_requests,
+                                       query_start_loc)
     out = torch.empty(T, HEADS, w, dtype=BF16, device=q_lat.device)
-    lse, _ = _history(q_lat, cache, block_table, ctx, scale, token_requests, splits, workspace, plan, min(kind, 2),
-                      max_query_len > 1, out)
+    lse, _ = _history(q_lat, cache, geometry, block_table, table, ctx, scale, token_requests, splits, workspace, plan,
+                      min(kind, 2), max_query_len > 1, out)
     return out, lse
 
 
-def _shape(q, block_table, max_seq_len, token_requests, query_start_loc, max_query_len, plan):
-    T, w = q.shape[0], q.shape[2]
-    cus = _lib.device_cus(q.device.index)
+def _shape(q, table, max_seq_len, token_requests, query_start_loc, max_query_len, plan):
+    T, _, w = q.shape
+    cus = _lib.device_cus(q.get_device())
     if max_query_len == 1 or token_requests is None or plan is not None:
         return 1, kv_splits(max_seq_len, T, cus, w)
-    R = block_table.shape[0] if query_start_loc is None else query_start_loc.shape[0] - 1
+    R = table[2] if query_start_loc is None else query_start_loc.shape[0] - 1
     return history_shape(max_seq_len, T, R, cus, w)
 
 
-def _expanded_attention(q, cache, block_table, ctx, scale, longest, token_requests, query_start_loc):
+def _expanded_attention(q, cache, geometry, block_table, ctx, scale, longest, token_requests, query_start_loc):
     T, w = q.shape[0], q.shape[2]
     _same_device(cache, query_start_loc)
     R = query_start_loc.shape[0] - 1
     qsl = _vector('query_start_loc', query_start_loc, R + 1)
-    _table(block_table, R)
     pages = -(-longest // TILE)
     rows = torch.empty(R * pages, 1, TILE, 2 * w, dtype=BF16, device=q.device)
-    _load(cache, w, block_table, None, qsl, ctx, T, R, pages * TILE, rows.view(R, pages * TILE, 2 * w))
+    _load(cache, geometry, block_table, None, qsl, ctx, T, R, pages * TILE, rows.view(R, pages * TILE, 2 * w))
     table = torch.arange(R * pages, dtype=I32, device=q.device).view(R, pages)
     return s6_ops.history_attention_kv(q, rows[..., :w], rows[..., w:], table, ctx, scale, 1, None, None, None, s6_ops.HIP,
                                        bt_rows=token_requests, tokens_per_group=4, shared_rows=True)
@@ -307,13 +325,12 @@ def history_partials(q_lat, cache, block_table, ctx, scale, num_kv_splits, works
                      query_start_loc=None, max_query_len=1):
     """The split kernel of ``history_attention`` alone: its partials in ``workspace``, in the layout that
     ``s6_ops.history_reduce`` and ``s6_ops.split_epilogue`` read (``[T, 16, splits, w + 1]``, private)."""
-    T, w, ctx, token_requests = _operands(q_lat, cache, block_table, ctx, token_requests, plan)
+    T, w, geometry, table, ctx, token_requests = _operands(q_lat, cache, block_table, ctx, token_requests, plan)
     if workspace is None:
         raise RuntimeError('history partials need an S6Workspace')
-    kind, _ = _shape(q_lat, block_table, block_table.shape[1] * block_size(cache), token_requests, query_start_loc,
-                     max_query_len, plan)
-    _, ws = _history(q_lat, cache, block_table, ctx, scale, token_requests, int(num_kv_splits), workspace, plan, min(kind, 2),
-                     max_query_len > 1, None)
+    kind, _ = _shape(q_lat, table, table[1] * geometry[2], token_requests, query_start_loc, max_query_len, plan)
+    _, ws = _history(q_lat, cache, geometry, block_table, table, ctx, scale, token_requests, int(num_kv_splits), workspace,
+                     plan, min(kind, 2), max_query_len > 1, None)
     return ws
 
 
@@ -324,7 +341,8 @@ def history_partials(q_lat, cache, block_table, ctx, scale, num_kv_splits, works
 def _pages(cache, width=None):
     """Geometry of either kind of cache: ``(width, compact, page_stride, row_stride, block, num_blocks)``."""
     if is_compact(cache):
-        return _compact(cache, width), 1, cache.stride(0), 0, block_size(cache), cache.shape[0]
+        w, page_stride, block, pages = _compact(cache, width)
+        return w, 1, page_stride, 0, block, pages
     s6_ops._bf16('cache', cache)
     if cache.dim() != 4 or cache.shape[1] != 1 or cache.shape[3] % 2 or (width is not None and cache.shape[3] != 2 * width):
         raise ValueError(f'latent cache must be [num_blocks, 1, block, {2 * width if width else "2 w"}], got {tuple(cache.shape)}')
@@ -346,20 +364,19 @@ def attention_weights(q_lat, cache, block_table, query_start_loc, ctx, lse, scal
     R = query_start_loc.shape[0] - 1
     qsl = _vector('query_start_loc', query_start_loc, R + 1)
     ctx = _vector('ctx', ctx, T)
-    _table(block_table, R)
+    table_stride, cols, _ = _table(block_table, R)
     _rows2d('lse', lse, F32, (HEADS, T))
-    _rows2d('weights', weights, F32)
+    weights_stride, M = _rows2d('weights', weights, F32)
     if weights.shape[0] != R:
         raise ValueError(f'weights has {weights.shape[0]} rows for {R} requests')
     lse = lse.contiguous()
-    rows = min(block_table.shape[1] * block, weights.shape[1])
-    shares, keys = account_shape(T, R, rows, _lib.device_cus(q_lat.device.index), w)
-    ws = torch.empty(shares * R * weights.shape[1], dtype=F32, device=weights.device) if shares > 1 else None
-    _call('hla_s6_attention_weights', q_lat.device, _lib.ptr(q_lat), T, HEADS, w, q_lat.stride(0), q_lat.stride(1),
-          _lib.ptr(cache), compact, page_stride, row_stride, block, num_blocks, _lib.ptr(block_table),
-          block_table.stride(0), block_table.shape[1], _lib.ptr(qsl), R, _lib.ptr(ctx), _lib.ptr(lse), float(scale),
-          _lib.ptr(weights), weights.stride(0), weights.shape[1], keys, shares, _lib.ptr(ws),
-          0 if ws is None else ws.numel())
+    token_stride, head_stride, _ = q_lat.stride()
+    shares, keys = account_shape(T, R, min(cols * block, M), _lib.device_cus(q_lat.get_device()), w)
+    ws = torch.empty(shares * R * M, dtype=F32, device=weights.device) if shares > 1 else None
+    _call('hla_s6_attention_weights', q_lat.device, q_lat.data_ptr(), T, HEADS, w, token_stride, head_stride,
+          cache.data_ptr(), compact, page_stride, row_stride, block, num_blocks, block_table.data_ptr(), table_stride, cols,
+          qsl.data_ptr(), R, ctx.data_ptr(), lse.data_ptr(), float(scale), weights.data_ptr(), weights_stride, M, keys, shares,
+          _lib.ptr(ws), 0 if ws is None else ws.numel())
     return weights
 
 
@@ -387,9 +404,9 @@ def select_rows(weights, positions, lengths, budget, protect_from):
     their place, and the i-th row behind it that stays moves to the i-th place left free: order among rows is not kept
     (attention over latent rows does not depend on it), positions tell it. ``move_rows`` applies the moves to a cache."""
     _same_device(weights, positions, lengths, protect_from, budget if torch.is_tensor(budget) else None)
-    _rows2d('weights', weights, F32)
-    R, M = weights.shape
-    _rows2d('positions', positions, I32, (R, M))
+    weights_stride, M = _rows2d('weights', weights, F32)
+    R = weights.shape[0]
+    positions_stride, _ = _rows2d('positions', positions, I32, (R, M))
     lengths = _vector('lengths', lengths, R)
     protect_from = _vector('protect_from', protect_from, R)
     budgets = None
@@ -401,9 +418,9 @@ def select_rows(weights, positions, lengths, budget, protect_from):
     e = Eviction(torch.empty(R, dtype=I32, device=dev), torch.empty(R, M, dtype=F32, device=dev),
                  torch.empty(R, M, dtype=I32, device=dev), torch.empty(R, M // 2, dtype=I32, device=dev),
                  torch.empty(R, M // 2, dtype=I32, device=dev))
-    _call('hla_s6_select_rows', dev, _lib.ptr(weights), weights.stride(0), _lib.ptr(positions), positions.stride(0),
-          _lib.ptr(lengths), R, M, min(int(budget), 2 ** 31 - 1), _lib.ptr(budgets), _lib.ptr(protect_from),
-          _lib.ptr(e.lengths), _lib.ptr(e.weights), _lib.ptr(e.positions), _lib.ptr(e.source), _lib.ptr(e.target))
+    _call('hla_s6_select_rows', dev, weights.data_ptr(), weights_stride, positions.data_ptr(), positions_stride,
+          lengths.data_ptr(), R, M, min(int(budget), 2 ** 31 - 1), _lib.ptr(budgets), protect_from.data_ptr(),
+          *[t.data_ptr() for t in e])
     return e
 
 
@@ -414,12 +431,10 @@ def move_rows(cache, block_table, eviction):
     source, target = eviction.source, eviction.target
     _same_device(cache, block_table, source, target)
     w, compact, page_stride, row_stride, block, num_blocks = _pages(cache)
-    _rows2d('source', source, I32)
-    R, count = source.shape
-    _rows2d('target', target, I32, (R, count))
-    if source.stride(0) != target.stride(0):
-        source, target = source.contiguous(), target.contiguous()
-    _table(block_table, R)
-    _call('hla_s6_move_rows', cache.device, _lib.ptr(cache), w, compact, page_stride, row_stride, block, num_blocks,
-          _lib.ptr(block_table), block_table.stride(0), block_table.shape[1], _lib.ptr(source), _lib.ptr(target),
-          source.stride(0), count, R)
+    list_stride, count = _rows2d('source', source, I32)
+    R = source.shape[0]
+    if _rows2d('target', target, I32, (R, count))[0] != list_stride:
+        source, target, list_stride = source.contiguous(), target.contiguous(), count
+    table_stride, cols, _ = _table(block_table, R)
+    _call('hla_s6_move_rows', cache.device, cache.data_ptr(), w, compact, page_stride, row_stride, block, num_blocks,
+          block_table.data_ptr(), table_stride, cols, source.data_ptr(), target.data_ptr(), list_stride, count, R)
