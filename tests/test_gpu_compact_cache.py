@@ -598,6 +598,48 @@ def test_attend_over_a_compact_cache(cc, pkg, ops, w, chunk):
         assert (a1[r, max(c - 32, 0):] == 0).all()
 
 
+def test_attend_after_an_eviction(cc, pkg, ops):
+    """A layer with an exact window: the rows behind the window are evicted by the account that attend keeps, the window's rows
+    follow them, and the next step attends to what is left, as over a bf16 cache of the same rows."""
+    rng = np.random.default_rng(5)
+    contexts, w, block, W, b, H, D = [300, 200, 150, 120], 512, 16, 32, 40, 16, 128
+    ctx, T = layer_step(pkg, ops, rng, contexts, 1, None, w)
+    p = Pool(rng, [c + 1 for c in contexts], w, block)
+    cache, table = dev_u8(p.cache), dev_i32(p.table)
+    exact = dev_bf16(random_bits(rng, (len(p.cache), H, block, 2 * D)))
+    q_lat = dev_bf16(random_bits(rng, (T, H, w), 0.7))
+    q_rope, k_rope, v = (dev_bf16(random_bits(rng, (T, H, D))) for _ in range(3))
+    B = dev_bf16(random_bits(rng, (H, w, D), 1 / math.sqrt(w)))
+    layer = FakeLatentLayer(B, B, [B], [B])
+    layer.rank1 = layer.rank = w
+    account = torch.zeros(4, 300, device='cuda')
+    step = lambda c, x, **kw: pkg.s6_layer.attend(layer, 0, q_lat, q_rope, k_rope, v, c, table, None, None, x, (exact, table), **kw)
+    step(cache, ctx, weights=account)
+    behind = ctx.ctx_latent.clone()
+    assert behind.tolist() == [c - W for c in contexts]
+    positions = torch.arange(300, dtype=torch.int32, device='cuda').repeat(4, 1)
+    e = cc.select_rows(account, positions, behind, b, behind)          # nothing protected
+    cc.move_rows(cache, table, e)
+    i = torch.arange(W, dtype=torch.int32, device='cuda')
+    cc.move_rows(cache, table, cc.Eviction(None, None, None, behind[:, None] + i, e.lengths[:, None] + i))
+    assert e.lengths.tolist() == [b] * 4
+    got, plain = host_u8(cache), np.zeros((len(p.cache), 1, block, 2 * w), np.float32)
+    for r, c in enumerate(contexts):
+        kept = np.concatenate((e.positions[r, :b].cpu().numpy(), np.arange(c - W, c)))
+        assert len(set(kept)) == b + W and kept[:b].max() < c - W
+        slots = C.slots_of(p.table[r], block, b + W)
+        assert (C.load(got, slots) == p.rows(r)[kept]).all()
+        plain[slots // block, 0, slots % block] = p.rows(r)[kept]
+    steps = []
+    for _ in range(2):
+        x, _ = layer_step(pkg, ops, rng, contexts, 1, None, w)
+        x.ctx_latent.copy_(e.lengths)
+        steps.append(x)
+    want = step(torch.from_numpy(plain).to(torch.bfloat16).cuda(), steps[0]).float()
+    out = step(cache, steps[1]).float()
+    assert (out - want).abs().max() <= 4 * HALF * want.abs().max() and (out - want).norm() <= 2 * HALF * want.norm()
+
+
 def test_write_commit_into_a_compact_cache(cc, pkg, ops):
     """write_commit and store_rows put the same bytes into a compact cache as the quantised rows of the bf16 path."""
     rng = np.random.default_rng(31)
