@@ -189,19 +189,22 @@ def _load(cache, geometry, block_table, lengths, query_start_loc, ctx, T, R, max
 
 def kv_splits(max_seq_len, num_tokens, cu_count=256, width=512, small_step_tiles=768):
     """Split slots per row for ``history_attention`` over a compact cache, one token a workgroup. A split is a workgroup of
-    four waves that walk 128 rows at a time. Like ``s6_ops.mi355x_kv_splits`` this returns twice the count that gives every CU
-    one of them (the plan cuts rows so that about half of the slots get equal work; with two a CU the partials cost more than
-    the waves gain: 64 rows of 8160 at width 512 60.6 us with 8 slots, 70.6 with 16), at most two per 128 keys of the longest
-    row, or per 64 in small steps. One slot, without a reduction, for rows that a single pass covers and for steps with a row
-    for every other CU (130 rows of 4000: 71.9 us with one slot, 79.9 with two; 200 of 200 to 4000: 65.8 and 79.1; 128 of
-    2000: 39.4, with four 42.4; exactly so many rows of 4096 and more still take four: 128 of 8160 136.7 us with one, 123.6
-    with four). A function of constants and the row count only (graph-stable)."""
+    four waves that walk 128 rows at a time. The plan cuts rows so that about half of the slots get equal work, and this returns
+    the count that gives every CU one of them (64 rows of 8160 at width 512: 59.8 us with 8 slots, 66.7 with 16); half of that
+    up to 256 rows per CU (128 above width 512), where partials cost more than workgroups gain (8 of 8160: 21.2 us with 32
+    slots, 22.8 with 64; 1 of 32736: 18.5 with 256, 21.6 with 512); at most two per 128 keys of the longest row, and in small
+    steps two per 64 and one per two CUs (1 of 8160: 13.5 with 128, 15.1 with 256). One slot, without a reduction, for rows that
+    a single pass covers and for steps with a row for every other CU (130 rows of 4000: 67.9 us with one slot, 76.5 with two;
+    200 of 200 to 4000: 62.3 and 77.0; 128 of 2000: 39.1, with four 40.8; exactly so many rows of 4096 and more still take
+    four: 128 of 8160 132 us with one, 105 with four). A function of constants and the row count only (graph-stable)."""
     tokens = max(1, num_tokens)
     if max_seq_len <= 128 or 2 * tokens >= cu_count + (max_seq_len >= LONG_ROWS):
         return 1
-    small = tokens * -(-max_seq_len // TILE) < small_step_tiles
-    by_length = 2 * -(-max_seq_len // (64 if small else 128))
-    return max(2, min(2 * max(1, cu_count // tokens), by_length, 1024))
+    few = tokens * max_seq_len <= cu_count * (256 if width <= 512 else 128)
+    slots = (1 if few else 2) * max(1, cu_count // tokens)
+    if tokens * -(-max_seq_len // TILE) < small_step_tiles:
+        return max(2, min(slots, 2 * -(-max_seq_len // 64), cu_count // 2))
+    return max(2, min(slots, 2 * -(-max_seq_len // 128), 1024))
 
 
 def history_shape(max_seq_len, num_tokens, num_reqs, cu_count=256, width=512):
@@ -210,19 +213,21 @@ def history_shape(max_seq_len, num_tokens, num_reqs, cu_count=256, width=512):
     the multi-query kernels of the bf16 cache over them. In us at 1 / 2 / 3, best split counts:
 
         tokens x rows          w 256             w 512             w 1024
-        4 x 512 on 8160        447 / 318 / 372   776 / 674 / 577   2614 / 1996 / 4673
-        4 x 512 on 1000        78 / 55 / 71      132 / 115 / 106   410 / 302 / 613
-        16 x 128 on 4000       238 / 171 / 214   403 / 351 / 353   1329 / 1019 / 2519
-        1 x 512 on 8160        123 / 96 / 132    211 / 201 / 217   688 / 505 / 1320
-        1 x 512 on 300         14 / 12           21 / 20           51 / 39
-        1 x 256 on 2000        23 / 27           37 / 50           97 / 110
-        2 x 64 on 8160         44 / 36           71 / 69           202 / 167
-        4 x 8 on 8160          23 / 21           34 / 33           68 / 62
-        4 x 3 on 8160          18 / 24           26 / 34           45 / 59
-        2 x 64 on 2000         22 / 23           36 / 37           80 / 70
+        4 x 512 on 8160        447 / 315 / 397   743 / 638 / 555   2633 / 2020 / 4676
+        4 x 512 on 1000        76 / 56 / 76      114 / 109 / 105   419 / 308 / 616
+        16 x 128 on 4000       231 / 166 / 215   391 / 343 / 328   1335 / 1022 / 2514
+        1 x 512 on 8160        121 / 93          202 / 195         700 / 509
+        1 x 512 on 300         14 / 13           20 / 21           49 / 39
+        64 x 8 on 4000         85 / 55           156 / 121         395 / 274
+        1 x 256 on 2000        21 / 27           35 / 50           98 / 110
+        2 x 64 on 8160         45 / 37           71 / 69           205 / 169
+        4 x 8 on 8160          22 / 21           32 / 34           70 / 63
+        4 x 3 on 8160          17 / 25           24 / 33           46 / 59
+        2 x 64 on 2000         22 / 23           36 / 38           82 / 72
 
-    At width 128 a token per workgroup is fastest throughout (4 x 512 on 8160: 273, expanded 437). So two tokens from 2 per CU on, and on long rows from one
-    per 8 CUs on; expansion at width 512 alone, from 8 tokens per CU in chunks of 256 and more on average."""
+    At width 128 a token per workgroup is fastest throughout (4 x 512 on 8160: 273, expanded 437). So two tokens from 2 per CU
+    on, and on long rows from one per 8 CUs on; expansion at width 512 alone, from 8 tokens per CU in chunks of 256 and more on
+    average."""
     per_request = num_tokens / max(1, num_reqs)
     if width == 512 and num_tokens >= 8 * cu_count and per_request >= 256:
         return 3, 1
@@ -318,7 +323,7 @@ def _expanded_attention(q, cache, geometry, block_table, ctx, scale, longest, to
     _load(cache, geometry, block_table, None, qsl, ctx, T, R, pages * TILE, rows.view(R, pages * TILE, 2 * w))
     table = torch.arange(R * pages, dtype=I32, device=q.device).view(R, pages)
     return s6_ops.history_attention_kv(q, rows[..., :w], rows[..., w:], table, ctx, scale, 1, None, None, None, s6_ops.HIP,
-                                       bt_rows=token_requests, tokens_per_group=4, shared_rows=True)
+                                       bt_rows=token_requests.clamp(0, R - 1), tokens_per_group=4, shared_rows=True)
 
 
 def history_partials(q_lat, cache, block_table, ctx, scale, num_kv_splits, workspace, token_requests=None, plan=None,

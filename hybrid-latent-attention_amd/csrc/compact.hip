@@ -479,7 +479,7 @@ __global__ __launch_bounds__(256, W <= 512 ? 2 : 1) void compact_history_kernel(
 // parts of the scores through LDS (one barrier a step, the parts in two buffers), and go on with the softmax each for itself.
 // The queries lie in LDS. O^T needs 128 accumulators a lane at every width. Tokens of a pair that differ in request or
 // length go through their rows one after the other: a product spreads a NaN in one's rows to the other's sums.
-// 4 x 512 tokens on 8160 rows: w = 512 674 us (760 TFLOP/s; a token per workgroup 776), w = 256 318 (447), w = 1024 1996 (2614).
+// 4 x 512 tokens on 8160 rows: w = 512 638 us (860 TFLOP/s; a token per workgroup 743), w = 256 315 (447), w = 1024 2020 (2633).
 // Four tokens per workgroup convert half as often, but need registers that spill (w = 512: twice as long).
 template <int W>
 struct PairGeo {
@@ -725,6 +725,84 @@ __global__ __launch_bounds__(256, W <= 512 ? 2 : 1) void compact_pair_kernel(Com
   }
 }
 
+// The slots of (token t, head h) joined by their log-sum-exp, columns [4 L z, 4 L (z + 1)): groups of L lanes take every NG-th
+// slot, kAhead of them on their way together, and their sums meet in LDS, in order. Bound by latency: slots' lse, then their
+// partials. A slot without rows costs a read of the first one's partial, which is in the cache. 64 rows of 8160 in 8 slots: 4.9
+// us (reading the empty slots as well: 6.4), 8 of 32736 in 64: 4.4.
+template <int W, int L, int NG, int kAhead>
+__global__ __launch_bounds__(L* NG) void compact_join_kernel(CompactParams a) {
+  constexpr int THREADS = L * NG, WAVES = THREADS / 64;
+  __shared__ float lse_lds[kMaxSplits];
+  __shared__ float top_lds[WAVES], den_lds[NG];
+  __shared__ floatx4 acc_lds[NG][L];
+  const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, i = tid % L, q = tid / L, S = a.num_splits;
+  const int col = blockIdx.z * 4 * L + 4 * i;
+  const float* ls = a.ws_lse + (int64_t)t * S * kHeads + h;
+  float top = -INFINITY;
+  for (int s = tid; s < S; s += THREADS) {
+    const float v = ls[(int64_t)s * kHeads];
+    lse_lds[s] = v;
+    top = fmaxf(top, v);
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+  if (tid % 64 == 0) top_lds[tid / 64] = top;
+  __syncthreads();
+#pragma unroll
+  for (int x = 0; x < WAVES; ++x) top = fmaxf(top, top_lds[x]);
+  uint16_t* out = a.out + (int64_t)t * a.o_st + (int64_t)h * a.o_sh + col;
+  if (top == -INFINITY) {  // uniform over the workgroup
+    if (q == 0) *reinterpret_cast<uint2*>(out) = uint2{0u, 0u};
+    if (tid == 0 && blockIdx.z == 0) a.lse[(int64_t)h * a.T + t] = -INFINITY;
+    return;
+  }
+  const float* base = a.ws_o + ((int64_t)t * S * kHeads + h) * W + col;
+  floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+  float den = 0.f;
+  for (int s0 = q; s0 < S; s0 += kAhead * NG) {
+    floatx4 o[kAhead];
+    float w[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int s = s0 + u * NG;
+      const float v = s < S ? lse_lds[s] : -INFINITY;
+      w[u] = fast_exp2((v - top) * kLog2e);  // (infinity for a NaN: NaN)
+      o[u] = *reinterpret_cast<const floatx4*>(base + (int64_t)(v == -INFINITY ? 0 : s) * kHeads * W);
+      if (v == -INFINITY) w[u] = 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const floatx4 x = w[u] == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : o[u];  // (the first slot's may be anything)
+      den += w[u];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(x[e], w[u], acc[e]);
+    }
+  }
+  acc_lds[q][i] = acc;
+  if (i == 0) den_lds[q] = den;
+  __syncthreads();
+  if (q != 0) return;
+#pragma unroll
+  for (int x = 1; x < NG; ++x) {
+    acc += acc_lds[x][i];
+    den += den_lds[x];
+  }
+  acc = acc * (1.0f / den);
+  *reinterpret_cast<uint2*>(out) = uint2{pack2(acc[0], acc[1]), pack2(acc[2], acc[3])};
+  if (tid == 0 && blockIdx.z == 0) a.lse[(int64_t)h * a.T + t] = (top * kLog2e + log2f(den)) * kLn2;
+}
+
+template <int W>
+void launch_join(const CompactParams& p, hipStream_t st) {
+  // many slots come with few tokens: more groups, and more workgroups a head (1 token, 512 slots: 21.7 us for the call, 39.6
+  // with two workgroups a head; with few slots these are too many: 16 tokens of 32 slots 21.1, this way 22.8)
+  constexpr int L = W >= 256 ? 64 : 32;
+  if (p.num_splits >= 64)
+    hipLaunchKernelGGL((compact_join_kernel<W, 16, 16, 8>), dim3((unsigned)p.T, kHeads, W / 64), dim3(256), 0, st, p);
+  else
+    hipLaunchKernelGGL((compact_join_kernel<W, L, 256 / L, 4>), dim3((unsigned)p.T, kHeads, W / (4 * L)), dim3(256), 0, st, p);
+}
+
 template <int W>
 void launch_history(const CompactParams& p, int tokens_per_group, bool shared_rows, hipStream_t st) {
   if constexpr (W >= 256) {
@@ -735,8 +813,8 @@ void launch_history(const CompactParams& p, int tokens_per_group, bool shared_ro
     }
   }
   const dim3 grid(split_workgroups(p.T, p.num_splits));
-  // rows that one token reads stream past the caches from W = 512 on (64 rows of 8160: 68.8 -> 60.6 us, 8 of 32736: 41.8 ->
-  // 37.6); at 256 and below, where a lane's V pieces are shorter than a cached line's share, not (32 rows of up to 8160 at
+  // rows that one token reads stream past the caches from W = 512 on (64 rows of 8160: 68.5 -> 60.5 us, 8 of 32736: 41.9 ->
+  // 37.0); at 256 and below, where a lane's V pieces are shorter than a cached line's share, not (32 rows of up to 8160 at
   // 256: 20.0 -> 20.6)
   if (W >= 512 && !shared_rows)
     hipLaunchKernelGGL((compact_history_kernel<W, (W >= 512)>), grid, dim3(256), 0, st, p);
@@ -896,14 +974,25 @@ extern "C" int hla_s6_compact_history(const void* q, int32_t num_tokens, int32_t
     p.lse = lse;
   }
   const hipStream_t st = as_stream(stream);
-  switch (width) {
-    case 128: launch_history<128>(p, tokens_per_group, shared_rows != 0, st); break;
-    case 256: launch_history<256>(p, tokens_per_group, shared_rows != 0, st); break;
-    case 512: launch_history<512>(p, tokens_per_group, shared_rows != 0, st); break;
-    default: launch_history<1024>(p, tokens_per_group, shared_rows != 0, st); break;
+#define HLA_EACH_WIDTH(call)     \
+  switch (width) {               \
+    case 128: call(128); break;  \
+    case 256: call(256); break;  \
+    case 512: call(512); break;  \
+    default: call(1024); break;  \
   }
+#define HLA_HISTORY(W) launch_history<W>(p, tokens_per_group, shared_rows != 0, st)
+#define HLA_JOIN(W) launch_join<W>(p, st)
+  HLA_EACH_WIDTH(HLA_HISTORY)
   rc = check_launch("compact_history");
   if (rc != HLA_S6_OK || !out || !partials) return rc;
-  return hla_s6_history_reduce(workspace, workspace_floats, num_tokens, num_heads, width, num_splits, out, o_st, o_sh,
-                               lse, stream);
+  p.out = static_cast<uint16_t*>(out);
+  p.o_st = o_st;
+  p.o_sh = o_sh;
+  p.lse = lse;
+  HLA_EACH_WIDTH(HLA_JOIN)
+#undef HLA_JOIN
+#undef HLA_HISTORY
+#undef HLA_EACH_WIDTH
+  return check_launch("compact_history");
 }

@@ -59,6 +59,7 @@ def test_split_counts(cc):
     assert cc.kv_splits(128, 64, 256, 512) == 1
     assert cc.kv_splits(992, 1, 256, 512) == 32             # a small step: two slots per 64 keys
     assert cc.kv_splits(10 ** 6, 1, 256, 256) == 512
+    assert cc.kv_splits(8160, 8, 256, 512) == 32 and cc.kv_splits(8160, 8, 256, 1024) == 64 and cc.kv_splits(8160, 1, 256, 512) == 128
     assert cc.kv_splits(8160, 4096, 256, 512) == 1 and cc.kv_splits(8160, 100, 256, 512) == 4
 
 

@@ -208,8 +208,8 @@ def test_history_per_request_tables_plans_and_strides(cc, ops):
         want = (o, lse) if want is None else want
         assert torch.equal(o, want[0]) and torch.equal(lse, want[1])   # a plan changes who does the work, not the sums
     parts = cc.history_partials(q, cache, table, c, SCALE, 6, ws, token_requests=dev_i64(req))
-    o, lse = ops.history_reduce(parts)
-    assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
+    o, lse = ops.history_reduce(parts)   # the bf16 cache's reduction: the same slots, another order
+    check_attention(host_f32(o), host_f32(lse), bf16.to_f32(wide)[:, 1:17, 8:], lambda t: p.rows(req[t]), ctx)
 
 
 @pytest.mark.parametrize('width', [128, 256, 512, 1024])
@@ -264,6 +264,34 @@ def test_rows_expanded_once(cc, monkeypatch):
     o, lse = cc.history_attention(dev_bf16(q), dev_u8(p.cache), dev_i32(p.table), dev_i32(ctx), SCALE, 210,
                                   token_requests=dev_i64(req), query_start_loc=dev_i32(start), max_query_len=30)
     check_attention(host_f32(o), host_f32(lse), bf16.to_f32(q), lambda t: p.rows(req[t]), ctx)
+
+
+@pytest.mark.parametrize('shape', [(1, 2), (2, 1), (2, 3), (3, 1)])
+def test_captured_chunks(cc, monkeypatch, shape):
+    """Every form of a chunk step in a graph: replays with new queries and lengths, eager work between them, equal the eager
+    results bit for bit."""
+    monkeypatch.setattr(cc, 'history_shape', lambda *a: shape)
+    rng = np.random.default_rng(31)
+    n, chunk = [130, 60], [7, 6]
+    p = Pool(rng, n, 512, 16)
+    req = np.repeat([0, 1], chunk)
+    q, ctx = dev_bf16(random_bits(rng, (13, 16, 512), 0.5)), dev_i32(np.array(n)[req])
+    cache, table, start, treq = dev_u8(p.cache), dev_i32(p.table), dev_i32([0, 7, 13]), dev_i64(req)
+    call = lambda: cc.history_attention(q, cache, table, ctx, SCALE, 130, token_requests=treq, query_start_loc=start, max_query_len=7)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o, lse = call()
+    for turn in range(3):
+        q.copy_(dev_bf16(random_bits(rng, (13, 16, 512), 0.5)))
+        ctx.copy_(dev_i32(np.maximum(np.array(n)[req] - 9 * turn, 0)))
+        o.fill_(float('nan'))
+        graph.replay()
+        want, want_lse = call()
+        torch.cuda.synchronize()
+        assert torch.equal(o, want) and torch.equal(lse, want_lse)
+    check_attention(host_f32(o), host_f32(lse), host_f32(q), lambda t: p.rows(req[t]), ctx.cpu().numpy())
 
 
 @pytest.mark.parametrize('width,n', [(256, 60), (512, 4200), (1024, 40)])
