@@ -137,8 +137,10 @@ __global__ __launch_bounds__(256) void compact_load_kernel(LoadParams a) {
 //   * O^T[columns x 16 heads] += V^T P^T: a lane loads the same 8 keys' values of W / 16 consecutive columns (one scale
 //     per key and 32 columns); two keys' values of a column are joined by one v_perm_b32 per pair. Product c of a wave
 //     takes column c of every lane's range.
-// No value passes through LDS until the waves' partials are joined at the end. At W = 1024 two waves share 32 keys, each
-// with all of K and half of the columns of V.
+// No row passes through LDS (from W = 512 on the query does) until the waves' partials are joined at the end. At W = 1024 two
+// waves share 32 keys, each with all of K and half of the columns of V.
+// Bound by HBM where a row is read once: 64 rows of 8160 at W = 512 50 us, 5.7 TB/s with a fixed part of about 11 us (launch,
+// work list, page ids and query, first rows, join); by the conversions (8 clocks a pair of values) where rows come out of L2.
 struct CompactParams {
   const uint16_t* q;
   int64_t q_st, q_sh;

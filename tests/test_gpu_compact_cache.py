@@ -166,7 +166,21 @@ def test_history_attention(cc, width, block, splits):
     check_attention(host_f32(o), host_f32(lse), bf16.to_f32(q), p.rows, ctx)
 
 
-@pytest.mark.parametrize('splits', [1, 4])
+@pytest.mark.parametrize('splits', [2, 31, 64, 1024])
+@pytest.mark.parametrize('width', [128, 256, 512, 1024])
+def test_reduction_over_slots(cc, width, splits):
+    """Few and many slots, most of them without rows; a row without any; a strided order of tokens in the table."""
+    rng = np.random.default_rng(width + splits)
+    ctx = [1700, 0, 33, 64]
+    p = Pool(rng, ctx, width, 16)
+    q = random_bits(rng, (4, 16, width), 1.4 * math.sqrt(128 / width))
+    order = np.array([2, 0, 3, 1])
+    o, lse = cc.history_attention(dev_bf16(q), dev_u8(p.cache), dev_i32(p.table), dev_i32(np.array(ctx)[order]), SCALE, 1700,
+                                  token_requests=dev_i64(order), num_kv_splits=splits)
+    check_attention(host_f32(o), host_f32(lse), bf16.to_f32(q), lambda t: p.rows(order[t]), np.array(ctx)[order])
+
+
+@pytest.mark.parametrize('splits', [1, 4, 100])
 def test_rows_that_read_as_nan(cc, splits):
     """A NaN among a request's rows makes its output and lse NaN, in one slot or in every one, and no other request's."""
     rng = np.random.default_rng(21)
