@@ -687,7 +687,11 @@ struct MovePieces {
     for (int s = 0; s < STEPS; ++s) {
       uint8_t* p = address(cache, lo, hi, kMoveRows + first, s, lane);
       const int item = s * 64 + lane;
-      if (item < ITEMS && ((valid >> (first + item / kPer)) & 1)) *reinterpret_cast<T*>(p) = v[s];
+      if (item < ITEMS && ((valid >> (first + item / kPer)) & 1)) {
+        // rows past the caches; scales, many rows' to a line, through them
+        if constexpr (kBytes == 16) __builtin_nontemporal_store(v[s], reinterpret_cast<T*>(p));
+        else *reinterpret_cast<T*>(p) = v[s];
+      }
     }
   }
 };
@@ -708,9 +712,9 @@ struct AtRow {  // bf16
 };
 
 // One wave takes 16 moves. Its lanes first work out where the 16 sources and 16 targets begin, together, and then hand these
-// places to the lanes that move the pieces. 121,000 rows of 544 bytes (160 MB of traffic with the lines that are used in
-// part) take 39 us, 4.1 TB/s; with the divisions by the page size in every thread 84, with one row and its scales, byte by
-// byte, per instruction 50 (its values alone 34).
+// places to the lanes that move the pieces. 121,000 rows of 544 bytes (their pieces fill half of many lines: 200 MB in pieces of 64
+// bytes, both ways) out of a cold cache take 40 us, 5.0 TB/s; 49 with ordinary stores, 41 with those of the scales past the
+// caches too. 30,000 bf16 rows of 1 KB: 12.5, and 17.6 with ordinary ones.
 template <int W, bool kCompact>
 __global__ __launch_bounds__(256) void move_rows_kernel(MoveParams a) {
   const int r = blockIdx.y, lane = threadIdx.x & 63;
