@@ -327,13 +327,15 @@ def _expanded_attention(q, cache, geometry, block_table, ctx, scale, longest, to
 
 
 def history_partials(q_lat, cache, block_table, ctx, scale, num_kv_splits, workspace, token_requests=None, plan=None,
-                     query_start_loc=None, max_query_len=1):
+                     query_start_loc=None, max_query_len=1, max_seq_len=None):
     """The split kernel of ``history_attention`` alone: its partials in ``workspace``, in the layout that
-    ``s6_ops.history_reduce`` and ``s6_ops.split_epilogue`` read (``[T, 16, splits, w + 1]``, private)."""
+    ``s6_ops.history_reduce`` and ``s6_ops.split_epilogue`` read (``[T, 16, splits, w + 1]``, private). ``max_seq_len``
+    defaults to the rows that a row of the table holds."""
     T, w, geometry, table, ctx, token_requests = _operands(q_lat, cache, block_table, ctx, token_requests, plan)
     if workspace is None:
         raise RuntimeError('history partials need an S6Workspace')
-    kind, _ = _shape(q_lat, table, table[1] * geometry[2], token_requests, query_start_loc, max_query_len, plan)
+    longest = table[1] * geometry[2] if max_seq_len is None else int(max_seq_len)
+    kind, _ = _shape(q_lat, table, longest, token_requests, query_start_loc, max_query_len, plan)
     _, ws = _history(q_lat, cache, geometry, block_table, table, ctx, scale, token_requests, int(num_kv_splits), workspace,
                      plan, min(kind, 2), max_query_len > 1, None)
     return ws

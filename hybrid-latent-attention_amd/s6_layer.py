@@ -81,6 +81,9 @@ class StepContext:
     constants only (``max_query_len`` picks the kernel family, as ``history_group`` always has), so a graph captured
     for a batch size replays the counts it was captured with; a split count changes only the order of the fp32
     sums. ``kv_splits_by_width`` overrides the counts per width (the workspace must hold the largest of them).
+
+    ``ctx_latent`` may be assigned, or written by torch operations, between layers (caches that rows were evicted from hold
+    different numbers of them): what was worked out of the former lengths is worked out again.
     """
 
     def __init__(self, positions, query_start_loc, seq_lens, max_query_len, num_tokens, tables, scale, backends,
@@ -112,7 +115,8 @@ class StepContext:
         self.valid = torch.empty(num_tokens, dtype=torch.bool, device=device)
         self.invalid = torch.empty(num_tokens, dtype=torch.bool, device=device)
         self.ctx = torch.empty(num_tokens, dtype=torch.int32, device=device)
-        self.ctx_latent = torch.empty(num_tokens, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):   # (a tensor that counts its changes)
+            self.ctx_latent = torch.empty(num_tokens, dtype=torch.int32, device=device)
         _lib.call('hla_s6_step_metadata', _lib.ptr(qsl), R, _lib.ptr(seq), num_tokens, int(window or 0),
                   _lib.ptr(self.token_requests), _lib.ptr(self.valid), _lib.ptr(self.invalid), _lib.ptr(self.ctx),
                   _lib.ptr(self.ctx_latent), None, _lib.stream(device))
@@ -146,8 +150,26 @@ class StepContext:
         return self._empty
 
     @property
+    def ctx_latent(self):
+        """Latent rows of every token (int32 ``[num_tokens]``)."""
+        return self._ctx_latent
+
+    @ctx_latent.setter
+    def ctx_latent(self, lengths):
+        self._ctx_latent, self._lengths_seen = lengths, None
+
+    def _check_lengths(self):
+        """Drops what was worked out of other latent lengths than those of now (of a tensor made under inference mode, whose
+        changes in place nothing counts, always)."""
+        lengths = self._ctx_latent
+        version = None if lengths.is_inference() else lengths._version
+        if version is None or version != self._lengths_seen:
+            self._plans, self._empty_latent, self._lengths_seen = {}, None, version
+
+    @property
     def empty_latent(self):
         """Tokens without latent history (``ctx_latent == 0``), computed on first use."""
+        self._check_lengths()
         if self._empty_latent is None:
             self._empty_latent = self.ctx_latent == 0
         return self._empty_latent
@@ -161,6 +183,7 @@ class StepContext:
         ``cap`` addressable rows, read by every layer. The first request of a step makes, in the same launch, the
         plans of the other latent widths' slot counts for the same ``cap`` (``hla_s6_split_plans``: the widths'
         tables address the same pages), so a step computes its plans with one launch."""
+        self._check_lengths()
         key = (int(splits), int(cap))
         if key not in self._plans:
             qsl = self.query_start_loc if self.max_query_len > 1 else None   # short chunks share rows
@@ -275,7 +298,7 @@ def _attend_composed(q_lat, o_chunk, lse_chunk, B, cache, block_table, ctx, weig
         T, rows = q_lat.shape[0], block_table.shape[1] * compact_cache.block_size(cache)
         longest = min(int(ctx.max_seqlen_k), rows) if ctx.max_seqlen_k else rows
         requests = T if ctx.max_query_len == 1 else ctx.query_start_loc.shape[0] - 1
-        kind, splits = compact_cache.history_shape(longest, T, requests, _lib.device_cus(q_lat.device.index or 0), w)
+        splits = compact_cache.history_shape(longest, T, requests, _lib.device_cus(q_lat.device.index or 0), w)[1]
         workspace = ctx.workspace
         if workspace is not None and T * q_lat.shape[1] * splits * (w + 1) > workspace.floats:
             workspace = None
@@ -283,8 +306,7 @@ def _attend_composed(q_lat, o_chunk, lse_chunk, B, cache, block_table, ctx, weig
             if workspace is None:
                 workspace = s6_ops.S6Workspace(q_lat.shape[1], w, T * splits)
             ws = compact_cache.history_partials(q_lat, cache, block_table, ctx.ctx_latent, ctx.scale, splits, workspace,
-                                                ctx.token_requests, ctx.split_plan(splits, rows) if kind == 1 else None,
-                                                ctx.query_start_loc, ctx.max_query_len)
+                                                ctx.token_requests, None, ctx.query_start_loc, ctx.max_query_len, longest)
             return s6_ops.split_epilogue(ws, B, o_chunk, lse_chunk, ctx.invalid)
         o_hist, lse_hist = compact_cache.history_attention(
             q_lat, cache, block_table, ctx.ctx_latent, ctx.scale, longest, ctx.token_requests, ctx.query_start_loc,
