@@ -94,6 +94,7 @@ __global__ void merge_kernel(const uint16_t* oa, int64_t a_st, int64_t a_sh, con
   uint16_t* op = out + (int64_t)t * o_st + (int64_t)h * o_sh + c;
   if (mode == 0 && invalid && invalid[t]) {
     st16(op, u32x4{0u, 0u, 0u, 0u});
+    if (lse_out && c == 0) lse_out[(int64_t)h * T + t] = -INFINITY;
     return;
   }
   const u32x4 va = ld16(oa + (int64_t)t * a_st + (int64_t)h * a_sh + c);
@@ -111,7 +112,7 @@ __global__ void merge_kernel(const uint16_t* oa, int64_t a_st, int64_t a_sh, con
     r[e] = pack2(a0 * wa + b0 * wb, a1 * wa + b1 * wb);
   }
   st16(op, r);
-  if (mode == 1 && lse_out && c == 0) lse_out[(int64_t)h * T + t] = peak + logf(total);
+  if (lse_out && c == 0) lse_out[(int64_t)h * T + t] = peak + logf(total);
 }
 
 // ---- a10: slot mapping and row store --------------------------------------------------------------
@@ -201,7 +202,6 @@ extern "C" int hla_s6_merge_states(const void* o_a, int64_t a_st, int64_t a_sh, 
                                    int32_t num_tokens, int32_t num_heads, int32_t head_dim, int32_t mode, void* out,
                                    int64_t o_st, int64_t o_sh, float* lse_out, void* stream) {
   HLA_REQUIRE(mode == 0 || mode == 1, HLA_S6_EINVAL, "merge_states: mode must be 0 or 1");
-  HLA_REQUIRE(mode == 1 || lse_out == nullptr, HLA_S6_EINVAL, "merge_states: lse_out is only written by mode 1");
   HLA_REQUIRE(num_tokens >= 0 && num_heads >= 1 && head_dim > 0 && head_dim % 8 == 0, HLA_S6_EUNSUPPORTED,
               "merge_states: head_dim must be a multiple of 8");
   if (num_tokens == 0) return HLA_S6_OK;

@@ -319,9 +319,9 @@ def _attend_composed(q_lat, o_chunk, lse_chunk, B, cache, block_table, ctx, weig
     o_hist = absorb_out(o_hist, B)
     if weights is None:
         return s6_ops.merge_states(o_hist, lse_hist, o_chunk, lse_chunk, ctx.invalid, ctx.backends.merge)
-    out, lse = s6_ops.merge_lse(o_hist, lse_hist, o_chunk, lse_chunk)
+    out, lse = s6_ops.merge_states(o_hist, lse_hist, o_chunk, lse_chunk, ctx.invalid, ctx.backends.merge, return_lse=True)
     compact_cache.attention_weights(q_lat, cache, block_table, ctx.query_start_loc, ctx.ctx_latent, lse, ctx.scale, weights)
-    return out.masked_fill_(ctx.invalid[:, None, None], 0)
+    return out
 
 
 def _attend_decode(sl, loop, q_lat, q_rope, cache, block_table, ctx, window):

@@ -462,10 +462,11 @@ def chunk_window_attention(q, k, v, query_start_loc, seq_lens, cache, block_tabl
     return o, lse
 
 
-def merge_states(o_hist, lse_hist, o_chunk, lse_chunk, invalid, backend):
+def merge_states(o_hist, lse_hist, o_chunk, lse_chunk, invalid, backend, return_lse=False):
     """LSE merge of two partial softmaxes; ``[T,H,D]`` outputs, ``[H,T]`` fp32 lse; ``invalid`` rows are zeroed.
 
-    ``+inf`` lse counts as empty (the FA2 empty-key convention); both sides empty give 0.
+    ``+inf`` lse counts as empty (the FA2 empty-key convention); both sides empty give 0. With ``return_lse`` the merged lse
+    too (``[H,T]``, -inf for ``invalid`` rows); NaN passes into output and lse, where ``merge_lse`` takes it for scratch rows.
     """
     _backend('merge', backend)
     _dev(o_hist, lse_hist, o_chunk, lse_chunk)
@@ -473,11 +474,12 @@ def merge_states(o_hist, lse_hist, o_chunk, lse_chunk, invalid, backend):
     _bf16('o_chunk', o_chunk)
     T, H, D = o_chunk.shape
     out = torch.empty(T, H, D, dtype=BF16, device=o_chunk.device)
+    lse = torch.empty(H, T, dtype=torch.float32, device=o_chunk.device) if return_lse else None
     lh, lc = lse_hist.float().contiguous(), lse_chunk.float().contiguous()
     _lib.call('hla_s6_merge_states', _lib.ptr(o_hist), o_hist.stride(0), o_hist.stride(1), _lib.ptr(lh),
               _lib.ptr(o_chunk), o_chunk.stride(0), o_chunk.stride(1), _lib.ptr(lc), _lib.ptr(_mask(invalid)), T, H, D,
-              0, _lib.ptr(out), out.stride(0), out.stride(1), None, _lib.stream(out.device))
-    return out
+              0, _lib.ptr(out), out.stride(0), out.stride(1), _lib.ptr(lse), _lib.stream(out.device))
+    return (out, lse) if return_lse else out
 
 
 def merge_lse(o1, lse1, o2, lse2):

@@ -24,7 +24,7 @@
 extern "C" {
 #endif
 
-#define HLA_S6_ABI_VERSION 15
+#define HLA_S6_ABI_VERSION 16
 
 #define HLA_S6_OK 0
 #define HLA_S6_EINVAL 1       /* bad shape, stride or argument            (Python: ValueError)   */
@@ -207,9 +207,9 @@ int hla_s6_chunk_window_attention(const void *q, const void *k, const void *v, i
 
 /* ---- a8: LSE merge of two partial attentions -----------------------------------------------------
  * mode 0 replaces s6_ops.merge_states (hla/vllm_latent/s6_ops.py:262-284): +inf lse counts as empty,
- *   both empty -> 0, rows with invalid[t] != 0 -> 0 (invalid nullable); lse_out must be NULL.
- * mode 1 replaces s6_ops.merge_lse (hla/vllm_latent/s6_ops.py:353-361): NaN inputs become 0, the merged
- *   lse = peak + log(w_a + w_b) is written to lse_out ([H, T] fp32, nullable).
+ *   both empty -> 0, rows with invalid[t] != 0 -> 0 (invalid nullable), their lse -inf.
+ * mode 1 replaces s6_ops.merge_lse (hla/vllm_latent/s6_ops.py:353-361): NaN inputs become 0.
+ * Both modes write the merged lse = peak + log(w_a + w_b) to lse_out ([H, T] fp32, nullable).
  * head_dim % 8 == 0; o tensors need a unit last stride. */
 int hla_s6_merge_states(const void *o_a, int64_t a_st, int64_t a_sh, const float *lse_a, const void *o_b,
                         int64_t b_st, int64_t b_sh, const float *lse_b, const uint8_t *invalid,

@@ -74,3 +74,70 @@ def test_lengths_may_change_within_a_step(pkg, ops, w, chunk, compact):
         fresh = x.step()
         fresh.ctx_latent.copy_(lengths)
         assert torch.equal(x.attend(cache, ctx), x.attend(cache, fresh)), turn
+
+
+# ---- rows that read as NaN ------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize('where', ['key', 'value'])
+@pytest.mark.parametrize('chunk,shape', [(1, None), (3, None), (20, None), (20, (1, 1)), (20, (2, 1)), (20, (2, 3))])
+def test_attend_passes_nan_on(cc, pkg, ops, monkeypatch, chunk, shape, where):
+    """A NaN in a request's latent rows makes its output NaN, with an account and without, and no other's. A NaN key makes the
+    request's account NaN as well; with a NaN value the weights are what they were."""
+    rng = np.random.default_rng(chunk)
+    if shape:
+        monkeypatch.setattr(cc, 'history_shape', lambda *a: shape)
+    contexts, w, block = [300, 200, 90], 512, 16
+    x = Layer(pkg, ops, rng, contexts, chunk, w, block)
+    M = 300 + chunk
+    clean_account = torch.zeros(3, M, device='cuda')
+    clean = x.attend(x.compact, x.step(), weights=clean_account)
+    rows = x.pool.rows(1)[[77]]
+    rows[0, 40 if where == 'key' else w + 40] = np.nan
+    C.store(x.pool.cache, rows[:, :w], rows[:, w:], C.slots_of(x.pool.table[1], block, 78)[[77]])
+    account = torch.zeros(3, M, device='cuda')
+    bad = slice(chunk, 2 * chunk)
+    for out in (x.attend(x.compact, x.step(), weights=account), x.attend(x.compact, x.step())):
+        assert torch.isnan(out[bad]).all()
+        for good in (slice(0, chunk), slice(2 * chunk, 3 * chunk)):
+            assert (out[good].float() - clean[good].float()).abs().max() <= 4 * HALF * clean.float().abs().max()
+    assert torch.equal(account[[0, 2]], clean_account[[0, 2]])
+    behind = contexts[1] - 32
+    assert (account[1, behind:] == 0).all()
+    if where == 'key':
+        assert torch.isnan(account[1, :behind]).all()
+    else:
+        assert torch.equal(account[1], clean_account[1])
+
+
+def test_merged_lse(ops):
+    """merge_states with its lse: empty sides (-inf, and +inf as the window kernels of others mark them), both, rows of padding,
+    NaN. Bounds: an output rounds to bf16 once (half a step: 2^-8) over fp32 weights (2^-20)."""
+    rng = np.random.default_rng(6)
+    T, H, D = 9, 16, 128
+    a, b = (random_bits(rng, (T, H, D)) for _ in range(2))
+    la, lb = (rng.standard_normal((H, T)).astype(np.float32) * 3 for _ in range(2))
+    la[:, 1], lb[:, 2], la[:, 3], lb[:, 4], la[:, 5], lb[:, 5] = -np.inf, -np.inf, np.inf, np.inf, -np.inf, np.inf
+    a[5], b[5] = 0, 0
+    la[:, 6], a[6] = np.nan, bf16.from_f32(np.full((H, D), np.nan, np.float32))
+    invalid = np.arange(T) == 8
+    out, lse = ops.merge_states(dev_bf16(a), torch.from_numpy(la).cuda(), dev_bf16(b), torch.from_numpy(lb).cuda(),
+                                torch.from_numpy(invalid).cuda(), 'hip', return_lse=True)
+    plain = ops.merge_states(dev_bf16(a), torch.from_numpy(la).cuda(), dev_bf16(b), torch.from_numpy(lb).cuda(),
+                             torch.from_numpy(invalid).cuda(), 'hip')
+    assert torch.equal(out.view(torch.int16), plain.view(torch.int16))
+    assert torch.isnan(out[6]).all() and torch.isnan(lse[:, 6]).all()
+    for t in (0, 1, 2, 3, 4, 5, 7, 8):
+        x, y = (np.where(np.isinf(l[:, t]) | invalid[t], -np.inf, l[:, t]).astype(np.float64) for l in (la, lb))
+        top = np.maximum(np.maximum(x, y), -1e30)
+        p, r = np.exp(x - top), np.exp(y - top)
+        total = p + r
+        with np.errstate(divide='ignore'):
+            want_lse = np.where(total > 0, top + np.log(total), -np.inf)
+        total = np.maximum(total, 1e-300)
+        want = (p / total)[:, None] * bf16.to_f32(a[t]) + (r / total)[:, None] * bf16.to_f32(b[t])
+        size = (p / total)[:, None] * np.abs(bf16.to_f32(a[t])) + (r / total)[:, None] * np.abs(bf16.to_f32(b[t]))
+        assert (np.abs(host_f32(out[t]) - want) <= HALF * np.abs(want) + 2.0 ** -20 * size).all(), t
+        got = lse[:, t].cpu().numpy()
+        assert (np.isneginf(got) == np.isneginf(want_lse)).all(), t
+        fine = np.isfinite(want_lse)
+        assert (np.abs(got[fine] - want_lse[fine]) <= 2.0 ** -20 * (1 + np.abs(want_lse[fine]))).all(), t
