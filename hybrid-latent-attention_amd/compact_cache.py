@@ -294,7 +294,8 @@ def history_attention(q_lat, cache, block_table, ctx, scale, max_seq_len, token_
     if num_kv_splits is not None:
         splits = int(num_kv_splits)
     longest = min(max_seq_len, table[1] * geometry[2])
-    if kind == 3 and splits == 1 and query_start_loc is not None and longest > 0:
+    # (its kernel folds a positive scale)
+    if kind == 3 and splits == 1 and query_start_loc is not None and longest > 0 and scale > 0:
         with torch.cuda.device(q_lat.device):
             return _expanded_attention(q_lat, cache, geometry, block_table, ctx, scale, longest, token_requests,
                                        query_start_loc)
@@ -323,7 +324,8 @@ def _expanded_attention(q, cache, geometry, block_table, ctx, scale, longest, to
     _load(cache, geometry, block_table, None, qsl, ctx, T, R, pages * TILE, rows.view(R, pages * TILE, 2 * w))
     table = torch.arange(R * pages, dtype=I32, device=q.device).view(R, pages)
     return s6_ops.history_attention_kv(q, rows[..., :w], rows[..., w:], table, ctx, scale, 1, None, None, None, s6_ops.HIP,
-                                       bt_rows=token_requests.clamp(0, R - 1), tokens_per_group=4, shared_rows=True)
+                                       bt_rows=token_requests.clamp(0, R - 1), tokens_per_group=4, shared_rows=True,
+                                       nan_rows=True)
 
 
 def history_partials(q_lat, cache, block_table, ctx, scale, num_kv_splits, workspace, token_requests=None, plan=None,

@@ -92,6 +92,7 @@ struct HistoryParams {
   int tok_per_row;
   int keys;
   int64_t kv_sb;
+  bool nan_rows;   // history_mq5, paged rows: see there
   float raise_by;  // history_mq5: log2 units that a score may exceed the running maximum by before it is raised
   const uint8_t* mask;
   int64_t mask_st, mask_sb;
@@ -1012,6 +1013,10 @@ constexpr int kKhop1024Tokens = 2;      // tokens per workgroup of the 1024-wide
 // waited for explicitly (s_waitcnt vmcnt counting the copies issued after the awaited ones) and the loop
 // synchronizes with plain s_barrier behind those waits, so a copy still in flight for a later tile is never waited
 // for at a barrier.
+// Rows are taken to be finite: a token whose sum is NaN comes out as one without rows (lse -inf), and a NaN in a row of V
+// that only the longer ones of a pass's tokens see reaches the others as 0 * NaN. With nan_rows (compact rows, whose
+// blocks read as NaN where they held a value that was not finite) a NaN sum gives a NaN lse, and the tokens of a pass have
+// equal lengths, as those of a chunk do.
 //   R = 512: 8 waves of 1 token (the registers hold 16 query rows x 512 columns), 139 KB of LDS;
 //   R = 256: 74 KB of LDS; 4 waves of 2 tokens when the grid has more workgroups than CUs (two workgroups per CU,
 //   whose tiles run out of step), else 8 waves of 1 token (one workgroup per CU at two waves per SIMD instead of
@@ -1051,7 +1056,7 @@ __global__ __launch_bounds__((64 * Mq5Geo<R, kTpw>::NW), R == 256 ? 2 : 1) void 
   for (int tp = t_begin; tp < t_end;) {  // passes: runs of tokens that share a table row
     const int64_t row = table_row(a, tp);
     int te = tp + 1;
-    while (te < t_end && table_row(a, te) == row) ++te;
+    while (te < t_end && table_row(a, te) == row && (kContig || !a.nan_rows || a.ctx[te] == a.ctx[tp])) ++te;
     const int count = te - tp;
     int n_max = 0, n_tok[TPW];
 #pragma unroll
@@ -1255,7 +1260,7 @@ __global__ __launch_bounds__((64 * Mq5Geo<R, kTpw>::NW), R == 256 ? 2 : 1) void 
     for (int x = 0; x < TPW; ++x) {
       if (TPW * wave + x >= count) continue;
       const int t = tp + TPW * wave + x, h = l16;  // lane holds O^T[col 16cb + 4g + r][head l16] of token t
-      const bool any = l_own[x] > 0.f;
+      const bool any = !kContig && a.nan_rows ? l_own[x] != 0.f : l_own[x] > 0.f;
       const float inv = any ? 1.0f / l_own[x] : 0.f;
 #pragma unroll
       for (int cb = 0; cb < CB; ++cb) {
@@ -1906,8 +1911,11 @@ extern "C" int hla_s6_history_attention_grouped(
                         block_size, num_blocks, block_table, bt_stride, bt_cols, bt_rows, ctx, scale, num_splits,
                         workspace, workspace_floats, out, o_st, o_sh, lse);
   if (rc != HLA_S6_OK || num_tokens == 0) return rc;
+  HLA_REQUIRE(shared_rows != 2 || (group == 4 && num_splits == 1 && (width == 256 || width == 512) && scale > 0.f),
+              HLA_S6_EUNSUPPORTED, "history_attention: rows with NaN need groups of 4, one split, width 256 or 512, scale > 0");
   p.group = group;
   p.shared_rows = shared_rows != 0 || group > 1;
+  p.nan_rows = shared_rows == 2;
   return dispatch(p, width, as_stream(stream));
 }
 

@@ -111,7 +111,8 @@ int hla_s6_history_attention(const void *q, int32_t num_tokens, int32_t num_head
  * of them; a group spanning two rows takes one pass per row. Each token still sees its own ctx[t] rows. Same
  * arguments, outputs and checks as hla_s6_history_attention. shared_rows != 0 declares that several tokens read the
  * same rows (any multi-query step, also with group == 1): K/V loads are then cached for the re-reads instead of
- * non-temporal. */
+ * non-temporal. shared_rows == 2 (group 4, one split, width 256 or 512, scale > 0 only): the rows may hold NaN; a token with
+ * a NaN score gets lse = NaN (otherwise -inf), and a NaN reaches only tokens whose ctx[t] rows hold it. */
 int hla_s6_history_attention_grouped(const void *q, int32_t num_tokens, int32_t num_heads, int32_t width,
                                      int64_t q_st, int64_t q_sh, const void *k_cache, const void *v_cache,
                                      int64_t page_stride, int64_t row_stride, int32_t block_size, int64_t num_blocks,

@@ -79,7 +79,7 @@ def test_lengths_may_change_within_a_step(pkg, ops, w, chunk, compact):
 # ---- rows that read as NaN ------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize('where', ['key', 'value'])
-@pytest.mark.parametrize('chunk,shape', [(1, None), (3, None), (20, None), (20, (1, 1)), (20, (2, 1)), (20, (2, 3))])
+@pytest.mark.parametrize('chunk,shape', [(1, None), (3, None), (20, None), (20, (1, 1)), (20, (2, 1)), (20, (2, 3)), (20, (3, 1))])
 def test_attend_passes_nan_on(cc, pkg, ops, monkeypatch, chunk, shape, where):
     """A NaN in a request's latent rows makes its output NaN, with an account and without, and no other's. A NaN key makes the
     request's account NaN as well; with a NaN value the weights are what they were."""
@@ -141,3 +141,57 @@ def test_merged_lse(ops):
         assert (np.isneginf(got) == np.isneginf(want_lse)).all(), t
         fine = np.isfinite(want_lse)
         assert (np.abs(got[fine] - want_lse[fine]) <= 2.0 ** -20 * (1 + np.abs(want_lse[fine]))).all(), t
+
+
+@pytest.mark.parametrize('shape', [(1, 1), (1, 3), (2, 1), (2, 3), (3, 1)])
+def test_nan_rows_reach_the_tokens_that_see_them(cc, monkeypatch, shape):
+    """Every form of a chunk: NaN outputs and lse for tokens whose rows hold one, and neighbours of the same request whose rows
+    end before it are exact."""
+    monkeypatch.setattr(cc, 'history_shape', lambda *a: shape)
+    rng = np.random.default_rng(77)
+    n, chunk, w = [300, 130], [19, 14], 512
+    p = Pool(rng, n, w, 16)
+    req = np.repeat([0, 1], chunk)
+    ctx = np.array(n)[req]
+    ctx[[0, 3, 4, 9, 18]] = 150, 149, 7, 0, 64
+    clean = {0: p.rows(0), 1: p.rows(1)}
+    for part in (0, 1):
+        rows = clean[0][[150 + part]].copy()
+        rows[0, part * w:(part + 1) * w] = np.nan     # a key, and behind it a value
+        C.store(p.cache, rows[:, :w], rows[:, w:], C.slots_of(p.table[0], 16, 300)[[150 + part]])
+    q = random_bits(rng, (len(req), 16, w), 0.5)
+    start = dev_i32(np.concatenate(([0], np.cumsum(chunk))))
+    o, lse = cc.history_attention(dev_bf16(q), dev_u8(p.cache), dev_i32(p.table), dev_i32(ctx), SCALE, 300,
+                                  token_requests=dev_i64(req), query_start_loc=start, max_query_len=19)
+    bad = (req == 0) & (ctx > 150)
+    assert torch.isnan(o[torch.from_numpy(bad)]).all() and torch.isnan(lse[:, torch.from_numpy(bad)]).all()
+    keep = np.flatnonzero(~bad)
+    check_attention(host_f32(o)[keep], host_f32(lse)[:, keep], bf16.to_f32(q)[keep], lambda t: clean[req[keep[t]]], ctx[keep])
+
+
+@pytest.mark.parametrize('scale', [-SCALE, 0.0])
+def test_chunks_at_any_scale(cc, monkeypatch, scale):
+    """A negative scale, and none: the smallest scores count most, or all rows alike."""
+    monkeypatch.setattr(cc, 'history_shape', lambda *a: (3, 1))
+    rng = np.random.default_rng(79)
+    p = Pool(rng, [90], 512, 16)
+    q = random_bits(rng, (11, 16, 512), 0.5)
+    o, lse = cc.history_attention(dev_bf16(q), dev_u8(p.cache), dev_i32(p.table), dev_i32([90] * 11), scale, 90,
+                                  token_requests=dev_i64([0] * 11), query_start_loc=dev_i32([0, 11]), max_query_len=11)
+    for t in range(11):
+        want, want_lse, size = C.attention(bf16.to_f32(q)[t].astype(np.float64), p.rows(0), scale)
+        d = 514 * 2.0 ** -24 * abs(scale) * (np.abs(bf16.to_f32(q)[t]).astype(np.float64) @ np.abs(p.rows(0)[:, :512]).T).max()
+        bound = HALF * (size * 1.01 + np.abs(want)) + (math.expm1(2 * d) + 2.0 ** -20) * size
+        assert (np.abs(host_f32(o)[t] - want) <= bound).all()
+        assert (np.abs(host_f32(lse)[:, t] - want_lse) <= d + 2.0 ** -20 + 2.0 ** -22 * np.abs(want_lse)).all()
+
+
+def test_rows_with_nan_refusals(ops):
+    z = lambda *s, dtype=torch.bfloat16: torch.zeros(*s, dtype=dtype, device='cuda')
+    call = lambda w=512, splits=1, group=4, scale=1.0: ops.history_attention_kv(
+        z(2, 16, w), z(4, 1, 16, w), z(4, 1, 16, w), z(2, 3, dtype=torch.int32), z(2, dtype=torch.int32), scale, splits,
+        ops.S6Workspace(16, 1024, 8), None, None, 'hip', tokens_per_group=group, nan_rows=True)
+    assert torch.isneginf(call()[1]).all()
+    for kw in (dict(w=1024), dict(w=128), dict(splits=2), dict(group=1), dict(group=2), dict(scale=0.0), dict(scale=-1.0)):
+        with pytest.raises(ValueError, match='rows with NaN'):
+            call(**kw)
