@@ -282,8 +282,8 @@ def history_attention(q_lat, cache, block_table, ctx, scale, max_seq_len, token_
     sums are fp32; the weights are rounded to bf16 for their product with the rows, as over a bf16 cache.
 
     Requests of several tokens (``max_query_len`` above 1, a host number) share their rows: with ``token_requests`` two tokens
-    may go through a row together, and with ``query_start_loc`` (int32 ``[R + 1]``) too the rows of large chunks may be
-    expanded to bf16 once, into scratch of ``R * max_seq_len`` rows (``history_shape`` says when).
+    may go through a row together, and with ``query_start_loc`` (int32 ``[R + 1]``, of the same requests: a token outside all
+    of its chunks may name any) too the rows of large chunks may be expanded to bf16 once, into scratch of ``R * max_seq_len`` rows (``history_shape`` says when).
 
     ``num_kv_splits`` defaults to the count of ``history_shape``; ``workspace`` (an ``S6Workspace``) to a new buffer; ``plan`` is
     an optional ``s6_ops.split_plan`` for ``(ctx, columns * block, num_kv_splits)``, for a token per workgroup. Calls that share

@@ -87,16 +87,22 @@ struct LoadParams {
   const int32_t* lengths;  // or null: the largest ctx of the request's tokens
   const int32_t* qsl;
   const int32_t* ctx;
-  int T;
+  int T, R;
   uint16_t* out;
   int64_t o_sr, o_sj;  // elements per request and per row
   int max_rows;
 };
 
+// the largest ctx of request r's tokens, and of those outside all chunks (padding, which may name any request)
 __device__ int most_ctx(const LoadParams& a, int r) {
   __shared__ int red[4];
   int most = 0;
-  for (int t = max(a.qsl[r], 0) + (int)threadIdx.x; t < min(a.qsl[r + 1], a.T); t += 256) most = max(most, a.ctx[t]);
+  auto take = [&](int t0, int t1) {
+    for (int t = max(t0, 0) + (int)threadIdx.x; t < min(t1, a.T); t += 256) most = max(most, a.ctx[t]);
+  };
+  take(a.qsl[r], a.qsl[r + 1]);
+  take(0, a.qsl[0]);
+  take(a.qsl[a.R], a.T);
   for (int off = 32; off > 0; off >>= 1) most = max(most, __shfl_xor(most, off));
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = most;
   __syncthreads();
@@ -902,6 +908,7 @@ extern "C" int hla_s6_compact_load(const void* cache, int32_t width, int64_t pag
   p.qsl = query_start_loc;
   p.ctx = ctx;
   p.T = num_tokens;
+  p.R = num_reqs;
   p.out = static_cast<uint16_t*>(out);
   p.o_sr = o_sr;
   p.o_sj = o_sj;

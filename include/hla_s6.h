@@ -523,8 +523,8 @@ int hla_s6_compact_store(const void *key, int64_t k_st, const void *value, int64
 
 /* out[r, j, :] (bf16, strides o_sr, o_sj, 1; 16-byte aligned rows) = row j of request r, for j < max_rows. With `lengths`
  * [num_reqs], rows at and past lengths[r] are zero. With lengths NULL the length of request r is the largest ctx[t] of its
- * tokens query_start_loc[r] <= t < query_start_loc[r + 1] (below num_tokens), and rows past it are not written. Page ids
- * are clamped into the cache. num_reqs <= 65535. */
+ * tokens query_start_loc[r] <= t < query_start_loc[r + 1] (below num_tokens) and of the tokens outside all requests, and
+ * rows past it are not written. Page ids are clamped into the cache. num_reqs <= 65535. */
 int hla_s6_compact_load(const void *cache, int32_t width, int64_t page_stride, int32_t block_size, int64_t num_blocks,
                         const int32_t *block_table, int64_t bt_stride, int32_t bt_cols, const int32_t *lengths,
                         const int32_t *query_start_loc, const int32_t *ctx, int32_t num_tokens, int32_t num_reqs,

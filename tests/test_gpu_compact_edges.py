@@ -195,3 +195,22 @@ def test_rows_with_nan_refusals(ops):
     for kw in (dict(w=1024), dict(w=128), dict(splits=2), dict(group=1), dict(group=2), dict(scale=0.0), dict(scale=-1.0)):
         with pytest.raises(ValueError, match='rows with NaN'):
             call(**kw)
+
+
+@pytest.mark.parametrize('shape', [(1, 1), (2, 1), (3, 1)])
+def test_tokens_outside_the_chunks_have_rows_too(cc, monkeypatch, shape):
+    """Tokens in front of the first chunk and behind the last one that name a request attend to its first ctx rows, in every
+    form: none reads memory that nothing was written to (which holds NaN here)."""
+    monkeypatch.setattr(cc, 'history_shape', lambda *a: shape)
+    rng = np.random.default_rng(78)
+    n, w = [210, 64, 33], 512
+    p = Pool(rng, n, w, 16)
+    req = np.array([2, 0] + [0] * 9 + [1] * 5 + [0, 2, 2])
+    start, ctx = dev_i32([2, 11, 16, 16]), np.array(n)[req]
+    ctx[2:11] = 90                                             # behind it the request's rows are needed by others alone
+    q = random_bits(rng, (len(req), 16, w), 0.5)
+    args = (dev_bf16(q), dev_u8(p.cache), dev_i32(p.table), dev_i32(ctx), SCALE, 210)
+    used = [torch.full((3 * 14, 1, 16, 2 * w), float('nan'), dtype=torch.bfloat16, device='cuda') for _ in range(4)]
+    del used
+    o, lse = cc.history_attention(*args, token_requests=dev_i64(req), query_start_loc=start, max_query_len=9)
+    check_attention(host_f32(o), host_f32(lse), bf16.to_f32(q), lambda t: p.rows(req[t]), ctx)
