@@ -80,7 +80,8 @@ __device__ __forceinline__ float row_sum16(float v) {
   return v;
 }
 
-// weight of a score under its softmax's lse (+inf: an empty row, which weighs nothing)
+// weight of a score under its softmax's lse (+inf: an empty row, which weighs nothing; the callers drop a NaN or infinite
+// score's there)
 __device__ __forceinline__ float weight(float s, float scale, float lse) {
   return fast_exp2(__builtin_fmaf(s, scale, -lse) * kLog2e);
 }
@@ -166,7 +167,7 @@ __global__ __launch_bounds__(256) void account_step_kernel(AccountParams a) {
       for (int x = 0; x < NT; ++x) {
         float w[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = weight(s[x][e], a.scale, lse);
+        for (int e = 0; e < 4; ++e) w[e] = lse == INFINITY ? 0.f : weight(s[x][e], a.scale, lse);
         const float sum = head_sums(h, w);
         const int key = j + x * kTile + 4 * g + h;
         if (h < 4 && key < end) sum_lds[key - begin] += sum;  // (the same lane for every token)
@@ -315,7 +316,7 @@ __global__ __launch_bounds__(256, W <= 256 ? 2 : 1) void account_chunk_kernel(Ac
         for (int i = 0; i < GROUP; ++i) qa[i] = qb[i];
       }
       lse = lse_now;
-      limit = min(n_now, cap) - key0 - 4 * g;
+      limit = lse_now == INFINITY ? 0 : min(n_now, cap) - key0 - 4 * g;
 #pragma unroll
       for (int x = 0; x < NT; ++x) last[x] = s[x];
       slot = slot1;

@@ -214,3 +214,34 @@ def test_tokens_outside_the_chunks_have_rows_too(cc, monkeypatch, shape):
     del used
     o, lse = cc.history_attention(*args, token_requests=dev_i64(req), query_start_loc=start, max_query_len=9)
     check_attention(host_f32(o), host_f32(lse), bf16.to_f32(q), lambda t: p.rows(req[t]), ctx)
+
+
+# ---- accounts ------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize('compact', [True, False])
+@pytest.mark.parametrize('w,chunk', [(256, 1), (1024, 1), (512, 1), (128, 40), (512, 40), (1024, 40)])
+def test_tokens_with_an_infinite_lse_add_nothing(cc, w, chunk, compact):
+    """Whatever their queries and the rows hold."""
+    rng = np.random.default_rng(w + chunk)
+    n, block = [150, 60], 16
+    p = Pool(rng, n, w, block)
+    T = 2 * chunk
+    q = random_bits(rng, (T, 16, w), 1.4 * math.sqrt(128 / w))
+    lse = rng.standard_normal((16, T)).astype(np.float32) + 8
+    empty = chunk + chunk // 2                                  # a token of request 1
+    lse[:, empty] = np.where(np.arange(16) % 2, np.inf, -np.inf)
+    q[empty, :, ::5] = bf16.from_f32(np.array([np.nan], np.float32))[0]
+    q[empty, 3] = bf16.from_f32(np.array([np.inf], np.float32))[0]
+    req, ctx = np.repeat([0, 1], chunk), np.repeat(n, chunk)
+    cache = dev_u8(p.cache)
+    if not compact:
+        every = C.load(p.cache, np.arange(len(p.cache) * block))
+        cache = torch.from_numpy(every.reshape(len(p.cache), 1, block, 2 * w)).to(torch.bfloat16).cuda()
+    start = rng.random((2, 150)).astype(np.float32)
+    clean = bf16.to_f32(q).copy()
+    clean[empty] = 0
+    want, bound = want_account(start, clean, p.rows, w, lse, req, ctx, 150)
+    got = cc.attention_weights(dev_bf16(q), cache, dev_i32(p.table), dev_i32([0, chunk, T]), dev_i32(ctx),
+                               torch.from_numpy(lse).cuda(), SCALE, torch.from_numpy(start).cuda()).cpu().numpy()
+    assert (np.abs(got - want) <= bound).all()
+    assert chunk > 1 or (got[1] == start[1]).all()
