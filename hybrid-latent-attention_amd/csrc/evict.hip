@@ -336,14 +336,14 @@ __global__ __launch_bounds__(256, W <= 256 ? 2 : 1) void account_chunk_kernel(Ac
   }
 }
 
-// account += the shares' sums, in their order
+// account += the shares' sums, in their order (rows that nothing was given keep their bits)
 __global__ __launch_bounds__(256) void account_reduce_kernel(const float* partial, int shares, int R, int cols,
                                                              float* account, int64_t a_st) {
   const int j = blockIdx.x * 256 + threadIdx.x, r = blockIdx.y;
   if (j >= cols) return;
   float s = 0.f;
   for (int z = 0; z < shares; ++z) s += partial[((int64_t)z * R + r) * cols + j];
-  account[(int64_t)r * a_st + j] += s;
+  if (s != 0.f) account[(int64_t)r * a_st + j] += s;
 }
 
 // ---- selection -----------------------------------------------------------------------------------------------------

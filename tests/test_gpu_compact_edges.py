@@ -245,3 +245,21 @@ def test_tokens_with_an_infinite_lse_add_nothing(cc, w, chunk, compact):
                                torch.from_numpy(lse).cuda(), SCALE, torch.from_numpy(start).cuda()).cpu().numpy()
     assert (np.abs(got - want) <= bound).all()
     assert chunk > 1 or (got[1] == start[1]).all()
+
+
+@pytest.mark.parametrize('chunk', [1, 64])
+def test_rows_behind_the_requests_keep_their_bits(cc, chunk):
+    """Accounts behind a request's rows, and of requests without tokens: -0 stays -0, a NaN keeps its payload."""
+    rng = np.random.default_rng(chunk)
+    n, w, M = [100, 0, 40, 16], 256, 130
+    p = Pool(rng, n, w, 16)
+    T = 2 * chunk
+    assert cc.account_shape(T, 4, M, 256, w)[0] == 0 if chunk == 1 else cc.account_shape(T, 4, M, 256, w)[0] > 1
+    req = np.repeat([0, 2], chunk)                              # requests 1 and 3 have no tokens
+    bits = np.where(rng.random((4, M)) < 0.5, 0x80000000, 0x7f812345).astype(np.uint32)
+    account = torch.from_numpy(bits.view(np.int32)).cuda().view(torch.float32)
+    cc.attention_weights(dev_bf16(random_bits(rng, (T, 16, w))), dev_u8(p.cache), dev_i32(p.table),
+                         dev_i32([0, chunk, chunk, T, T]), dev_i32(np.array(n)[req]), torch.zeros(16, T, device='cuda'), SCALE, account)
+    got = account.view(torch.int32).cpu().numpy().view(np.uint32)
+    for r, rows in enumerate([100, 0, 40, 0]):
+        assert (got[r, rows:] == bits[r, rows:]).all(), r
