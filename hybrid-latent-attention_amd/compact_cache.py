@@ -269,6 +269,8 @@ def _operands(q, cache, block_table, ctx, token_requests, plan=None):
     table = _table(block_table, T if token_requests is None else min(T, 1))
     if token_requests is not None:
         token_requests = _vector('token_requests', token_requests, T, I64)
+    if plan is not None and (plan.dtype != I32 or plan.dim() != 1 or not plan.is_contiguous()):
+        raise ValueError(f'plan must be a contiguous 1-d int32 tensor (s6_ops.split_plan), got {plan.dtype} {list(plan.shape)}')
     return T, w, geometry, table, ctx, token_requests
 
 

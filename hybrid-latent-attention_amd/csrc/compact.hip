@@ -295,8 +295,8 @@ __global__ __launch_bounds__(256, W <= 512 ? 2 : 1) void compact_history_kernel(
   s = __builtin_amdgcn_readfirstlane(s);
   const int n = (int)min((int64_t)max(from_lanes ? __builtin_amdgcn_readlane(ctx_of_lane, t) : a.ctx[t], 0), cap);
   const int tiles = (n + kTile - 1) / kTile;
-  if (S == 1) chunk = tiles;
-  const int j_begin = s * chunk, j_end = min(tiles, j_begin + chunk);
+  chunk = S == 1 ? tiles : min(max(chunk, 1), tiles);  // (whatever a plan holds: tiles of this row, and no overflow)
+  const int j_begin = (int)min((int64_t)s * chunk, (int64_t)tiles), j_end = min(tiles, j_begin + chunk);
   const int64_t part_row = ((int64_t)t * S + s) * kHeads;
 
   if (j_begin >= j_end) {  // a row without history

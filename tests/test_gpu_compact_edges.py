@@ -263,3 +263,27 @@ def test_rows_behind_the_requests_keep_their_bits(cc, chunk):
     got = account.view(torch.int32).cpu().numpy().view(np.uint32)
     for r, rows in enumerate([100, 0, 40, 0]):
         assert (got[r, rows:] == bits[r, rows:]).all(), r
+
+
+# ---- operands ------------------------------------------------------------------------------------------------------
+
+def test_plans_of_other_kinds(cc, ops):
+    """A plan of another type is refused; one whose chunk and slots would overflow stays inside the rows."""
+    rng = np.random.default_rng(17)
+    n, w, S = [200, 77], 256, 3
+    p = Pool(rng, n, w, 16)
+    q = random_bits(rng, (2, 16, w))
+    args = (dev_bf16(q), dev_u8(p.cache), dev_i32(p.table), dev_i32(n), SCALE)
+    plan = ops.split_plan(dev_i32(n), p.table.shape[1] * 16, S)
+    for bad in (plan.long(), plan.float(), plan[None], plan.repeat_interleave(2)[::2]):
+        with pytest.raises(ValueError, match='plan'):
+            cc.history_attention(*args, 200, num_kv_splits=S, plan=bad)
+        with pytest.raises(ValueError, match='plan'):
+            cc.history_partials(*args, S, ops.S6Workspace(16, w, 8), plan=bad)
+    items = (len(plan) - 3) // 2
+    rows, slots = np.full(items, -1), np.zeros(items)
+    rows[:6], slots[:6] = [0, 1, 0, 1, 0, 1], [0, 0, 2, 2, 1, 1]
+    for chunk in (2 ** 31 - 1, 2 ** 30, 13):                   # slot 0 holds whole rows; 2 * chunk passes 32 bits
+        made = dev_i32(np.concatenate(([chunk, S, S], rows, slots)))
+        o, lse = cc.history_attention(*args, 200, num_kv_splits=S, plan=made)
+        check_attention(host_f32(o), host_f32(lse), bf16.to_f32(q), p.rows, n)
