@@ -252,6 +252,7 @@ def _history(q, cache, geometry, block_table, table, ctx, scale, token_requests,
         need = T * HEADS * splits * (w + 1)
         ws = (torch.empty(need, dtype=F32, device=dev) if workspace is None
               else workspace.attn_logits(T, HEADS, splits, w, dev))
+        _same_device(q, ws)   # (a workspace keeps the device of its first use)
     if out is not None:
         lse = torch.empty(HEADS, T, dtype=F32, device=dev)
     _call('hla_s6_compact_history', dev, q.data_ptr(), T, HEADS, w, token_stride, head_stride, cache.data_ptr(), page_stride,

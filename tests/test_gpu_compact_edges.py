@@ -287,3 +287,15 @@ def test_plans_of_other_kinds(cc, ops):
         made = dev_i32(np.concatenate(([chunk, S, S], rows, slots)))
         o, lse = cc.history_attention(*args, 200, num_kv_splits=S, plan=made)
         check_attention(host_f32(o), host_f32(lse), bf16.to_f32(q), p.rows, n)
+
+
+def test_a_workspace_of_another_device_is_refused(cc, ops):
+    z = lambda *s, dtype=torch.bfloat16: torch.zeros(*s, dtype=dtype, device='cuda')
+    ws = ops.S6Workspace(16, 256, 8)
+    ws.ensure('cpu')
+    args = (z(2, 16, 256), z(4, 1, 17 * 256, dtype=torch.uint8), z(2, 3, dtype=torch.int32), z(2, dtype=torch.int32), SCALE)
+    with pytest.raises(RuntimeError, match='GPU only'):
+        cc.history_attention(*args, 48, num_kv_splits=4, workspace=ws)
+    with pytest.raises(RuntimeError, match='GPU only'):
+        cc.history_partials(*args, 4, ws)
+    cc.history_attention(*args, 48, num_kv_splits=1, workspace=ws)     # needs none
