@@ -30,6 +30,8 @@ WIDTHS = (128, 256, 512, 1024)
 HEADS, TILE = 16, 16
 # rows from which a history is long enough to be cut between workgroups in steps that could do without
 LONG_ROWS = 4096
+# rows of all requests up to which a step may expand them to bf16: 256 MiB of scratch at width 512
+EXPANDED_ROWS = 1 << 17
 
 #: What ``select_rows`` returns. ``lengths [R]``: rows per request from now on; ``weights``, ``positions [R, M]``: the account
 #: and positions in the new order (0 and -1 behind the last row); ``source``, ``target [R, M // 2]``: the row moves, ended by -1.
@@ -227,9 +229,9 @@ def history_shape(max_seq_len, num_tokens, num_reqs, cu_count=256, width=512):
 
     At width 128 a token per workgroup is fastest throughout (4 x 512 on 8160: 273, expanded 437). So two tokens from 2 per CU
     on, and on long rows from one per 8 CUs on; expansion at width 512 alone, from 8 tokens per CU in chunks of 256 and more on
-    average."""
+    average, for up to ``EXPANDED_ROWS`` rows: its scratch stays below 256 MiB where memory is what a compact cache is for."""
     per_request = num_tokens / max(1, num_reqs)
-    if width == 512 and num_tokens >= 8 * cu_count and per_request >= 256:
+    if width == 512 and num_tokens >= 8 * cu_count and per_request >= 256 and 0 < num_reqs * max_seq_len <= EXPANDED_ROWS:
         return 3, 1
     if width >= 256 and per_request >= 4:
         if num_tokens >= 2 * cu_count:
@@ -286,7 +288,7 @@ def history_attention(q_lat, cache, block_table, ctx, scale, max_seq_len, token_
 
     Requests of several tokens (``max_query_len`` above 1, a host number) share their rows: with ``token_requests`` two tokens
     may go through a row together, and with ``query_start_loc`` (int32 ``[R + 1]``, of the same requests: a token outside all
-    of its chunks may name any) too the rows of large chunks may be expanded to bf16 once, into scratch of ``R * max_seq_len`` rows (``history_shape`` says when).
+    of its chunks may name any) too the rows of large chunks may be expanded to bf16 once, into scratch of ``R * max_seq_len`` rows (``history_shape`` says when, and up to how many).
 
     ``num_kv_splits`` defaults to the count of ``history_shape``; ``workspace`` (an ``S6Workspace``) to a new buffer; ``plan`` is
     an optional ``s6_ops.split_plan`` for ``(ctx, columns * block, num_kv_splits)``, for a token per workgroup. Calls that share

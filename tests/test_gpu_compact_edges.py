@@ -299,3 +299,16 @@ def test_a_workspace_of_another_device_is_refused(cc, ops):
     with pytest.raises(RuntimeError, match='GPU only'):
         cc.history_partials(*args, 4, ws)
     cc.history_attention(*args, 48, num_kv_splits=1, workspace=ws)     # needs none
+
+
+def test_a_large_step_without_requests(cc):
+    """query_start_loc of no request: all tokens lie outside the chunks, and attend to the rows that they name."""
+    rng = np.random.default_rng(18)
+    p = Pool(rng, [33], 512, 16)
+    T = 2100
+    q = random_bits(rng, (T, 16, 512), 0.5)
+    assert cc.history_shape(33, T, 1, 256, 512)[0] == 3
+    o, lse = cc.history_attention(dev_bf16(q), dev_u8(p.cache), dev_i32(p.table), dev_i32([33] * T), SCALE, 33,
+                                  token_requests=dev_i64([0] * T), query_start_loc=dev_i32([0]), max_query_len=T)
+    some = [0, 1, 1050, T - 1]
+    check_attention(host_f32(o[some]), host_f32(lse[:, some]), bf16.to_f32(q)[some], lambda t: p.rows(0), [33] * 4)

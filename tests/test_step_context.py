@@ -1,4 +1,5 @@
-"""CPU checks of what a StepContext keeps about its latent lengths (the GPU side: test_gpu_compact_edges.py)."""
+"""CPU checks of what a StepContext keeps about its latent lengths, and of how much scratch a step may take (the GPU side:
+test_gpu_compact_edges.py)."""
 import contextlib
 
 import pytest
@@ -40,3 +41,11 @@ def test_plans_follow_the_lengths(step, mode):
         ctx.ctx_latent.add_(1)
         assert ctx.split_plan(4, 64) == (4, [1, 4]) and ctx.empty_latent.tolist() == [False, False]
         assert ctx.split_plan(4, 128) == (4, [1, 4])
+
+
+def test_scratch_of_expanded_rows_is_bounded(pkg):
+    shape = pkg.compact_cache.history_shape
+    assert shape(32736, 2048, 4, 256, 512) == (3, 1) and shape(32768, 2048, 4, 256, 512) == (3, 1)
+    assert shape(32769, 2048, 4, 256, 512) == (2, 1) and shape(32736, 16384, 32, 256, 512) == (2, 1)
+    assert shape(131072, 4096, 1, 256, 512) == (3, 1) and shape(131073, 4096, 1, 256, 512) == (2, 1)
+    assert shape(300, 4096, 0, 256, 512) == (2, 1)             # no requests: nothing to expand
