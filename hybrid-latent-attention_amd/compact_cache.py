@@ -441,7 +441,8 @@ def select_rows(weights, positions, lengths, budget, protect_from):
 def move_rows(cache, block_table, eviction):
     """Apply the row moves of ``select_rows`` to a cache (compact or bf16) in place, through the per-request
     ``block_table``. A request's pages must be its own: a page in two rows of the table would change for both. Moves through
-    page ids outside the cache are skipped."""
+    page ids outside the cache are skipped. The moves of a call run at once: in lists of a caller's own no source may be another
+    move's target, nor a target named twice (``select_rows`` makes none such)."""
     source, target = eviction.source, eviction.target
     _same_device(cache, block_table, source, target)
     w, compact, page_stride, row_stride, block, num_blocks = _pages(cache)

@@ -312,3 +312,42 @@ def test_a_large_step_without_requests(cc):
                                   token_requests=dev_i64([0] * T), query_start_loc=dev_i32([0]), max_query_len=T)
     some = [0, 1, 1050, T - 1]
     check_attention(host_f32(o[some]), host_f32(lse[:, some]), bf16.to_f32(q)[some], lambda t: p.rows(0), [33] * 4)
+
+
+# ---- eviction beside an exact window ----------------------------------------------------------------------------------
+
+@pytest.mark.parametrize('compact', [True, False])
+def test_eviction_beside_a_window_in_a_ragged_batch(cc, compact):
+    """Requests with none, few, exactly W and many rows above the budget, shorter than the window, with pages of the others in
+    their unused table entries: rows go where at least W are to go, and the W rows behind follow them in order."""
+    rng = np.random.default_rng(19)
+    W, top, w, block = 32, 64, 256, 16
+    n = np.array([64, 69, 95, 96, 97, 300, 0, 40, 128])        # rows behind the window's
+    p = Pool(rng, n + W, w, block)
+    p.table[6, 2:] = p.table[5, :len(p.table[6]) - 2]           # beyond its 32 rows: pages of request 5
+    p.table[7, 5:] = p.table[8, :len(p.table[7]) - 5]
+    R, M = len(n), 300
+    if compact:
+        cache = dev_u8(p.cache)
+    else:
+        every = np.nan_to_num(C.load(p.cache, np.arange(len(p.cache) * block)))
+        cache = torch.from_numpy(every.reshape(len(p.cache), 1, block, 2 * w)).to(torch.bfloat16).cuda()
+    before = [p.rows(r) for r in range(R)]
+    table, lengths = dev_i32(p.table), dev_i32(n)
+    account = torch.rand(R, M, device='cuda')
+    positions = torch.arange(M, dtype=torch.int32, device='cuda').repeat(R, 1)
+    budget = torch.where(lengths >= top + W, top, lengths)
+    e = cc.select_rows(account, positions, lengths, budget, lengths)
+    cc.move_rows(cache, table, e)
+    i, gone = torch.arange(W, dtype=torch.int32, device='cuda'), (e.lengths < lengths)[:, None]
+    source, target = (torch.where(gone, x[:, None] + i, -1) for x in (lengths, e.lengths))
+    cc.move_rows(cache, table, cc.Eviction(None, None, None, source, target))
+    assert e.lengths.tolist() == [64, 69, 95, 64, 64, 64, 0, 40, 64]
+    got = host_u8(cache) if compact else host_f32(cache).reshape(-1, 2 * w)
+    for r in range(R):
+        b = int(e.lengths[r])
+        kept = np.concatenate((e.positions[r, :b].cpu().numpy(), n[r] + np.arange(W)))
+        slots = C.slots_of(p.table[r], block, b + W)
+        assert ((C.load(got, slots) if compact else got[slots]) == before[r][kept]).all(), r
+        assert b == n[r] or kept[:b].max() < n[r] and len(set(kept)) == b + W
+        assert b < n[r] or (kept == np.arange(b + W)).all()
