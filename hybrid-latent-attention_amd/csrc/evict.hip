@@ -122,18 +122,14 @@ __global__ __launch_bounds__(256) void account_step_kernel(AccountParams a) {
     const int end = min(min(a.ctx[t], cap), begin + a.per_wg);
     if (begin >= end) continue;  // uniform over the workgroup
     int j = begin + wave * NT * kTile;
-    // places of the wave's next 64 / NT steps' tiles, one per lane; the last step loads nothing (see compact_history_kernel)
-    uint32_t at_lo, at_hi;
-    auto look_up = [&](int j0) {
-      const int64_t at = K::place(a, btr, min(j0 + lane / NT * SPAN + lane % NT * kTile, (end - 1) / kTile * kTile));
-      at_lo = (uint32_t)at;
-      at_hi = (uint32_t)((uint64_t)at >> 32);
-    };
+    // places of the tiles of all the wave's steps, one per lane; the last step loads nothing (see compact_history_kernel)
+    static_assert(kMaxStepKeys <= 64 / NT * SPAN, "a wave's lanes hold the places of all its tiles");
+    const int64_t at = K::place(a, btr, min(j + lane / NT * SPAN + lane % NT * kTile, (end - 1) / kTile * kTile));
+    const uint32_t at_lo = (uint32_t)at, at_hi = (uint32_t)((uint64_t)at >> 32);
     auto tile = [&](int i) {
       const uint32_t lo = __builtin_amdgcn_readlane(at_lo, i), hi = __builtin_amdgcn_readlane(at_hi, i);
       return (int64_t)(((uint64_t)hi << 32) | lo);
     };
-    look_up(j);
     u32x4 q[STEPS / 4];
     const uint16_t* qp = a.q + (int64_t)t * a.q_st + (int64_t)h * a.q_sh;
 #pragma unroll
@@ -158,10 +154,8 @@ __global__ __launch_bounds__(256) void account_step_kernel(AccountParams a) {
         for (int x = 0; x < NT; ++x) s[x] = mfma16x16x32(k[x].operand(i), qi, s[x]);
       }
       if constexpr (!last.value) {
-        const int i0 = step % (64 / NT) * NT;
-        if (i0 == 0) look_up(j + SPAN);
 #pragma unroll
-        for (int x = 0; x < NT; ++x) k[x].template load<kOnce>(a, tile(i0 + x), h, g);
+        for (int x = 0; x < NT; ++x) k[x].template load<kOnce>(a, tile(step * NT + x), h, g);
       }
 #pragma unroll
       for (int x = 0; x < NT; ++x) {

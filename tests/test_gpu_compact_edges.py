@@ -351,3 +351,118 @@ def test_eviction_beside_a_window_in_a_ragged_batch(cc, compact):
         assert ((C.load(got, slots) if compact else got[slots]) == before[r][kept]).all(), r
         assert b == n[r] or kept[:b].max() < n[r] and len(set(kept)) == b + W
         assert b < n[r] or (kept == np.arange(b + W)).all()
+
+
+# ---- long walks ----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize('shape', [(1, 1), (2, 1)])
+@pytest.mark.parametrize('width,block', [(128, 16), (256, 48), (512, 16), (1024, 32)])
+def test_one_workgroup_walks_past_its_page_look_ups(cc, monkeypatch, width, block, shape):
+    """A wave looks up the pages of 32 steps at a time (4096 rows, with two tokens 2048 at width 512, and 1024 rows at 1024):
+    rows of more than two look-ups in one slot, in scattered pages, and rows that end with a look-up."""
+    if shape[0] == 2 and width == 128:
+        shape = (1, 1)                                          # (no form for two tokens there)
+    monkeypatch.setattr(cc, 'history_shape', lambda *a: shape)
+    rng = np.random.default_rng(width)
+    n = [8192 + 73, 4096, 2049] if width < 1024 else [4096 + 73, 2048, 1025]
+    p = Pool(rng, n, width, block)
+    req = np.array([0, 0, 1, 1, 2])
+    ctx = np.array(n)[req]
+    q = random_bits(rng, (5, 16, width), 1.4 * math.sqrt(128 / width))
+    rows = [p.rows(r) for r in range(3)]
+    for length in (2, 1):                                       # rows that tokens share, and rows that stream past the caches
+        o, lse = cc.history_attention(dev_bf16(q), dev_u8(p.cache), dev_i32(p.table), dev_i32(ctx), SCALE, max(n),
+                                      token_requests=dev_i64(req), max_query_len=length, num_kv_splits=1)
+        check_attention(host_f32(o), host_f32(lse), bf16.to_f32(q), lambda t: rows[req[t]], ctx)
+
+
+@pytest.mark.parametrize('compact', [True, False])
+@pytest.mark.parametrize('width,keys', [(128, 1024), (256, 4096), (512, 1024), (512, 4096), (1024, 2048), (1024, 64)])
+def test_accounts_of_many_rows_per_workgroup(cc, monkeypatch, width, keys, compact):
+    """Single tokens, requests of two and three tokens and of none in the kernel that streams K, over rows that fill the places
+    a wave looks up, and end in the middle."""
+    monkeypatch.setattr(cc, 'account_shape', lambda *a: (0, keys))
+    rng = np.random.default_rng(width + keys)
+    n, chunk = [4100, 1030, 16, 333], [1, 3, 0, 2]
+    p = Pool(rng, n, width, 16)
+    cache = dev_u8(p.cache)
+    if not compact:
+        every = C.load(p.cache, np.arange(len(p.cache) * 16))
+        cache = torch.from_numpy(every.reshape(len(p.cache), 1, 16, 2 * width)).to(torch.bfloat16).cuda()
+    req = np.repeat(np.arange(4), chunk)
+    ctx = np.array(n)[req]
+    ctx[2] = 517
+    q = random_bits(rng, (6, 16, width), 1.4 * math.sqrt(128 / width))
+    lse = rng.standard_normal((16, 6)).astype(np.float32) + 8
+    start = rng.random((4, 4100)).astype(np.float32)
+    rows = [p.rows(r) for r in range(4)]
+    want, bound = want_account(start, bf16.to_f32(q), lambda r: rows[r], width, lse, req, ctx, 4100)
+    got = cc.attention_weights(dev_bf16(q), cache, dev_i32(p.table), dev_i32(np.concatenate(([0], np.cumsum(chunk)))), dev_i32(ctx),
+                               torch.from_numpy(lse).cuda(), SCALE, torch.from_numpy(start).cuda()).cpu().numpy()
+    assert (np.abs(got - want) <= bound).all(), float((np.abs(got - want) - bound).max())
+
+
+# ---- steps that mix chunks and single tokens ----------------------------------------------------------------------------
+
+@pytest.mark.parametrize('chunk', [9, 10])
+@pytest.mark.parametrize('width', [256, 512])
+def test_accounts_of_mixed_steps(cc, width, chunk):
+    """Eight single tokens and one chunk, on both sides of the rule that picks the kernel."""
+    rng = np.random.default_rng(width + chunk)
+    n = [40, 300, 17, 1, 0, 64, 130, 222, 180]
+    count = [1] * 8 + [chunk]
+    T = sum(count)
+    assert (cc.account_shape(T, 9, 300, 256, width)[0] == 0) == (chunk == 9)
+    p = Pool(rng, n, width, 16)
+    req = np.repeat(np.arange(9), count)
+    ctx = np.array(n)[req]
+    q = random_bits(rng, (T, 16, width), 1.4 * math.sqrt(128 / width))
+    lse = rng.standard_normal((16, T)).astype(np.float32) + 8
+    start = rng.random((9, 300)).astype(np.float32)
+    want, bound = want_account(start, bf16.to_f32(q), p.rows, width, lse, req, ctx, 300)
+    got = cc.attention_weights(dev_bf16(q), dev_u8(p.cache), dev_i32(p.table), dev_i32(np.concatenate(([0], np.cumsum(count)))),
+                               dev_i32(ctx), torch.from_numpy(lse).cuda(), SCALE, torch.from_numpy(start).cuda()).cpu().numpy()
+    assert (np.abs(got - want) <= bound).all()
+
+
+@pytest.mark.parametrize('singles,chunk,width,n', [(100, 412, 256, 60), (100, 412, 512, 60), (30, 100, 512, 4200), (7, 2057, 512, 50)])
+def test_history_of_mixed_steps(cc, singles, chunk, width, n):
+    """Single tokens and one chunk in the forms that their numbers on average ask for: two tokens a workgroup, in splits, expanded."""
+    rng = np.random.default_rng(singles)
+    R, T = singles + 1, singles + chunk
+    kind, splits = cc.history_shape(n, T, R, 256, width)
+    assert (kind, splits > 1) == {60: (2, False), 4200: (2, True), 50: (3, False)}[n]
+    lengths = rng.integers(0, 41, R)
+    lengths[0], lengths[singles] = n, n - 3
+    p = Pool(rng, lengths, width, 16)
+    count = [1] * singles + [chunk]
+    req = np.repeat(np.arange(R), count)
+    ctx = lengths[req]
+    q = random_bits(rng, (T, 16, width), 1.4 * math.sqrt(128 / width))
+    o, lse = cc.history_attention(dev_bf16(q), dev_u8(p.cache), dev_i32(p.table), dev_i32(ctx), SCALE, n,
+                                  token_requests=dev_i64(req), query_start_loc=dev_i32(np.concatenate(([0], np.cumsum(count)))),
+                                  max_query_len=chunk)
+    some = np.concatenate((np.arange(singles + 2), [T - 2, T - 1]))
+    last = p.rows(singles)
+    check_attention(host_f32(o[some]), host_f32(lse[:, some]), bf16.to_f32(q)[some],
+                    lambda t: last if req[some[t]] == singles else p.rows(req[some[t]]), ctx[some])
+
+
+@pytest.mark.parametrize('w,contexts,chunk,kind', [(256, [330, 90, 20, 600], 130, 2), (512, [330, 90, 20, 600], 130, 2),
+                                                   (512, [330, 90, 20, 600], 512, 3), (512, [4200, 4100], 17, 2)])
+def test_attend_in_every_form(cc, pkg, ops, monkeypatch, w, contexts, chunk, kind):
+    """s6_layer.attend over a compact cache against the bf16 cache of the same values at sizes that take two tokens a workgroup,
+    split and not, and the expanded form; bounds as in test_attend_over_a_compact_cache."""
+    rng = np.random.default_rng(w + chunk)
+    taken, shape = [], cc.history_shape
+    monkeypatch.setattr(cc, 'history_shape', lambda *a: taken.append(shape(*a)) or taken[-1])
+    x = Layer(pkg, ops, rng, contexts, chunk, w)
+    M, R = max(contexts) + chunk, len(contexts)
+    a1, a2 = torch.zeros(R, M, device='cuda'), torch.zeros(R, M, device='cuda')
+    cache, plain = x.compact, x.plain
+    want = x.attend(plain, x.step()).float()
+    for got in (x.attend(cache, x.step()), x.attend(cache, x.step(), weights=a1), x.attend(plain, x.step(), weights=a2)):
+        assert (got.float() - want).abs().max() <= 4 * HALF * want.abs().max()
+        assert (got.float() - want).norm() <= 2 * HALF * want.norm()
+    assert {k for k, _ in taken} == {kind}
+    assert torch.allclose(a1, a2, rtol=2.0 ** -10, atol=1e-6)
