@@ -192,13 +192,15 @@ def _load(cache, geometry, block_table, lengths, query_start_loc, ctx, T, R, max
 def kv_splits(max_seq_len, num_tokens, cu_count=256, width=512, small_step_tiles=768):
     """Split slots per row for ``history_attention`` over a compact cache, one token a workgroup. A split is a workgroup of
     four waves that walk 128 rows at a time. The plan cuts rows so that about half of the slots get equal work, and this returns
-    the count that gives every CU one of them (64 rows of 8160 at width 512: 59.8 us with 8 slots, 66.7 with 16); half of that
-    up to 256 rows per CU (128 above width 512), where partials cost more than workgroups gain (8 of 8160: 21.2 us with 32
-    slots, 22.8 with 64; 1 of 32736: 18.5 with 256, 21.6 with 512); at most two per 128 keys of the longest row, and in small
-    steps two per 64 and one per two CUs (1 of 8160: 13.5 with 128, 15.1 with 256). One slot, without a reduction, for rows that
-    a single pass covers and for steps with a row for every other CU (130 rows of 4000: 67.9 us with one slot, 76.5 with two;
-    200 of 200 to 4000: 62.3 and 77.0; 128 of 2000: 39.1, with four 40.8; exactly so many rows of 4096 and more still take
-    four: 128 of 8160 132 us with one, 105 with four). A function of constants and the row count only (graph-stable)."""
+    the count that gives every CU one of them (64 rows of 8160 at width 512: 57.6 us with 8 slots, 62.9 with 16); half of that
+    up to 256 rows per CU (128 above width 512), where partials cost more than workgroups gain (8 of 8160: 21.8 us with 32
+    slots, 22.8 with 64; 1 of 32736: 18.6 with 256, 21.7 with 512); at most two per 128 keys of the longest row, and in small
+    steps two per 64 and one per two CUs (1 of 8160: 14.5 with 128, 15.3 with 256). One slot, without a reduction, for rows that
+    a single pass covers and for steps with a row for every other CU (130 rows of 4000: 67.5 us with one slot, 75.5 with two, 81.3
+    with four, 67.3 with six; 200 of 200 to 4000: 62.3 with one, 68.3 with four; 128 of 2000: 38.8 with either). On long rows
+    four slots pay as long as their items, two per row, are no more than the CUs: 128 of 8160 129 us with one slot, 102 with
+    four; 129 of 8160 131 and 144 (six: 119, the most that one slot gives away there; 160 rows 140, 152, 133; 200 161, 171, 176;
+    250 175, 196, 207). A function of constants and the row count only (graph-stable)."""
     tokens = max(1, num_tokens)
     if max_seq_len <= 128 or 2 * tokens >= cu_count + (max_seq_len >= LONG_ROWS):
         return 1
@@ -215,21 +217,22 @@ def history_shape(max_seq_len, num_tokens, num_reqs, cu_count=256, width=512):
     the multi-query kernels of the bf16 cache over them. In us at 1 / 2 / 3, best split counts:
 
         tokens x rows          w 256             w 512             w 1024
-        4 x 512 on 8160        447 / 315 / 397   743 / 638 / 555   2633 / 2020 / 4676
-        4 x 512 on 1000        76 / 56 / 76      114 / 109 / 105   419 / 308 / 616
-        16 x 128 on 4000       231 / 166 / 215   391 / 343 / 328   1335 / 1022 / 2514
-        1 x 512 on 8160        121 / 93          202 / 195         700 / 509
-        1 x 512 on 300         14 / 13           20 / 21           49 / 39
-        64 x 8 on 4000         85 / 55           156 / 121         395 / 274
-        1 x 256 on 2000        21 / 27           35 / 50           98 / 110
-        2 x 64 on 8160         45 / 37           71 / 69           205 / 169
-        4 x 8 on 8160          22 / 21           32 / 34           70 / 63
-        4 x 3 on 8160          17 / 25           24 / 33           46 / 59
-        2 x 64 on 2000         22 / 23           36 / 38           82 / 72
+        4 x 512 on 8160        458 / 322 / 403   765 / 668 / 567   2645 / 2025
+        4 x 512 on 1000        76 / 54 / 74      115 / 110 / 105   401 / 307
+        16 x 128 on 4000       234 / 169 / 215   397 / 353 / 337   1340 / 1025
+        1 x 512 on 8160        127 / 95          212 / 194         690 / 512
+        1 x 512 on 300         13 / 12           18 / 20           48 / 39
+        64 x 8 on 4000         86 / 53           146 / 127         390 / 275
+        1 x 256 on 2000        23 / 27           38 / 50           102 / 100
+        2 x 64 on 8160         44 / 36           68 / 67           197 / 162
+        4 x 8 on 8160          21 / 20           32 / 32           65 / 60
+        4 x 3 on 8160          16 / 23           24 / 33           42 / 57
+        2 x 64 on 2000         22 / 22           35 / 36           73 / 64
 
-    At width 128 a token per workgroup is fastest throughout (4 x 512 on 8160: 273, expanded 437). So two tokens from 2 per CU
+    At width 128 there is a token per workgroup alone (4 x 512 on 8160: 278). So two tokens from 2 per CU
     on, and on long rows from one per 8 CUs on; expansion at width 512 alone, from 8 tokens per CU in chunks of 256 and more on
-    average, for up to ``EXPANDED_ROWS`` rows: its scratch stays below 256 MiB where memory is what a compact cache is for."""
+    average, for up to ``EXPANDED_ROWS`` rows: its scratch stays below 256 MiB where memory is what a compact cache is for.
+    (Measured on steps of equal chunks; of others the rule sees averages.)"""
     per_request = num_tokens / max(1, num_reqs)
     if width == 512 and num_tokens >= 8 * cu_count and per_request >= 256 and 0 < num_reqs * max_seq_len <= EXPANDED_ROWS:
         return 3, 1
@@ -288,7 +291,8 @@ def history_attention(q_lat, cache, block_table, ctx, scale, max_seq_len, token_
 
     Requests of several tokens (``max_query_len`` above 1, a host number) share their rows: with ``token_requests`` two tokens
     may go through a row together, and with ``query_start_loc`` (int32 ``[R + 1]``, of the same requests: a token outside all
-    of its chunks may name any) too the rows of large chunks may be expanded to bf16 once, into scratch of ``R * max_seq_len`` rows (``history_shape`` says when, and up to how many).
+    of its chunks may name any) too the rows of large chunks may be expanded to bf16 once, into scratch of ``R * max_seq_len``
+    rows (``history_shape`` says when, and up to how many).
 
     ``num_kv_splits`` defaults to the count of ``history_shape``; ``workspace`` (an ``S6Workspace``) to a new buffer; ``plan`` is
     an optional ``s6_ops.split_plan`` for ``(ctx, columns * block, num_kv_splits)``, for a token per workgroup. Calls that share

@@ -75,7 +75,7 @@ __global__ __launch_bounds__(256) void compact_store_kernel(StoreParams a) {
 // out[r, j, :] = row j of request r in bf16 for j < lengths[r], 0 behind it (without lengths: of a step's tokens, and
 // nothing behind it). One thread per eight columns: 4 bytes in, 16 out. HBM-bound by the writes (64 W bytes of every 81 W).
 // They go past the caches (16 x 4096 rows at W = 512: 27.5 us, 6.2 TB/s; through them 43), but for a step's, which the attention
-// reads next (4 x 512 tokens on 7000 to 8160: 619 us with it, past the caches 648).
+// reads next (4 x 512 tokens on 7000 to 8160: 562 us with it, past the caches 609).
 struct LoadParams {
   const uint8_t* cache;
   int64_t page_stride;
@@ -414,7 +414,8 @@ __global__ __launch_bounds__(256, W <= 512 ? 2 : 1) void compact_history_kernel(
       load_v<W, kOnce>(t1, h, g, half, v[1]);
     }
   };
-  if constexpr (W >= 256) {  // (at 128, where four waves a SIMD hide it, the second body costs more: 64 rows of 8160 27 us, 33)
+  if constexpr (W >= 256) {  // (at 128, where four waves a SIMD hide it, the second body costs more: 64 rows of 8160 27 us and 33
+                             // with it; 22.6 since slots are joined by compact_join_kernel)
     for (; j + stride < j_end; j += stride, ++step) one_step(std::false_type{});
     if (j < j_end) one_step(std::true_type{});
   } else {
@@ -491,7 +492,7 @@ __global__ __launch_bounds__(256, W <= 512 ? 2 : 1) void compact_history_kernel(
 // parts of the scores through LDS (one barrier a step, the parts in two buffers), and go on with the softmax each for itself.
 // The queries lie in LDS. O^T needs 128 accumulators a lane at every width. Tokens of a pair that differ in request or
 // length go through their rows one after the other: a product spreads a NaN in one's rows to the other's sums.
-// 4 x 512 tokens on 8160 rows: w = 512 638 us (860 TFLOP/s; a token per workgroup 743), w = 256 315 (447), w = 1024 2020 (2633).
+// 4 x 512 tokens on 8160 rows: w = 512 668 us (820 TFLOP/s; a token per workgroup 765), w = 256 322 (458), w = 1024 2025 (2645).
 // Four tokens per workgroup convert half as often, but need registers that spill (w = 512: twice as long).
 template <int W>
 struct PairGeo {
