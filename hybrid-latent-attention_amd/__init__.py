@@ -9,8 +9,10 @@ reference's own loader reads it back); ``history_gemm`` is
 the differentiable history attention over contiguous rows (multi-query for K-hop replay, single-query for the HF
 engine); ``batched_engine`` is the HF rolling engine's joint attention over history rows and the current chunk.
 ``compact_cache`` holds latent rows in 4 bits per value, attends to them, and evicts rows from either kind of cache by the
-attention they received; it has no counterpart in the reference.
+attention they received; ``exact_cache`` attends to whole exact caches, in bf16 or 8 bits; ``pages`` shares, takes, drops and
+compacts the pages of any cache. These three have no counterpart in the reference.
 """
-from . import _lib, batched_engine, compact_cache, history_gemm, rollout_cache, s6_layer, s6_ops
+from . import _lib, batched_engine, compact_cache, exact_cache, history_gemm, pages, rollout_cache, s6_layer, s6_ops
 
-__all__ = ['_lib', 'batched_engine', 'compact_cache', 'history_gemm', 'rollout_cache', 's6_layer', 's6_ops']
+__all__ = ['_lib', 'batched_engine', 'compact_cache', 'exact_cache', 'history_gemm', 'pages', 'rollout_cache', 's6_layer',
+           's6_ops']

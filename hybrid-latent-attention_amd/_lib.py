@@ -13,11 +13,13 @@ import torch
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get('HLA_S6_LIBRARY') or os.path.join(HERE, 'libhla_s6.so')   # override: another build
-ABI_VERSION = 16
+ABI_VERSION = 17
 
 OK, EINVAL, EUNSUPPORTED, EWORKSPACE, ELAUNCH, EDEVICE = range(6)
 
 P, I32, I64, F32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
+
+POOL = (P, I64, I32, I32, P, P, I64, P, I32)   # tables and their row stride, requests, columns, lengths, refs, pages, free, block
 
 # name -> argument types, in the order of include/hla_s6.h
 SIGNATURES = {
@@ -94,6 +96,14 @@ SIGNATURES = {
                                  P, I64, I32, I32, I32, P, I64, P],
     'hla_s6_select_rows': [P, I64, P, I64, P, I32, I32, I32, P, P, P, P, P, P, P, P],
     'hla_s6_move_rows': [P, I32, I32, I64, I64, I32, I64, P, I64, I32, P, P, I64, I32, I32, P],
+    'hla_s6_exact_attention': [P, I32, I32, I32, I64, I64, P, I32, I32, I64, I64, I64, I32, I64, P, I64, I32, I32, P, P, I32,
+                               F32, P, P, I32, I32, P, I64, P, I64, I64, P, P],
+    'hla_s6_exact_store': [P, I64, I64, P, I64, I64, I32, I32, I32, P, P, P, P, I32, I64, I64, I64, I32, I64, P],
+    'hla_s6_pool_release': [*POOL, P, P, I32, P],
+    'hla_s6_pool_fork': [*POOL, P, P, I32, P, P],
+    'hla_s6_pool_extend': [*POOL, P, P, P, P, P, P, P],
+    'hla_s6_pool_compact': [*POOL, P, P, P, P],
+    'hla_s6_copy_pages': [P, I32, I64, I64, I64, P, P, I64, P],
 }
 
 RESTYPES = {'hla_s6_last_error': ctypes.c_char_p, 'hla_s6_split_plan_ints': ctypes.c_int64,

@@ -1,0 +1,529 @@
+// A pool of cache pages: requests that share, drop and take pages, the compaction of the pages in use, and page copies.
+//
+// tables [R, cols]: the pages of request r, -1 behind its last; lengths [R]: its rows; refs [N]: how many requests hold a page;
+// free: bit p % 32 of word p / 32 is set where refs[p] == 0. Every result is a function of the pool and the arguments alone
+// (free pages are taken lowest first, in the order of requests and of their columns), whatever the order of the atomics.
+// The bookkeeping is a few KB to a MB of scattered words: latency, not bytes. One workgroup takes what needs an order (the
+// bit per page makes 200,000 pages 25 KB of it); drops and forks go a workgroup per request.
+#include "common.h"
+
+namespace hla {
+namespace {
+
+constexpr int kPoolThreads = 1024, kPoolWaves = kPoolThreads / 64;
+constexpr int kMaxRequests = 8192;
+
+struct Pool {
+  int32_t* tables;
+  int64_t t_st;
+  int R, cols;
+  int32_t* lengths;
+  int32_t* refs;
+  int N;
+  uint32_t* free;
+  int block;
+};
+
+__device__ __forceinline__ int pages_of(const Pool& p, int64_t rows) { return (int)((rows + p.block - 1) / p.block); }
+__device__ __forceinline__ int rows_of(const Pool& p, int32_t length) {  // a length that the table can hold
+  return (int)min((int64_t)max(length, 0), min((int64_t)p.cols * p.block, (int64_t)INT32_MAX));
+}
+__device__ __forceinline__ bool is_page(const Pool& p, int32_t page) { return page >= 0 && page < p.N; }
+
+__device__ __forceinline__ void drop_page(const Pool& p, int32_t page) {
+  if (is_page(p, page) && atomicSub(&p.refs[page], 1) == 1) atomicOr(&p.free[page >> 5], 1u << (page & 31));
+}
+
+// ---- release -----------------------------------------------------------------------------------------------------
+// Request requests[i] keeps its first to[i] rows (none without `to`). The lengths are lowered atomically: a request named
+// twice drops each of its columns once, in whatever order.
+__global__ __launch_bounds__(256) void pool_release_kernel(Pool p, const int32_t* requests, const int32_t* to) {
+  __shared__ int32_t before;
+  const int r = requests[blockIdx.x];
+  if (r < 0 || r >= p.R) return;
+  const int left = to ? max(to[blockIdx.x], 0) : 0;
+  if (threadIdx.x == 0) before = atomicMin(&p.lengths[r], left);
+  __syncthreads();
+  const int had = pages_of(p, rows_of(p, before));
+  for (int c = pages_of(p, left) + threadIdx.x; c < had; c += 256) {
+    int32_t* entry = p.tables + r * p.t_st + c;
+    drop_page(p, *entry);
+    *entry = -1;
+  }
+}
+
+// ---- fork --------------------------------------------------------------------------------------------------------
+// Request children[i] takes over the pages and the length of parents[i]. Refused: numbers outside the pool, children with rows,
+// children named before, parents that the list names as children (what they hold would depend on the order).
+__global__ __launch_bounds__(256) void pool_fork_kernel(Pool p, const int32_t* parents, const int32_t* children, int n,
+                                                        uint8_t* ok) {
+  const int i = blockIdx.x;
+  const int parent = parents[i], child = children[i];
+  bool bad = parent < 0 || parent >= p.R || child < 0 || child >= p.R;
+  if (!bad)
+    for (int j = threadIdx.x; j < n; j += 256) {
+      const int c = children[j];
+      bad = bad || c == parent || (c == child && j < i);
+    }
+  if (__syncthreads_or(bad)) {
+    if (threadIdx.x == 0) ok[i] = 0;
+    return;
+  }
+  const int had = p.lengths[child];   // (written by this workgroup alone, below)
+  const int32_t length = p.lengths[parent];
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    ok[i] = had <= 0;
+    if (had <= 0) p.lengths[child] = length;
+  }
+  if (had > 0) return;
+  const int held = pages_of(p, rows_of(p, length));
+  for (int c = threadIdx.x; c < held; c += 256) {
+    const int32_t page = p.tables[parent * p.t_st + c];
+    p.tables[child * p.t_st + c] = page;
+    if (is_page(p, page)) atomicAdd(&p.refs[page], 1);
+  }
+}
+
+// ---- scans of a workgroup ------------------------------------------------------------------------------------------
+// Exclusive prefix sum over the workgroup's threads; `total` is their sum. `sums` holds kPoolWaves + 1 entries.
+__device__ __forceinline__ int64_t pool_scan(int64_t v, int64_t* sums, int64_t& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t x = v;
+  for (int off = 1; off < 64; off <<= 1) {
+    const int64_t y = __shfl_up(x, off);
+    if (lane >= off) x += y;
+  }
+  __syncthreads();   // sums may still be read from a call before
+  if (lane == 63) sums[wave] = x;
+  __syncthreads();
+  int64_t at = 0;
+  total = 0;
+  for (int w = 0; w < kPoolWaves; ++w) {
+    if (w == wave) at = total;
+    total += sums[w];
+  }
+  return at + x - v;
+}
+
+// Set bits of word w of the pool's bitmap that are pages
+__device__ __forceinline__ uint32_t page_bits(const Pool& p, int w) {
+  const int words = (p.N + 31) / 32;
+  if (w >= words) return 0;
+  const int last = p.N & 31;
+  return w == words - 1 && last ? (1u << last) - 1 : ~0u;
+}
+
+// ---- extend ------------------------------------------------------------------------------------------------------
+// Room for the rows [from, to) of every request: columns behind its last get a free page each, columns that hold a shared page
+// a free page that the caller fills with a copy of it (the pairs source, target). Requests are served in order as long as what
+// they and those before them ask for is there; the others stay as they are.
+//
+// kFrom: from = write_from[r], and lists have an entry per table entry; a wave goes through a request's columns. Else from =
+// lengths[r], at most one column of a request is shared and lists have an entry per request; free pages find their places.
+struct ExtendParams {
+  Pool p;
+  const int32_t* to;
+  const int32_t* from;  // null: the lengths
+  uint8_t* ok;
+  int32_t *source, *target;
+  int32_t* ids;  // kFrom: [R * cols] scratch
+};
+
+template <bool kFrom>
+__global__ __launch_bounds__(kPoolThreads) void pool_extend_kernel(ExtendParams a) {
+  __shared__ int64_t sums[kPoolWaves + 1];
+  __shared__ int start[kMaxRequests + 1];   // first rank of a request's pages; requests that get none have no ranks
+  __shared__ uint8_t shared_last[kFrom ? 1 : kMaxRequests];
+  const Pool& p = a.p;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int words = (p.N + 31) / 32;
+
+  // columns [c0, c1) that may change: those with rows to write
+  auto columns = [&](int r, int& length, int& want, int& c0, int& c1) {
+    length = rows_of(p, p.lengths[r]);
+    want = max(a.to[r], length);
+    const int from = kFrom ? min(max(a.from[r], 0), length) : length;
+    const bool fits = want <= (int64_t)p.cols * p.block;
+    c0 = from / p.block;
+    c1 = fits && want > from ? pages_of(p, want) : c0;
+    return fits;
+  };
+  auto is_shared = [&](int r, int c) {
+    const int32_t page = p.tables[r * p.t_st + c];
+    return is_page(p, page) && p.refs[page] > 1;
+  };
+
+  // free pages
+  int64_t have = 0;
+  for (int w0 = 0; w0 < words; w0 += kPoolThreads) {
+    int64_t total;
+    pool_scan(__popc(w0 + tid < words ? p.free[w0 + tid] & page_bits(p, w0 + tid) : 0u), sums, total);
+    have += total;
+  }
+
+  // what every request asks for, and who gets it
+  if (kFrom) {
+    for (int r = wave; r < p.R; r += kPoolWaves) {
+      int length, want, c0, c1;
+      columns(r, length, want, c0, c1);
+      const int held = pages_of(p, length);
+      int need = max(0, c1 - max(c0, held));
+      for (int c = c0; c < min(c1, held); c += 64) {
+        const int at = c + lane;
+        const bool sh = at < min(c1, held) && is_shared(r, at);
+        need += __popcll(__ballot(sh));
+      }
+      if (lane == 0) start[r] = need;
+    }
+    __syncthreads();
+  }
+  int64_t asked = 0;
+  int given = 0;   // ranks handed out
+  for (int r0 = 0; r0 < p.R; r0 += kPoolThreads) {
+    const int r = r0 + tid;
+    int need = 0, length = 0, want = 0, c0 = 0, c1 = 0;
+    bool fits = true, last = false;
+    if (r < p.R) {
+      fits = columns(r, length, want, c0, c1);
+      if (kFrom) {
+        need = start[r];
+      } else {
+        const int held = pages_of(p, length);
+        last = c0 < held && c0 < c1 && is_shared(r, c0);
+        need = c1 - max(c0, held) + last;
+        if (c1 <= c0) need = 0;
+      }
+    }
+    int64_t total;
+    const int64_t before = asked + pool_scan(need, sums, total);
+    asked += total;
+    const bool served = need == 0 || before + need <= have;
+    const int got = served ? need : 0;
+    int64_t sum;
+    const int rank = given + (int)pool_scan(got, sums, sum);
+    given += (int)sum;
+    if (r < p.R) {
+      start[r] = rank;
+      if (!kFrom) {
+        shared_last[r] = last && served;
+        a.source[r] = -1;
+        a.target[r] = -1;
+      }
+      const bool done = fits && served;
+      a.ok[r] = done;
+      // (kFrom: below, after the columns have been read once more)
+      if (!kFrom && got == 0 && done && want > length) p.lengths[r] = want;
+    }
+  }
+  if (tid == 0) start[p.R] = given;
+  __syncthreads();
+
+  // the lowest free pages, in rank order
+  int base = 0;
+  for (int w0 = 0; base < given; w0 += kPoolThreads) {
+    const int w = w0 + tid;
+    uint32_t bits = w < words ? p.free[w] & page_bits(p, w) : 0u;
+    int64_t total;
+    int rank = base + (int)pool_scan(__popc(bits), sums, total);
+    base += (int)total;
+    if (bits && rank < given) {
+      uint32_t kept = p.free[w];
+      int r = 0;
+      if (!kFrom) {   // the request of the first rank: the last one that starts at or before it
+        int lo = 0, hi = p.R;
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (start[mid] <= rank) lo = mid;
+          else hi = mid;
+        }
+        r = lo;
+      }
+      for (; bits && rank < given; ++rank) {
+        const int bit = __ffs((int)bits) - 1, page = w * 32 + bit;
+        bits &= bits - 1;
+        kept &= ~(1u << bit);
+        p.refs[page] = 1;
+        if (kFrom) {
+          a.ids[rank] = page;
+        } else {
+          while (start[r + 1] <= rank) ++r;
+          int length, want, c0, c1;
+          columns(r, length, want, c0, c1);
+          const int j = rank - start[r], held = pages_of(p, length);
+          const bool copy = shared_last[r] && j == 0;
+          const int c = copy ? c0 : held + j - shared_last[r];
+          int32_t* entry = p.tables + r * p.t_st + c;
+          if (copy) {
+            a.source[r] = *entry;
+            a.target[r] = page;
+          }
+          *entry = page;
+        }
+      }
+      p.free[w] = kept;
+    }
+  }
+  __syncthreads();
+
+  if (!kFrom) {
+    // lengths, and the pages that were copied from lose a holder (after all free bits have been read)
+    for (int r = tid; r < p.R; r += kPoolThreads)
+      if (start[r + 1] > start[r]) {
+        if (shared_last[r]) drop_page(p, a.source[r]);
+        p.lengths[r] = a.to[r];
+      }
+  } else {
+    for (int r = wave; r < p.R; r += kPoolWaves) {
+      int length, want, c0, c1;
+      columns(r, length, want, c0, c1);
+      const int held = pages_of(p, length), n = start[r + 1] - start[r];
+      int rank = start[r];
+      // (shared pages are looked for as they were: counts of copied pages change behind the barrier below)
+      for (int c = 0; c < p.cols; c += 64) {
+        const int at = c + lane;
+        const bool takes = n > 0 && at >= c0 && at < c1 && (at >= held || is_shared(r, at));
+        const uint64_t mask = __ballot(takes);
+        int32_t from = -1, page = -1;
+        if (takes) {
+          page = a.ids[rank + __popcll(mask & ((1ull << lane) - 1))];
+          int32_t* entry = p.tables + r * p.t_st + at;
+          if (at < held) from = *entry;
+          *entry = page;
+        }
+        rank += __popcll(mask);
+        if (at < p.cols) {
+          a.source[(int64_t)r * p.cols + at] = from;
+          a.target[(int64_t)r * p.cols + at] = from >= 0 ? page : -1;
+        }
+      }
+      if (lane == 0 && a.ok[r] && want > length) p.lengths[r] = want;
+    }
+    __syncthreads();
+    for (int64_t i = tid; i < (int64_t)p.R * p.cols; i += kPoolThreads)
+      if (a.source[i] >= 0) drop_page(p, a.source[i]);
+  }
+}
+
+// ---- compaction --------------------------------------------------------------------------------------------------
+// With U pages in use, the i-th page in use at or behind U moves to the i-th free place before it. pool_pairs_kernel finds the
+// pairs, place[page] for the pages that move, place[N] = U and place[N + 1] = their number; pool_compact_kernel then rewrites tables, counts and bits.
+__global__ __launch_bounds__(kPoolThreads) void pool_pairs_kernel(Pool p, int32_t* source, int32_t* target, int32_t* place) {
+  __shared__ int64_t sums[kPoolWaves + 1];
+  const int tid = threadIdx.x, words = (p.N + 31) / 32;
+  int64_t total, empty = 0;
+  for (int w0 = 0; w0 < words; w0 += kPoolThreads) {
+    pool_scan(__popc(w0 + tid < words ? p.free[w0 + tid] & page_bits(p, w0 + tid) : 0u), sums, total);
+    empty += total;
+  }
+  const int used = p.N - (int)empty;
+  int moved = 0;
+  for (int pass = 0; pass < 2; ++pass) {   // holes, then movers
+    const int first = pass ? used / 32 : 0, end = pass ? words : (used + 31) / 32;
+    int base = 0;
+    for (int w0 = first; w0 < end; w0 += kPoolThreads) {
+      const int w = w0 + tid;
+      uint32_t bits = 0;
+      if (w < end) {
+        bits = p.free[w];
+        const int cut = used - 32 * w;   // pages of this word before U
+        const uint32_t below = cut >= 32 ? ~0u : cut <= 0 ? 0u : (1u << cut) - 1;
+        bits = pass ? ~bits & ~below & page_bits(p, w) : bits & below;
+      }
+      int rank = base + (int)pool_scan(__popc(bits), sums, total);
+      base += (int)total;
+      for (; bits; bits &= bits - 1, ++rank) {
+        const int page = w * 32 + __ffs((int)bits) - 1;
+        (pass ? source : target)[rank] = page;
+      }
+    }
+    moved = base;
+    __syncthreads();
+  }
+  for (int i = tid; i < p.N / 2; i += kPoolThreads) {
+    if (i < moved) place[source[i]] = target[i];
+    else source[i] = target[i] = -1;
+  }
+  if (tid == 0) {
+    place[p.N] = used;
+    place[p.N + 1] = moved;
+  }
+}
+
+__global__ __launch_bounds__(256) void pool_compact_kernel(Pool p, const int32_t* source, const int32_t* target,
+                                                           const int32_t* place, int words) {
+  const int used = place[p.N], moved = place[p.N + 1];
+  const int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
+  for (int64_t i = i0; i < (int64_t)p.R * p.cols; i += step) {
+    const int r = (int)(i / p.cols), c = (int)(i % p.cols);
+    if (c >= pages_of(p, rows_of(p, p.lengths[r]))) continue;
+    int32_t* entry = p.tables + r * p.t_st + c;
+    const int32_t page = *entry;
+    if (page >= used && page < p.N) *entry = place[page];
+  }
+  for (int64_t i = i0; i < moved; i += step) {
+    p.refs[target[i]] = p.refs[source[i]];
+    p.refs[source[i]] = 0;
+  }
+  for (int64_t w = i0; w < words; w += step) {
+    const int64_t cut = used - 32 * w;
+    const uint32_t below = cut >= 32 ? ~0u : cut <= 0 ? 0u : (1u << cut) - 1;
+    p.free[w] = ~below & page_bits(p, (int)w);
+  }
+}
+
+// ---- copies ------------------------------------------------------------------------------------------------------
+// Page target[i] of every cache becomes page source[i], in units of 16 bytes (or single ones). A workgroup takes kPiece bytes
+// of a page, of `per` list entries one after the other (64 of a list that may be mostly -1: a look at 64 at a time).
+constexpr int kMaxCaches = 128;
+constexpr int kPiece = 16384;
+
+struct CopyParams {
+  uint8_t* caches[kMaxCaches];
+  int64_t page_stride, page_bytes, num_pages;
+  const int32_t *source, *target;
+  int64_t count;
+  int per, pieces;
+};
+
+template <typename Unit>
+__global__ __launch_bounds__(256) void copy_pages_kernel(CopyParams a) {
+  constexpr int U = kPiece / sizeof(Unit) / 256;
+  const int lane = threadIdx.x & 63;
+  uint8_t* cache = a.caches[blockIdx.y];
+  const int64_t at = (int64_t)(blockIdx.x % a.pieces) * kPiece;
+  const int64_t units = min((int64_t)kPiece, a.page_bytes - at) / (int64_t)sizeof(Unit);
+  const int64_t e0 = (int64_t)(blockIdx.x / a.pieces) * a.per;
+  int32_t s = -1, d = -1;
+  if (lane < a.per && e0 + lane < a.count) {
+    s = a.source[e0 + lane];
+    d = a.target[e0 + lane];
+  }
+  const bool valid = s >= 0 && s < a.num_pages && d >= 0 && d < a.num_pages && s != d;
+  for (uint64_t left = __ballot(valid); left; left &= left - 1) {
+    const int i = __ffsll((unsigned long long)left) - 1;
+    const Unit* from = reinterpret_cast<const Unit*>(cache + (int64_t)__shfl(s, i) * a.page_stride + at);
+    Unit* to = reinterpret_cast<Unit*>(cache + (int64_t)__shfl(d, i) * a.page_stride + at);
+    if constexpr (sizeof(Unit) == 16) {
+      Unit v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (threadIdx.x + 256 * u < units) v[u] = from[threadIdx.x + 256 * u];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (threadIdx.x + 256 * u < units) to[threadIdx.x + 256 * u] = v[u];
+    } else {
+      for (int64_t u = threadIdx.x; u < units; u += 256) to[u] = from[u];
+    }
+  }
+}
+
+int check_pool(const char* what, const int32_t* tables, int64_t t_st, int R, int cols, const int32_t* lengths,
+               const int32_t* refs, int64_t N, const void* free, int block) {
+  HLA_REQUIRE(R >= 0 && R <= kMaxRequests && cols >= 0 && N >= 0 && N <= INT32_MAX - 64 && block >= 1, HLA_S6_EINVAL,
+              "%s: bad request count (0..%d), table width, page count or block size", what, kMaxRequests);
+  HLA_REQUIRE(R == 0 || lengths, HLA_S6_EINVAL, "%s: null lengths", what);
+  HLA_REQUIRE(R == 0 || cols == 0 || tables, HLA_S6_EINVAL, "%s: null tables", what);
+  HLA_REQUIRE(N == 0 || (refs && free), HLA_S6_EINVAL, "%s: null page state", what);
+  HLA_REQUIRE(t_st >= cols || R <= 1, HLA_S6_EINVAL, "%s: table rows overlap", what);
+  return HLA_S6_OK;
+}
+
+}  // namespace
+}  // namespace hla
+
+#define HLA_POOL(what)                                                                                       \
+  int rc = check_pool(what, tables, t_st, num_reqs, cols, lengths, refs, num_pages, free_bits, block_size);  \
+  if (rc != HLA_S6_OK) return rc;                                                                            \
+  const Pool p = {tables, t_st, num_reqs, cols, lengths, refs, (int)num_pages, free_bits, block_size}
+
+extern "C" int hla_s6_pool_release(int32_t* tables, int64_t t_st, int32_t num_reqs, int32_t cols, int32_t* lengths,
+                                   int32_t* refs, int64_t num_pages, uint32_t* free_bits, int32_t block_size,
+                                   const int32_t* requests, const int32_t* to, int32_t count, void* stream) {
+  using namespace hla;
+  HLA_POOL("pool_release");
+  HLA_REQUIRE(count >= 0 && (count == 0 || requests), HLA_S6_EINVAL, "pool_release: bad list");
+  if (count == 0 || num_reqs == 0) return HLA_S6_OK;
+  hipLaunchKernelGGL(pool_release_kernel, dim3((unsigned)count), dim3(256), 0, as_stream(stream), p, requests, to);
+  return check_launch("pool_release");
+}
+
+extern "C" int hla_s6_pool_fork(int32_t* tables, int64_t t_st, int32_t num_reqs, int32_t cols, int32_t* lengths,
+                                int32_t* refs, int64_t num_pages, uint32_t* free_bits, int32_t block_size,
+                                const int32_t* parents, const int32_t* children, int32_t count, uint8_t* ok, void* stream) {
+  using namespace hla;
+  HLA_POOL("pool_fork");
+  HLA_REQUIRE(count >= 0 && count <= kMaxRequests && (count == 0 || (parents && children && ok)), HLA_S6_EINVAL,
+              "pool_fork: bad lists (at most %d entries)", kMaxRequests);
+  if (count == 0) return HLA_S6_OK;
+  hipLaunchKernelGGL(pool_fork_kernel, dim3((unsigned)count), dim3(256), 0, as_stream(stream), p, parents, children, count, ok);
+  return check_launch("pool_fork");
+}
+
+extern "C" int hla_s6_pool_extend(int32_t* tables, int64_t t_st, int32_t num_reqs, int32_t cols, int32_t* lengths,
+                                  int32_t* refs, int64_t num_pages, uint32_t* free_bits, int32_t block_size,
+                                  const int32_t* to, const int32_t* from, uint8_t* ok, int32_t* source, int32_t* target,
+                                  int32_t* scratch, void* stream) {
+  using namespace hla;
+  HLA_POOL("pool_extend");
+  if (num_reqs == 0) return HLA_S6_OK;
+  HLA_REQUIRE(to && ok && ((source && target && (!from || scratch)) || (from && cols == 0)), HLA_S6_EINVAL,
+              "pool_extend: null pointer argument");
+  HLA_REQUIRE(!from || (int64_t)num_reqs * cols <= INT32_MAX, HLA_S6_EINVAL, "pool_extend: too many table entries");
+  const ExtendParams a = {p, to, from, ok, source, target, scratch};
+  if (from) hipLaunchKernelGGL(pool_extend_kernel<true>, dim3(1), dim3(kPoolThreads), 0, as_stream(stream), a);
+  else hipLaunchKernelGGL(pool_extend_kernel<false>, dim3(1), dim3(kPoolThreads), 0, as_stream(stream), a);
+  return check_launch("pool_extend");
+}
+
+extern "C" int hla_s6_pool_compact(int32_t* tables, int64_t t_st, int32_t num_reqs, int32_t cols, int32_t* lengths,
+                                   int32_t* refs, int64_t num_pages, uint32_t* free_bits, int32_t block_size,
+                                   int32_t* source, int32_t* target, int32_t* scratch, void* stream) {
+  using namespace hla;
+  HLA_POOL("pool_compact");
+  if (num_pages == 0) return HLA_S6_OK;
+  HLA_REQUIRE(scratch && (num_pages < 2 || (source && target)), HLA_S6_EINVAL, "pool_compact: null pointer argument");
+  const hipStream_t st = as_stream(stream);
+  hipLaunchKernelGGL(pool_pairs_kernel, dim3(1), dim3(kPoolThreads), 0, st, p, source, target, scratch);
+  const int words = (int)((num_pages + 31) / 32);
+  const int64_t most = (int64_t)num_reqs * cols > num_pages ? (int64_t)num_reqs * cols : num_pages;
+  const unsigned grid = (unsigned)((most + 1023) / 1024 < 1024 ? (most + 1023) / 1024 : 1024);
+  hipLaunchKernelGGL(pool_compact_kernel, dim3(grid), dim3(256), 0, st, p, source, target, scratch, words);
+  return check_launch("pool_compact");
+}
+
+extern "C" int hla_s6_copy_pages(void* const* caches, int32_t num_caches, int64_t page_stride, int64_t page_bytes,
+                                 int64_t num_pages, const int32_t* source, const int32_t* target, int64_t count,
+                                 void* stream) {
+  using namespace hla;
+  HLA_REQUIRE(num_caches >= 0 && page_bytes >= 0 && num_pages >= 0 && count >= 0, HLA_S6_EINVAL, "copy_pages: negative size");
+  HLA_REQUIRE(page_stride >= page_bytes || num_pages <= 1, HLA_S6_EINVAL, "copy_pages: pages overlap");
+  if (num_caches == 0 || page_bytes == 0 || count == 0 || num_pages == 0) return HLA_S6_OK;
+  HLA_REQUIRE(caches && source && target, HLA_S6_EINVAL, "copy_pages: null pointer argument");
+  const hipStream_t st = as_stream(stream);
+  CopyParams a = {};
+  a.page_stride = page_stride;
+  a.page_bytes = page_bytes;
+  a.num_pages = num_pages;
+  a.source = source;
+  a.target = target;
+  a.count = count;
+  const int64_t pieces = (page_bytes + kPiece - 1) / kPiece;
+  a.per = count > 4096 ? 64 : 1;
+  const int64_t groups = (count + a.per - 1) / a.per;
+  HLA_REQUIRE(groups * pieces <= INT32_MAX, HLA_S6_EINVAL, "copy_pages: lists or pages too long");
+  a.pieces = (int)pieces;
+  for (int c0 = 0; c0 < num_caches; c0 += kMaxCaches) {
+    const int n = num_caches - c0 < kMaxCaches ? num_caches - c0 : kMaxCaches;
+    bool vec = page_stride % 16 == 0 && page_bytes % 16 == 0;
+    for (int c = 0; c < n; ++c) {
+      HLA_REQUIRE(caches[c0 + c], HLA_S6_EINVAL, "copy_pages: null cache");
+      a.caches[c] = static_cast<uint8_t*>(caches[c0 + c]);
+      vec = vec && (reinterpret_cast<uintptr_t>(caches[c0 + c]) & 15u) == 0;
+    }
+    const dim3 grid((unsigned)(groups * pieces), (unsigned)n);
+    if (vec) hipLaunchKernelGGL(copy_pages_kernel<u32x4>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(copy_pages_kernel<uint8_t>, grid, dim3(256), 0, st, a);
+  }
+  return check_launch("copy_pages");
+}

@@ -1,0 +1,116 @@
+"""Whole exact caches on MI355X: attention of new tokens over all rows of a paged per-head K / V cache, and the store into it.
+
+The S6 path reads exact K / V in a window of a few rows. Layers and loops that keep their exact cache, and the teacher that a
+latent model is measured against, attend to all of it: ``attention`` does, for single tokens, with any number of query heads per
+KV head, and ``store_rows`` writes the rows of new tokens.
+
+A cache is ``[num_blocks, KV heads, block, 2d]`` (K then V, the layout of the exact window; any strides, the last one 1), ``d`` 64,
+128 or 256, in bf16 or in ``torch.float8_e4m3fn``. The values of an e4m3 cache count times a scale per KV head (``k_scale``,
+``v_scale``: fp32 ``[KV heads]``; None: 1). A page has any number of rows.
+
+Checks, streams and errors are those of ``compact_cache``.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib, s6_ops
+from .compact_cache import _call, _same_device, _table, _vector
+
+BF16, E4M3, F32, I32, I64 = torch.bfloat16, torch.float8_e4m3fn, torch.float32, torch.int32, torch.int64
+DIMS = (64, 128, 256)
+MAX_SPLITS = 256
+
+
+def _cache(cache, k_scale, v_scale):
+    """``(KV heads, d, e4m3, page, head and row stride, block, pages)`` of an exact cache, checked."""
+    shape, stride = cache.shape, cache.stride()
+    if cache.dtype != BF16 and cache.dtype != E4M3:
+        raise ValueError(f'an exact cache is bfloat16 or float8_e4m3fn, got {cache.dtype}')
+    if len(shape) != 4 or shape[3] % 2 or shape[3] // 2 not in DIMS:
+        raise ValueError(f'an exact cache is [num_blocks, KV heads, block, 2d] with d in {DIMS}, got {tuple(shape)}')
+    if stride[3] != 1:
+        raise ValueError('an exact cache needs a unit last-dim stride')
+    e4m3 = cache.dtype == E4M3
+    for name, scale in (('k_scale', k_scale), ('v_scale', v_scale)):
+        if scale is not None:
+            if not e4m3:
+                raise ValueError(f'{name} belongs to a float8_e4m3fn cache, got {cache.dtype}')
+            if scale.dtype != F32 or tuple(scale.shape) != (shape[1],) or not scale.is_contiguous():
+                raise ValueError(f'{name} must be contiguous fp32 [{shape[1]}], got {scale.dtype} {tuple(scale.shape)}')
+    return shape[1], shape[3] // 2, e4m3, stride[0], stride[1], stride[2], shape[2], shape[0]
+
+
+def store_rows(key, value, slots, cache, k_scale=None, v_scale=None):
+    """``key`` and ``value`` (bf16 ``[T, KV heads, d]``, any token and head strides) into slots (int64 ``[T]``, ``page * block +
+    row``) of an exact cache; slots outside the cache are skipped, and the slots of a call must differ.
+
+    Into an e4m3 cache goes ``x / scale`` (fp32), clamped to +-448 and rounded to the nearest value, ties to the even one; NaN
+    stays NaN."""
+    _same_device(cache, key, value, slots, k_scale, v_scale)
+    kv_heads, d, e4m3, page, head, row, block, pages = _cache(cache, k_scale, v_scale)
+    s6_ops._bf16('key', key)
+    s6_ops._bf16('value', value)
+    if key.dim() != 3 or key.shape != value.shape or key.shape[1] != kv_heads or key.shape[2] != d:
+        raise ValueError(f'key and value must be [T, {kv_heads}, {d}] alike, got {tuple(key.shape)} and {tuple(value.shape)}')
+    T = key.shape[0]
+    slots = _vector('slots', slots, T, I64)
+    _call('hla_s6_exact_store', cache.device, key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
+          value.stride(1), T, kv_heads, d, slots.data_ptr(), _lib.ptr(k_scale), _lib.ptr(v_scale), cache.data_ptr(), int(e4m3),
+          page, head, row, block, pages)
+
+
+def kv_splits(max_rows, groups, cu_count=256):
+    """``(split slots per row, workgroups wanted)`` of ``attention`` for rows of at most ``max_rows`` and ``groups`` (token, KV
+    head) pairs. A function of constants and the row count only (graph-stable)."""
+    wanted = 4 * cu_count
+    slots = min(MAX_SPLITS, -(-max_rows // 128), -(-2 * wanted // max(1, groups)))
+    return max(1, slots), wanted
+
+
+def attention(q, cache, block_table, ctx, scale, max_seq_len, token_requests=None, window=0, k_scale=None, v_scale=None,
+              num_kv_splits=None, workspace=None):
+    """Attention of ``q [T, H, d]`` (bf16, any token and head strides) over the rows ``[max(0, n - window), n)`` of ``n = ctx[t]``
+    (int32; ``window`` 0: over all ``n``) of an exact cache: ``(o [T, H, d] bf16, lse [H, T] fp32)``. ``H`` is a multiple of the
+    cache's KV heads, and query head ``h`` reads KV head ``h // (H / KV heads)``. Tokens without rows give ``o = 0``, ``lse = -inf``.
+
+    The rows of a token are those before it and its own, once ``store_rows`` has written it; tokens of one request (a chunk) have a
+    ``ctx`` of their own each. ``block_table`` (int32) is per token, or per request with ``token_requests[t]`` (int64) naming the
+    row of token ``t``. No entry of ``ctx`` should be above ``max_seq_len`` (a host number, which sets how rows are cut). Scores,
+    softmax statistics and sums are fp32; the weights are rounded to bf16 for their product with V.
+
+    ``num_kv_splits`` (slots per row, 1 to 256) defaults to ``kv_splits``; ``workspace`` (an ``S6Workspace``) to a new buffer. Calls
+    that share a workspace must not overlap."""
+    _same_device(cache, q, block_table, ctx, token_requests, k_scale, v_scale)
+    kv_heads, d, e4m3, page, head, row, block, pages = _cache(cache, k_scale, v_scale)
+    s6_ops._bf16('q', q)
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != d or shape[1] % kv_heads or not shape[1]:
+        raise ValueError(f'q must be [T, a multiple of {kv_heads} heads, {d}], got {tuple(shape)}')
+    T, H, _ = shape
+    ctx = _vector('ctx', ctx, T)
+    table_stride, cols, count = _table(block_table, T if token_requests is None else min(T, 1))
+    if token_requests is not None:
+        token_requests = _vector('token_requests', token_requests, T, I64)
+    window = int(window)
+    if window < 0:
+        raise ValueError(f'window must not be negative, got {window}')
+    dev = q.device
+    longest = min(int(max_seq_len), cols * block, window or cols * block)
+    groups = T * kv_heads * -(-H // kv_heads // 16)
+    splits, wanted = kv_splits(longest, groups, _lib.device_cus(dev.index))
+    if num_kv_splits is not None:
+        splits = int(num_kv_splits)
+    ws = None
+    if splits > 1:
+        ws = (torch.empty(T * H * splits * (d + 1), dtype=F32, device=dev) if workspace is None
+              else workspace.attn_logits(T, H, splits, d, dev))
+        _same_device(q, ws)   # (a workspace keeps the device of its first use)
+    out = torch.empty(T, H, d, dtype=BF16, device=dev)
+    lse = torch.empty(H, T, dtype=F32, device=dev)
+    token_stride, head_stride, _ = q.stride()
+    _call('hla_s6_exact_attention', dev, q.data_ptr(), T, H, d, token_stride, head_stride, cache.data_ptr(), int(e4m3), kv_heads,
+          page, head, row, block, pages, block_table.data_ptr(), table_stride, cols, count, _lib.ptr(token_requests),
+          ctx.data_ptr(), window, float(scale), _lib.ptr(k_scale), _lib.ptr(v_scale), splits, wanted, _lib.ptr(ws),
+          0 if ws is None else ws.numel(), out.data_ptr(), H * d, d, lse.data_ptr())
+    return out, lse

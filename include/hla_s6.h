@@ -24,7 +24,7 @@
 extern "C" {
 #endif
 
-#define HLA_S6_ABI_VERSION 16
+#define HLA_S6_ABI_VERSION 17
 
 #define HLA_S6_OK 0
 #define HLA_S6_EINVAL 1       /* bad shape, stride or argument            (Python: ValueError)   */
@@ -579,6 +579,71 @@ int hla_s6_move_rows(void *cache, int32_t width, int32_t compact, int64_t page_s
                      int32_t block_size, int64_t num_blocks, const int32_t *block_table, int64_t bt_stride,
                      int32_t bt_cols, const int32_t *source, const int32_t *target, int64_t list_st, int32_t count,
                      int32_t num_reqs, void *stream);
+
+/* ---- exact paged caches ------------------------------------------------------------------------------
+ * Pages of block_size rows (any count >= 1) of kv_heads heads, [K | V] of 2 * head_dim values each: bf16, or (e4m3 != 0) e4m3
+ * bytes times a scale per KV head (k_scale, v_scale fp32 [kv_heads]; NULL: 1). Strides in elements of the cache, multiples of
+ * 16 bytes; head_dim in {64, 128, 256}.
+ *
+ * hla_s6_exact_attention: out[t, h] (bf16) = softmax over the rows [max(0, n - window), n) of n = ctx[t] (window 0: all) of
+ * scale * q[t, h] . K[row, h / (num_heads / kv_heads)], times V; lse [num_heads, num_tokens]. Token t reads row bt_rows ?
+ * bt_rows[t] : t of the table, clamped into its bt_count rows; page ids are clamped into the cache; at most bt_cols * block_size
+ * rows. num_splits (1..256) slots per row, cut so that about `workgroups` of them hold rows; with more than one the workspace
+ * holds num_tokens * num_heads * num_splits * (head_dim + 1) floats. */
+int hla_s6_exact_attention(const void *q, int32_t num_tokens, int32_t num_heads, int32_t head_dim, int64_t q_st,
+                           int64_t q_sh, const void *cache, int32_t e4m3, int32_t kv_heads, int64_t page_stride,
+                           int64_t head_stride, int64_t row_stride, int32_t block_size, int64_t num_blocks,
+                           const int32_t *block_table, int64_t bt_stride, int32_t bt_cols, int32_t bt_count,
+                           const int64_t *bt_rows, const int32_t *ctx, int32_t window, float scale,
+                           const float *k_scale, const float *v_scale, int32_t num_splits, int32_t workgroups,
+                           float *workspace, int64_t workspace_floats, void *out, int64_t o_st, int64_t o_sh, float *lse,
+                           void *stream);
+
+/* Row t of key / value (bf16 [num_tokens, kv_heads, head_dim]) into slot slots[t] (page * block_size + row; outside the cache:
+ * skipped; the slots of a call differ). e4m3: x / scale, clamped to +-448, to the nearest, ties to even; NaN stays NaN. */
+int hla_s6_exact_store(const void *key, int64_t k_st, int64_t k_sh, const void *value, int64_t v_st, int64_t v_sh,
+                       int32_t num_tokens, int32_t kv_heads, int32_t head_dim, const int64_t *slots,
+                       const float *k_scale, const float *v_scale, void *cache, int32_t e4m3, int64_t page_stride,
+                       int64_t head_stride, int64_t row_stride, int32_t block_size, int64_t num_blocks, void *stream);
+
+/* ---- pools of pages ----------------------------------------------------------------------------------
+ * tables [num_reqs, cols] (row stride t_st): the pages of request r, -1 behind its last; lengths [num_reqs]: its rows; refs
+ * [num_pages]: requests that hold a page; free_bits [ceil(num_pages / 32)]: bit p % 32 of word p / 32 is set where refs[p] ==
+ * 0. num_reqs <= 8192. Results do not depend on the order in which requests are worked on.
+ *
+ * hla_s6_pool_release: request requests[i] (outside the pool: skipped) keeps its first to[i] rows (to NULL: none); pages behind
+ * them lose a holder. Of a request named twice the shorter length holds. */
+int hla_s6_pool_release(int32_t *tables, int64_t t_st, int32_t num_reqs, int32_t cols, int32_t *lengths, int32_t *refs,
+                        int64_t num_pages, uint32_t *free_bits, int32_t block_size, const int32_t *requests,
+                        const int32_t *to, int32_t count, void *stream);
+
+/* Request children[i] takes over the pages and length of parents[i]; ok[i] 0 and nothing done where a number is outside the
+ * pool, the child has rows or was named before, or the parent is among the children. count <= 8192. */
+int hla_s6_pool_fork(int32_t *tables, int64_t t_st, int32_t num_reqs, int32_t cols, int32_t *lengths, int32_t *refs,
+                     int64_t num_pages, uint32_t *free_bits, int32_t block_size, const int32_t *parents,
+                     const int32_t *children, int32_t count, uint8_t *ok, void *stream);
+
+/* Room for the rows [from[r], to[r]) of every request (from NULL: lengths[r]), whose length becomes max(lengths[r], to[r]):
+ * columns behind its last page get the lowest free pages, in the order of requests and columns; columns with rows to write
+ * whose page others hold too get one that takes its place, and (source, target) say what to copy. A request is served if it and
+ * those before it that ask for pages ask for no more than there are, and to[r] fits the table; else ok[r] is 0 and nothing is
+ * changed. Lists: [num_reqs], or with `from` [num_reqs, cols], -1 where nothing is to be copied; scratch [num_reqs * cols] with
+ * `from`. */
+int hla_s6_pool_extend(int32_t *tables, int64_t t_st, int32_t num_reqs, int32_t cols, int32_t *lengths, int32_t *refs,
+                       int64_t num_pages, uint32_t *free_bits, int32_t block_size, const int32_t *to,
+                       const int32_t *from, uint8_t *ok, int32_t *source, int32_t *target, int32_t *scratch, void *stream);
+
+/* With U pages in use, the i-th page in use at or behind U takes the i-th free place before it, in tables, refs and free_bits;
+ * (source, target) [num_pages / 2], -1 behind the last, say what to copy. scratch [num_pages + 2]. */
+int hla_s6_pool_compact(int32_t *tables, int64_t t_st, int32_t num_reqs, int32_t cols, int32_t *lengths, int32_t *refs,
+                        int64_t num_pages, uint32_t *free_bits, int32_t block_size, int32_t *source, int32_t *target,
+                        int32_t *scratch, void *stream);
+
+/* Page target[i] of every cache becomes its page source[i] (pairs with a number outside [0, num_pages) are skipped), whole
+ * pages of page_bytes at a stride of page_stride bytes. `caches` is a host array of device pointers. No source may be another
+ * pair's target, nor a target named twice. */
+int hla_s6_copy_pages(void *const *caches, int32_t num_caches, int64_t page_stride, int64_t page_bytes,
+                      int64_t num_pages, const int32_t *source, const int32_t *target, int64_t count, void *stream);
 
 #ifdef __cplusplus
 }
