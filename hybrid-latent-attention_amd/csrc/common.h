@@ -155,12 +155,17 @@ __device__ __forceinline__ void copy16_to_lds_v(const void* src, const void* lds
                : "memory", "m0");
 }
 
-// The same where the compiler may hold the (uniform) LDS address in a VGPR.
+// The same where the compiler may hold the (uniform) LDS address in a VGPR; kOnce: past the caches, for bytes read once.
+template <bool kOnce>
 __device__ __forceinline__ void copy16_to_lds_rfl_v(const void* src, const void* lds) {
   const uint32_t dst = __builtin_amdgcn_readfirstlane(
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src)
-               : "memory", "m0");
+  if (kOnce)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(dst), "v"(src)
+                 : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src)
+                 : "memory", "m0");
 }
 
 // 4 bytes per lane from a per-lane source address to LDS address lds + 4 i (a gather of scattered words).

@@ -3,8 +3,10 @@
 // A cache page holds `block` rows of every KV head, [K | V] of 2d values in bf16 or e4m3; G query heads read one KV head.
 //   o[t, h] = sum_j softmax_j(scale q[t, h] . K[j]) V[j], j over the rows [max(0, n - window), n) of n = ctx[t].
 //
-// A workgroup takes the rows of one (token, KV head, up to 16 of its query heads, slot): the token's rows are cut in slots of
-// equal length, whose partials exact_join_kernel joins. Each of its waves walks tiles of kKeys rows of its own:
+// A workgroup takes a share of the rows of one KV head for up to 16 of its query heads. The rows of all tokens, one token behind
+// the other, are cut in shares of equal length: every workgroup has as much to stream, however ragged the lengths are. What a
+// share holds of a token is a part, whole tokens are written at once, and exact_join_kernel joins the parts of the others. (With
+// rows enough for the device, or short ones, a workgroup takes all rows of a token.) Each wave walks tiles of its own:
 //   * a tile's K and V rows come by direct copies into LDS, a KB each, NB - 1 tiles ahead (the stream is what bounds the
 //     kernel: 2d values per row and head are read once and meet 4 G d flops); the 16-byte pieces of a row lie swizzled, so
 //     that both ways of reading them below touch every bank once;
@@ -15,18 +17,17 @@
 //     LDS loads. bf16 tiles have 16 keys (16x16x16 products), e4m3 ones 32, in the order of keys that the two halves of the
 //     scores have (16x16x32), and e4m3 values become bf16, exactly, on their way into the operands.
 // P is rounded to bf16 for its product (half a step, 2^-9 of each weight; the output is bf16); sums are fp32.
-#include <type_traits>
-
 #include "common.h"
 
 namespace hla {
 namespace {
 
 constexpr int kMaxTile = 16;     // query heads per workgroup
-constexpr int kMaxSlots = 256;
+constexpr int kMaxShares = 1024;
 constexpr float kRaise = 8.f;    // log2 by which a score may exceed the running maximum
-// rows below which a slot is not worth a workgroup of its own (its partial is written and read once more)
-constexpr int kMinRows = 64;
+constexpr int kStep = 64;        // rows that shares are counted in
+// steps below which a share is not worth a workgroup of its own (its partial is written and read once more)
+constexpr int kMinSteps = 2;
 
 struct ExactCacheParams {
   const uint16_t* q;
@@ -44,9 +45,9 @@ struct ExactCacheParams {
   float scale_log2;
   const float *k_scale, *v_scale;
   int T, H, KH, G, tiles;  // tiles: workgroups of query heads per KV head
-  int S;
-  int64_t rows_wanted;     // workgroups that the rows of all tokens are spread over
-  float *ws_o, *ws_lse;    // [T][H][S][D], [T][H][S]
+  int shares;              // 0: a workgroup takes all rows of a token
+  float *ws_o, *ws_lse;    // [shares][2][H][D], [shares][2][H]
+  int32_t* split;          // [T][2]: first and last share of a token's rows
   uint16_t* out;
   int64_t o_st, o_sh;
   float* lse;  // [H][T]
@@ -58,11 +59,11 @@ struct ExactGeo {
   static constexpr bool kE4 = kE4m3;
   static constexpr int ES = kE4 ? 1 : 2;
   static constexpr int KEYS = kE4 ? 32 : 16;
-  static constexpr int RB = D * ES;              // bytes of a row's K (or V)
-  static constexpr int CPR = RB / 16;            // pieces of 16 bytes in them
+  static constexpr int RB = 2 * D * ES;          // bytes of a row, K and V
+  static constexpr int CPR = RB / 16;            // pieces of 16 bytes in it
   static constexpr int RPI = 64 / CPR;           // rows per copy of a wave
-  static constexpr int NI = KEYS / RPI;          // copies per tile, K and V each
-  static constexpr int TILE = 2 * KEYS * RB;     // bytes of a tile
+  static constexpr int NI = KEYS / RPI;          // copies per tile
+  static constexpr int TILE = KEYS * RB;         // bytes of a tile
   static constexpr int NB = !kE4 && TILE <= 4096 ? 4 : 2;
   static constexpr int WAVES = TILE > 8192 ? 2 : 4;
   static constexpr int BATCH = 64 / KEYS;        // tiles whose row addresses are worked out at a time
@@ -71,16 +72,12 @@ struct ExactGeo {
 
 // Where the pieces of row x of a tile lie: piece c at c ^ swizzle(x). Both reads go over 256 bytes of banks at a time: K by 16
 // lanes that take one piece of rows 0..15 (or 16..31), V by 32 lanes that take 32 bytes of rows 0..7 or 8..15 (bf16), or 16
-// bytes of rows 0..7 and 16..23, or 8..15 and 24..31 (e4m3). Rows share the 256 bytes where they are shorter.
+// bytes of rows 0..7 and 16..23, or 8..15 and 24..31 (e4m3). Rows of 128 bytes share the 256.
 template <class G>
 __device__ __forceinline__ int swizzle(int x) {
-  if (G::kE4) {
-    if (G::CPR == 4) return ((x >> 2) & 1) | ((((x >> 3) ^ (x >> 4)) & 1) << 1);
-    if (G::CPR == 8) return ((x >> 1) & 3) | ((((x >> 3) ^ (x >> 4)) & 1) << 2);
-    return (x & 7) | ((((x >> 3) ^ (x >> 4)) & 1) << 3);
-  }
-  if (G::CPR == 8) return (((x >> 1) & 3) << 1) | ((x >> 3) & 1);
-  return ((x & 7) << 1) | ((x >> 3) & 1);
+  if (!G::kE4) return ((x & 7) << 1) | ((x >> 3) & 1);
+  if (G::CPR == 8) return ((x >> 1) & 3) | ((((x >> 3) ^ (x >> 4)) & 1) << 2);
+  return (x & 7) | ((((x >> 3) ^ (x >> 4)) & 1) << 3);
 }
 
 // Waits that no memory access moves across, in either direction: for the copies into LDS but the N newest, and for LDS reads
@@ -97,32 +94,73 @@ __device__ __forceinline__ u32x4 e4m3_to_bf16(uint32_t lo, uint32_t hi) {
                __builtin_bit_cast(uint32_t, (bf16x2_t)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true))};
 }
 
+// A weight in two bf16 parts: its upper half, and the rest rounded. The rest of a weight that is not 0 is not 0 and not negative,
+// so that an infinity in V stays one.
+__device__ __forceinline__ uint32_t upper_halves(float a, float b) {
+  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+__device__ __forceinline__ uint32_t rests(float a, float b, uint32_t upper) {
+  return pack2(fmaxf(a - lo_bf(upper), a * 0x1p-40f), fmaxf(b - hi_bf(upper), b * 0x1p-40f));
+}
+
 // Rows of a token: [first, n)
 __device__ __forceinline__ void token_rows(const ExactCacheParams& a, int t, int& first, int& n) {
-  n = (int)min((int64_t)max(a.ctx[t], 0), min((int64_t)a.bt_cols * a.block, (int64_t)INT32_MAX));
+  n = (int)min((int64_t)max(a.ctx[t], 0), min((int64_t)a.bt_cols * a.block, (int64_t)INT32_MAX - kStep));
   first = a.window > 0 ? max(0, n - a.window) : 0;
 }
 
-// Rows per slot, the same for every token: no token has more than S slots, and the rows of all tokens and heads make about
-// rows_wanted workgroups, however many rows the longest has. Each wave works it out by itself.
-__device__ __forceinline__ int slot_rows(const ExactCacheParams& a, int lane, int step) {
-  int64_t most = 0, sum = 0;
-  for (int t = lane; t < a.T; t += 64) {
-    int first, n;
-    token_rows(a, t, first, n);
-    most = max(most, (int64_t)(n - first));
-    sum += n - first;
-  }
-  for (int off = 32; off > 0; off >>= 1) {
-    most = max(most, __shfl_xor(most, off));
-    sum += __shfl_xor(sum, off);
-  }
-  const int64_t share = (sum * a.KH * a.tiles + a.rows_wanted - 1) / a.rows_wanted;
-  const int64_t rows = max(max((most + a.S - 1) / a.S, share), (int64_t)kMinRows);
-  return (int)min((rows + step - 1) / step * step, (int64_t)INT32_MAX / 2);
+// Steps of a token's rows
+__device__ __forceinline__ int token_steps(const ExactCacheParams& a, int t) {
+  int first, n;
+  token_rows(a, t, first, n);
+  return (n - first + kStep - 1) / kStep;
 }
 
-template <class G>
+// Share k of the steps of all tokens, one token behind the other: a share is ceil(total / shares) of them, kMinSteps at least.
+// `left` steps of it (0: none) begin at step `at` of token t, whose first step is the `before`-th of all.
+__device__ __forceinline__ void find_share(const ExactCacheParams& a, int k, int threads, int64_t* sums, int64_t* found, int& t,
+                                           int& at, int64_t& left, int64_t& before, int64_t& share) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int seg = (a.T + threads - 1) / threads, t0 = min(a.T, tid * seg), t1 = min(a.T, t0 + seg);
+  int64_t mine = 0;
+  for (int i = t0; i < t1; ++i) mine += token_steps(a, i);
+  int64_t x = mine;
+  for (int off = 1; off < 64; off <<= 1) {
+    const int64_t y = __shfl_up(x, off);
+    if (lane >= off) x += y;
+  }
+  if (lane == 63) sums[wave] = x;
+  __syncthreads();
+  int64_t total = 0;
+  for (int w = 0; w < threads / 64; ++w) {
+    if (w < wave) x += sums[w];
+    total += sums[w];
+  }
+  total = uniform64(total);
+  share = max((total + a.shares - 1) / a.shares, (int64_t)kMinSteps);
+  const int64_t begin = k * share;
+  left = min(share, total - begin);
+  if (left <= 0) return;
+  int64_t base = x - mine;
+  if (begin >= base && begin < x)   // one thread's tokens hold it
+    for (int i = t0; i < t1; ++i) {
+      const int steps = token_steps(a, i);
+      if (begin < base + steps) {
+        found[0] = i;
+        found[1] = base;
+        break;
+      }
+      base += steps;
+    }
+  __syncthreads();
+  t = __builtin_amdgcn_readfirstlane((int)found[0]);
+  before = uniform64(found[1]);
+  at = (int)(begin - before);
+}
+
+// kOnce: rows are read by one workgroup and stream past the caches. kTwice: up to 8 query heads per workgroup, columns 8.. are
+// heads 0.. again.
+template <class G, bool kOnce, bool kTwice>
 __global__ __launch_bounds__(64 * G::WAVES) void exact_cache_kernel(ExactCacheParams a) {
   constexpr int D = G::D;
   constexpr bool kE4 = G::kE4;
@@ -134,293 +172,312 @@ __global__ __launch_bounds__(64 * G::WAVES) void exact_cache_kernel(ExactCachePa
   __shared__ int64_t offsets[WAVES][64];
   __shared__ int32_t page_ids[WAVES][64];
   __shared__ float stats[WAVES][2][16];
+  __shared__ int64_t sums[WAVES], found[2];
 
   const int tid = threadIdx.x, lane = tid & 63, x = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // item: heads innermost (workgroups dispatched one behind the other read the same rows' heads), then slots, then tokens
-  int item = blockIdx.x;
-  const int part = item % (a.KH * a.tiles);
-  item /= a.KH * a.tiles;
-  const int slot = item % a.S, t = item / a.S;
+  // heads innermost: workgroups dispatched one behind the other read the same rows' heads
+  const int parts = a.KH * a.tiles, part = blockIdx.x % parts, k = blockIdx.x / parts;
   const int kh = part / a.tiles, j0 = part % a.tiles * kMaxTile;
   const int heads = min(kMaxTile, a.G - j0), h0 = kh * a.G + j0;
+  const int head = kTwice ? x & 7 : x;
+  const uint8_t* cache = a.cache + kh * a.head_stride;
 
-  int first, n;
-  token_rows(a, t, first, n);
-  int lo = first, hi = n;
-  if (a.S > 1) {
-    const int rows = slot_rows(a, lane, WAVES * KEYS);
-    lo = (int)min((int64_t)n, first + (int64_t)slot * rows);
-    hi = (int)min((int64_t)n, (int64_t)lo + rows);
+  int t = k, at = 0;
+  int64_t left_steps = INT32_MAX, before = 0, share = 1;
+  if (a.shares) {
+    find_share(a, k, 64 * WAVES, sums, found, t, at, left_steps, before, share);
+    if (left_steps <= 0) return;
   }
-  const int64_t base = (int64_t)t * a.H + h0;  // row of the workgroup's first head in [T][H]
-  if (lo >= hi) {
-    if (a.S > 1) {
-      for (int j = tid; j < heads; j += 64 * WAVES) a.ws_lse[(base + j) * a.S + slot] = -INFINITY;
-    } else {
+  for (;;) {   // the tokens of the share
+    int first, n;
+    token_rows(a, t, first, n);
+    const int steps = (n - first + kStep - 1) / kStep;
+    const int taken = (int)min((int64_t)steps - at, left_steps);
+    const int lo = first + at * kStep, hi = (int)min((int64_t)n, (int64_t)lo + (int64_t)taken * kStep);
+    const bool whole = taken == steps;
+    if (a.shares && part == 0 && tid == 0 && at == 0 && steps > 0) {
+      a.split[2 * t] = k;
+      a.split[2 * t + 1] = (int)((before + steps - 1) / share);
+    }
+    if (lo >= hi && !a.shares) {
       for (int i = tid; i < heads * (D / 8); i += 64 * WAVES)
         st16(a.out + (int64_t)t * a.o_st + (int64_t)(h0 + i / (D / 8)) * a.o_sh + i % (D / 8) * 8, u32x4{0u, 0u, 0u, 0u});
       for (int j = tid; j < heads; j += 64 * WAVES) a.lse[(int64_t)(h0 + j) * a.T + t] = -INFINITY;
+      return;
     }
-    return;
-  }
+    if (lo < hi) {
+      const int64_t row = a.bt_rows ? min(max(a.bt_rows[t], (int64_t)0), (int64_t)a.bt_count - 1) : t;
+      const int32_t* btr = a.bt + row * a.bt_stride;
+      const int tiles = (hi - lo + KEYS - 1) / KEYS;
+      const int mine = tiles > wave ? (tiles - wave + WAVES - 1) / WAVES : 0;  // tiles wave, wave + WAVES, ...
 
-  const int64_t row = a.bt_rows ? min(max(a.bt_rows[t], (int64_t)0), (int64_t)a.bt_count - 1) : t;
-  const int32_t* btr = a.bt + row * a.bt_stride;
-  const uint8_t* cache = a.cache + kh * a.head_stride;
-  const int tiles = (hi - lo + KEYS - 1) / KEYS;
-  const int mine = tiles > wave ? (tiles - wave + WAVES - 1) / WAVES : 0;  // tiles wave, wave + WAVES, ...
-
-  // row of lane `lane` in the batch of tiles b: rows past the last are the last one again
-  auto batch_row = [&](int b) {
-    return (int)min((int64_t)hi - 1, lo + ((int64_t)wave + (int64_t)(b * G::BATCH + lane / KEYS) * WAVES) * KEYS + lane % KEYS);
-  };
-  auto fetch_ids = [&](int b) { copy4_to_lds_v(btr + (uint32_t)batch_row(b) / (uint32_t)a.block, page_ids[wave]); };
-  auto work_out = [&](int b) {
-    const int64_t page = min(max((int64_t)page_ids[wave][lane], (int64_t)0), a.num_blocks - 1);
-    offsets[wave][lane] = page * a.page_stride + (uint32_t)batch_row(b) % (uint32_t)a.block * a.row_stride;
-    wait_reads();   // (other lanes' writes, read by the requests)
-  };
-  const uint8_t* buf0 = lds + wave * (NB * G::TILE);
-  const int in_copy = lane / CPR, piece = lane % CPR;
-  // tile i of the wave on its way into buffer i % NB
-  auto request = [&](int i) {
-    const uint8_t* buf = buf0 + i % NB * G::TILE;
+      // row of lane `lane` in the batch of tiles b: rows past the last are the last one again
+      auto batch_row = [&](int b) {
+        return (int)min((int64_t)hi - 1, lo + ((int64_t)wave + (int64_t)(b * G::BATCH + lane / KEYS) * WAVES) * KEYS + lane % KEYS);
+      };
+      auto fetch_ids = [&](int b) { copy4_to_lds_v(btr + (uint32_t)batch_row(b) / (uint32_t)a.block, page_ids[wave]); };
+      auto work_out = [&](int b) {
+        const int64_t page = min(max((int64_t)page_ids[wave][lane], (int64_t)0), a.num_blocks - 1);
+        offsets[wave][lane] = page * a.page_stride + (uint32_t)batch_row(b) % (uint32_t)a.block * a.row_stride;
+        wait_reads();   // (other lanes' writes, read by the requests)
+      };
+      const uint8_t* buf0 = lds + wave * (NB * G::TILE);
+      const int in_copy = lane / CPR, piece = lane % CPR;
+      // tile i of the wave on its way into buffer i % NB
+      auto request = [&](int i) {
+        const uint8_t* buf = buf0 + i % NB * G::TILE;
 #pragma unroll
-    for (int c = 0; c < NI; ++c) {
-      const int r = RPI * c + in_copy;
-      const uint8_t* src = cache + offsets[wave][i % G::BATCH * KEYS + r] + 16 * (piece ^ swizzle<G>(r));
-      copy16_to_lds_rfl_v(src, buf + 1024 * c);
-      copy16_to_lds_rfl_v(src + RB, buf + KEYS * RB + 1024 * c);
-    }
-  };
+        for (int c = 0; c < NI; ++c) {
+          const int r = RPI * c + in_copy;
+          const uint8_t* src = cache + offsets[wave][i % G::BATCH * KEYS + r] + 16 * (piece ^ swizzle<G>(r));
+          copy16_to_lds_rfl_v<kOnce>(src, buf + 1024 * c);
+        }
+      };
 
-  // Q^T: the columns of step s that lane group g holds are those of K's pieces
-  u32x4 qo[D / 32];
-  {
-    const uint16_t* qp = a.q + (int64_t)t * a.q_st + (int64_t)(h0 + min(x, heads - 1)) * a.q_sh;
+      // Q^T: the columns of step s that lane group g holds are those of K's pieces
+      const float scale = a.scale_log2 * (kE4 && a.k_scale ? a.k_scale[kh] : 1.f);
+      u32x4 qo[D / 32];
+      {
+        const uint16_t* qp = a.q + (int64_t)t * a.q_st + (int64_t)(h0 + min(head, heads - 1)) * a.q_sh;
+        const uint32_t flip = scale < 0.f ? 0x80008000u : 0u;   // scores of -q, so that the largest one has the largest weight
 #pragma unroll
-    for (int s = 0; s < D / 32; ++s) {
-      const int col = kE4 ? 16 * (g + 4 * (s / 2)) + 8 * (s % 2) : 32 * s + 8 * g;
-      qo[s] = x < heads ? ld16(qp + col) : u32x4{0u, 0u, 0u, 0u};
-    }
-  }
-  const float scale = a.scale_log2 * (kE4 && a.k_scale ? a.k_scale[kh] : 1.f);
-
-  float m = -INFINITY, l = 0.f;
-  floatx4 o[CT];
-#pragma unroll
-  for (int c = 0; c < CT; ++c) o[c] = floatx4{0.f, 0.f, 0.f, 0.f};
-
-  if (mine > 0) {
-    fetch_ids(0);
-    wait_copies<0>();
-    work_out(0);
-    if (mine > G::BATCH) fetch_ids(1);
-    for (int i = 0; i < NB - 1 && i < mine; ++i) request(i);   // (NB - 1 <= BATCH)
-  }
-  for (int i = 0; i < mine; ++i) {
-    const int ahead = i + NB - 1;
-    if (ahead < mine) {
-      if (ahead % G::BATCH == 0 && ahead > 0) {
-        // the ids were requested a batch ago, before copies that have been waited for
-        work_out(ahead / G::BATCH);
-        if ((ahead / G::BATCH + 1) * G::BATCH < mine) {
-          wait_reads();   // page_ids has been read
-          fetch_ids(ahead / G::BATCH + 1);
+        for (int s = 0; s < D / 32; ++s) {
+          const int col = kE4 ? 16 * (g + 4 * (s / 2)) + 8 * (s % 2) : 32 * s + 8 * g;
+          qo[s] = head < heads ? ld16(qp + col) ^ flip : u32x4{0u, 0u, 0u, 0u};
         }
       }
-      wait_reads();       // so has the buffer
-      request(ahead);
-      wait_copies<2 * NI * (NB - 1)>();
-    } else {
-      wait_copies<0>();
-    }
-    const uint8_t *kb = buf0 + i % NB * G::TILE, *vb = kb + KEYS * RB;
+      const float factor = fabsf(scale);
 
-    constexpr int KB = KEYS / 16;
-    floatx4 s[KB];
+      float m = -INFINITY, l = 0.f;
+      floatx4 o[CT];
 #pragma unroll
-    for (int b = 0; b < KB; ++b) {
-      s[b] = floatx4{0.f, 0.f, 0.f, 0.f};
-      const int key = 16 * b + x;
-#pragma unroll
-      for (int c = 0; c < CPR / 4; ++c) {
-        const u32x4 v = ld16(kb + key * RB + 16 * ((4 * c + g) ^ swizzle<G>(key)));
-        if (kE4) {
-          s[b] = mfma16x16x32(e4m3_to_bf16(v[0], v[1]), qo[2 * c], s[b]);
-          s[b] = mfma16x16x32(e4m3_to_bf16(v[2], v[3]), qo[2 * c + 1], s[b]);
+      for (int c = 0; c < CT; ++c) o[c] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+      if (mine > 0) {
+        fetch_ids(0);
+        wait_copies<0>();
+        work_out(0);
+        if (mine > G::BATCH) fetch_ids(1);
+        for (int i = 0; i < NB - 1 && i < mine; ++i) request(i);   // (NB - 1 <= BATCH)
+      }
+      for (int i = 0; i < mine; ++i) {
+        const int ahead = i + NB - 1;
+        if (ahead < mine) {
+          if (ahead % G::BATCH == 0 && ahead > 0) {
+            // the ids were requested a batch ago, before copies that have been waited for
+            work_out(ahead / G::BATCH);
+            if ((ahead / G::BATCH + 1) * G::BATCH < mine) {
+              wait_reads();   // page_ids has been read
+              fetch_ids(ahead / G::BATCH + 1);
+            }
+          }
+          wait_reads();       // so has the buffer
+          request(ahead);
+          wait_copies<NI * (NB - 1)>();
         } else {
-          s[b] = mfma16x16x32(v, qo[c], s[b]);
+          wait_copies<0>();
         }
-      }
-    }
-    const int left = hi - (lo + (wave + i * WAVES) * KEYS);   // keys of the tile
-    float top = -INFINITY;
+        const uint8_t* buf = buf0 + i % NB * G::TILE;
+
+        constexpr int KB = KEYS / 16;
+        floatx4 s[KB];
 #pragma unroll
-    for (int b = 0; b < KB; ++b)
+        for (int b = 0; b < KB; ++b) {
+          s[b] = floatx4{0.f, 0.f, 0.f, 0.f};
+          const int key = 16 * b + x;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        s[b][r] = 16 * b + 4 * g + r < left ? s[b][r] * scale : -INFINITY;
-        top = fmaxf(top, s[b][r]);
-      }
-    top = wave_max16x4(top);
-    if (__any(top > m + kRaise)) {
-      const float raised = fmaxf(m, top);
-      const float alpha = raised == -INFINITY ? 1.f : fast_exp2(m - raised);
-      m = raised;
-      l *= alpha;
+          for (int c = 0; c < CPR / 8; ++c) {
+            const u32x4 v = ld16(buf + key * RB + 16 * ((4 * c + g) ^ swizzle<G>(key)));
+            if (kE4) {
+              s[b] = mfma16x16x32(e4m3_to_bf16(v[0], v[1]), qo[2 * c], s[b]);
+              s[b] = mfma16x16x32(e4m3_to_bf16(v[2], v[3]), qo[2 * c + 1], s[b]);
+            } else {
+              s[b] = mfma16x16x32(v, qo[c], s[b]);
+            }
+          }
+        }
+        const int left = hi - (lo + (wave + i * WAVES) * KEYS);   // keys of the tile
+        if (left < KEYS) {
+          // rows past the last repeat it: no weight, and values of 0 (0 * inf is not)
 #pragma unroll
-      for (int c = 0; c < CT; ++c)
+          for (int b = 0; b < KB; ++b)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[c][r] *= alpha;
-    }
-    const float at = m == -INFINITY ? 0.f : m;   // (nothing but scores of -inf so far: weights of zero)
-    u32x2 p[KB];
+            for (int r = 0; r < 4; ++r)
+              if (16 * b + 4 * g + r >= left) s[b][r] = -INFINITY;
+          for (int j = left * CPR + lane; j < KEYS * CPR; j += 64) st16(const_cast<uint8_t*>(buf) + 16 * j, u32x4{0u, 0u, 0u, 0u});
+          wait_reads();
+        }
+        float top = -INFINITY;
 #pragma unroll
-    for (int b = 0; b < KB; ++b) {
-      float w[4];
+        for (int b = 0; b < KB; ++b)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) l += w[r] = fast_exp2(s[b][r] - at);
-      p[b] = u32x2{pack2(w[0], w[1]), pack2(w[2], w[3])};
-    }
-    // the keys of a lane's values of V, in the order of the contraction: 4g .. and, e4m3, 16 + 4g ..
-    auto sum_values = [&](auto last) {
-      uint32_t seen[2] = {~0u, ~0u};   // rows past the last repeat it: their values count as 0 (0 * inf is not)
-      if constexpr (decltype(last)::value) {
+          for (int r = 0; r < 4; ++r) top = fmaxf(top, s[b][r]);
+        top = wave_max16x4(top) * factor;
+        if (__any(top > m + kRaise)) {
+          const float raised = fmaxf(m, top);
+          const float alpha = raised == -INFINITY ? 1.f : fast_exp2(m - raised);
+          m = raised;
+          l *= alpha;
+#pragma unroll
+          for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[c][r] *= alpha;
+        }
+        const float from = m == -INFINITY ? 0.f : m;   // (nothing but scores of -inf so far: weights of zero)
+        u32x2 p[KB], p2[KB];   // the column's part of P; with more than 8 heads p2 has the rests
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+          float w[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) l += w[r] = fast_exp2(fmaf(s[b][r], factor, -from));
+          p[b] = u32x2{upper_halves(w[0], w[1]), upper_halves(w[2], w[3])};
+          p2[b] = u32x2{rests(w[0], w[1], p[b][0]), rests(w[2], w[3], p[b][1])};
+          if (kTwice && x >= 8) p[b] = p2[b];
+        }
         if constexpr (kE4) {
-          for (int b = 0; b < 2; ++b) {
-            const int k = min(max(left - 16 * b - 4 * g, 0), 4);
-            seen[b] = k == 4 ? ~0u : (1u << (8 * k)) - 1;
+          const u32x4 pt = u32x4{p[0][0], p[0][1], p[1][0], p[1][1]};
+          // lane x of group g reads half a piece of key 4g + x/2 (x < 8) or 16 + 4g + x/2 - 4
+          const int key = (x < 8 ? 0 : 12) + 4 * g + (x >> 1);
+          const uint8_t* vr = buf + key * RB + 8 * (x & 1);
+#pragma unroll
+          for (int c = 0; c < CT; ++c) {
+            typedef int int2v __attribute__((ext_vector_type(2)));
+            const int2v v = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                (__attribute__((address_space(3))) int2v*)(vr + 16 * ((CPR / 2 + c) ^ swizzle<G>(key))));
+            const u32x4 vt = e4m3_to_bf16((uint32_t)v[0], (uint32_t)v[1]);
+            o[c] = mfma16x16x32(vt, pt, o[c]);
+            if (!kTwice) o[c] = mfma16x16x32(vt, u32x4{p2[0][0], p2[0][1], p2[1][0], p2[1][1]}, o[c]);
           }
         } else {
-          const int k = min(max(left - 4 * g, 0), 4);
-          seen[0] = k >= 2 ? ~0u : k == 1 ? 0xffffu : 0u;
-          seen[1] = k >= 4 ? ~0u : k == 3 ? 0xffffu : 0u;
+          const short4v pt = __builtin_bit_cast(short4v, p[0]);
+          const int key = 4 * g + (x >> 2);
+          const uint8_t* vr = buf + key * RB + 8 * (x & 1);
+#pragma unroll
+          for (int c = 0; c < CT; ++c) {
+            const short4v vt = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) short4v*)(vr + 16 * ((CPR / 2 + 2 * c + ((x >> 1) & 1)) ^ swizzle<G>(key))));
+            o[c] = mfma16x16x16(vt, pt, o[c]);
+            if (!kTwice) o[c] = mfma16x16x16(vt, __builtin_bit_cast(short4v, p2[0]), o[c]);
+          }
         }
       }
-      if constexpr (kE4) {
-        const u32x4 pt = u32x4{p[0][0], p[0][1], p[1][0], p[1][1]};
-        // lane x of group g reads half a piece of key 4g + x/2 (x < 8) or 16 + 4g + x/2 - 4
-        const int key = (x < 8 ? 0 : 12) + 4 * g + (x >> 1);
-        const uint8_t* vr = vb + key * RB + 8 * (x & 1);
-#pragma unroll
-        for (int c = 0; c < CT; ++c) {
-          typedef int int2v __attribute__((ext_vector_type(2)));
-          const int2v v = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-              (__attribute__((address_space(3))) int2v*)(vr + 16 * (c ^ swizzle<G>(key))));
-          o[c] = mfma16x16x32(e4m3_to_bf16((uint32_t)v[0] & seen[0], (uint32_t)v[1] & seen[1]), pt, o[c]);
-        }
-      } else {
-        const short4v pt = __builtin_bit_cast(short4v, p[0]);
-        const int key = 4 * g + (x >> 2);
-        const uint8_t* vr = vb + key * RB + 8 * (x & 1);
-#pragma unroll
-        for (int c = 0; c < CT; ++c) {
-          const short4v v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) short4v*)(vr + 16 * ((2 * c + ((x >> 1) & 1)) ^ swizzle<G>(key))));
-          const u32x2 w = __builtin_bit_cast(u32x2, v);
-          o[c] = mfma16x16x16(__builtin_bit_cast(short4v, u32x2{w[0] & seen[0], w[1] & seen[1]}), pt, o[c]);
-        }
-      }
-    };
-    if (left < KEYS) sum_values(std::true_type{});
-    else sum_values(std::false_type{});
-  }
 
-  // the waves' parts together
-  l = wave_sum16x4(l);
-  if (g == 0) {
-    stats[wave][0][x] = m;
-    stats[wave][1][x] = l;
-  }
-  __syncthreads();   // (and every wave has read its last tile)
-  float* joined = reinterpret_cast<float*>(lds);
-  {
-    float top = -INFINITY;
-    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stats[w][0][x]);
-    const float f = m == -INFINITY ? 0.f : fast_exp2(m - top);
-    // (a NaN among the scores is in l, and where m is -inf nothing but zeros and NaN are in o)
-    if (x < heads) {
+      // the waves' parts together
+      l = wave_sum16x4(l);
+      if (g == 0) {
+        stats[wave][0][x] = m;
+        stats[wave][1][x] = l;
+      }
+      __syncthreads();   // (and every wave has read its last tile)
+      float* joined = reinterpret_cast<float*>(lds);
+      {
+        float top = -INFINITY;
+        for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stats[w][0][x]);
+        const float f = m == -INFINITY ? 0.f : fast_exp2(m - top);
+        // (a NaN among the scores is in l, and where m is -inf nothing but zeros and NaN are in o)
+        if (head < heads) {
 #pragma unroll
-      for (int c = 0; c < CT; ++c) *reinterpret_cast<floatx4*>(joined + (wave * 16 + x) * OS + 16 * c + 4 * g) = o[c] * f;
+          for (int c = 0; c < CT; ++c) *reinterpret_cast<floatx4*>(joined + (wave * 16 + x) * OS + 16 * c + 4 * g) = o[c] * f;
+        }
+      }
+      __syncthreads();
+      for (int i = tid; i < heads * (D / 4); i += 64 * WAVES) {
+        const int j = i / (D / 4), col = i % (D / 4) * 4;
+        float top = -INFINITY, sum = 0.f;
+        for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stats[w][0][j]);
+        floatx4 v = floatx4{0.f, 0.f, 0.f, 0.f};
+        for (int w = 0; w < WAVES; ++w) {
+          const float mw = stats[w][0][j];
+          sum += stats[w][1][j] * (mw == -INFINITY ? 0.f : fast_exp2(mw - top));
+          v += *reinterpret_cast<floatx4*>(joined + (w * 16 + j) * OS + col);
+          if (kTwice) v += *reinterpret_cast<floatx4*>(joined + (w * 16 + j + 8) * OS + col);
+        }
+        const bool none = sum == 0.f;
+        const float inv = none ? 0.f : (kE4 && a.v_scale ? a.v_scale[kh] : 1.f) / sum;
+        const float lse = none ? -INFINITY : (top + log2f(sum)) * kLn2;
+        if (!whole) {   // rows that began in an earlier share, or that go on in the next
+          const int64_t place = ((int64_t)2 * k + (at == 0)) * a.H + h0 + j;
+          *reinterpret_cast<floatx4*>(a.ws_o + place * D + col) = v * inv;
+          if (col == 0) a.ws_lse[place] = lse;
+        } else {
+          *reinterpret_cast<u32x2*>(a.out + (int64_t)t * a.o_st + (int64_t)(h0 + j) * a.o_sh + col) =
+              u32x2{pack2(v[0] * inv, v[1] * inv), pack2(v[2] * inv, v[3] * inv)};
+          if (col == 0) a.lse[(int64_t)(h0 + j) * a.T + t] = lse;
+        }
+      }
     }
-  }
-  __syncthreads();
-  for (int i = tid; i < heads * (D / 4); i += 64 * WAVES) {
-    const int j = i / (D / 4), col = i % (D / 4) * 4;
-    float top = -INFINITY, sum = 0.f;
-    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stats[w][0][j]);
-    floatx4 v = floatx4{0.f, 0.f, 0.f, 0.f};
-    for (int w = 0; w < WAVES; ++w) {
-      const float mw = stats[w][0][j];
-      sum += stats[w][1][j] * (mw == -INFINITY ? 0.f : fast_exp2(mw - top));
-      v += *reinterpret_cast<floatx4*>(joined + (w * 16 + j) * OS + col);
-    }
-    const bool none = sum == 0.f;
-    const float inv = none ? 0.f : (kE4 && a.v_scale ? a.v_scale[kh] : 1.f) / sum;
-    const float lse = none ? -INFINITY : (top + log2f(sum)) * kLn2;
-    if (a.S > 1) {
-      *reinterpret_cast<floatx4*>(a.ws_o + ((base + j) * a.S + slot) * D + col) = v * inv;
-      if (col == 0) a.ws_lse[(base + j) * a.S + slot] = lse;
-    } else {
-      *reinterpret_cast<u32x2*>(a.out + (int64_t)t * a.o_st + (int64_t)(h0 + j) * a.o_sh + col) =
-          u32x2{pack2(v[0] * inv, v[1] * inv), pack2(v[2] * inv, v[3] * inv)};
-      if (col == 0) a.lse[(int64_t)(h0 + j) * a.T + t] = lse;
-    }
+    left_steps -= taken;
+    if (!a.shares || left_steps <= 0) return;
+    before += steps;
+    at = 0;
+    ++t;             // (steps are left, so a token with rows follows)
+    __syncthreads(); // the parts in LDS have been read
   }
 }
 
-// The slots of one (token, head) joined by their lse: one workgroup, D / 4 threads per slot.
+// The parts of one (token, head) joined by their lse, where its rows lie in several shares; tokens without rows. One workgroup,
+// D / 4 threads per part.
 template <int D>
-__global__ __launch_bounds__(256) void exact_join_kernel(const float* ws_o, const float* ws_lse, int T, int H, int S,
-                                                         uint16_t* out, int64_t o_st, int64_t o_sh, float* lse) {
+__global__ __launch_bounds__(256) void exact_join_kernel(ExactCacheParams a) {
   constexpr int PER = D / 4, ROWS = 256 / PER;
-  __shared__ float weight[kMaxSlots];
+  __shared__ float weight[kMaxShares];
   __shared__ floatx4 sums[ROWS][PER];
   __shared__ float red[2][4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t row = blockIdx.x;
-  const float mine = tid < S ? ws_lse[row * S + tid] : -INFINITY;
-  float top = mine;
+  const int t = blockIdx.x / a.H, h = blockIdx.x % a.H;
+  int first, n;
+  token_rows(a, t, first, n);
+  int k0 = 0, count = 0;
+  if (n > first) {
+    k0 = a.split[2 * t];
+    count = a.split[2 * t + 1] - k0 + 1;
+    if (count == 1) return;   // written by its workgroup
+  }
+  // part s: the rows' end of share k0 (s = 0), or their beginning in share k0 + s
+  const int64_t place = ((int64_t)2 * k0 + 1) * a.H + h;
+  auto where = [&](int s) { return place + (s ? (2 * (int64_t)s - 1) * a.H : 0); };
+  float top = -INFINITY;
+  for (int s = tid; s < count; s += 256) top = fmaxf(top, weight[s] = a.ws_lse[where(s)]);
   for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
   if (lane == 0) red[0][wave] = top;
   __syncthreads();
   top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-  // (a slot with a NaN lse has a NaN weight; a slot without rows none, and its partial was not written)
-  float w = mine == -INFINITY ? 0.f : fast_exp2((mine - top) * kLog2e);
-  if (tid < S) weight[tid] = w;
+  float w = 0.f;
+  for (int s = tid; s < count; s += 256) {
+    // (a part with a NaN lse has a NaN weight; one with nothing but scores of -inf none)
+    const float mine = weight[s];
+    w += weight[s] = mine == -INFINITY ? 0.f : fast_exp2((mine - top) * kLog2e);
+  }
   for (int off = 32; off > 0; off >>= 1) w += __shfl_xor(w, off);
   if (lane == 0) red[1][wave] = w;
   __syncthreads();
   const float sum = red[1][0] + red[1][1] + red[1][2] + red[1][3];
   floatx4 v = floatx4{0.f, 0.f, 0.f, 0.f};
-  const float* src = ws_o + row * S * D + tid % PER * 4;
 #pragma unroll 4
-  for (int s = tid / PER; s < S; s += ROWS) {
-    const float f = weight[s];
-    if (f != 0.f) v += *reinterpret_cast<const floatx4*>(src + (int64_t)s * D) * f;
-  }
+  for (int s = tid / PER; s < count; s += ROWS)
+    v += *reinterpret_cast<const floatx4*>(a.ws_o + where(s) * D + tid % PER * 4) * weight[s];
   sums[tid / PER][tid % PER] = v;
   __syncthreads();
   if (tid >= PER) return;
   for (int i = 1; i < ROWS; ++i) v += sums[i][tid];
-  const int t = (int)(row / H), h = (int)(row % H);
   const bool none = sum == 0.f;
   const float inv = none ? 0.f : 1.f / sum;
-  *reinterpret_cast<u32x2*>(out + (int64_t)t * o_st + (int64_t)h * o_sh + 4 * tid) =
+  *reinterpret_cast<u32x2*>(a.out + (int64_t)t * a.o_st + (int64_t)h * a.o_sh + 4 * tid) =
       u32x2{pack2(v[0] * inv, v[1] * inv), pack2(v[2] * inv, v[3] * inv)};
-  if (tid == 0) lse[(int64_t)h * T + t] = none ? -INFINITY : top + logf(sum);
+  if (tid == 0) a.lse[(int64_t)h * a.T + t] = none ? -INFINITY : top + logf(sum);
 }
 
 template <int D, bool kE4>
 void launch_exact_cache(const ExactCacheParams& p, hipStream_t st) {
-  const unsigned grid = (unsigned)((int64_t)p.T * p.S * p.KH * p.tiles);
+  const unsigned grid = (unsigned)((int64_t)(p.shares ? p.shares : p.T) * p.KH * p.tiles);
   using G = ExactGeo<D, kE4>;
-  hipLaunchKernelGGL(exact_cache_kernel<G>, dim3(grid), dim3(64 * G::WAVES), 0, st, p);
-  if (p.S > 1)
-    hipLaunchKernelGGL(exact_join_kernel<D>, dim3((unsigned)((int64_t)p.T * p.H)), dim3(256), 0, st, p.ws_o, p.ws_lse, p.T,
-                       p.H, p.S, p.out, p.o_st, p.o_sh, p.lse);
+  const bool once = p.tiles == 1 && p.T <= p.bt_count;   // a table row for every token
+  void (*const kernel)(ExactCacheParams) = p.G <= 8 ? (once ? exact_cache_kernel<G, true, true> : exact_cache_kernel<G, false, true>)
+                                                    : (once ? exact_cache_kernel<G, true, false> : exact_cache_kernel<G, false, false>);
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * G::WAVES), 0, st, p);
+  if (p.shares)
+    hipLaunchKernelGGL(exact_join_kernel<D>, dim3((unsigned)((int64_t)p.T * p.H)), dim3(256), 0, st, p);
 }
 
 // ---- store -------------------------------------------------------------------------------------------------------
@@ -497,7 +554,7 @@ extern "C" int hla_s6_exact_attention(const void* q, int32_t num_tokens, int32_t
                                       int64_t head_stride, int64_t row_stride, int32_t block_size, int64_t num_blocks,
                                       const int32_t* block_table, int64_t bt_stride, int32_t bt_cols, int32_t bt_count,
                                       const int64_t* bt_rows, const int32_t* ctx, int32_t window, float scale,
-                                      const float* k_scale, const float* v_scale, int32_t num_splits, int32_t workgroups,
+                                      const float* k_scale, const float* v_scale, int32_t shares,
                                       float* workspace, int64_t workspace_floats, void* out, int64_t o_st, int64_t o_sh,
                                       float* lse, void* stream) {
   using namespace hla;
@@ -507,9 +564,8 @@ extern "C" int hla_s6_exact_attention(const void* q, int32_t num_tokens, int32_t
   if (rc != HLA_S6_OK) return rc;
   HLA_REQUIRE(num_heads >= kv_heads && num_heads % kv_heads == 0, HLA_S6_EINVAL,
               "exact_attention: %d query heads over %d KV heads", num_heads, kv_heads);
-  HLA_REQUIRE(num_splits >= 1 && num_splits <= kMaxSlots, HLA_S6_EINVAL, "exact_attention: %d splits (1..%d)", num_splits,
-              kMaxSlots);
-  HLA_REQUIRE(window >= 0 && bt_cols >= 0 && workgroups >= 1, HLA_S6_EINVAL, "exact_attention: bad window, table or grid");
+  HLA_REQUIRE(shares >= 0 && shares <= kMaxShares, HLA_S6_EINVAL, "exact_attention: %d shares (0..%d)", shares, kMaxShares);
+  HLA_REQUIRE(window >= 0 && bt_cols >= 0, HLA_S6_EINVAL, "exact_attention: bad window or table");
   HLA_REQUIRE(e4m3 || (!k_scale && !v_scale), HLA_S6_EINVAL, "exact_attention: scales belong to e4m3 caches");
   if (num_tokens == 0) return HLA_S6_OK;
   HLA_REQUIRE(bt_count >= (bt_rows ? 1 : num_tokens), HLA_S6_EINVAL, "exact_attention: %d table rows", bt_count);
@@ -542,18 +598,17 @@ extern "C" int hla_s6_exact_attention(const void* q, int32_t num_tokens, int32_t
   p.KH = kv_heads;
   p.G = num_heads / kv_heads;
   p.tiles = (p.G + kMaxTile - 1) / kMaxTile;
-  p.S = num_splits;
-  p.rows_wanted = workgroups;
-  HLA_REQUIRE((int64_t)p.T * p.S * p.KH * p.tiles <= INT32_MAX && (int64_t)p.T * p.H <= INT32_MAX, HLA_S6_EINVAL,
+  p.shares = shares;
+  HLA_REQUIRE((int64_t)max(p.T, shares) * p.KH * p.tiles <= INT32_MAX && (int64_t)p.T * p.H <= INT32_MAX, HLA_S6_EINVAL,
               "exact_attention: too many rows");
-  if (p.S > 1) {
-    const int64_t rows = (int64_t)p.T * p.H * p.S;
-    HLA_REQUIRE(workspace && workspace_floats >= rows * (head_dim + 1), HLA_S6_EWORKSPACE,
-                "exact_attention: workspace of %lld floats, need %lld", (long long)workspace_floats,
-                (long long)(rows * (head_dim + 1)));
+  if (shares) {
+    const int64_t rows = (int64_t)2 * shares * p.H, need = rows * (head_dim + 1) + 2 * (int64_t)p.T;
+    HLA_REQUIRE(workspace && workspace_floats >= need, HLA_S6_EWORKSPACE,
+                "exact_attention: workspace overflow: %lld floats, have %lld", (long long)need, (long long)workspace_floats);
     HLA_REQUIRE(aligned16(workspace), HLA_S6_EINVAL, "exact_attention: workspace must be 16-byte aligned");
     p.ws_o = workspace;
     p.ws_lse = workspace + rows * head_dim;
+    p.split = reinterpret_cast<int32_t*>(p.ws_lse + rows);
   }
   p.out = static_cast<uint16_t*>(out);
   p.o_st = o_st;

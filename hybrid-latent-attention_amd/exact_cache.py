@@ -19,7 +19,7 @@ from .compact_cache import _call, _same_device, _table, _vector
 
 BF16, E4M3, F32, I32, I64 = torch.bfloat16, torch.float8_e4m3fn, torch.float32, torch.int32, torch.int64
 DIMS = (64, 128, 256)
-MAX_SPLITS = 256
+MAX_SHARES = 1024
 
 
 def _cache(cache, k_scale, v_scale):
@@ -60,16 +60,17 @@ def store_rows(key, value, slots, cache, k_scale=None, v_scale=None):
           page, head, row, block, pages)
 
 
-def kv_splits(max_rows, groups, cu_count=256):
-    """``(split slots per row, workgroups wanted)`` of ``attention`` for rows of at most ``max_rows`` and ``groups`` (token, KV
-    head) pairs. A function of constants and the row count only (graph-stable)."""
-    wanted = 4 * cu_count
-    slots = min(MAX_SPLITS, -(-max_rows // 128), -(-2 * wanted // max(1, groups)))
-    return max(1, slots), wanted
+def row_shares(max_rows, groups, parts, cu_count=256):
+    """``shares`` of ``attention`` for rows of at most ``max_rows`` and ``groups`` (token, KV head) pairs over ``parts`` KV heads: two
+    workgroups per CU, or 0 (a workgroup per group) where the rows are short or the groups many. A function of constants and the
+    row count only (graph-stable)."""
+    if max_rows <= 256 or groups >= 16 * cu_count:
+        return 0
+    return max(1, min(MAX_SHARES, 2 * cu_count // parts))
 
 
 def attention(q, cache, block_table, ctx, scale, max_seq_len, token_requests=None, window=0, k_scale=None, v_scale=None,
-              num_kv_splits=None, workspace=None):
+              shares=None, workspace=None):
     """Attention of ``q [T, H, d]`` (bf16, any token and head strides) over the rows ``[max(0, n - window), n)`` of ``n = ctx[t]``
     (int32; ``window`` 0: over all ``n``) of an exact cache: ``(o [T, H, d] bf16, lse [H, T] fp32)``. ``H`` is a multiple of the
     cache's KV heads, and query head ``h`` reads KV head ``h // (H / KV heads)``. Tokens without rows give ``o = 0``, ``lse = -inf``.
@@ -77,10 +78,11 @@ def attention(q, cache, block_table, ctx, scale, max_seq_len, token_requests=Non
     The rows of a token are those before it and its own, once ``store_rows`` has written it; tokens of one request (a chunk) have a
     ``ctx`` of their own each. ``block_table`` (int32) is per token, or per request with ``token_requests[t]`` (int64) naming the
     row of token ``t``. No entry of ``ctx`` should be above ``max_seq_len`` (a host number, which sets how rows are cut). Scores,
-    softmax statistics and sums are fp32; the weights are rounded to bf16 for their product with V.
+    softmax statistics and sums are fp32; weights keep 16 bits in their product with V.
 
-    ``num_kv_splits`` (slots per row, 1 to 256) defaults to ``kv_splits``; ``workspace`` (an ``S6Workspace``) to a new buffer. Calls
-    that share a workspace must not overlap."""
+    The rows of all tokens are cut in ``shares`` equal parts per KV head (0: a workgroup takes all rows of a token; defaults to
+    ``row_shares``); their partial results go through ``workspace`` (an ``S6Workspace`` of ``2 * shares * H * (d + 1) + 2 * T`` floats;
+    defaults to a new buffer). Calls that share a workspace must not overlap."""
     _same_device(cache, q, block_table, ctx, token_requests, k_scale, v_scale)
     kv_heads, d, e4m3, page, head, row, block, pages = _cache(cache, k_scale, v_scale)
     s6_ops._bf16('q', q)
@@ -97,20 +99,22 @@ def attention(q, cache, block_table, ctx, scale, max_seq_len, token_requests=Non
         raise ValueError(f'window must not be negative, got {window}')
     dev = q.device
     longest = min(int(max_seq_len), cols * block, window or cols * block)
-    groups = T * kv_heads * -(-H // kv_heads // 16)
-    splits, wanted = kv_splits(longest, groups, _lib.device_cus(dev.index))
-    if num_kv_splits is not None:
-        splits = int(num_kv_splits)
+    parts = kv_heads * -(-H // kv_heads // 16)
+    shares = row_shares(longest, T * parts, parts, _lib.device_cus(dev.index)) if shares is None else int(shares)
+    if not 0 <= shares <= MAX_SHARES:
+        raise ValueError(f'shares must be 0 to {MAX_SHARES}, got {shares}')
     ws = None
-    if splits > 1:
-        ws = (torch.empty(T * H * splits * (d + 1), dtype=F32, device=dev) if workspace is None
-              else workspace.attn_logits(T, H, splits, d, dev))
+    if shares:
+        need = 2 * shares * H * (d + 1) + 2 * T
+        ws = torch.empty(need, dtype=F32, device=dev) if workspace is None else workspace.ensure(dev)
+        if ws.numel() < need:
+            raise RuntimeError(f'S6 workspace overflow: need {need} floats, have {ws.numel()}')
         _same_device(q, ws)   # (a workspace keeps the device of its first use)
     out = torch.empty(T, H, d, dtype=BF16, device=dev)
     lse = torch.empty(H, T, dtype=F32, device=dev)
     token_stride, head_stride, _ = q.stride()
     _call('hla_s6_exact_attention', dev, q.data_ptr(), T, H, d, token_stride, head_stride, cache.data_ptr(), int(e4m3), kv_heads,
           page, head, row, block, pages, block_table.data_ptr(), table_stride, cols, count, _lib.ptr(token_requests),
-          ctx.data_ptr(), window, float(scale), _lib.ptr(k_scale), _lib.ptr(v_scale), splits, wanted, _lib.ptr(ws),
+          ctx.data_ptr(), window, float(scale), _lib.ptr(k_scale), _lib.ptr(v_scale), shares, _lib.ptr(ws),
           0 if ws is None else ws.numel(), out.data_ptr(), H * d, d, lse.data_ptr())
     return out, lse

@@ -103,17 +103,17 @@ def test_attention(ec, kv_heads, G, block, d, e4m3):
 
 
 @pytest.mark.parametrize('e4m3', [False, True])
-@pytest.mark.parametrize('splits', [1, 2, 3, 7, 64, 256])
-def test_every_split_count(ec, splits, e4m3):
+@pytest.mark.parametrize('splits', [0, 1, 2, 3, 7, 64, 1024])
+def test_every_share_count(ec, splits, e4m3):
     n = [5000, 1, 700, 0, 4097, 64, 65]
     c = Cache(splits, n, 2, 128, 16, e4m3)
     q = query(splits, len(n), 8, 128)
-    o, lse = attend(ec, q, c, n, num_kv_splits=splits)
+    o, lse = attend(ec, q, c, n, shares=splits)
     check(o, lse, q, c, range(len(n)), n, 128 ** -0.5)
 
 
 @pytest.mark.parametrize('window', [1, 15, 32, 100, 4096])
-@pytest.mark.parametrize('splits', [None, 1, 9])
+@pytest.mark.parametrize('splits', [None, 0, 9])
 def test_windows(ec, window, splits):
     n = [3000, 1, 0, 32, 33, 99, 777]
     c = Cache(window, n, 4, 128, 16)
@@ -121,7 +121,7 @@ def test_windows(ec, window, splits):
         at = torch.arange(max(0, n[r] - window), device='cuda')
         c.cache[c.table[r].long()[at // 16], :, at % 16] = math.nan
     q = query(window, len(n), 8, 128)
-    o, lse = attend(ec, q, c, n, window=window, num_kv_splits=splits)
+    o, lse = attend(ec, q, c, n, window=window, shares=splits)
     check(o, lse, q, c, range(len(n)), n, 128 ** -0.5, window)
 
 
@@ -190,7 +190,7 @@ def test_scales_of_scores(ec):
     check(o, lse, q, c, range(2), n, 0.5)
 
 
-@pytest.mark.parametrize('splits', [1, 8])
+@pytest.mark.parametrize('splits', [0, 8])
 def test_values_that_are_not_finite(ec, splits):
     """NaN in a row of K reaches output and lse of the heads that see it, NaN and infinities in V the output alone; -inf scores
     have no weight; a row of nothing else is an empty one. No other token, head or window sees any of it."""
@@ -210,7 +210,7 @@ def test_values_that_are_not_finite(ec, splits):
     for j in range(40):
         p, _, x = page(4, j)
         c.cache[p, :, x, 0] = -math.inf
-    o, lse = attend(ec, base, c, n, num_kv_splits=splits)
+    o, lse = attend(ec, base, c, n, shares=splits)
     assert torch.isnan(o[0, 2:]).all() and torch.isnan(lse[2:, 0]).all()
     assert torch.isposinf(o[1, :2, 9]).all() and torch.isnan(o[2, 2:]).all()
     assert torch.isfinite(o[1, :, :9]).all() and torch.isfinite(o[1, 2:]).all() and torch.isfinite(lse[:, 1:4]).all()
@@ -220,7 +220,7 @@ def test_values_that_are_not_finite(ec, splits):
         part = Cache.__new__(Cache)
         part.h, part.rows = 1 if keep.stop - keep.start == 2 else 2, [c.rows[t][:, keep.start // 2:-(-keep.stop // 2)]]
         check(o[t:t + 1, keep].contiguous(), lse[keep, t:t + 1], base[t:t + 1, keep], part, [0], [c.rows[t].shape[0]], 128 ** -0.5)
-    o, lse = attend(ec, base, c, n[:3] + [500] + [0], window=30, num_kv_splits=splits)
+    o, lse = attend(ec, base, c, n[:3] + [500] + [0], window=30, shares=splits)
     assert torch.isfinite(o[0]).all() and torch.isfinite(o[2:4]).all()      # the rows in question lie before the window
 
 
@@ -275,16 +275,16 @@ def test_streams_and_workspaces(ec, pkg):
     n = [4000, 3000]
     c = Cache(28, n, 2, 128, 16)
     q = query(29, 2, 4, 128)
-    want = attend(ec, q, c, n, num_kv_splits=16)
-    ws = pkg.s6_ops.S6Workspace.for_splits(4, 2, {128: 16})
-    got = attend(ec, q, c, n, num_kv_splits=16, workspace=ws)
+    want = attend(ec, q, c, n, shares=16)
+    ws = pkg.s6_ops.S6Workspace(4, 128, 2 * 16 + 1)
+    got = attend(ec, q, c, n, shares=16, workspace=ws)
     assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
     with pytest.raises(RuntimeError, match='workspace overflow'):
-        attend(ec, q, c, n, num_kv_splits=17, workspace=ws)
+        attend(ec, q, c, n, shares=17, workspace=ws)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
-        got = attend(ec, q, c, n, num_kv_splits=16)
+        got = attend(ec, q, c, n, shares=16)
     side.synchronize()
     assert torch.equal(want[0], got[0])
 
@@ -311,7 +311,7 @@ def test_refusals(ec):
                         ((q, c.cache, t.long(), n, 1.0, 5), 'block_table'), ((q, c.cache, t, n, 1.0, 5, n), 'token_requests'),
                         ((q, c.cache, t, n, 1.0, 5, None, -1), 'window'), ((q, c.cache, t, n, 1.0, 5, None, 0, scale), 'k_scale'),
                         ((q, e4, t, n, 1.0, 5, None, 0, None, scale[:1]), 'v_scale'), ((q, e4, t, n, 1.0, 5, None, 0, scale.half()), 'k_scale'),
-                        ((q, c.cache, t, n, 1.0, 5, None, 0, None, None, 300), 'splits'), ((q, c.cache, t, n, 1.0, 5, None, 0, None, None, 0), 'splits')):
+                        ((q, c.cache, t, n, 1.0, 5, None, 0, None, None, 1025), 'shares'), ((q, c.cache, t, n, 1.0, 5, None, 0, None, None, -1), 'shares')):
         with pytest.raises(ValueError, match=match):
             ec.attention(*args)
     with pytest.raises(RuntimeError):
