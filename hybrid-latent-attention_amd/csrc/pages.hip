@@ -117,33 +117,155 @@ __device__ __forceinline__ uint32_t page_bits(const Pool& p, int w) {
 // ---- extend ------------------------------------------------------------------------------------------------------
 // Room for the rows [from, to) of every request: columns behind its last get a free page each, columns that hold a shared page
 // a free page that the caller fills with a copy of it (the pairs source, target). Requests are served in order as long as what
-// they and those before them ask for is there; the others stay as they are.
-//
-// kFrom: from = write_from[r], and lists have an entry per table entry; a wave goes through a request's columns. Else from =
-// lengths[r], at most one column of a request is shared and lists have an entry per request; free pages find their places.
+// they and those before them ask for is there; the others stay as they are. So the pages that served requests get are ranks
+// 0, 1, .. of the free pages, and a request's first rank is what those before it ask for.
 struct ExtendParams {
   Pool p;
   const int32_t* to;
   const int32_t* from;  // null: the lengths
   uint8_t* ok;
   int32_t *source, *target;
-  int32_t* ids;  // kFrom: [R * cols] scratch
+  int32_t* ids;  // with `from`: [R * cols] scratch
 };
 
-template <bool kFrom>
+__device__ __forceinline__ int64_t count_free(const Pool& p, int64_t* sums) {
+  const int words = (p.N + 31) / 32;
+  int n = 0;
+  for (int w = threadIdx.x; w < words; w += kPoolThreads) n += __popc(p.free[w] & page_bits(p, w));
+  int64_t have;
+  pool_scan(n, sums, have);
+  return have;
+}
+
+// The `given` lowest free pages, which are free no longer: 32 * kPoolThreads pages of the pool at a time, place(base, n, page0) with
+// the pages of ranks base .. base + n - 1 in `found`, less page0.
+constexpr int kAtOnce = 32 * kPoolThreads;
+
+template <typename Place>
+__device__ __forceinline__ void hand_out(const Pool& p, int given, int64_t* sums, uint16_t* found, Place place) {
+  for (int w0 = 0, base = 0; base < given; w0 += kPoolThreads) {   // (given is no more than there are)
+    const int w = w0 + threadIdx.x;
+    const uint32_t all = w < (p.N + 31) / 32 ? p.free[w] : 0u;
+    uint32_t bits = all & page_bits(p, w), kept = all;
+    int64_t total;
+    int at = (int)pool_scan(__popc(bits), sums, total);
+    const int n = min((int)total, given - base);
+    for (; bits && at < n; bits &= bits - 1, ++at) {
+      const int bit = __ffs((int)bits) - 1;
+      kept &= ~(1u << bit);
+      found[at] = (uint16_t)(threadIdx.x * 32 + bit);
+    }
+    if (kept != all) p.free[w] = kept;
+    __syncthreads();
+    place(base, n, w0 * 32);
+    __syncthreads();
+    base += n;
+  }
+}
+
+// from = lengths[r]: at most one column of a request, its last, is shared, and lists have an entry per request. A call of few
+// pages is a chain of loads and barriers; one of many is bound by the instructions of its one workgroup, so a wave places the
+// pages of a request 64 at a time, in consecutive columns, and only requests of up to kFew pages are left to their threads.
+constexpr int kFew = 4;
+
 __global__ __launch_bounds__(kPoolThreads) void pool_extend_kernel(ExtendParams a) {
   __shared__ int64_t sums[kPoolWaves + 1];
-  __shared__ int start[kMaxRequests + 1];   // first rank of a request's pages; requests that get none have no ranks
-  __shared__ uint8_t shared_last[kFrom ? 1 : kMaxRequests];
+  __shared__ int start[kMaxRequests + 1];   // first rank of a request's pages
+  __shared__ int column[kMaxRequests];      // where the first of them goes; negative: ~column, in place of a shared page
+  __shared__ uint16_t found[kAtOnce];
+  __shared__ int given;                     // ranks handed out
+  const Pool& p = a.p;
+  const int tid = threadIdx.x, lane = tid & 63;
+
+  int64_t asked = 0, have = 0;
+  if (tid == 0) given = 0;
+  for (int r0 = 0; r0 < p.R; r0 += kPoolThreads) {
+    const int r = r0 + tid;
+    int need = 0, first = 0, want = 0, length = 0;
+    bool fits = true;
+    if (r < p.R) {
+      length = rows_of(p, p.lengths[r]);
+      want = max(a.to[r], length);
+      fits = want <= (int64_t)p.cols * p.block;
+      if (fits && want > length) {
+        const int held = pages_of(p, length), last = length / p.block;
+        first = held;
+        if (last < held) {   // rows go into the last page
+          const int32_t page = p.tables[r * p.t_st + last];
+          if (is_page(p, page) && p.refs[page] > 1) first = ~last;
+        }
+        need = pages_of(p, want) - held + (first < 0);
+      }
+    }
+    if (r0 == 0) have = count_free(p, sums);
+    int64_t total;
+    const int64_t before = asked + pool_scan(need, sums, total);
+    asked += total;
+    const bool served = need == 0 || before + need <= have;
+    if (r < p.R) {
+      start[r] = (int)min(before, have);
+      column[r] = first;
+      a.source[r] = -1;
+      a.target[r] = -1;
+      a.ok[r] = fits && served;
+      if (served && need) atomicMax(&given, (int)(before + need));
+      if (fits && served && want > length) p.lengths[r] = want;
+    }
+  }
+  if (tid == 0) start[p.R] = (int)min(asked, have);
+  __syncthreads();
+  const int pages = given;   // (the request that is not served first, and all behind it, start at `pages` or later)
+  hand_out(p, pages, sums, found, [&](int base, int n, int page0) {
+    // pages of ranks k, k + step, .. below `last` of request r, whose ranks start at `first_rank`
+    auto place = [&](int r, int first_rank, int k, int last, int step) {
+      const int c = column[r];
+      int32_t* entry = p.tables + r * p.t_st + (c < 0 ? ~c : c) - first_rank;
+      if (c < 0 && k == first_rank) {
+        a.source[r] = entry[k];
+        a.target[r] = page0 + found[k - base];
+      }
+#pragma unroll 4
+      for (; k < last; k += step) {
+        const int page = page0 + found[k - base];
+        entry[k] = page;
+        p.refs[page] = 1;
+      }
+    };
+    for (int r0 = 0; r0 < p.R; r0 += kPoolThreads) {
+      const int r = r0 + lane * kPoolWaves + (tid >> 6);   // (neighbours with different waves)
+      int lo = 0, hi = 0, first_rank = 0;
+      if (r < p.R) {
+        first_rank = start[r];
+        lo = max(first_rank, base);
+        hi = min(start[r + 1], base + n);
+      }
+      if (hi - lo <= kFew && lo < hi) place(r, first_rank, lo, hi, 1);
+      for (uint64_t many = __ballot(hi - lo > kFew); many; many &= many - 1) {
+        const int from = __ffsll((unsigned long long)many) - 1;
+        place(__shfl(r, from), __shfl(first_rank, from), __shfl(lo, from) + lane, __shfl(hi, from), 64);
+      }
+    }
+  });
+  // the pages that were copied from lose a holder, after all free bits have been read
+  for (int r = tid; r < p.R; r += kPoolThreads)
+    if (column[r] < 0 && a.source[r] >= 0) drop_page(p, a.source[r]);
+}
+
+// from = write_from[r]: any column may be shared, lists have an entry per table entry. A wave goes through a request's columns,
+// first to count them and then to fill them.
+__global__ __launch_bounds__(kPoolThreads) void pool_extend_from_kernel(ExtendParams a) {
+  __shared__ int64_t sums[kPoolWaves + 1];
+  __shared__ int start[kMaxRequests + 1];
+  __shared__ uint16_t found[kAtOnce];
+  __shared__ int given;
   const Pool& p = a.p;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int words = (p.N + 31) / 32;
 
   // columns [c0, c1) that may change: those with rows to write
   auto columns = [&](int r, int& length, int& want, int& c0, int& c1) {
     length = rows_of(p, p.lengths[r]);
     want = max(a.to[r], length);
-    const int from = kFrom ? min(max(a.from[r], 0), length) : length;
+    const int from = min(max(a.from[r], 0), length);
     const bool fits = want <= (int64_t)p.cols * p.block;
     c0 = from / p.block;
     c1 = fits && want > from ? pages_of(p, want) : c0;
@@ -154,155 +276,72 @@ __global__ __launch_bounds__(kPoolThreads) void pool_extend_kernel(ExtendParams 
     return is_page(p, page) && p.refs[page] > 1;
   };
 
-  // free pages
-  int64_t have = 0;
-  for (int w0 = 0; w0 < words; w0 += kPoolThreads) {
-    int64_t total;
-    pool_scan(__popc(w0 + tid < words ? p.free[w0 + tid] & page_bits(p, w0 + tid) : 0u), sums, total);
-    have += total;
-  }
-
-  // what every request asks for, and who gets it
-  if (kFrom) {
-    for (int r = wave; r < p.R; r += kPoolWaves) {
-      int length, want, c0, c1;
-      columns(r, length, want, c0, c1);
-      const int held = pages_of(p, length);
-      int need = max(0, c1 - max(c0, held));
-      for (int c = c0; c < min(c1, held); c += 64) {
-        const int at = c + lane;
-        const bool sh = at < min(c1, held) && is_shared(r, at);
-        need += __popcll(__ballot(sh));
-      }
-      if (lane == 0) start[r] = need;
+  if (tid == 0) given = 0;
+  const int64_t have = count_free(p, sums);
+  for (int r = wave; r < p.R; r += kPoolWaves) {
+    int length, want, c0, c1;
+    columns(r, length, want, c0, c1);
+    const int held = pages_of(p, length);
+    int need = max(0, c1 - max(c0, held));
+    for (int c = c0; c < min(c1, held); c += 64) {
+      const int at = c + lane;
+      const bool sh = at < min(c1, held) && is_shared(r, at);
+      need += __popcll(__ballot(sh));
     }
-    __syncthreads();
+    if (lane == 0) start[r] = need;
   }
+  __syncthreads();
   int64_t asked = 0;
-  int given = 0;   // ranks handed out
   for (int r0 = 0; r0 < p.R; r0 += kPoolThreads) {
     const int r = r0 + tid;
-    int need = 0, length = 0, want = 0, c0 = 0, c1 = 0;
-    bool fits = true, last = false;
-    if (r < p.R) {
-      fits = columns(r, length, want, c0, c1);
-      if (kFrom) {
-        need = start[r];
-      } else {
-        const int held = pages_of(p, length);
-        last = c0 < held && c0 < c1 && is_shared(r, c0);
-        need = c1 - max(c0, held) + last;
-        if (c1 <= c0) need = 0;
-      }
-    }
+    const int need = r < p.R ? start[r] : 0;
     int64_t total;
     const int64_t before = asked + pool_scan(need, sums, total);
     asked += total;
-    const bool served = need == 0 || before + need <= have;
-    const int got = served ? need : 0;
-    int64_t sum;
-    const int rank = given + (int)pool_scan(got, sums, sum);
-    given += (int)sum;
     if (r < p.R) {
-      start[r] = rank;
-      if (!kFrom) {
-        shared_last[r] = last && served;
-        a.source[r] = -1;
-        a.target[r] = -1;
-      }
-      const bool done = fits && served;
-      a.ok[r] = done;
-      // (kFrom: below, after the columns have been read once more)
-      if (!kFrom && got == 0 && done && want > length) p.lengths[r] = want;
-    }
-  }
-  if (tid == 0) start[p.R] = given;
-  __syncthreads();
-
-  // the lowest free pages, in rank order
-  int base = 0;
-  for (int w0 = 0; base < given; w0 += kPoolThreads) {
-    const int w = w0 + tid;
-    uint32_t bits = w < words ? p.free[w] & page_bits(p, w) : 0u;
-    int64_t total;
-    int rank = base + (int)pool_scan(__popc(bits), sums, total);
-    base += (int)total;
-    if (bits && rank < given) {
-      uint32_t kept = p.free[w];
-      int r = 0;
-      if (!kFrom) {   // the request of the first rank: the last one that starts at or before it
-        int lo = 0, hi = p.R;
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) >> 1;
-          if (start[mid] <= rank) lo = mid;
-          else hi = mid;
-        }
-        r = lo;
-      }
-      for (; bits && rank < given; ++rank) {
-        const int bit = __ffs((int)bits) - 1, page = w * 32 + bit;
-        bits &= bits - 1;
-        kept &= ~(1u << bit);
-        p.refs[page] = 1;
-        if (kFrom) {
-          a.ids[rank] = page;
-        } else {
-          while (start[r + 1] <= rank) ++r;
-          int length, want, c0, c1;
-          columns(r, length, want, c0, c1);
-          const int j = rank - start[r], held = pages_of(p, length);
-          const bool copy = shared_last[r] && j == 0;
-          const int c = copy ? c0 : held + j - shared_last[r];
-          int32_t* entry = p.tables + r * p.t_st + c;
-          if (copy) {
-            a.source[r] = *entry;
-            a.target[r] = page;
-          }
-          *entry = page;
-        }
-      }
-      p.free[w] = kept;
-    }
-  }
-  __syncthreads();
-
-  if (!kFrom) {
-    // lengths, and the pages that were copied from lose a holder (after all free bits have been read)
-    for (int r = tid; r < p.R; r += kPoolThreads)
-      if (start[r + 1] > start[r]) {
-        if (shared_last[r]) drop_page(p, a.source[r]);
-        p.lengths[r] = a.to[r];
-      }
-  } else {
-    for (int r = wave; r < p.R; r += kPoolWaves) {
       int length, want, c0, c1;
-      columns(r, length, want, c0, c1);
-      const int held = pages_of(p, length), n = start[r + 1] - start[r];
-      int rank = start[r];
-      // (shared pages are looked for as they were: counts of copied pages change behind the barrier below)
-      for (int c = 0; c < p.cols; c += 64) {
-        const int at = c + lane;
-        const bool takes = n > 0 && at >= c0 && at < c1 && (at >= held || is_shared(r, at));
-        const uint64_t mask = __ballot(takes);
-        int32_t from = -1, page = -1;
-        if (takes) {
-          page = a.ids[rank + __popcll(mask & ((1ull << lane) - 1))];
-          int32_t* entry = p.tables + r * p.t_st + at;
-          if (at < held) from = *entry;
-          *entry = page;
-        }
-        rank += __popcll(mask);
-        if (at < p.cols) {
-          a.source[(int64_t)r * p.cols + at] = from;
-          a.target[(int64_t)r * p.cols + at] = from >= 0 ? page : -1;
-        }
-      }
-      if (lane == 0 && a.ok[r] && want > length) p.lengths[r] = want;
+      const bool fits = columns(r, length, want, c0, c1), served = need == 0 || before + need <= have;
+      start[r] = served ? (int)before : -1;
+      a.ok[r] = fits && served;
+      if (served && need) atomicMax(&given, (int)(before + need));
     }
-    __syncthreads();
-    for (int64_t i = tid; i < (int64_t)p.R * p.cols; i += kPoolThreads)
-      if (a.source[i] >= 0) drop_page(p, a.source[i]);
   }
+  __syncthreads();
+  hand_out(p, given, sums, found, [&](int base, int n, int page0) {
+    for (int i = tid; i < n; i += kPoolThreads) {
+      a.ids[base + i] = page0 + found[i];
+      p.refs[page0 + found[i]] = 1;
+    }
+  });
+  for (int r = wave; r < p.R; r += kPoolWaves) {
+    int length, want, c0, c1;
+    columns(r, length, want, c0, c1);
+    const int held = pages_of(p, length);
+    int k = start[r];
+    const bool served = k >= 0;
+    // (shared pages are looked for as they were: counts of copied pages change behind the barrier below)
+    for (int c = 0; c < p.cols; c += 64) {
+      const int at = c + lane;
+      const bool takes = served && at >= c0 && at < c1 && (at >= held || is_shared(r, at));
+      const uint64_t mask = __ballot(takes);
+      int32_t from = -1, page = -1;
+      if (takes) {
+        page = a.ids[k + __popcll(mask & ((1ull << lane) - 1))];
+        int32_t* entry = p.tables + r * p.t_st + at;
+        if (at < held) from = *entry;
+        *entry = page;
+      }
+      k += __popcll(mask);
+      if (at < p.cols) {
+        a.source[(int64_t)r * p.cols + at] = from;
+        a.target[(int64_t)r * p.cols + at] = from >= 0 ? page : -1;
+      }
+    }
+    if (lane == 0 && a.ok[r] && want > length) p.lengths[r] = want;
+  }
+  __syncthreads();
+  for (int64_t i = tid; i < (int64_t)p.R * p.cols; i += kPoolThreads)
+    if (a.source[i] >= 0) drop_page(p, a.source[i]);
 }
 
 // ---- compaction --------------------------------------------------------------------------------------------------
@@ -408,10 +447,10 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(CopyParams a) {
       Unit v[U];
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (threadIdx.x + 256 * u < units) v[u] = from[threadIdx.x + 256 * u];
+        if (threadIdx.x + 256 * u < units) v[u] = __builtin_nontemporal_load(from + threadIdx.x + 256 * u);
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (threadIdx.x + 256 * u < units) to[threadIdx.x + 256 * u] = v[u];
+        if (threadIdx.x + 256 * u < units) __builtin_nontemporal_store(v[u], to + threadIdx.x + 256 * u);
     } else {
       for (int64_t u = threadIdx.x; u < units; u += 256) to[u] = from[u];
     }
@@ -471,8 +510,8 @@ extern "C" int hla_s6_pool_extend(int32_t* tables, int64_t t_st, int32_t num_req
               "pool_extend: null pointer argument");
   HLA_REQUIRE(!from || (int64_t)num_reqs * cols <= INT32_MAX, HLA_S6_EINVAL, "pool_extend: too many table entries");
   const ExtendParams a = {p, to, from, ok, source, target, scratch};
-  if (from) hipLaunchKernelGGL(pool_extend_kernel<true>, dim3(1), dim3(kPoolThreads), 0, as_stream(stream), a);
-  else hipLaunchKernelGGL(pool_extend_kernel<false>, dim3(1), dim3(kPoolThreads), 0, as_stream(stream), a);
+  if (from) hipLaunchKernelGGL(pool_extend_from_kernel, dim3(1), dim3(kPoolThreads), 0, as_stream(stream), a);
+  else hipLaunchKernelGGL(pool_extend_kernel, dim3(1), dim3(kPoolThreads), 0, as_stream(stream), a);
   return check_launch("pool_extend");
 }
 

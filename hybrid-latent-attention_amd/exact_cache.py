@@ -62,9 +62,10 @@ def store_rows(key, value, slots, cache, k_scale=None, v_scale=None):
 
 def row_shares(max_rows, groups, parts, cu_count=256):
     """``shares`` of ``attention`` for rows of at most ``max_rows`` and ``groups`` (token, KV head) pairs over ``parts`` KV heads: two
-    workgroups per CU, or 0 (a workgroup per group) where the rows are short or the groups many. A function of constants and the
-    row count only (graph-stable)."""
-    if max_rows <= 256 or groups >= 16 * cu_count:
+    workgroups per CU together, which is what fits one at a time (32 tokens of 1000 to 8160 rows on 8 KV heads: 115 us with a half
+    of them, 101, 102 with twice as many), or 0, a workgroup per group, where the second launch costs more than it evens out: on
+    short rows, and where the groups are many. A function of constants and the row count only (graph-stable)."""
+    if max_rows <= 512 or groups >= 16 * cu_count or (max_rows <= 1024 and groups >= 2 * cu_count):
         return 0
     return max(1, min(MAX_SHARES, 2 * cu_count // parts))
 

@@ -107,8 +107,9 @@ def extend_requests(pool, lengths, write_from=None):
         write_from = _vector('write_from', write_from, R)
     dev = tables.device
     ok = torch.empty(R, dtype=torch.bool, device=dev)
-    lists = torch.empty((2, R) if write_from is None else (3, R, C), dtype=I32, device=dev)
-    source, target, scratch = lists[0], lists[1], None if write_from is None else lists[2]
+    shape = (R,) if write_from is None else (R, C)
+    source, target = torch.empty(shape, dtype=I32, device=dev), torch.empty(shape, dtype=I32, device=dev)
+    scratch = None if write_from is None else torch.empty(shape, dtype=I32, device=dev)
     _call('hla_s6_pool_extend', dev, *args, lengths.data_ptr(), _lib.ptr(write_from), ok.data_ptr(), source.data_ptr(),
           target.data_ptr(), _lib.ptr(scratch))
     return Extension(ok, source, target)
@@ -120,10 +121,10 @@ def compact_pages(pool):
     pool before anything reads it; pages from ``U`` on are free then. Holders that no table knows find their pages by the moves."""
     args = _pool(pool)
     dev, N = pool.refs.device, pool.refs.shape[0]
-    lists = torch.empty(2, N // 2, dtype=I32, device=dev)
+    source, target = torch.empty(N // 2, dtype=I32, device=dev), torch.empty(N // 2, dtype=I32, device=dev)
     scratch = torch.empty(N + 2, dtype=I32, device=dev)
-    _call('hla_s6_pool_compact', dev, *args, lists[0].data_ptr(), lists[1].data_ptr(), scratch.data_ptr())
-    return Moves(lists[0], lists[1])
+    _call('hla_s6_pool_compact', dev, *args, source.data_ptr(), target.data_ptr(), scratch.data_ptr())
+    return Moves(source, target)
 
 
 def copy_pages(caches, source, target):
