@@ -64,8 +64,13 @@ def row_shares(max_rows, groups, parts, cu_count=256):
     """``shares`` of ``attention`` for rows of at most ``max_rows`` and ``groups`` (token, KV head) pairs over ``parts`` KV heads: two
     workgroups per CU together, which is what fits one at a time (32 tokens of 1000 to 8160 rows on 8 KV heads: 115 us with a half
     of them, 101, 102 with twice as many), or 0, a workgroup per group, where the second launch costs more than it evens out: on
-    short rows, and where the groups are many. A function of constants and the row count only (graph-stable)."""
-    if max_rows <= 512 or groups >= 16 * cu_count or (max_rows <= 1024 and groups >= 2 * cu_count):
+    short rows, and where the groups are many. GPU time in us with shares / a workgroup per group, 8 KV heads:
+
+        tokens x rows   1 x 512     1 x 768     1 x 1024    4 x 1024    16 x 1024   16 x 1536   32 x 1536   64 x 1024
+                        11.1 / 9.1  11.1 / 11.3 11.2 / 13.4 11.6 / 14.0 19.7 / 17.9 24.5 / 24.0 41.9 / 35.8 48.9 / 45.9
+
+    (a call on the host takes 16 / 11). A function of constants and the row count only (graph-stable)."""
+    if max_rows <= (1536 if 2 * groups >= cu_count else 1024) or groups >= 16 * cu_count:
         return 0
     return max(1, min(MAX_SHARES, 2 * cu_count // parts))
 

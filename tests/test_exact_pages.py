@@ -60,10 +60,10 @@ def test_new_pools(pg):
 
 def test_how_rows_are_cut(ec):
     """Two workgroups per CU between the KV heads; a workgroup per group for short rows and for very many groups."""
-    assert ec.row_shares(993, 16, 16, 256) == 32 and ec.row_shares(131000, 16, 8, 256) == 64
+    assert ec.row_shares(8160, 16, 16, 256) == 32 and ec.row_shares(131000, 16, 8, 256) == 64
     assert ec.row_shares(4096, 1024, 16, 256) == 32 and ec.row_shares(10 ** 6, 1, 1, 256) == 512
-    assert ec.row_shares(131000, 10 ** 6, 8, 256) == 0 and ec.row_shares(512, 4, 4, 256) == 0 and ec.row_shares(0, 4, 4, 256) == 0
-    assert ec.row_shares(513, 4, 4, 256) == 128 and ec.row_shares(1024, 512, 8, 256) == 0 and ec.row_shares(1025, 512, 8, 256) == 64
+    assert ec.row_shares(131000, 10 ** 6, 8, 256) == 0 and ec.row_shares(1024, 4, 4, 256) == 0 and ec.row_shares(0, 4, 4, 256) == 0
+    assert ec.row_shares(1025, 4, 4, 256) == 128 and ec.row_shares(1536, 128, 8, 256) == 0 and ec.row_shares(1537, 128, 8, 256) == 64
     assert ec.row_shares(4096, 3000, 3000, 256) == 1
 
 
