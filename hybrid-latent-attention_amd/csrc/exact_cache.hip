@@ -248,7 +248,7 @@ __global__ __launch_bounds__(64 * G::WAVES) void exact_cache_kernel(ExactCachePa
           qo[s] = head < heads ? ld16(qp + col) ^ flip : u32x4{0u, 0u, 0u, 0u};
         }
       }
-      const float factor = fabsf(scale);
+      const float factor = scale == 0.f ? 0x1p-126f : fabsf(scale);   // (a masked score stays -inf)
 
       float m = -INFINITY, l = 0.f;
       floatx4 o[CT];

@@ -28,13 +28,31 @@ from .compact_cache import _call, _rows2d, _same_device, _vector
 I32 = torch.int32
 MAX_REQUESTS = 8192
 
-#: ``tables [R, C]``: the pages of request ``r``, -1 behind its last; ``lengths [R]``: its rows; ``refs [N]``: requests that hold a
-#: page; ``free [ceil(N / 32)]``: bit ``p % 32`` of word ``p // 32`` is set where ``refs[p]`` is 0 (all int32); ``block``: rows per page.
-Pool = namedtuple('Pool', 'tables lengths refs free block')
 #: What ``extend_requests`` returns: ``ok [R]`` (bool), and the pages to copy.
 Extension = namedtuple('Extension', 'ok source target')
 #: Pages to copy: int32 lists, -1 where there is nothing to do.
 Moves = namedtuple('Moves', 'source target')
+
+
+class Pool:
+    """The state of a pool, int32 tensors on one device: ``tables [R, C]`` (any row stride), the pages of request ``r``, -1 behind its
+    last; ``lengths [R]``, its rows; ``refs [N]``, the requests that hold a page; ``free [ceil(N / 32)]``, bit ``p % 32`` of word ``p //
+    32`` set where ``refs[p]`` is 0; and ``block``, the rows per page. Checked here, once; the operators below change it in place."""
+
+    __slots__ = ('tables', 'lengths', 'refs', 'free', 'block', '_args')
+
+    def __init__(self, tables, lengths, refs, free, block):
+        stride, cols = _rows2d('tables', tables, I32)
+        R, N, block = tables.shape[0], refs.shape[0], int(block)
+        if R > MAX_REQUESTS or block < 1:
+            raise ValueError(f'no pool for {R} requests (at most {MAX_REQUESTS}) with pages of {block} rows')
+        for name, t, n in (('lengths', lengths, R), ('refs', refs, N), ('free', free, -(-N // 32))):
+            if _vector(name, t, n) is not t:
+                raise ValueError(f'{name} must be contiguous')
+            if t.device != tables.device:
+                raise RuntimeError(f'tensors on {tables.device} and {t.device}')
+        self.tables, self.lengths, self.refs, self.free, self.block = tables, lengths, refs, free, block
+        self._args = (tables.data_ptr(), stride, R, cols, lengths.data_ptr(), refs.data_ptr(), N, free.data_ptr(), block)
 
 
 def new_pool(num_pages, block, max_requests, max_rows, device, reserved=0):
@@ -54,28 +72,16 @@ def new_pool(num_pages, block, max_requests, max_rows, device, reserved=0):
                 torch.where(words >> 31 > 0, words - (1 << 32), words).to(I32), block)
 
 
-def _pool(pool, *others):
-    """The pool's arguments of an entry point, checked."""
-    tables, lengths, refs, free, block = pool
-    _same_device(tables, lengths, refs, free, *others)
-    stride, cols = _rows2d('tables', tables, I32)
-    R, N = tables.shape[0], refs.shape[0]
-    for name, t, n in (('lengths', lengths, R), ('refs', refs, N), ('free', free, -(-N // 32))):
-        if _vector(name, t, n) is not t:
-            raise ValueError(f'{name} must be contiguous')
-    return (tables.data_ptr(), stride, R, cols, lengths.data_ptr(), refs.data_ptr(), N, free.data_ptr(), int(block))
-
-
 def release_requests(pool, requests, lengths=None):
     """Requests ``requests`` (int32 ``[n]``) keep their first ``lengths[i]`` rows (int32 ``[n]``; none without it; more than a request
     has: all) and give back the pages behind them; a page is free once nobody holds it. Numbers outside the pool are skipped; of a
     request named twice the shorter length holds."""
     n = requests.shape[0]
-    args = _pool(pool, requests, lengths)
+    _same_device(pool.tables, requests, lengths)
     requests = _vector('requests', requests, n)
     if lengths is not None:
         lengths = _vector('lengths', lengths, n)
-    _call('hla_s6_pool_release', pool.tables.device, *args, requests.data_ptr(), _lib.ptr(lengths), n)
+    _call('hla_s6_pool_release', pool.tables.device, *pool._args, requests.data_ptr(), _lib.ptr(lengths), n)
 
 
 def fork_requests(pool, parents, children):
@@ -83,10 +89,10 @@ def fork_requests(pool, parents, children):
     shared, nothing is copied. Returns ``ok [n]`` (bool): False, and nothing done, where a number is outside the pool, the child
     has rows or was named before in the list, or the parent is itself among the children."""
     n = parents.shape[0]
-    args = _pool(pool, parents, children)
+    _same_device(pool.tables, parents, children)
     parents, children = _vector('parents', parents, n), _vector('children', children, n)
     ok = torch.empty(n, dtype=torch.bool, device=pool.tables.device)
-    _call('hla_s6_pool_fork', ok.device, *args, parents.data_ptr(), children.data_ptr(), n, ok.data_ptr())
+    _call('hla_s6_pool_fork', ok.device, *pool._args, parents.data_ptr(), children.data_ptr(), n, ok.data_ptr())
     return ok
 
 
@@ -99,7 +105,7 @@ def extend_requests(pool, lengths, write_from=None):
     ``ok[r]`` is False, and the request as it was, where ``lengths[r]`` does not fit the table or it and the requests before it ask for
     more pages than are free: no request overtakes one that waits. (Requests that share a page and write to it in the same call get a
     copy each.) The lists are ``[R]``, or with ``write_from`` ``[R, C]``, an entry per entry of the table."""
-    args = _pool(pool, lengths, write_from)
+    _same_device(pool.tables, lengths, write_from)
     tables = pool.tables
     R, C = tables.shape
     lengths = _vector('lengths', lengths, R)
@@ -110,7 +116,7 @@ def extend_requests(pool, lengths, write_from=None):
     shape = (R,) if write_from is None else (R, C)
     source, target = torch.empty(shape, dtype=I32, device=dev), torch.empty(shape, dtype=I32, device=dev)
     scratch = None if write_from is None else torch.empty(shape, dtype=I32, device=dev)
-    _call('hla_s6_pool_extend', dev, *args, lengths.data_ptr(), _lib.ptr(write_from), ok.data_ptr(), source.data_ptr(),
+    _call('hla_s6_pool_extend', dev, *pool._args, lengths.data_ptr(), _lib.ptr(write_from), ok.data_ptr(), source.data_ptr(),
           target.data_ptr(), _lib.ptr(scratch))
     return Extension(ok, source, target)
 
@@ -119,11 +125,11 @@ def compact_pages(pool):
     """Pages in use move to the front: with ``U`` of them, the i-th page in use at or behind ``U`` takes the i-th free place before it,
     in the tables and counts. The returned ``Moves`` (int32 ``[N // 2]``, -1 behind the last) are to be copied in every cache of the
     pool before anything reads it; pages from ``U`` on are free then. Holders that no table knows find their pages by the moves."""
-    args = _pool(pool)
+    _same_device(pool.tables)
     dev, N = pool.refs.device, pool.refs.shape[0]
     source, target = torch.empty(N // 2, dtype=I32, device=dev), torch.empty(N // 2, dtype=I32, device=dev)
     scratch = torch.empty(N + 2, dtype=I32, device=dev)
-    _call('hla_s6_pool_compact', dev, *args, source.data_ptr(), target.data_ptr(), scratch.data_ptr())
+    _call('hla_s6_pool_compact', dev, *pool._args, source.data_ptr(), target.data_ptr(), scratch.data_ptr())
     return Moves(source, target)
 
 

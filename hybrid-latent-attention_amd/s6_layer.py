@@ -12,7 +12,7 @@ from dataclasses import dataclass
 
 import torch
 
-from . import _lib, compact_cache, s6_ops
+from . import _lib, compact_cache, exact_cache, s6_ops
 
 
 def latent_inv_freq(head_dim, theta):
@@ -120,7 +120,7 @@ class StepContext:
         _lib.call('hla_s6_step_metadata', _lib.ptr(qsl), R, _lib.ptr(seq), num_tokens, int(window or 0),
                   _lib.ptr(self.token_requests), _lib.ptr(self.valid), _lib.ptr(self.invalid), _lib.ptr(self.ctx),
                   _lib.ptr(self.ctx_latent), None, _lib.stream(device))
-        self._empty = self._empty_latent = None
+        self._empty = self._empty_latent = self._row_counts = None
         self._block_tables = {}
         self._plans = {}
         self._slots = {}
@@ -157,6 +157,14 @@ class StepContext:
     @ctx_latent.setter
     def ctx_latent(self, lengths):
         self._ctx_latent, self._lengths_seen = lengths, None
+
+    @property
+    def row_counts(self):
+        """Rows of an exact cache that every token sees, its own the last (int32 ``[num_tokens]``; 0 on padding), computed on first
+        use."""
+        if self._row_counts is None:
+            self._row_counts = ((self.positions + 1) * self.valid).to(torch.int32)
+        return self._row_counts
 
     def _check_lengths(self):
         """Drops what was worked out of other latent lengths than those of now (of a tensor made under inference mode, whose
@@ -376,6 +384,25 @@ def _attend_decode(sl, loop, q_lat, q_rope, cache, block_table, ctx, window):
               _lib.ptr(o_hist),
               _lib.ptr(lse_hist), _lib.ptr(o_win), _lib.ptr(lse_win), _lib.ptr(out), out.stride(0), out.stride(1),
               _lib.stream(dev))
+    return out
+
+
+def attend_exact(q_rope, k_rope, v, cache, block_table, ctx, k_scale=None, v_scale=None):
+    """Attention of a layer and loop that keeps its exact cache and reads all of it (no reference counterpart: the S6 layers read
+    it in a window; a layer left exact, or the teacher on the same pages, does not).
+
+    ``q_rope`` is ``[T, H, d]``; ``k_rope`` and ``v`` (``[T, KV heads, d]``) are stored at the tokens' positions in ``cache`` (an exact
+    cache, bf16 or e4m3 with its scales, see ``exact_cache``) through the per-request ``block_table``, or None where the caller has
+    written them. Every token attends to its request's rows up to its own position. Returns ``[T, H, d]`` with ``~valid`` rows
+    zero. A step without metadata (profiling) has neither rows nor cache writes and returns zeros."""
+    if not ctx.md_present:
+        return torch.zeros_like(q_rope)
+    if k_rope is not None:
+        exact_cache.store_rows(k_rope, v, ctx.slots(block_table, cache.shape[2]), cache, k_scale, v_scale)
+    rows = block_table.shape[1] * cache.shape[2]
+    longest = min(int(ctx.max_seqlen_k), rows) if ctx.max_seqlen_k else rows
+    out, _ = exact_cache.attention(q_rope, cache, block_table, ctx.row_counts, ctx.scale, longest, ctx.token_requests,
+                                   k_scale=k_scale, v_scale=v_scale)
     return out
 
 

@@ -175,7 +175,7 @@ def test_scales_of_scores(ec):
     n = [2000, 500]
     c = Cache(13, n, 1, 128, 16)
     q = query(14, 2, 4, 128, 12.0)
-    for scale in (0.5, -0.3, 1e-4):
+    for scale in (0.5, -0.3, 1e-4, 0.0):
         o, lse = attend(ec, q, c, n, scale)
         if scale < 0:
             check(o, lse, -q, c, range(2), n, -scale)

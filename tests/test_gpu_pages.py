@@ -231,15 +231,18 @@ def test_refusals(pg):
     for call, match in ((lambda: pg.release_requests(pool, one.long()), 'requests'), (lambda: pg.release_requests(pool, one, two), 'lengths'),
                         (lambda: pg.fork_requests(pool, one, two), 'children'), (lambda: pg.extend_requests(pool, one), 'lengths'),
                         (lambda: pg.extend_requests(pool, two, one), 'write_from'),
-                        (lambda: pg.compact_pages(pool._replace(lengths=one)), 'lengths'),
-                        (lambda: pg.compact_pages(pool._replace(refs=torch.zeros(40, dtype=torch.int32, device='cuda'))), 'free'),
-                        (lambda: pg.compact_pages(pool._replace(tables=pool.tables.t())), 'tables'),
-                        (lambda: pg.compact_pages(pool._replace(refs=torch.zeros(16, dtype=torch.int32, device='cuda')[::2])), 'contiguous'),
-                        (lambda: pg.compact_pages(pool._replace(block=0)), 'block size')):
+                        (lambda: pg.Pool(pool.tables, one, pool.refs, pool.free, 16), 'lengths'),
+                        (lambda: pg.Pool(pool.tables, pool.lengths, torch.zeros(40, dtype=torch.int32, device='cuda'), pool.free, 16), 'free'),
+                        (lambda: pg.Pool(pool.tables.t(), pool.lengths, pool.refs, pool.free, 16), 'tables'),
+                        (lambda: pg.Pool(pool.tables, pool.lengths, torch.zeros(16, dtype=torch.int32, device='cuda')[::2], pool.free, 16),
+                         'contiguous'),
+                        (lambda: pg.Pool(pool.tables, pool.lengths.long(), pool.refs, pool.free, 16), 'lengths'),
+                        (lambda: pg.Pool(pool.tables, pool.lengths, pool.refs, pool.free, 0), 'no pool')):
         with pytest.raises(ValueError, match=match):
             call()
-    with pytest.raises(RuntimeError):
-        pg.fork_requests(pool, one, one.cpu())
+    for call in (lambda: pg.fork_requests(pool, one, one.cpu()), lambda: pg.Pool(pool.tables, pool.lengths.cpu(), pool.refs, pool.free, 16)):
+        with pytest.raises(RuntimeError):
+            call()
     c = torch.zeros(8, 4, 6, device='cuda')
     for caches, a, b, match in (([c, c[:4]], one, one, 'one shape'), ([c, c.half()], one, one, 'one shape'), (c[:, :, :5], one, one, 'dense'),
                                 (c[:, ::2], one, one, 'dense'), (c[:1].expand(8, 4, 6), one, one, 'apart'), (c, one, two, 'one shape'),
