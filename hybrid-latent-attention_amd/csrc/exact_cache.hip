@@ -46,7 +46,8 @@ struct ExactCacheParams {
   float scale_log2;
   const float *k_scale, *v_scale;
   int T, H, KH, G, tiles;  // tiles: workgroups of query heads per KV head
-  int shares;              // 0: a workgroup takes all rows of a token
+  int shares;              // 0: a workgroup takes all rows of a token, or (grouped) of 16 / G tokens
+  bool grouped;
   float *ws_o, *ws_lse;    // [shares][2][H][D], [shares][2][H]
   int32_t* split;          // [T][2]: first and last share of a token's rows
   uint16_t* out;
@@ -159,9 +160,15 @@ __device__ __forceinline__ void find_share(const ExactCacheParams& a, int k, int
   at = (int)(begin - before);
 }
 
-// kOnce: rows are read by one workgroup and stream past the caches. kTwice: up to 8 query heads per workgroup, columns 8.. are
-// heads 0.. again.
-template <class G, bool kOnce, bool kTwice>
+// What the 16 columns of the scores are
+enum Columns {
+  kHeads,    // query heads of a token
+  kTwice,    // up to 8 of them, and the same again
+  kTokens,   // those of several tokens, which share the rows of a request (the queries of a chunk)
+};
+
+// kOnce: rows are read by one workgroup and stream past the caches
+template <class G, bool kOnce, Columns kColumns>
 __global__ __launch_bounds__(64 * G::WAVES) void exact_cache_kernel(ExactCacheParams a) {
   constexpr int D = G::D;
   constexpr bool kE4 = G::kE4;
@@ -181,18 +188,42 @@ __global__ __launch_bounds__(64 * G::WAVES) void exact_cache_kernel(ExactCachePa
   const int parts = a.KH * a.tiles, part = blockIdx.x % parts, k = blockIdx.x / parts;
   const int kh = part / a.tiles, j0 = part % a.tiles * kMaxTile;
   const int heads = min(kMaxTile, a.G - j0), h0 = kh * a.G + j0;
-  const int head = kTwice ? x & 7 : x;
   const uint8_t* cache = a.cache + kh * a.head_stride;
+  // column x: head `head` of token k, or with several of token t_group + x / G
+  const int group = kColumns == kTokens ? kMaxTile / a.G : 1, t_group = k * group, t_end = min(a.T, t_group + group);
+  const int head = kColumns == kTwice ? x & 7 : kColumns == kTokens ? x % a.G : x;
+  const int token = t_group + (kColumns == kTokens ? x / a.G : 0);
+  auto table_row = [&](int i) { return a.bt_rows ? min(max(a.bt_rows[i], (int64_t)0), (int64_t)a.bt_count - 1) : i; };
 
-  int t = k, at = 0;
+  int t = t_group, at = 0;
   int64_t left_steps = INT32_MAX, before = 0, share = 1;
   if (a.shares) {
     find_share(a, k, 64 * WAVES, sums, found, t, at, left_steps, before, share);
     if (left_steps <= 0) return;
   }
-  for (;;) {   // the tokens of the share
+  for (;;) {   // the tokens of the share, or the requests of the group
     int first, n;
     token_rows(a, t, first, n);
+    const int64_t row = table_row(t);
+    // tokens [t, t_last) of a request: rows [first, n) are seen by any of them, [all_first, all_n) by all that see any
+    int t_last = t + 1, all_first = first, all_n = n, my_first = 0, my_n = 0;
+    if constexpr (kColumns == kTokens) {
+      int any_first = INT32_MAX, any_n = 0;
+      all_first = 0;
+      all_n = INT32_MAX;
+      for (t_last = t; t_last < t_end && table_row(t_last) == row; ++t_last) {
+        int f, c;
+        token_rows(a, t_last, f, c);
+        if (c <= f) continue;
+        any_first = min(any_first, f);
+        any_n = max(any_n, c);
+        all_first = max(all_first, f);
+        all_n = min(all_n, c);
+      }
+      first = min(any_first, any_n);
+      n = any_n;
+      if (token >= t && token < t_last) token_rows(a, token, my_first, my_n);
+    }
     const int steps = (n - first + kStep - 1) / kStep;
     const int taken = (int)min((int64_t)steps - at, left_steps);
     const int lo = first + at * kStep, hi = (int)min((int64_t)n, (int64_t)lo + (int64_t)taken * kStep);
@@ -202,13 +233,13 @@ __global__ __launch_bounds__(64 * G::WAVES) void exact_cache_kernel(ExactCachePa
       a.split[2 * t + 1] = (int)((before + steps - 1) / share);
     }
     if (lo >= hi && !a.shares) {
-      for (int i = tid; i < heads * (D / 8); i += 64 * WAVES)
-        st16(a.out + (int64_t)t * a.o_st + (int64_t)(h0 + i / (D / 8)) * a.o_sh + i % (D / 8) * 8, u32x4{0u, 0u, 0u, 0u});
-      for (int j = tid; j < heads; j += 64 * WAVES) a.lse[(int64_t)(h0 + j) * a.T + t] = -INFINITY;
-      return;
+      for (int u = t; u < t_last; ++u) {
+        for (int i = tid; i < heads * (D / 8); i += 64 * WAVES)
+          st16(a.out + (int64_t)u * a.o_st + (int64_t)(h0 + i / (D / 8)) * a.o_sh + i % (D / 8) * 8, u32x4{0u, 0u, 0u, 0u});
+        for (int j = tid; j < heads; j += 64 * WAVES) a.lse[(int64_t)(h0 + j) * a.T + u] = -INFINITY;
+      }
     }
     if (lo < hi) {
-      const int64_t row = a.bt_rows ? min(max(a.bt_rows[t], (int64_t)0), (int64_t)a.bt_count - 1) : t;
       const int32_t* btr = a.bt + row * a.bt_stride;
       const int tiles = (hi - lo + KEYS - 1) / KEYS;
       const int mine = tiles > wave ? (tiles - wave + WAVES - 1) / WAVES : 0;  // tiles wave, wave + WAVES, ...
@@ -240,12 +271,13 @@ __global__ __launch_bounds__(64 * G::WAVES) void exact_cache_kernel(ExactCachePa
       const float scale = a.scale_log2 * (kE4 && a.k_scale ? a.k_scale[kh] : 1.f);
       u32x4 qo[D / 32];
       {
-        const uint16_t* qp = a.q + (int64_t)t * a.q_st + (int64_t)(h0 + min(head, heads - 1)) * a.q_sh;
+        const bool used = kColumns == kTokens ? token >= t && token < t_last : head < heads;
+        const uint16_t* qp = a.q + (int64_t)(kColumns == kTokens && used ? token : t) * a.q_st + (int64_t)(h0 + (used ? head : 0)) * a.q_sh;
         const uint32_t flip = scale < 0.f ? 0x80008000u : 0u;   // scores of -q, so that the largest one has the largest weight
 #pragma unroll
         for (int s = 0; s < D / 32; ++s) {
           const int col = kE4 ? 16 * (g + 4 * (s / 2)) + 8 * (s % 2) : 32 * s + 8 * g;
-          qo[s] = head < heads ? ld16(qp + col) ^ flip : u32x4{0u, 0u, 0u, 0u};
+          qo[s] = used ? ld16(qp + col) ^ flip : u32x4{0u, 0u, 0u, 0u};
         }
       }
       const float factor = scale == 0.f ? 0x1p-126f : fabsf(scale);   // (a masked score stays -inf)
@@ -298,8 +330,19 @@ __global__ __launch_bounds__(64 * G::WAVES) void exact_cache_kernel(ExactCachePa
             }
           }
         }
-        const int left = hi - (lo + (wave + i * WAVES) * KEYS);   // keys of the tile
-        if (left < KEYS) {
+        const int row0 = lo + (wave + i * WAVES) * KEYS, left = hi - row0;   // keys of the tile
+        const bool mixed = kColumns == kTokens && (row0 < all_first || row0 + KEYS > all_n);   // some tokens see some of them
+        if (kColumns == kTokens) {
+          if (mixed) {
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const int j = row0 + 16 * b + 4 * g + r;
+                if (j < my_first || j >= my_n) s[b][r] = -INFINITY;
+              }
+          }
+        } else if (left < KEYS) {
           // rows past the last repeat it: no weight, and values of 0 (0 * inf is not)
 #pragma unroll
           for (int b = 0; b < KB; ++b)
@@ -334,33 +377,54 @@ __global__ __launch_bounds__(64 * G::WAVES) void exact_cache_kernel(ExactCachePa
           for (int r = 0; r < 4; ++r) l += w[r] = fast_exp2(fmaf(s[b][r], factor, -from));
           p[b] = u32x2{upper_halves(w[0], w[1]), upper_halves(w[2], w[3])};
           p2[b] = u32x2{rests(w[0], w[1], p[b][0]), rests(w[2], w[3], p[b][1])};
-          if (kTwice && x >= 8) p[b] = p2[b];
+          if (kColumns == kTwice && x >= 8) p[b] = p2[b];
         }
-        if constexpr (kE4) {
-          const u32x4 pt = u32x4{p[0][0], p[0][1], p[1][0], p[1][1]};
-          // lane x of group g reads half a piece of key 4g + x/2 (x < 8) or 16 + 4g + x/2 - 4
-          const int key = (x < 8 ? 0 : 12) + 4 * g + (x >> 1);
-          const uint8_t* vr = buf + key * RB + 8 * (x & 1);
-#pragma unroll
-          for (int c = 0; c < CT; ++c) {
+        // V^T of 16 columns, as the A operand
+        // e4m3: lane x of group g reads half a piece of key 4g + x/2 (x < 8) or 16 + 4g + x/2 - 4; bf16: of key 4g + x/4
+        const int key = kE4 ? (x < 8 ? 0 : 12) + 4 * g + (x >> 1) : 4 * g + (x >> 2);
+        const uint8_t* vr = buf + key * RB + 8 * (x & 1);
+        auto add = [&](floatx4 to, int c, const uint32_t* seen, bool both) {
+          if constexpr (kE4) {
             typedef int int2v __attribute__((ext_vector_type(2)));
-            const int2v v = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+            int2v v = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
                 (__attribute__((address_space(3))) int2v*)(vr + 16 * ((CPR / 2 + c) ^ swizzle<G>(key))));
+            if (seen) v = int2v{(int)(v[0] & seen[0]), (int)(v[1] & seen[1])};
             const u32x4 vt = e4m3_to_bf16((uint32_t)v[0], (uint32_t)v[1]);
-            o[c] = mfma16x16x32(vt, pt, o[c]);
-            if (!kTwice) o[c] = mfma16x16x32(vt, u32x4{p2[0][0], p2[0][1], p2[1][0], p2[1][1]}, o[c]);
+            to = mfma16x16x32(vt, u32x4{p[0][0], p[0][1], p[1][0], p[1][1]}, to);
+            return both ? mfma16x16x32(vt, u32x4{p2[0][0], p2[0][1], p2[1][0], p2[1][1]}, to) : to;
+          } else {
+            u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) short4v*)(vr + 16 * ((CPR / 2 + 2 * c + ((x >> 1) & 1)) ^ swizzle<G>(key)))));
+            if (seen) v = u32x2{v[0] & seen[0], v[1] & seen[1]};
+            const short4v vt = __builtin_bit_cast(short4v, v);
+            to = mfma16x16x16(vt, __builtin_bit_cast(short4v, p[0]), to);
+            return both ? mfma16x16x16(vt, __builtin_bit_cast(short4v, p2[0]), to) : to;
+          }
+        };
+        if (kColumns == kTokens && mixed) {
+          // rows that a token does not see may hold anything, and 0 * NaN is not 0: a token at a time, its rows and its columns
+          for (int u = t; u < t_last; ++u) {
+            int f, c1;
+            token_rows(a, u, f, c1);
+            uint32_t seen[2];   // of keys 4g .. and 16 + 4g .. (a byte each), or of 4g, 4g + 1 and 4g + 2, 4g + 3 (a half each)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              seen[w] = 0;
+#pragma unroll
+              for (int e = 0; e < (kE4 ? 4 : 2); ++e) {
+                const int j = row0 + 4 * g + (kE4 ? 16 * w : 2 * w) + e;
+                if (j >= f && j < c1) seen[w] |= (kE4 ? 0xffu : 0xffffu) << (kE4 ? 8 : 16) * e;
+              }
+            }
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+              const floatx4 more = add(floatx4{0.f, 0.f, 0.f, 0.f}, c, seen, true);
+              if (token == u) o[c] += more;
+            }
           }
         } else {
-          const short4v pt = __builtin_bit_cast(short4v, p[0]);
-          const int key = 4 * g + (x >> 2);
-          const uint8_t* vr = buf + key * RB + 8 * (x & 1);
 #pragma unroll
-          for (int c = 0; c < CT; ++c) {
-            const short4v vt = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) short4v*)(vr + 16 * ((CPR / 2 + 2 * c + ((x >> 1) & 1)) ^ swizzle<G>(key))));
-            o[c] = mfma16x16x16(vt, pt, o[c]);
-            if (!kTwice) o[c] = mfma16x16x16(vt, __builtin_bit_cast(short4v, p2[0]), o[c]);
-          }
+          for (int c = 0; c < CT; ++c) o[c] = add(o[c], c, nullptr, kColumns != kTwice);
         }
       }
 
@@ -377,14 +441,16 @@ __global__ __launch_bounds__(64 * G::WAVES) void exact_cache_kernel(ExactCachePa
         for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stats[w][0][x]);
         const float f = m == -INFINITY ? 0.f : fast_exp2(m - top);
         // (a NaN among the scores is in l, and where m is -inf nothing but zeros and NaN are in o)
-        if (head < heads) {
+        if (kColumns == kTokens || head < heads) {
 #pragma unroll
           for (int c = 0; c < CT; ++c) *reinterpret_cast<floatx4*>(joined + (wave * 16 + x) * OS + 16 * c + 4 * g) = o[c] * f;
         }
       }
       __syncthreads();
-      for (int i = tid; i < heads * (D / 4); i += 64 * WAVES) {
-        const int j = i / (D / 4), col = i % (D / 4) * 4;
+      const int j_first = (t - t_group) * heads, j_count = (t_last - t) * heads;   // its columns (the tokens' ones)
+      for (int i = tid; i < (kColumns == kTokens ? j_count : heads) * (D / 4); i += 64 * WAVES) {
+        const int j = (kColumns == kTokens ? j_first : 0) + i / (D / 4), col = i % (D / 4) * 4;
+        const int u = kColumns == kTokens ? t_group + j / heads : t, h = h0 + (kColumns == kTokens ? j % heads : j);
         float top = -INFINITY, sum = 0.f;
         for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stats[w][0][j]);
         floatx4 v = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -392,27 +458,33 @@ __global__ __launch_bounds__(64 * G::WAVES) void exact_cache_kernel(ExactCachePa
           const float mw = stats[w][0][j];
           sum += stats[w][1][j] * (mw == -INFINITY ? 0.f : fast_exp2(mw - top));
           v += *reinterpret_cast<floatx4*>(joined + (w * 16 + j) * OS + col);
-          if (kTwice) v += *reinterpret_cast<floatx4*>(joined + (w * 16 + j + 8) * OS + col);
+          if (kColumns == kTwice) v += *reinterpret_cast<floatx4*>(joined + (w * 16 + j + 8) * OS + col);
         }
-        const bool none = sum == 0.f;
+        bool none = sum == 0.f;
+        if (kColumns == kTokens) {
+          int f, c;
+          token_rows(a, u, f, c);
+          none = none || c <= f;   // (its columns took part in what the others see)
+          if (none) v = floatx4{0.f, 0.f, 0.f, 0.f};
+        }
         const float inv = none ? 0.f : (kE4 && a.v_scale ? a.v_scale[kh] : 1.f) / sum;
         const float lse = none ? -INFINITY : (top + log2f(sum)) * kLn2;
         if (!whole) {   // rows that began in an earlier share, or that go on in the next
-          const int64_t place = ((int64_t)2 * k + (at == 0)) * a.H + h0 + j;
+          const int64_t place = ((int64_t)2 * k + (at == 0)) * a.H + h;
           *reinterpret_cast<floatx4*>(a.ws_o + place * D + col) = v * inv;
           if (col == 0) a.ws_lse[place] = lse;
         } else {
-          *reinterpret_cast<u32x2*>(a.out + (int64_t)t * a.o_st + (int64_t)(h0 + j) * a.o_sh + col) =
+          *reinterpret_cast<u32x2*>(a.out + (int64_t)u * a.o_st + (int64_t)h * a.o_sh + col) =
               u32x2{pack2(v[0] * inv, v[1] * inv), pack2(v[2] * inv, v[3] * inv)};
-          if (col == 0) a.lse[(int64_t)(h0 + j) * a.T + t] = lse;
+          if (col == 0) a.lse[(int64_t)h * a.T + u] = lse;
         }
       }
     }
     left_steps -= taken;
-    if (!a.shares || left_steps <= 0) return;
+    if (a.shares ? left_steps <= 0 : t_last >= t_end) return;
     before += steps;
     at = 0;
-    ++t;             // (steps are left, so a token with rows follows)
+    t = t_last;      // (steps are left, so a token with rows follows)
     __syncthreads(); // the parts in LDS have been read
   }
 }
@@ -471,17 +543,19 @@ __global__ __launch_bounds__(256) void exact_join_kernel(ExactCacheParams a) {
 
 template <int D, bool kE4>
 void launch_exact_cache(const ExactCacheParams& p, hipStream_t st) {
-  const unsigned grid = (unsigned)((int64_t)(p.shares ? p.shares : p.T) * p.KH * p.tiles);
+  const int group = p.grouped ? kMaxTile / p.G : 1;
+  const unsigned grid = (unsigned)((int64_t)(p.shares ? p.shares : (p.T + group - 1) / group) * p.KH * p.tiles);
   const bool once = p.tiles == 1 && p.T <= p.bt_count;   // a table row for every token
   // whole tokens for at most a workgroup per CU: twice the waves (one token of 16 heads, 993 rows: 17.4 us with 4, 12.9 with 8)
-  const bool wide = !p.shares && (int64_t)p.T * p.KH * p.tiles <= kCus;
+  const bool wide = !p.shares && !p.grouped && (int64_t)p.T * p.KH * p.tiles <= kCus;
   using G = ExactGeo<D, kE4, false>;
   using W = ExactGeo<D, kE4, true>;
-  void (*const kernels[8])(ExactCacheParams) = {
-      exact_cache_kernel<G, false, false>, exact_cache_kernel<G, false, true>, exact_cache_kernel<G, true, false>,
-      exact_cache_kernel<G, true, true>,   exact_cache_kernel<W, false, false>, exact_cache_kernel<W, false, true>,
-      exact_cache_kernel<W, true, false>,  exact_cache_kernel<W, true, true>};
-  hipLaunchKernelGGL(kernels[4 * wide + 2 * once + (p.G <= 8)], dim3(grid), dim3(64 * (wide ? W::WAVES : G::WAVES)), 0, st, p);
+  void (*const kernels[9])(ExactCacheParams) = {
+      exact_cache_kernel<G, false, kHeads>, exact_cache_kernel<G, false, kTwice>, exact_cache_kernel<G, true, kHeads>,
+      exact_cache_kernel<G, true, kTwice>,  exact_cache_kernel<W, false, kHeads>, exact_cache_kernel<W, false, kTwice>,
+      exact_cache_kernel<W, true, kHeads>,  exact_cache_kernel<W, true, kTwice>,  exact_cache_kernel<G, false, kTokens>};
+  hipLaunchKernelGGL(kernels[p.grouped ? 8 : 4 * wide + 2 * once + (p.G <= 8)], dim3(grid), dim3(64 * (wide ? W::WAVES : G::WAVES)),
+                     0, st, p);
   if (p.shares)
     hipLaunchKernelGGL(exact_join_kernel<D>, dim3((unsigned)((int64_t)p.T * p.H)), dim3(256), 0, st, p);
 }
@@ -562,7 +636,7 @@ extern "C" int hla_s6_exact_attention(const void* q, int32_t num_tokens, int32_t
                                       const int32_t* block_table, int64_t bt_stride, int32_t bt_cols, int32_t bt_count,
                                       const int64_t* bt_rows, const int32_t* ctx, int32_t window, float scale,
                                       const float* k_scale, const float* v_scale, int32_t shares,
-                                      float* workspace, int64_t workspace_floats, void* out, int64_t o_st, int64_t o_sh,
+                                      int32_t grouped, float* workspace, int64_t workspace_floats, void* out, int64_t o_st, int64_t o_sh,
                                       float* lse, void* stream) {
   using namespace hla;
   HLA_REQUIRE(num_tokens >= 0, HLA_S6_EINVAL, "exact_attention: negative token count");
@@ -606,6 +680,9 @@ extern "C" int hla_s6_exact_attention(const void* q, int32_t num_tokens, int32_t
   p.G = num_heads / kv_heads;
   p.tiles = (p.G + kMaxTile - 1) / kMaxTile;
   p.shares = shares;
+  p.grouped = grouped != 0;
+  HLA_REQUIRE(!grouped || (shares == 0 && p.G <= kMaxTile / 2), HLA_S6_EINVAL,
+              "exact_attention: groups of tokens need shares 0 and at most %d query heads per KV head", kMaxTile / 2);
   HLA_REQUIRE((int64_t)max(p.T, shares) * p.KH * p.tiles <= INT32_MAX && (int64_t)p.T * p.H <= INT32_MAX, HLA_S6_EINVAL,
               "exact_attention: too many rows");
   if (shares) {

@@ -75,6 +75,13 @@ def row_shares(max_rows, groups, parts, cu_count=256):
     return max(1, min(MAX_SHARES, 2 * cu_count // parts))
 
 
+def _grouped(tokens, heads, kv_heads, cu_count=256):
+    """Whether workgroups take ``16 // heads`` tokens (``heads`` query heads per KV head) together: with one of them for every CU.
+    Chunks on top of histories, us with groups / a workgroup per token: 4 x 512 tokens on 8160 rows of 16 heads 613 / 6863, of 8 KV
+    heads for 32 1030 / 3445, a prompt of 4000 of 16 heads 396 / 3764, 8 x 64 on 4000 (8 KV heads for 32) 152 / 464."""
+    return heads <= 8 and -(-tokens // (16 // heads)) * kv_heads >= cu_count
+
+
 def attention(q, cache, block_table, ctx, scale, max_seq_len, token_requests=None, window=0, k_scale=None, v_scale=None,
               shares=None, workspace=None):
     """Attention of ``q [T, H, d]`` (bf16, any token and head strides) over the rows ``[max(0, n - window), n)`` of ``n = ctx[t]``
@@ -83,7 +90,7 @@ def attention(q, cache, block_table, ctx, scale, max_seq_len, token_requests=Non
 
     The rows of a token are those before it and its own, once ``store_rows`` has written it; tokens of one request (a chunk) have a
     ``ctx`` of their own each. ``block_table`` (int32) is per token, or per request with ``token_requests[t]`` (int64) naming the
-    row of token ``t``. No entry of ``ctx`` should be above ``max_seq_len`` (a host number, which sets how rows are cut). Scores,
+    row of token ``t`` (tokens of a request that lie one behind the other go through its rows together in large steps). No entry of ``ctx`` should be above ``max_seq_len`` (a host number, which sets how rows are cut). Scores,
     softmax statistics and sums are fp32; weights keep 16 bits in their product with V.
 
     The rows of all tokens are cut in ``shares`` equal parts per KV head (0: a workgroup takes all rows of a token; defaults to
@@ -106,7 +113,13 @@ def attention(q, cache, block_table, ctx, scale, max_seq_len, token_requests=Non
     dev = q.device
     longest = min(int(max_seq_len), cols * block, window or cols * block)
     parts = kv_heads * -(-H // kv_heads // 16)
-    shares = row_shares(longest, T * parts, parts, _lib.device_cus(dev.index)) if shares is None else int(shares)
+    cus = _lib.device_cus(dev.index)
+    grouped = False
+    if shares is None:
+        grouped = T > count and _grouped(T, H // kv_heads, kv_heads, cus)   # (more tokens than table rows: chunks)
+        shares = 0 if grouped else row_shares(longest, T * parts, parts, cus)
+    else:
+        shares = int(shares)
     if not 0 <= shares <= MAX_SHARES:
         raise ValueError(f'shares must be 0 to {MAX_SHARES}, got {shares}')
     ws = None
@@ -121,6 +134,6 @@ def attention(q, cache, block_table, ctx, scale, max_seq_len, token_requests=Non
     token_stride, head_stride, _ = q.stride()
     _call('hla_s6_exact_attention', dev, q.data_ptr(), T, H, d, token_stride, head_stride, cache.data_ptr(), int(e4m3), kv_heads,
           page, head, row, block, pages, block_table.data_ptr(), table_stride, cols, count, _lib.ptr(token_requests),
-          ctx.data_ptr(), window, float(scale), _lib.ptr(k_scale), _lib.ptr(v_scale), shares, _lib.ptr(ws),
+          ctx.data_ptr(), window, float(scale), _lib.ptr(k_scale), _lib.ptr(v_scale), shares, int(grouped), _lib.ptr(ws),
           0 if ws is None else ws.numel(), out.data_ptr(), H * d, d, lse.data_ptr())
     return out, lse

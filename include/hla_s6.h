@@ -589,14 +589,16 @@ int hla_s6_move_rows(void *cache, int32_t width, int32_t compact, int64_t page_s
  * scale * q[t, h] . K[row, h / (num_heads / kv_heads)], times V; lse [num_heads, num_tokens]. Token t reads row bt_rows ?
  * bt_rows[t] : t of the table, clamped into its bt_count rows; page ids are clamped into the cache; at most bt_cols * block_size
  * rows. shares 0: a workgroup takes all rows of a (token, KV head); else (at most 1024) the rows of all tokens together are cut in
- * that many equal shares per KV head, and the workspace holds 2 * shares * num_heads * (head_dim + 1) + 2 * num_tokens floats. */
+ * that many equal shares per KV head, and the workspace holds 2 * shares * num_heads * (head_dim + 1) + 2 * num_tokens floats.
+ * grouped != 0 (shares 0, at most 8 query heads per KV head): a workgroup takes 16 / (num_heads / kv_heads) tokens one behind the
+ * other, those that read the same table row together. */
 int hla_s6_exact_attention(const void *q, int32_t num_tokens, int32_t num_heads, int32_t head_dim, int64_t q_st,
                            int64_t q_sh, const void *cache, int32_t e4m3, int32_t kv_heads, int64_t page_stride,
                            int64_t head_stride, int64_t row_stride, int32_t block_size, int64_t num_blocks,
                            const int32_t *block_table, int64_t bt_stride, int32_t bt_cols, int32_t bt_count,
                            const int64_t *bt_rows, const int32_t *ctx, int32_t window, float scale,
-                           const float *k_scale, const float *v_scale, int32_t shares, float *workspace,
-                           int64_t workspace_floats, void *out, int64_t o_st, int64_t o_sh, float *lse, void *stream);
+                           const float *k_scale, const float *v_scale, int32_t shares, int32_t grouped,
+                           float *workspace, int64_t workspace_floats, void *out, int64_t o_st, int64_t o_sh, float *lse, void *stream);
 
 /* Row t of key / value (bf16 [num_tokens, kv_heads, head_dim]) into slot slots[t] (page * block_size + row; outside the cache:
  * skipped; the slots of a call differ). e4m3: x / scale, clamped to +-448, to the nearest, ties to even; NaN stays NaN. */

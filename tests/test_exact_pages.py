@@ -93,15 +93,16 @@ def test_entry_points_check_before_they_launch(pkg):
                 call(name, {**good, **change})
 
     attention = {0: 16, 1: 1, 2: 8, 3: 64, 4: 512, 5: 64, 6: 16, 8: 2, 9: 4096, 10: 128, 11: 256, 12: 16, 13: 2, 14: 16, 15: 1, 16: 1,
-                 17: 1, 19: 16, 27: 16, 28: 512, 29: 64, 30: 16}
+                 17: 1, 19: 16, 28: 16, 29: 512, 30: 64, 31: 16}
     refused('hla_s6_exact_attention', attention, [
         ({1: -1}, 'token count'), ({3: 96}, 'head dim'), ({8: 0}, 'KV heads'), ({8: 3}, '8 query heads over 3'), ({2: 1}, 'query heads'),
         ({12: 0}, 'block size'), ({13: 0}, 'page count'), ({6: 8}, 'aligned'), ({9: 4097}, 'multiples of 16'), ({11: 255}, 'multiples of 16'),
         ({10: 64}, 'overlap'), ({11: 64}, 'overlap'), ({24: -1}, 'shares'), ({24: 1025}, 'shares'), ({20: -1}, 'window'),
         ({22: 16}, 'scales'), ({23: 16}, 'scales'), ({17: 0}, 'table rows'), ({0: None}, 'null pointer'), ({14: None}, 'null pointer'),
-        ({19: None}, 'null pointer'), ({27: None}, 'null pointer'), ({30: None}, 'null pointer'), ({4: 4}, 'aligned'), ({0: 8}, 'aligned'),
-        ({29: 4}, 'aligned'), ({1: 2 ** 30, 17: 2 ** 30}, 'too many rows'), ({24: 2, 25: 8, 26: 10 ** 6}, 'aligned')])
-    refused('hla_s6_exact_attention', attention, [({24: 2, 25: 16, 26: 10}, 'workspace'), ({24: 2, 26: 10 ** 6}, 'workspace')], RuntimeError)
+        ({19: None}, 'null pointer'), ({28: None}, 'null pointer'), ({31: None}, 'null pointer'), ({4: 4}, 'aligned'), ({0: 8}, 'aligned'),
+        ({30: 4}, 'aligned'), ({1: 2 ** 30, 17: 2 ** 30}, 'too many rows'), ({24: 2, 26: 8, 27: 10 ** 6}, 'aligned'),
+        ({24: 2, 25: 1, 26: 16, 27: 10 ** 6}, 'groups of tokens'), ({25: 1, 2: 18}, 'groups of tokens')])
+    refused('hla_s6_exact_attention', attention, [({24: 2, 26: 16, 27: 10}, 'workspace'), ({24: 2, 27: 10 ** 6}, 'workspace')], RuntimeError)
     call('hla_s6_exact_attention', {**attention, 1: 0, 0: None})      # no tokens, nothing to do
     store = {0: 16, 1: 128, 2: 64, 3: 16, 4: 128, 5: 64, 6: 1, 7: 2, 8: 64, 9: 16, 12: 16, 14: 4096, 15: 128, 16: 256, 17: 16, 18: 2}
     refused('hla_s6_exact_store', store, [

@@ -377,3 +377,79 @@ def test_store_divides_by_the_scale(ec):
     want = (torch.cat((key, value), -1).double() / scale.double()[:, None]).clamp(-448, 448)
     step = 2.0 ** (torch.floor(torch.log2(want.abs().clamp(min=2.0 ** -6))) - 3)
     assert ((got - want).abs() <= step / 2 * (1 + 2.0 ** -19)).all()
+
+
+# ---- tokens that go through the rows of a request together --------------------------------------------------------------
+
+def chunks(n, lens, order):
+    """Requests and lengths of the tokens of causal chunks, request after request."""
+    requests = sum(([r] * lens[r] for r in order), [])
+    return requests, sum(([n[r] - lens[r] + i + 1 for i in range(lens[r])] for r in order), [])
+
+
+@pytest.mark.parametrize('e4m3', [False, True])
+@pytest.mark.parametrize('kv_heads,G,d,block', [(2, 1, 128, 16), (1, 2, 64, 24), (2, 3, 128, 32), (1, 4, 256, 16), (1, 5, 64, 16),
+                                               (2, 8, 128, 1), (3, 7, 128, 16)])
+@pytest.mark.parametrize('window', [0, 21])
+def test_groups_of_tokens(ec, monkeypatch, kv_heads, G, d, block, e4m3, window):
+    """Chunks that begin and end inside a group of tokens, single tokens among them, tokens without rows, lengths in any order."""
+    monkeypatch.setattr(ec, '_grouped', lambda *a: True)
+    n, lens = [300, 40, 17, 900, 33], [37, 40, 1, 5, 33]
+    c = Cache(G + d, n, kv_heads, d, block, e4m3)
+    requests, ctx = chunks(n, lens, (3, 0, 1, 2, 4))
+    ctx[7], ctx[60], ctx[-1] = 0, -4, 12
+    requests, ctx = requests + [2, 0, 2], ctx + [17, 300, 5]
+    q = query(G, len(ctx), kv_heads * G, d)
+    o, lse = ec.attention(q, c.cache, c.table, dev_i32(np.array(ctx)), d ** -0.5, max(n), dev_i64(np.array(requests)), window,
+                          c.k_scale, c.v_scale)
+    check(o, lse, q, c, requests, ctx, d ** -0.5, window)
+
+
+@pytest.mark.parametrize('e4m3', [False, True])
+def test_rows_that_a_token_of_a_group_does_not_see(ec, monkeypatch, e4m3):
+    """NaN and infinities in the rows behind a token's last, and before its window, reach only the tokens that see them."""
+    monkeypatch.setattr(ec, '_grouped', lambda *a: True)
+    n = [200]
+    c = Cache(40, n, 2, 128, 16, e4m3)
+    ctx = [170, 171, 200, 172, 190, 1, 173, 174, 176, 177, 180, 179, 178, 175, 0, 169]
+    requests = [0] * 15 + [0]
+    base = query(41, 16, 4, 128)
+    want = ec.attention(base, c.cache, c.table, dev_i32(np.array(ctx)), 0.1, 200, dev_i64(np.array(requests)), 0, c.k_scale, c.v_scale)
+    check(*want, base, c, requests, ctx, 0.1)
+    raw = c.cache.view(torch.uint8) if e4m3 else c.cache
+    bad = 0x7F if e4m3 else math.nan
+    at = torch.arange(176, 200, device='cuda')
+    raw[c.table[0].long()[at // 16], :, at % 16] = bad
+    o, lse = ec.attention(base, c.cache, c.table, dev_i32(np.array(ctx)), 0.1, 200, dev_i64(np.array(requests)), 0, c.k_scale, c.v_scale)
+    sees = torch.tensor([x > 176 for x in ctx], device='cuda')
+    assert torch.isnan(o[sees]).all() and torch.isnan(lse[:, sees]).all()
+    assert torch.equal(o[~sees], want[0][~sees]) and torch.equal(lse[:, ~sees], want[1][:, ~sees])
+    if not e4m3:
+        c.cache[c.table[0, 176 // 16].long(), :, 176 % 16, 128:] = math.inf      # and an infinity in V alone
+        c.cache[c.table[0, 176 // 16].long(), :, 176 % 16, :128] = 1
+        o, lse = ec.attention(base, c.cache, c.table, dev_i32(np.array(ctx)), 0.1, 200, dev_i64(np.array(requests)), 0)
+        assert torch.isposinf(o[ctx.index(177)]).all() and torch.isfinite(lse[:, ctx.index(177)]).all()
+        assert torch.equal(o[~sees], want[0][~sees])
+    raw[c.table[0].long()[at // 16], :, at % 16] = 0
+    before = torch.arange(0, 150, device='cuda')
+    window = 20
+    clean = ec.attention(base, c.cache, c.table, dev_i32(np.array(ctx)), 0.1, 200, dev_i64(np.array(requests)), window, c.k_scale, c.v_scale)
+    raw[c.table[0].long()[before // 16], :, before % 16] = bad
+    o, lse = ec.attention(base, c.cache, c.table, dev_i32(np.array(ctx)), 0.1, 200, dev_i64(np.array(requests)), window, c.k_scale, c.v_scale)
+    sees = torch.tensor([0 < x < 170 for x in ctx], device='cuda')
+    assert torch.isnan(o[sees]).all() and torch.equal(o[~sees], clean[0][~sees]) and torch.equal(lse[:, ~sees], clean[1][:, ~sees])
+
+
+@pytest.mark.parametrize('kv_heads,G', [(16, 1), (8, 4)])
+def test_large_chunks(ec, kv_heads, G):
+    """Steps large enough for groups by the rule, prompts without history among them."""
+    n, lens = [1500, 700, 513, 3000], [300, 700, 1, 400]
+    c = Cache(50 + G, n, kv_heads, 128, 16)
+    requests, ctx = chunks(n, lens, range(4))
+    assert ec._grouped(len(ctx), G, kv_heads)
+    q = query(51, len(ctx), kv_heads * G, 128)
+    o, lse = ec.attention(q, c.cache, c.table, dev_i32(np.array(ctx)), 0.09, 3000, dev_i64(np.array(requests)))
+    some = list(range(0, len(ctx), 61)) + [len(ctx) - 1]
+    check(o[some], lse[:, some], q[some], c, [requests[t] for t in some], [ctx[t] for t in some], 0.09)
+    alone = ec.attention(q, c.cache, c.table, dev_i32(np.array(ctx)), 0.09, 3000, dev_i64(np.array(requests)), shares=0)
+    assert (o.float() - alone[0].float()).abs().max() <= 2.0 ** -6 * alone[0].float().abs().max()
