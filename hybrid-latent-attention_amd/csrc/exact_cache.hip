@@ -545,7 +545,7 @@ template <int D, bool kE4>
 void launch_exact_cache(const ExactCacheParams& p, hipStream_t st) {
   const int group = p.grouped ? kMaxTile / p.G : 1;
   const unsigned grid = (unsigned)((int64_t)(p.shares ? p.shares : (p.T + group - 1) / group) * p.KH * p.tiles);
-  const bool once = p.tiles == 1 && p.T <= p.bt_count;   // a table row for every token
+  const bool once = p.tiles == 1 && p.T < 2 * (int64_t)p.bt_count;   // a table row for every token, but for padding
   // whole tokens for at most a workgroup per CU: twice the waves (one token of 16 heads, 993 rows: 17.4 us with 4, 12.9 with 8)
   const bool wide = !p.shares && !p.grouped && (int64_t)p.T * p.KH * p.tiles <= kCus;
   using G = ExactGeo<D, kE4, false>;

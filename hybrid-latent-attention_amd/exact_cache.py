@@ -29,6 +29,8 @@ def _cache(cache, k_scale, v_scale):
         raise ValueError(f'an exact cache is bfloat16 or float8_e4m3fn, got {cache.dtype}')
     if len(shape) != 4 or shape[3] % 2 or shape[3] // 2 not in DIMS:
         raise ValueError(f'an exact cache is [num_blocks, KV heads, block, 2d] with d in {DIMS}, got {tuple(shape)}')
+    if not shape[1]:
+        raise ValueError('an exact cache has at least one KV head')
     if stride[3] != 1:
         raise ValueError('an exact cache needs a unit last-dim stride')
     e4m3 = cache.dtype == E4M3
@@ -116,7 +118,7 @@ def attention(q, cache, block_table, ctx, scale, max_seq_len, token_requests=Non
     cus = _lib.device_cus(dev.index)
     grouped = False
     if shares is None:
-        grouped = T > count and _grouped(T, H // kv_heads, kv_heads, cus)   # (more tokens than table rows: chunks)
+        grouped = T >= 4 * count and _grouped(T, H // kv_heads, kv_heads, cus)   # (chunks: several tokens per table row)
         shares = 0 if grouped else row_shares(longest, T * parts, parts, cus)
     else:
         shares = int(shares)

@@ -37,7 +37,8 @@ Moves = namedtuple('Moves', 'source target')
 class Pool:
     """The state of a pool, int32 tensors on one device: ``tables [R, C]`` (any row stride), the pages of request ``r``, -1 behind its
     last; ``lengths [R]``, its rows; ``refs [N]``, the requests that hold a page; ``free [ceil(N / 32)]``, bit ``p % 32`` of word ``p //
-    32`` set where ``refs[p]`` is 0; and ``block``, the rows per page. Checked here, once; the operators below change it in place."""
+    32`` set where ``refs[p]`` is 0; and ``block``, the rows per page. Checked here, once; the operators below write into the tensors,
+    which cannot be exchanged for others."""
 
     __slots__ = ('tables', 'lengths', 'refs', 'free', 'block', '_args')
 
@@ -51,8 +52,15 @@ class Pool:
                 raise ValueError(f'{name} must be contiguous')
             if t.device != tables.device:
                 raise RuntimeError(f'tensors on {tables.device} and {t.device}')
-        self.tables, self.lengths, self.refs, self.free, self.block = tables, lengths, refs, free, block
-        self._args = (tables.data_ptr(), stride, R, cols, lengths.data_ptr(), refs.data_ptr(), N, free.data_ptr(), block)
+        args = (tables.data_ptr(), stride, R, cols, lengths.data_ptr(), refs.data_ptr(), N, free.data_ptr(), block)
+        for name, value in zip(self.__slots__, (tables, lengths, refs, free, block, args)):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f'{name} of a pool is written into, not exchanged')
+
+    def __reduce__(self):
+        return Pool, (self.tables, self.lengths, self.refs, self.free, self.block)
 
 
 def new_pool(num_pages, block, max_requests, max_rows, device, reserved=0):
@@ -81,6 +89,8 @@ def release_requests(pool, requests, lengths=None):
     requests = _vector('requests', requests, n)
     if lengths is not None:
         lengths = _vector('lengths', lengths, n)
+        if lengths.data_ptr() == pool.lengths.data_ptr():
+            lengths = lengths.clone()   # (they change while requests are worked on)
     _call('hla_s6_pool_release', pool.tables.device, *pool._args, requests.data_ptr(), _lib.ptr(lengths), n)
 
 

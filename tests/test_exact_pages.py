@@ -1,4 +1,6 @@
 """CPU checks of whole exact caches and of pools of pages: the plain pool by hand, how rows are cut, refusals before any launch."""
+import copy
+
 import numpy as np
 import pytest
 import torch
@@ -56,6 +58,16 @@ def test_new_pools(pg):
             pg.new_pool(*args, 'cpu')
     with pytest.raises(ValueError, match='no pool'):
         pg.new_pool(4, 16, 1, 1, 'cpu', reserved=5)
+
+
+def test_a_pool_keeps_its_tensors(pg):
+    """Operators hold the addresses: a tensor of a pool is not exchanged, and a copy of a pool has tensors of its own."""
+    pool = pg.new_pool(5, 4, 2, 12, 'cpu')
+    with pytest.raises(AttributeError, match='written into'):
+        pool.lengths = torch.zeros(2, dtype=torch.int32)
+    other = copy.deepcopy(pool)
+    other.lengths[0] = 3
+    assert pool.lengths.tolist() == [0, 0] and other._args[4] == other.lengths.data_ptr() != pool.lengths.data_ptr()
 
 
 def test_how_rows_are_cut(ec):

@@ -306,7 +306,7 @@ def test_refusals(ec):
     for args, match in (((q.float(), c.cache, t, n, 1.0, 5), 'bfloat16'), ((q, c.cache.float(), t, n, 1.0, 5), 'float8_e4m3fn'),
                         ((q[:, :3], c.cache, t, n, 1.0, 5), 'multiple of 2 heads'), ((q[0], c.cache, t, n, 1.0, 5), 'q must be'),
                         ((query(1, 2, 4, 128), c.cache, t, n, 1.0, 5), '64'), ((q, c.cache[0], t, n, 1.0, 5), 'exact cache'),
-                        ((q, c.cache[..., :96], t, n, 1.0, 5), 'exact cache'), ((q, c.cache, t, n[:1], 1.0, 5), 'ctx'),
+                        ((q, c.cache[..., :96], t, n, 1.0, 5), 'exact cache'), ((q, c.cache[:, :0], t, n, 1.0, 5), 'one KV head'), ((q, c.cache, t, n[:1], 1.0, 5), 'ctx'),
                         ((q, c.cache, t, n.long(), 1.0, 5), 'ctx'), ((q, c.cache, t[:1], n, 1.0, 5), 'block_table'),
                         ((q, c.cache, t.long(), n, 1.0, 5), 'block_table'), ((q, c.cache, t, n, 1.0, 5, n), 'token_requests'),
                         ((q, c.cache, t, n, 1.0, 5, None, -1), 'window'), ((q, c.cache, t, n, 1.0, 5, None, 0, scale), 'k_scale'),
@@ -399,6 +399,7 @@ def test_groups_of_tokens(ec, monkeypatch, kv_heads, G, d, block, e4m3, window):
     requests, ctx = chunks(n, lens, (3, 0, 1, 2, 4))
     ctx[7], ctx[60], ctx[-1] = 0, -4, 12
     requests, ctx = requests + [2, 0, 2], ctx + [17, 300, 5]
+    assert len(ctx) >= 4 * len(n)
     q = query(G, len(ctx), kv_heads * G, d)
     o, lse = ec.attention(q, c.cache, c.table, dev_i32(np.array(ctx)), d ** -0.5, max(n), dev_i64(np.array(requests)), window,
                           c.k_scale, c.v_scale)
@@ -410,7 +411,7 @@ def test_rows_that_a_token_of_a_group_does_not_see(ec, monkeypatch, e4m3):
     """NaN and infinities in the rows behind a token's last, and before its window, reach only the tokens that see them."""
     monkeypatch.setattr(ec, '_grouped', lambda *a: True)
     n = [200]
-    c = Cache(40, n, 2, 128, 16, e4m3)
+    c = Cache(40, n, 2, 128, 16, e4m3)      # (one table row, sixteen tokens)
     ctx = [170, 171, 200, 172, 190, 1, 173, 174, 176, 177, 180, 179, 178, 175, 0, 169]
     requests = [0] * 15 + [0]
     base = query(41, 16, 4, 128)

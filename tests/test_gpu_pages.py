@@ -112,6 +112,21 @@ def test_extend(pg, R, rows, block, spare, full):
             pg.release_requests(dev, dev_i32(np.asarray(gone)))
 
 
+def test_lengths_of_the_pool_itself(pg):
+    """The pool's own lengths as an argument: what they were before the call."""
+    rng = np.random.default_rng(9)
+    pool = Pool.random(rng, [100, 20, 64, 7], 16, 8, 40)
+    dev = up(pg, pool)
+    order = [2, 0, 3, 1]
+    pool.release(order, list(pool.lengths))
+    pg.release_requests(dev, dev_i32(np.asarray(order)), dev.lengths)
+    same(dev, pool)
+    ok, _ = pool.extend(list(pool.lengths), list(pool.lengths))
+    got = pg.extend_requests(dev, dev.lengths, dev.lengths)
+    assert got.ok.tolist() == ok and (got.source == -1).all()
+    same(dev, pool)
+
+
 def test_pages_run_out(pg):
     """The first request that asks for more than there is waits, and those behind it that ask for any."""
     pool = Pool.empty(10, 4, 6, 8)
