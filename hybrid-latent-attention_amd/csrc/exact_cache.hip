@@ -8,15 +8,24 @@
 // share holds of a token is a part, whole tokens are written at once, and exact_join_kernel joins the parts of the others. (With
 // rows enough for the device, or short ones, a workgroup takes all rows of a token.) Each wave walks tiles of its own:
 //   * a tile's K and V rows come by direct copies into LDS, a KB each, NB - 1 tiles ahead (the stream is what bounds the
-//     kernel: 2d values per row and head are read once and meet 4 G d flops); the 16-byte pieces of a row lie swizzled, so
-//     that both ways of reading them below touch every bank once;
+//     kernel: 2d values per row and head are read once and meet 4 G d flops); the 16-byte pieces of a row lie swizzled, which
+//     spreads both ways of reading them below over the banks;
 //   * S^T[keys x 16 heads] = K Q^T on 16x16x32 bf16 products: K is the A operand (a row's pieces as they lie), Q^T stays in
 //     registers; heads past the group's are zero columns, whose work is cheaper than the bytes;
 //   * softmax in the exp2 domain, fp32, with a running maximum that is raised only when a score exceeds it by 2^8;
 //   * O^T[d x 16 heads] += V^T P^T: P^T comes out of the scores' registers as the B operand, V^T is read by the transposing
 //     LDS loads. bf16 tiles have 16 keys (16x16x16 products), e4m3 ones 32, in the order of keys that the two halves of the
 //     scores have (16x16x32), and e4m3 values become bf16, exactly, on their way into the operands.
-// P is rounded to bf16 for its product (half a step, 2^-9 of each weight; the output is bf16); sums are fp32.
+// P goes into its product as two bf16 parts, upper half and rounded rest (2^-16 of a weight is left; one part alone would add about
+// two thirds of the output's own rounding to it: 0.0024 relative to the 64-bit result, now 0.0017). Up to 8 query heads have their
+// rests in the 8 columns that would be zero: the scores of a head are made twice, for free. More heads take a second product.
+//
+// Large steps of many tokens per request (chunks) put the heads of 16 / G tokens in the columns (kTokens).
+//
+// Bound by HBM: 64 tokens of 4096 rows and 16 heads (2.1 GB) 320 us, 6.7 TB/s, the vector units at 24 %; a call is its bytes at
+// that rate and about 11 us (launch, lengths, table entries, first rows, joining waves, the second launch). Past the caches
+// (kOnce) 7 % faster. Two workgroups of four waves per CU, a tile of each wave on its way: three waves, eight, or one workgroup
+// with twice the tiles measured the same or slower, so did dealing the heads of a share to one XCD.
 #include "common.h"
 
 namespace hla {
@@ -465,8 +474,8 @@ __global__ __launch_bounds__(64 * G::WAVES) void exact_cache_kernel(ExactCachePa
           int f, c;
           token_rows(a, u, f, c);
           none = none || c <= f;   // (its columns took part in what the others see)
-          if (none) v = floatx4{0.f, 0.f, 0.f, 0.f};
         }
+        if (none) v = floatx4{0.f, 0.f, 0.f, 0.f};   // (weights of 0, of which a NaN in V made NaN)
         const float inv = none ? 0.f : (kE4 && a.v_scale ? a.v_scale[kh] : 1.f) / sum;
         const float lse = none ? -INFINITY : (top + log2f(sum)) * kLn2;
         if (!whole) {   // rows that began in an earlier share, or that go on in the next

@@ -346,16 +346,13 @@ __global__ __launch_bounds__(kPoolThreads) void pool_extend_from_kernel(ExtendPa
 
 // ---- compaction --------------------------------------------------------------------------------------------------
 // With U pages in use, the i-th page in use at or behind U moves to the i-th free place before it. pool_pairs_kernel finds the
-// pairs, place[page] for the pages that move, place[N] = U and place[N + 1] = their number; pool_compact_kernel then rewrites tables, counts and bits.
+// pairs, place[page] for the pages that move, place[N] = U and place[N + 1] = their number; pool_compact_kernel then rewrites
+// tables, counts and bits, and ends the lists.
 __global__ __launch_bounds__(kPoolThreads) void pool_pairs_kernel(Pool p, int32_t* source, int32_t* target, int32_t* place) {
   __shared__ int64_t sums[kPoolWaves + 1];
   const int tid = threadIdx.x, words = (p.N + 31) / 32;
-  int64_t total, empty = 0;
-  for (int w0 = 0; w0 < words; w0 += kPoolThreads) {
-    pool_scan(__popc(w0 + tid < words ? p.free[w0 + tid] & page_bits(p, w0 + tid) : 0u), sums, total);
-    empty += total;
-  }
-  const int used = p.N - (int)empty;
+  const int used = p.N - (int)count_free(p, sums);
+  int64_t total;
   int moved = 0;
   for (int pass = 0; pass < 2; ++pass) {   // holes, then movers
     const int first = pass ? used / 32 : 0, end = pass ? words : (used + 31) / 32;
@@ -379,18 +376,15 @@ __global__ __launch_bounds__(kPoolThreads) void pool_pairs_kernel(Pool p, int32_
     moved = base;
     __syncthreads();
   }
-  for (int i = tid; i < p.N / 2; i += kPoolThreads) {
-    if (i < moved) place[source[i]] = target[i];
-    else source[i] = target[i] = -1;
-  }
+  for (int i = tid; i < moved; i += kPoolThreads) place[source[i]] = target[i];
   if (tid == 0) {
     place[p.N] = used;
     place[p.N + 1] = moved;
   }
 }
 
-__global__ __launch_bounds__(256) void pool_compact_kernel(Pool p, const int32_t* source, const int32_t* target,
-                                                           const int32_t* place, int words) {
+__global__ __launch_bounds__(256) void pool_compact_kernel(Pool p, int32_t* source, int32_t* target, const int32_t* place,
+                                                           int words) {
   const int used = place[p.N], moved = place[p.N + 1];
   const int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
   for (int64_t i = i0; i < (int64_t)p.R * p.cols; i += step) {
@@ -404,6 +398,7 @@ __global__ __launch_bounds__(256) void pool_compact_kernel(Pool p, const int32_t
     p.refs[target[i]] = p.refs[source[i]];
     p.refs[source[i]] = 0;
   }
+  for (int64_t i = moved + i0; i < p.N / 2; i += step) source[i] = target[i] = -1;
   for (int64_t w = i0; w < words; w += step) {
     const int64_t cut = used - 32 * w;
     const uint32_t below = cut >= 32 ? ~0u : cut <= 0 ? 0u : (1u << cut) - 1;

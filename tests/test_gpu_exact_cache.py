@@ -210,6 +210,7 @@ def test_values_that_are_not_finite(ec, splits):
     for j in range(40):
         p, _, x = page(4, j)
         c.cache[p, :, x, 0] = -math.inf
+        c.cache[p, 1, x, 128:] = (math.nan, math.inf)[j % 2]      # values without any weight
     o, lse = attend(ec, base, c, n, shares=splits)
     assert torch.isnan(o[0, 2:]).all() and torch.isnan(lse[2:, 0]).all()
     assert torch.isposinf(o[1, :2, 9]).all() and torch.isnan(o[2, 2:]).all()
