@@ -125,7 +125,7 @@ def extend_requests(pool, lengths, write_from=None):
     ok = torch.empty(R, dtype=torch.bool, device=dev)
     shape = (R,) if write_from is None else (R, C)
     source, target = torch.empty(shape, dtype=I32, device=dev), torch.empty(shape, dtype=I32, device=dev)
-    scratch = None if write_from is None else torch.empty(shape, dtype=I32, device=dev)
+    scratch = None if write_from is None else torch.empty(R * (C + 1), dtype=I32, device=dev)
     _call('hla_s6_pool_extend', dev, *pool._args, lengths.data_ptr(), _lib.ptr(write_from), ok.data_ptr(), source.data_ptr(),
           target.data_ptr(), _lib.ptr(scratch))
     return Extension(ok, source, target)

@@ -628,8 +628,8 @@ int hla_s6_pool_fork(int32_t *tables, int64_t t_st, int32_t num_reqs, int32_t co
  * columns behind its last page get the lowest free pages, in the order of requests and columns; columns with rows to write
  * whose page others hold too get one that takes its place, and (source, target) say what to copy. A request is served if it and
  * those before it that ask for pages ask for no more than there are, and to[r] fits the table; else ok[r] is 0 and nothing is
- * changed. Lists: [num_reqs], or with `from` [num_reqs, cols], -1 where nothing is to be copied; scratch [num_reqs * cols] with
- * `from`. */
+ * changed. Lists: [num_reqs], or with `from` [num_reqs, cols], -1 where nothing is to be copied; scratch
+ * [num_reqs * (cols + 1)] with `from`. */
 int hla_s6_pool_extend(int32_t *tables, int64_t t_st, int32_t num_reqs, int32_t cols, int32_t *lengths, int32_t *refs,
                        int64_t num_pages, uint32_t *free_bits, int32_t block_size, const int32_t *to,
                        const int32_t *from, uint8_t *ok, int32_t *source, int32_t *target, int32_t *scratch, void *stream);
