@@ -56,7 +56,7 @@ struct ExactCacheParams {
   const float *k_scale, *v_scale;
   int T, H, KH, G, tiles;  // tiles: workgroups of query heads per KV head
   int shares;              // 0: a workgroup takes all rows of a token, or (grouped) of 16 / G tokens
-  bool grouped;
+  int grouped;             // workgroups among which the requests of a group are dealt; 0: a token by itself
   float *ws_o, *ws_lse;    // [shares][2][H][D], [shares][2][H]
   int32_t* split;          // [T][2]: first and last share of a token's rows
   uint16_t* out;
@@ -194,7 +194,11 @@ __global__ __launch_bounds__(64 * G::WAVES) void exact_cache_kernel(ExactCachePa
   const int tid = threadIdx.x, lane = tid & 63, x = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // heads innermost: workgroups dispatched one behind the other read the same rows' heads
-  const int parts = a.KH * a.tiles, part = blockIdx.x % parts, k = blockIdx.x / parts;
+  const int parts = a.KH * a.tiles, part = blockIdx.x % parts;
+  // a group's requests (runs of tokens with one table row) are dealt to `turns` workgroups
+  const int groups = kColumns == kTokens ? (a.T + kMaxTile / a.G - 1) / (kMaxTile / a.G) : 0;
+  const int k = kColumns == kTokens ? (int)(blockIdx.x / parts) % groups : (int)(blockIdx.x / parts);
+  const int turn = kColumns == kTokens ? (int)(blockIdx.x / parts) / groups : 0;
   const int kh = part / a.tiles, j0 = part % a.tiles * kMaxTile;
   const int heads = min(kMaxTile, a.G - j0), h0 = kh * a.G + j0;
   const uint8_t* cache = a.cache + kh * a.head_stride;
@@ -204,34 +208,62 @@ __global__ __launch_bounds__(64 * G::WAVES) void exact_cache_kernel(ExactCachePa
   const int token = t_group + (kColumns == kTokens ? x / a.G : 0);
   auto table_row = [&](int i) { return a.bt_rows ? min(max(a.bt_rows[i], (int64_t)0), (int64_t)a.bt_count - 1) : i; };
 
-  int t = t_group, at = 0;
+  // lane i: what token t_group + i reads and sees; a bit for every token that begins a run
+  int64_t lane_row = 0;
+  int lane_first = 0, lane_n = 0;
+  uint32_t heads_of_runs = 0;
+  if constexpr (kColumns == kTokens) {
+    const int i = t_group + lane;
+    if (i < t_end) {
+      lane_row = table_row(i);
+      token_rows(a, i, lane_first, lane_n);
+    }
+    const int64_t before = __shfl_up(lane_row, 1);
+    heads_of_runs = (uint32_t)__ballot(i < t_end && (lane == 0 || lane_row != before));
+    for (int skip = 0; skip < turn; ++skip) heads_of_runs &= heads_of_runs - 1;
+    if (!heads_of_runs) return;
+  }
+
+  int t = kColumns == kTokens ? t_group + __ffs((int)heads_of_runs) - 1 : t_group, at = 0;
   int64_t left_steps = INT32_MAX, before = 0, share = 1;
   if (a.shares) {
     find_share(a, k, 64 * WAVES, sums, found, t, at, left_steps, before, share);
     if (left_steps <= 0) return;
   }
   for (;;) {   // the tokens of the share, or the requests of the group
-    int first, n;
-    token_rows(a, t, first, n);
-    const int64_t row = table_row(t);
     // tokens [t, t_last) of a request: rows [first, n) are seen by any of them, [all_first, all_n) by all that see any
-    int t_last = t + 1, all_first = first, all_n = n, my_first = 0, my_n = 0;
+    int first, n, t_last = t + 1, all_first, all_n, my_first = 0, my_n = 0;
+    int64_t row;
     if constexpr (kColumns == kTokens) {
-      int any_first = INT32_MAX, any_n = 0;
-      all_first = 0;
-      all_n = INT32_MAX;
-      for (t_last = t; t_last < t_end && table_row(t_last) == row; ++t_last) {
-        int f, c;
-        token_rows(a, t_last, f, c);
-        if (c <= f) continue;
-        any_first = min(any_first, f);
-        any_n = max(any_n, c);
-        all_first = max(all_first, f);
-        all_n = min(all_n, c);
+      const int at_lane = t - t_group;
+      row = __shfl(lane_row, at_lane);
+      const uint64_t others = __ballot(lane > at_lane && (t_group + lane >= t_end || lane_row != row));
+      t_last = min(t_end, t_group + (others ? __ffsll((unsigned long long)others) - 1 : 64));
+      const bool sees = lane >= at_lane && t_group + lane < t_last && lane_n > lane_first;
+      first = sees ? lane_first : INT32_MAX;
+      n = sees ? lane_n : 0;
+      all_first = sees ? lane_first : 0;
+      all_n = sees ? lane_n : INT32_MAX;
+      for (int off = kMaxTile / 2; off > 0; off >>= 1) {   // (a group is in the first 16 lanes)
+        first = min(first, __shfl_xor(first, off));
+        n = max(n, __shfl_xor(n, off));
+        all_first = max(all_first, __shfl_xor(all_first, off));
+        all_n = min(all_n, __shfl_xor(all_n, off));
       }
-      first = min(any_first, any_n);
-      n = any_n;
-      if (token >= t && token < t_last) token_rows(a, token, my_first, my_n);
+      n = __builtin_amdgcn_readfirstlane(n);
+      first = min(__builtin_amdgcn_readfirstlane(first), n);
+      all_first = __builtin_amdgcn_readfirstlane(all_first);
+      all_n = __builtin_amdgcn_readfirstlane(all_n);
+      const int f = __shfl(lane_first, token - t_group), c = __shfl(lane_n, token - t_group);
+      if (token >= t && token < t_last) {
+        my_first = f;
+        my_n = c;
+      }
+    } else {
+      token_rows(a, t, first, n);
+      row = table_row(t);
+      all_first = first;
+      all_n = n;
     }
     const int steps = (n - first + kStep - 1) / kStep;
     const int taken = (int)min((int64_t)steps - at, left_steps);
@@ -413,8 +445,7 @@ __global__ __launch_bounds__(64 * G::WAVES) void exact_cache_kernel(ExactCachePa
         if (kColumns == kTokens && mixed) {
           // rows that a token does not see may hold anything, and 0 * NaN is not 0: a token at a time, its rows and its columns
           for (int u = t; u < t_last; ++u) {
-            int f, c1;
-            token_rows(a, u, f, c1);
+            const int f = __shfl(lane_first, u - t_group), c1 = __shfl(lane_n, u - t_group);
             uint32_t seen[2];   // of keys 4g .. and 16 + 4g .. (a byte each), or of 4g, 4g + 1 and 4g + 2, 4g + 3 (a half each)
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
@@ -489,11 +520,17 @@ __global__ __launch_bounds__(64 * G::WAVES) void exact_cache_kernel(ExactCachePa
         }
       }
     }
-    left_steps -= taken;
-    if (a.shares ? left_steps <= 0 : t_last >= t_end) return;
-    before += steps;
-    at = 0;
-    t = t_last;      // (steps are left, so a token with rows follows)
+    if constexpr (kColumns == kTokens) {
+      for (int skip = 0; skip < a.grouped; ++skip) heads_of_runs &= heads_of_runs - 1;
+      if (!heads_of_runs) return;
+      t = t_group + __ffs((int)heads_of_runs) - 1;
+    } else {
+      left_steps -= taken;
+      if (!a.shares || left_steps <= 0) return;
+      before += steps;
+      at = 0;
+      ++t;           // (steps are left, so a token with rows follows)
+    }
     __syncthreads(); // the parts in LDS have been read
   }
 }
@@ -552,8 +589,8 @@ __global__ __launch_bounds__(256) void exact_join_kernel(ExactCacheParams a) {
 
 template <int D, bool kE4>
 void launch_exact_cache(const ExactCacheParams& p, hipStream_t st) {
-  const int group = p.grouped ? kMaxTile / p.G : 1;
-  const unsigned grid = (unsigned)((int64_t)(p.shares ? p.shares : (p.T + group - 1) / group) * p.KH * p.tiles);
+  const int group = p.grouped ? kMaxTile / p.G : 1, turns = p.grouped ? p.grouped : 1;
+  const unsigned grid = (unsigned)((int64_t)(p.shares ? p.shares : (p.T + group - 1) / group) * turns * p.KH * p.tiles);
   const bool once = p.tiles == 1 && p.T < 2 * (int64_t)p.bt_count;   // a table row for every token, but for padding
   // whole tokens for at most a workgroup per CU: twice the waves (one token of 16 heads, 993 rows: 17.4 us with 4, 12.9 with 8)
   const bool wide = !p.shares && !p.grouped && (int64_t)p.T * p.KH * p.tiles <= kCus;
@@ -689,10 +726,11 @@ extern "C" int hla_s6_exact_attention(const void* q, int32_t num_tokens, int32_t
   p.G = num_heads / kv_heads;
   p.tiles = (p.G + kMaxTile - 1) / kMaxTile;
   p.shares = shares;
-  p.grouped = grouped != 0;
-  HLA_REQUIRE(!grouped || (shares == 0 && p.G <= kMaxTile / 2), HLA_S6_EINVAL,
-              "exact_attention: groups of tokens need shares 0 and at most %d query heads per KV head", kMaxTile / 2);
-  HLA_REQUIRE((int64_t)max(p.T, shares) * p.KH * p.tiles <= INT32_MAX && (int64_t)p.T * p.H <= INT32_MAX, HLA_S6_EINVAL,
+  p.grouped = grouped;
+  HLA_REQUIRE(grouped >= 0 && grouped <= kMaxTile && (!grouped || (shares == 0 && p.G <= kMaxTile / 2)), HLA_S6_EINVAL,
+              "exact_attention: groups of tokens need shares 0, at most %d query heads per KV head and at most %d turns", kMaxTile / 2,
+              kMaxTile);
+  HLA_REQUIRE((int64_t)max(grouped ? p.T + kMaxTile * kMaxTile : p.T, shares) * p.KH * p.tiles <= INT32_MAX / (grouped ? 2 : 1) && (int64_t)p.T * p.H <= INT32_MAX, HLA_S6_EINVAL,
               "exact_attention: too many rows");
   if (shares) {
     const int64_t rows = (int64_t)2 * shares * p.H, need = rows * (head_dim + 1) + 2 * (int64_t)p.T;

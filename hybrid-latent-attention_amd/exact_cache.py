@@ -77,22 +77,28 @@ def row_shares(max_rows, groups, parts, cu_count=256):
     return max(1, min(MAX_SHARES, 2 * cu_count // parts))
 
 
-def _grouped(tokens, heads, kv_heads, cu_count=256):
-    """Whether workgroups take ``16 // heads`` tokens (``heads`` query heads per KV head) together: with one of them for every CU.
-    Chunks on top of histories, us with groups / a workgroup per token: 4 x 512 tokens on 8160 rows of 16 heads 613 / 6863, of 8 KV
-    heads for 32 1030 / 3445, a prompt of 4000 of 16 heads 396 / 3764, 8 x 64 on 4000 (8 KV heads for 32) 152 / 464."""
-    return heads <= 8 and -(-tokens // (16 // heads)) * kv_heads >= cu_count
+def _turns(tokens, heads, kv_heads, cu_count=256, per_request=1):
+    """0, or the workgroups per group of ``16 // heads`` tokens (``heads`` query heads per KV head) that go through rows together, where
+    there is a group for every CU. Chunks on top of histories, us with groups / a workgroup per token: 4 x 512 tokens on 8160 rows of
+    16 heads 593 / 6863, of 8 KV heads for 32 1028 / 3445, a prompt of 4000 of 16 heads 358 / 3764, 8 x 64 on 4000 (8 KV heads for
+    32) 153 / 464.
+    A group of single tokens (which a step may have beside its chunks) has as many requests as tokens: with few tokens per request
+    on average a workgroup for each; else 4, since most find nothing to do."""
+    if heads > 8 or -(-tokens // (16 // heads)) * kv_heads < cu_count:
+        return 0
+    return 16 // heads if per_request < 32 else min(4, 16 // heads)
 
 
 def attention(q, cache, block_table, ctx, scale, max_seq_len, token_requests=None, window=0, k_scale=None, v_scale=None,
-              shares=None, workspace=None):
+              shares=None, workspace=None, max_query_len=None):
     """Attention of ``q [T, H, d]`` (bf16, any token and head strides) over the rows ``[max(0, n - window), n)`` of ``n = ctx[t]``
     (int32; ``window`` 0: over all ``n``) of an exact cache: ``(o [T, H, d] bf16, lse [H, T] fp32)``. ``H`` is a multiple of the
     cache's KV heads, and query head ``h`` reads KV head ``h // (H / KV heads)``. Tokens without rows give ``o = 0``, ``lse = -inf``.
 
     The rows of a token are those before it and its own, once ``store_rows`` has written it; tokens of one request (a chunk) have a
     ``ctx`` of their own each. ``block_table`` (int32) is per token, or per request with ``token_requests[t]`` (int64) naming the
-    row of token ``t`` (tokens of a request that lie one behind the other go through its rows together in large steps). No entry of ``ctx`` should be above ``max_seq_len`` (a host number, which sets how rows are cut). Scores,
+    row of token ``t``. Tokens of a request that lie one behind the other go through its rows together in large steps of chunks:
+    ``max_query_len`` (a host number, the most tokens of a request) defaults to the tokens per row of the table. No entry of ``ctx`` should be above ``max_seq_len`` (a host number, which sets how rows are cut). Scores,
     softmax statistics and sums are fp32; weights keep 16 bits in their product with V.
 
     The rows of all tokens are cut in ``shares`` equal parts per KV head (0: a workgroup takes all rows of a token; defaults to
@@ -116,10 +122,11 @@ def attention(q, cache, block_table, ctx, scale, max_seq_len, token_requests=Non
     longest = min(int(max_seq_len), cols * block, window or cols * block)
     parts = kv_heads * -(-H // kv_heads // 16)
     cus = _lib.device_cus(dev.index)
-    grouped = False
+    turns = 0
     if shares is None:
-        grouped = T >= 4 * count and _grouped(T, H // kv_heads, kv_heads, cus)   # (chunks: several tokens per table row)
-        shares = 0 if grouped else row_shares(longest, T * parts, parts, cus)
+        chunk = T // max(1, count) if max_query_len is None else max_query_len
+        turns = _turns(T, H // kv_heads, kv_heads, cus, T // max(1, count)) if token_requests is not None and chunk >= 4 else 0
+        shares = 0 if turns else row_shares(longest, T * parts, parts, cus)
     else:
         shares = int(shares)
     if not 0 <= shares <= MAX_SHARES:
@@ -136,6 +143,6 @@ def attention(q, cache, block_table, ctx, scale, max_seq_len, token_requests=Non
     token_stride, head_stride, _ = q.stride()
     _call('hla_s6_exact_attention', dev, q.data_ptr(), T, H, d, token_stride, head_stride, cache.data_ptr(), int(e4m3), kv_heads,
           page, head, row, block, pages, block_table.data_ptr(), table_stride, cols, count, _lib.ptr(token_requests),
-          ctx.data_ptr(), window, float(scale), _lib.ptr(k_scale), _lib.ptr(v_scale), shares, int(grouped), _lib.ptr(ws),
+          ctx.data_ptr(), window, float(scale), _lib.ptr(k_scale), _lib.ptr(v_scale), shares, turns, _lib.ptr(ws),
           0 if ws is None else ws.numel(), out.data_ptr(), H * d, d, lse.data_ptr())
     return out, lse

@@ -402,7 +402,7 @@ def attend_exact(q_rope, k_rope, v, cache, block_table, ctx, k_scale=None, v_sca
     rows = block_table.shape[1] * cache.shape[2]
     longest = min(int(ctx.max_seqlen_k), rows) if ctx.max_seqlen_k else rows
     out, _ = exact_cache.attention(q_rope, cache, block_table, ctx.row_counts, ctx.scale, longest, ctx.token_requests,
-                                   k_scale=k_scale, v_scale=v_scale)
+                                   k_scale=k_scale, v_scale=v_scale, max_query_len=ctx.max_query_len)
     return out
 
 

@@ -79,6 +79,13 @@ def test_how_rows_are_cut(ec):
     assert ec.row_shares(4096, 3000, 3000, 256) == 1
 
 
+def test_which_steps_are_grouped(ec):
+    """A group of tokens for every CU, eight heads at most; a workgroup per token of a group where requests are short."""
+    assert ec._turns(2048, 1, 16, 256, 512) == 4 and ec._turns(2048, 4, 8, 256, 512) == 4 and ec._turns(2048, 8, 8, 256, 512) == 2
+    assert ec._turns(256, 1, 16, 256, 8) == 16 and ec._turns(255, 1, 16, 256, 8) == 16 and ec._turns(240, 1, 16, 256, 8) == 0
+    assert ec._turns(10 ** 5, 9, 16, 256, 512) == 0 and ec._turns(0, 1, 16, 256, 0) == 0 and ec._turns(300, 5, 8, 256, 8) == 3
+
+
 def test_host_tensors_are_refused(ec, pg):
     i32, rows, cache = torch.zeros(1, dtype=torch.int32), torch.zeros(1, 2, 64, dtype=torch.bfloat16), \
         torch.zeros(2, 2, 16, 128, dtype=torch.bfloat16)
@@ -113,7 +120,8 @@ def test_entry_points_check_before_they_launch(pkg):
         ({22: 16}, 'scales'), ({23: 16}, 'scales'), ({17: 0}, 'table rows'), ({0: None}, 'null pointer'), ({14: None}, 'null pointer'),
         ({19: None}, 'null pointer'), ({28: None}, 'null pointer'), ({31: None}, 'null pointer'), ({4: 4}, 'aligned'), ({0: 8}, 'aligned'),
         ({30: 4}, 'aligned'), ({1: 2 ** 30, 17: 2 ** 30}, 'too many rows'), ({24: 2, 26: 8, 27: 10 ** 6}, 'aligned'),
-        ({24: 2, 25: 1, 26: 16, 27: 10 ** 6}, 'groups of tokens'), ({25: 1, 2: 18}, 'groups of tokens')])
+        ({24: 2, 25: 1, 26: 16, 27: 10 ** 6}, 'groups of tokens'), ({25: 1, 2: 18}, 'groups of tokens'), ({25: 17}, 'groups of tokens'),
+        ({25: -1}, 'groups of tokens')])
     refused('hla_s6_exact_attention', attention, [({24: 2, 26: 16, 27: 10}, 'workspace'), ({24: 2, 27: 10 ** 6}, 'workspace')], RuntimeError)
     call('hla_s6_exact_attention', {**attention, 1: 0, 0: None})      # no tokens, nothing to do
     store = {0: 16, 1: 128, 2: 64, 3: 16, 4: 128, 5: 64, 6: 1, 7: 2, 8: 64, 9: 16, 12: 16, 14: 4096, 15: 128, 16: 256, 17: 16, 18: 2}

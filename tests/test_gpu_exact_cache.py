@@ -425,10 +425,10 @@ def chunks(n, lens, order):
 @pytest.mark.parametrize('e4m3', [False, True])
 @pytest.mark.parametrize('kv_heads,G,d,block', [(2, 1, 128, 16), (1, 2, 64, 24), (2, 3, 128, 32), (1, 4, 256, 16), (1, 5, 64, 16),
                                                (2, 8, 128, 1), (3, 7, 128, 16)])
-@pytest.mark.parametrize('window', [0, 21])
-def test_groups_of_tokens(ec, monkeypatch, kv_heads, G, d, block, e4m3, window):
+@pytest.mark.parametrize('window,turns', [(0, 1), (0, 4), (21, 2), (0, 16)])
+def test_groups_of_tokens(ec, monkeypatch, kv_heads, G, d, block, e4m3, window, turns):
     """Chunks that begin and end inside a group of tokens, single tokens among them, tokens without rows, lengths in any order."""
-    monkeypatch.setattr(ec, '_grouped', lambda *a: True)
+    monkeypatch.setattr(ec, '_turns', lambda *a: turns)
     n, lens = [300, 40, 17, 900, 33], [37, 40, 1, 5, 33]
     c = Cache(G + d, n, kv_heads, d, block, e4m3)
     requests, ctx = chunks(n, lens, (3, 0, 1, 2, 4))
@@ -444,7 +444,7 @@ def test_groups_of_tokens(ec, monkeypatch, kv_heads, G, d, block, e4m3, window):
 @pytest.mark.parametrize('e4m3', [False, True])
 def test_rows_that_a_token_of_a_group_does_not_see(ec, monkeypatch, e4m3):
     """NaN and infinities in the rows behind a token's last, and before its window, reach only the tokens that see them."""
-    monkeypatch.setattr(ec, '_grouped', lambda *a: True)
+    monkeypatch.setattr(ec, '_turns', lambda *a: 3)
     n = [200]
     c = Cache(40, n, 2, 128, 16, e4m3)      # (one table row, sixteen tokens)
     ctx = [170, 171, 200, 172, 190, 1, 173, 174, 176, 177, 180, 179, 178, 175, 0, 169]
@@ -476,13 +476,26 @@ def test_rows_that_a_token_of_a_group_does_not_see(ec, monkeypatch, e4m3):
     assert torch.isnan(o[sees]).all() and torch.equal(o[~sees], clean[0][~sees]) and torch.equal(lse[:, ~sees], clean[1][:, ~sees])
 
 
+def test_a_chunk_beside_single_tokens(ec):
+    """Many single tokens and one chunk, through a table with rows to spare; the chunk's length as the hint."""
+    n, lens = [400 + 13 * r for r in range(60)] + [900], [1] * 60 + [200]
+    c = Cache(70, n, 16, 128, 16)
+    requests, ctx = chunks(n, lens, range(61))
+    q = query(71, len(ctx), 16, 128)
+    table = torch.zeros(300, c.table.shape[1], dtype=torch.int32, device='cuda')
+    table[:61] = c.table
+    o, lse = ec.attention(q, c.cache, table, dev_i32(np.array(ctx)), 0.09, max(n), dev_i64(np.array(requests)), max_query_len=200)
+    some = list(range(60)) + list(range(60, 260, 17)) + [259]
+    check(o[some], lse[:, some], q[some], c, [requests[t] for t in some], [ctx[t] for t in some], 0.09)
+
+
 @pytest.mark.parametrize('kv_heads,G', [(16, 1), (8, 4)])
 def test_large_chunks(ec, kv_heads, G):
     """Steps large enough for groups by the rule, prompts without history among them."""
     n, lens = [1500, 700, 513, 3000], [300, 700, 1, 400]
     c = Cache(50 + G, n, kv_heads, 128, 16)
     requests, ctx = chunks(n, lens, range(4))
-    assert ec._grouped(len(ctx), G, kv_heads)
+    assert ec._turns(len(ctx), G, kv_heads, 256, len(ctx) // 4) == 4
     q = query(51, len(ctx), kv_heads * G, 128)
     o, lse = ec.attention(q, c.cache, c.table, dev_i32(np.array(ctx)), 0.09, 3000, dev_i64(np.array(requests)))
     some = list(range(0, len(ctx), 61)) + [len(ctx) - 1]
