@@ -155,11 +155,10 @@ __device__ __forceinline__ void copy16_to_lds_v(const void* src, const void* lds
                : "memory", "m0");
 }
 
-// The same where the compiler may hold the (uniform) LDS address in a VGPR; kOnce: past the caches, for bytes read once.
+// The same to LDS byte address dst (uniform, which may be in a VGPR); kOnce: past the caches, for bytes read once.
 template <bool kOnce>
-__device__ __forceinline__ void copy16_to_lds_rfl_v(const void* src, const void* lds) {
-  const uint32_t dst = __builtin_amdgcn_readfirstlane(
-      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)lds);
+__device__ __forceinline__ void copy16_to_lds_rfl_v(const void* src, uint32_t dst) {
+  dst = __builtin_amdgcn_readfirstlane(dst);
   if (kOnce)
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(dst), "v"(src)
                  : "memory", "m0");

@@ -77,6 +77,9 @@ struct ExactGeo {
   static constexpr int TILE = KEYS * RB;         // bytes of a tile
   static constexpr int NB = !kE4 && TILE <= 4096 ? 4 : 2;
   static constexpr int WAVES = (TILE > 8192 ? 2 : 4) * (kWide ? 2 : 1);   // two workgroups per CU by their LDS, or a wide one
+  // (two are what LDS holds; said to the compiler, it keeps the sums out of the accumulation registers, from which it would copy
+  // them to others and back in every tile)
+  static constexpr int kWavesPerSimd = D <= 128 ? 2 : 1;
   static constexpr int BATCH = 64 / KEYS;        // tiles whose row addresses are worked out at a time
   static_assert(NB <= BATCH, "page ids are requested a batch ahead and waited for with the tile before");
 };
@@ -178,7 +181,7 @@ enum Columns {
 
 // kOnce: rows are read by one workgroup and stream past the caches
 template <class G, bool kOnce, Columns kColumns>
-__global__ __launch_bounds__(64 * G::WAVES) void exact_cache_kernel(ExactCacheParams a) {
+__global__ __launch_bounds__(64 * G::WAVES, G::kWavesPerSimd) void exact_cache_kernel(ExactCacheParams a) {
   constexpr int D = G::D;
   constexpr bool kE4 = G::kE4;
   constexpr int KEYS = G::KEYS, RB = G::RB, CPR = G::CPR, RPI = G::RPI, NI = G::NI, NB = G::NB, WAVES = G::WAVES;
@@ -297,9 +300,10 @@ __global__ __launch_bounds__(64 * G::WAVES) void exact_cache_kernel(ExactCachePa
       };
       const uint8_t* buf0 = lds + wave * (NB * G::TILE);
       const int in_copy = lane / CPR, piece = lane % CPR;
+      const uint32_t at_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)buf0;
       // tile i of the wave on its way into buffer i % NB
       auto request = [&](int i) {
-        const uint8_t* buf = buf0 + i % NB * G::TILE;
+        const uint32_t buf = at_lds + i % NB * G::TILE;
 #pragma unroll
         for (int c = 0; c < NI; ++c) {
           const int r = RPI * c + in_copy;
