@@ -22,7 +22,7 @@
 //
 // Large steps of many tokens per request (chunks) put the heads of 16 / G tokens in the columns (kTokens).
 //
-// Bound by HBM: 64 tokens of 4096 rows and 16 heads (2.1 GB) 320 us, 6.7 TB/s, the vector units at 24 %; a call is its bytes at
+// Bound by HBM: 64 tokens of 4096 rows and 16 heads (2.1 GB) 320 us, 6.7 TB/s, the vector units at 15 %; a call is its bytes at
 // that rate and about 11 us (launch, lengths, table entries, first rows, joining waves, the second launch). Past the caches
 // (kOnce) 7 % faster. Two workgroups of four waves per CU, a tile of each wave on its way: three waves, eight, or one workgroup
 // with twice the tiles measured the same or slower, so did dealing the heads of a share to one XCD.
@@ -596,7 +596,7 @@ void launch_exact_cache(const ExactCacheParams& p, hipStream_t st) {
   const int group = p.grouped ? kMaxTile / p.G : 1, turns = p.grouped ? p.grouped : 1;
   const unsigned grid = (unsigned)((int64_t)(p.shares ? p.shares : (p.T + group - 1) / group) * turns * p.KH * p.tiles);
   const bool once = p.tiles == 1 && p.T < 2 * (int64_t)p.bt_count;   // a table row for every token, but for padding
-  // whole tokens for at most a workgroup per CU: twice the waves (one token of 16 heads, 993 rows: 17.4 us with 4, 12.9 with 8)
+  // whole tokens for at most a workgroup per CU: twice the waves (one token of 16 heads, 993 rows: 17.4 us with 4, 11.7 with 8)
   const bool wide = !p.shares && !p.grouped && (int64_t)p.T * p.KH * p.tiles <= kCus;
   using G = ExactGeo<D, kE4, false>;
   using W = ExactGeo<D, kE4, true>;

@@ -69,7 +69,7 @@ def row_shares(max_rows, groups, parts, cu_count=256):
     short rows, and where the groups are many. GPU time in us with shares / a workgroup per group, 8 KV heads:
 
         tokens x rows   1 x 512     1 x 768     1 x 1024    4 x 1024    16 x 1024   16 x 1536   32 x 1536   64 x 1024
-                        11.1 / 9.1  11.1 / 11.3 11.2 / 13.4 11.6 / 14.0 19.7 / 17.9 24.5 / 24.0 41.9 / 35.8 48.9 / 45.9
+                        10.8 / 8.9  10.9 / 10.7 10.9 / 11.2 11.4 / 13.5 19.7 / 17.5 25.1 / 23.6 41.8 / 35.0 51.9 / 47.6
 
     (a call on the host takes 16 / 11). A function of constants and the row count only (graph-stable)."""
     if max_rows <= (1536 if 2 * groups >= cu_count else 1024) or groups >= 16 * cu_count:
@@ -80,8 +80,8 @@ def row_shares(max_rows, groups, parts, cu_count=256):
 def _turns(tokens, heads, kv_heads, cu_count=256, per_request=1):
     """0, or the workgroups per group of ``16 // heads`` tokens (``heads`` query heads per KV head) that go through rows together, where
     there is a group for every CU. Chunks on top of histories, us with groups / a workgroup per token: 4 x 512 tokens on 8160 rows of
-    16 heads 593 / 6863, of 8 KV heads for 32 1028 / 3445, a prompt of 4000 of 16 heads 358 / 3764, 8 x 64 on 4000 (8 KV heads for
-    32) 153 / 464.
+    16 heads 550 / 5861, of 8 KV heads for 32 945 / 2939, a prompt of 4000 of 16 heads 361 / 3219, 8 x 64 on 4000 (8 KV heads for
+    32) 140 / 397.
     A group of single tokens (which a step may have beside its chunks) has as many requests as tokens: with few tokens per request
     on average a workgroup for each; else 4, since most find nothing to do."""
     if heads > 8 or -(-tokens // (16 // heads)) * kv_heads < cu_count:
