@@ -80,6 +80,15 @@ def new_pool(num_pages, block, max_requests, max_rows, device, reserved=0):
                 torch.where(words >> 31 > 0, words - (1 << 32), words).to(I32), block)
 
 
+def _apart(pool, vector, in_place):
+    """``vector``, or a copy of it where it lies on the pool's lengths, which change while requests are worked on; the lengths
+    themselves are fine where a request reads no entry but its own (``in_place``)."""
+    offset, held = vector.data_ptr() - pool._args[4], pool.lengths.shape[0]
+    if -4 * vector.shape[0] < offset < 4 * held and not (in_place and offset == 0):
+        return vector.clone()
+    return vector
+
+
 def release_requests(pool, requests, lengths=None):
     """Requests ``requests`` (int32 ``[n]``) keep their first ``lengths[i]`` rows (int32 ``[n]``; none without it; more than a request
     has: all) and give back the pages behind them; a page is free once nobody holds it. Numbers outside the pool are skipped; of a
@@ -88,9 +97,7 @@ def release_requests(pool, requests, lengths=None):
     _same_device(pool.tables, requests, lengths)
     requests = _vector('requests', requests, n)
     if lengths is not None:
-        lengths = _vector('lengths', lengths, n)
-        if lengths.data_ptr() == pool.lengths.data_ptr():
-            lengths = lengths.clone()   # (they change while requests are worked on)
+        lengths = _apart(pool, _vector('lengths', lengths, n), False)
     _call('hla_s6_pool_release', pool.tables.device, *pool._args, requests.data_ptr(), _lib.ptr(lengths), n)
 
 
@@ -118,9 +125,9 @@ def extend_requests(pool, lengths, write_from=None):
     _same_device(pool.tables, lengths, write_from)
     tables = pool.tables
     R, C = tables.shape
-    lengths = _vector('lengths', lengths, R)
+    lengths = _apart(pool, _vector('lengths', lengths, R), True)
     if write_from is not None:
-        write_from = _vector('write_from', write_from, R)
+        write_from = _apart(pool, _vector('write_from', write_from, R), True)
     dev = tables.device
     ok = torch.empty(R, dtype=torch.bool, device=dev)
     shape = (R,) if write_from is None else (R, C)

@@ -127,6 +127,27 @@ def test_lengths_of_the_pool_itself(pg):
     same(dev, pool)
 
 
+def test_parts_of_the_lengths(pg):
+    """Arguments that lie on the pool's lengths, entries apart from those that they are for: what they were before the call."""
+    rng = np.random.default_rng(10)
+    n = rng.integers(0, 400, 300).tolist()
+    pool = Pool.random(rng, n, 16, 30, sum(held(x, 16) for x in n) + 6000, 0.3)
+    dev = up(pg, pool)
+    order = list(range(299))
+    pool.release(order, list(pool.lengths[1:]))
+    pg.release_requests(dev, dev_i32(np.asarray(order)), dev.lengths[1:])
+    same(dev, pool)
+    for full in (False, True):
+        long = torch.cat([dev.lengths, dev_i32(np.asarray([90]))])
+        dev = pg.Pool(dev.tables, long[:-1], dev.refs, dev.free, dev.block)
+        want, start = list(pool.lengths[1:]) + [90], [0] * 300 if full else None
+        ok, pairs = pool.extend(want, start)
+        got = pg.extend_requests(dev, long[1:], torch.zeros_like(dev.lengths) if full else None)
+        assert got.ok.tolist() == ok
+        lists(got, pairs, 300, 30, full)
+        same(dev, pool)
+
+
 def test_pages_run_out(pg):
     """The first request that asks for more than there is waits, and those behind it that ask for any."""
     pool = Pool.empty(10, 4, 6, 8)
