@@ -147,15 +147,13 @@ __device__ __forceinline__ void hand_out(const Pool& p, int given, int64_t* sums
   for (int w0 = 0, base = 0; base < given; w0 += kPoolThreads) {   // (given is no more than there are)
     const int w = w0 + threadIdx.x;
     const uint32_t all = w < (p.N + 31) / 32 ? p.free[w] : 0u;
-    uint32_t bits = all & page_bits(p, w), kept = all;
+    uint32_t bits = all & page_bits(p, w);
+    const uint32_t others = all ^ bits;
     int64_t total;
     int at = (int)pool_scan(__popc(bits), sums, total);
-    const int n = min((int)total, given - base);
-    for (; bits && at < n; bits &= bits - 1, ++at) {
-      const int bit = __ffs((int)bits) - 1;
-      kept &= ~(1u << bit);
-      found[at] = (uint16_t)(threadIdx.x * 32 + bit);
-    }
+    const int n = min((int)total, given - base), end = min(n, at + __popc(bits));
+    for (; at < end; ++at, bits &= bits - 1) found[at] = (uint16_t)(threadIdx.x * 32 + __ffs((int)bits) - 1);
+    const uint32_t kept = others | bits;
     if (kept != all) p.free[w] = kept;
     __syncthreads();
     place(base, n, w0 * 32);
@@ -165,8 +163,10 @@ __device__ __forceinline__ void hand_out(const Pool& p, int given, int64_t* sums
 }
 
 // from = lengths[r]: at most one column of a request, its last, is shared, and lists have an entry per request. A call of few
-// pages is a chain of loads and barriers; one of many is bound by the instructions of its one workgroup, so a wave places the
-// pages of a request 64 at a time, in consecutive columns, and only requests of up to kFew pages are left to their threads.
+// pages is a chain of loads and barriers; one of many is bound by the instructions of its one workgroup (80,000 of 143,619 pages 31 us: for every
+// 32,768 pages of the pool 0.8 in the scan, 2.1 in `found`, 3.4 in tables and counts, whose stores are what they wait for: barriers
+// that leave them in flight gain nothing), so a wave places the pages of a request 64 at a time, in consecutive columns, and only
+// requests of up to kFew pages are left to their threads. (A wave per 64 pages of the pool in `found`: 42.)
 constexpr int kFew = 4;
 
 __global__ __launch_bounds__(kPoolThreads) void pool_extend_kernel(ExtendParams a) {
@@ -217,33 +217,32 @@ __global__ __launch_bounds__(kPoolThreads) void pool_extend_kernel(ExtendParams 
   __syncthreads();
   const int pages = given;   // (the request that is not served first, and all behind it, start at `pages` or later)
   hand_out(p, pages, sums, found, [&](int base, int n, int page0) {
-    // pages of ranks k, k + step, .. below `last` of request r, whose ranks start at `first_rank`
-    auto place = [&](int r, int first_rank, int k, int last, int step) {
-      const int c = column[r];
-      int32_t* entry = p.tables + r * p.t_st + (c < 0 ? ~c : c) - first_rank;
-      if (c < 0 && k == first_rank) {
-        a.source[r] = entry[k];
-        a.target[r] = page0 + found[k - base];
-      }
-#pragma unroll 4
-      for (; k < last; k += step) {
-        const int page = page0 + found[k - base];
-        entry[k] = page;
-        p.refs[page] = 1;
-      }
-    };
     for (int r0 = 0; r0 < p.R; r0 += kPoolThreads) {
       const int r = r0 + lane * kPoolWaves + (tid >> 6);   // (neighbours with different waves)
-      int lo = 0, hi = 0, first_rank = 0;
+      int lo = 0, hi = 0;
+      int64_t entry = 0;   // that of rank k is entry + k
       if (r < p.R) {
-        first_rank = start[r];
+        const int first_rank = start[r], c = column[r];
         lo = max(first_rank, base);
         hi = min(start[r + 1], base + n);
+        entry = r * p.t_st + (c < 0 ? ~c : c) - first_rank;
+        if (c < 0 && lo == first_rank && lo < hi) {
+          a.source[r] = p.tables[entry + lo];
+          a.target[r] = page0 + found[lo - base];
+        }
       }
-      if (hi - lo <= kFew && lo < hi) place(r, first_rank, lo, hi, 1);
+      auto place = [&](int32_t* entries, int k) {
+        const int page = page0 + found[k - base];
+        entries[k] = page;
+        p.refs[page] = 1;
+      };
+      if (hi - lo <= kFew)
+        for (int k = lo; k < hi; ++k) place(p.tables + entry, k);
       for (uint64_t many = __ballot(hi - lo > kFew); many; many &= many - 1) {
-        const int from = __ffsll((unsigned long long)many) - 1;
-        place(__shfl(r, from), __shfl(first_rank, from), __shfl(lo, from) + lane, __shfl(hi, from), 64);
+        const int from = __ffsll((unsigned long long)many) - 1, end = __builtin_amdgcn_readlane(hi, from);
+        int32_t* entries = p.tables + uniform64(__shfl(entry, from));
+#pragma unroll 2
+        for (int k = __builtin_amdgcn_readlane(lo, from) + lane; k < end; k += 64) place(entries, k);
       }
     }
   });
