@@ -20,7 +20,8 @@
 // two thirds of the output's own rounding to it: 0.0024 relative to the 64-bit result, now 0.0017). Up to 8 query heads have their
 // rests in the 8 columns that would be zero: the scores of a head are made twice, for free. More heads take a second product.
 //
-// Large steps of many tokens per request (chunks) put the heads of 16 / G tokens in the columns (kTokens).
+// Large steps of many tokens per request (chunks) put the heads of 16 / G or 32 / G tokens in the columns: 4 x 512 tokens on
+// 8160 rows, 16 heads, 454 us, 292 TFLOP/s (matrix units 29 %, vector units 42 %, and the chain of the two between two waves).
 //
 // Bound by HBM: 64 tokens of 4096 rows and 16 heads (2.1 GB) 320 us, 6.7 TB/s, the vector units at 15 %; a call is its bytes at
 // that rate and about 11 us (launch, lengths, table entries, first rows, joining waves, the second launch). Past the caches
@@ -55,7 +56,7 @@ struct ExactCacheParams {
   float scale_log2;
   const float *k_scale, *v_scale;
   int T, H, KH, G, tiles;  // tiles: workgroups of query heads per KV head
-  int shares;              // 0: a workgroup takes all rows of a token, or (grouped) of 16 / G tokens
+  int shares;              // 0: a workgroup takes all rows of a token, or (grouped) of 16 / G or 32 / G tokens
   int grouped;             // workgroups among which the requests of a group are dealt; 0: a token by itself
   float *ws_o, *ws_lse;    // [shares][2][H][D], [shares][2][H]
   int32_t* split;          // [T][2]: first and last share of a token's rows
@@ -176,7 +177,8 @@ __device__ __forceinline__ void find_share(const ExactCacheParams& a, int k, int
 enum Columns {
   kHeads,    // query heads of a token
   kTwice,    // up to 8 of them, and the same again
-  kTokens,   // those of several tokens, which share the rows of a request (the queries of a chunk)
+  kTokens16, // those of several tokens, which share the rows of a request (the queries of a chunk)
+  kTokens32, // the same with 32 columns
 };
 
 // kOnce: rows are read by one workgroup and stream past the caches
@@ -187,11 +189,13 @@ __global__ __launch_bounds__(64 * G::WAVES, G::kWavesPerSimd) void exact_cache_k
   constexpr int KEYS = G::KEYS, RB = G::RB, CPR = G::CPR, RPI = G::RPI, NI = G::NI, NB = G::NB, WAVES = G::WAVES;
   constexpr int CT = D / 16;       // 16-column tiles of O^T
   constexpr int OS = D + 4;        // LDS row stride of a wave's partial output, in floats
-  constexpr int kTiles = WAVES * NB * G::TILE, kJoin = WAVES * 16 * OS * 4;
+  constexpr bool kTokens = kColumns >= kTokens16;
+  constexpr int COLS = kColumns == kTokens32 ? 32 : 16, Y = COLS / 16;   // columns of the scores, 16 per product
+  constexpr int kTiles = WAVES * NB * G::TILE, kJoin = WAVES * COLS * OS * 4;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kTiles > kJoin ? kTiles : kJoin];
   __shared__ int64_t offsets[WAVES][64];
   __shared__ int32_t page_ids[WAVES][64];
-  __shared__ float stats[WAVES][2][16];
+  __shared__ float stats[WAVES][2][COLS];
   __shared__ int64_t sums[WAVES], found[2];
 
   const int tid = threadIdx.x, lane = tid & 63, x = lane & 15, g = lane >> 4;
@@ -199,23 +203,27 @@ __global__ __launch_bounds__(64 * G::WAVES, G::kWavesPerSimd) void exact_cache_k
   // heads innermost: workgroups dispatched one behind the other read the same rows' heads
   const int parts = a.KH * a.tiles, part = blockIdx.x % parts;
   // a group's requests (runs of tokens with one table row) are dealt to `turns` workgroups
-  const int groups = kColumns == kTokens ? (a.T + kMaxTile / a.G - 1) / (kMaxTile / a.G) : 0;
-  const int k = kColumns == kTokens ? (int)(blockIdx.x / parts) % groups : (int)(blockIdx.x / parts);
-  const int turn = kColumns == kTokens ? (int)(blockIdx.x / parts) / groups : 0;
+  const int groups = kTokens ? (a.T + COLS / a.G - 1) / (COLS / a.G) : 0;
+  const int k = kTokens ? (int)(blockIdx.x / parts) % groups : (int)(blockIdx.x / parts);
+  const int turn = kTokens ? (int)(blockIdx.x / parts) / groups : 0;
   const int kh = part / a.tiles, j0 = part % a.tiles * kMaxTile;
   const int heads = min(kMaxTile, a.G - j0), h0 = kh * a.G + j0;
   const uint8_t* cache = a.cache + kh * a.head_stride;
-  // column x: head `head` of token k, or with several of token t_group + x / G
-  const int group = kColumns == kTokens ? kMaxTile / a.G : 1, t_group = k * group, t_end = min(a.T, t_group + group);
-  const int head = kColumns == kTwice ? x & 7 : kColumns == kTokens ? x % a.G : x;
-  const int token = t_group + (kColumns == kTokens ? x / a.G : 0);
+  // column x: head `head` of token k; with several, column 16 y + x: that of token t_group + (16 y + x) / G
+  const int group = kTokens ? COLS / a.G : 1, t_group = k * group, t_end = min(a.T, t_group + group);
+  int head[Y], token[Y];
+#pragma unroll
+  for (int y = 0; y < Y; ++y) {
+    head[y] = kColumns == kTwice ? x & 7 : kTokens ? (16 * y + x) % a.G : x;
+    token[y] = t_group + (kTokens ? (16 * y + x) / a.G : 0);
+  }
   auto table_row = [&](int i) { return a.bt_rows ? min(max(a.bt_rows[i], (int64_t)0), (int64_t)a.bt_count - 1) : i; };
 
   // lane i: what token t_group + i reads and sees; a bit for every token that begins a run
   int64_t lane_row = 0;
   int lane_first = 0, lane_n = 0;
   uint32_t heads_of_runs = 0;
-  if constexpr (kColumns == kTokens) {
+  if constexpr (kTokens) {
     const int i = t_group + lane;
     if (i < t_end) {
       lane_row = table_row(i);
@@ -227,7 +235,7 @@ __global__ __launch_bounds__(64 * G::WAVES, G::kWavesPerSimd) void exact_cache_k
     if (!heads_of_runs) return;
   }
 
-  int t = kColumns == kTokens ? t_group + __ffs((int)heads_of_runs) - 1 : t_group, at = 0;
+  int t = kTokens ? t_group + __ffs((int)heads_of_runs) - 1 : t_group, at = 0;
   int64_t left_steps = INT32_MAX, before = 0, share = 1;
   if (a.shares) {
     find_share(a, k, 64 * WAVES, sums, found, t, at, left_steps, before, share);
@@ -235,9 +243,9 @@ __global__ __launch_bounds__(64 * G::WAVES, G::kWavesPerSimd) void exact_cache_k
   }
   for (;;) {   // the tokens of the share, or the requests of the group
     // tokens [t, t_last) of a request: rows [first, n) are seen by any of them, [all_first, all_n) by all that see any
-    int first, n, t_last = t + 1, all_first, all_n, my_first = 0, my_n = 0;
+    int first, n, t_last = t + 1, all_first, all_n, my_first[Y] = {}, my_n[Y] = {};
     int64_t row;
-    if constexpr (kColumns == kTokens) {
+    if constexpr (kTokens) {
       const int at_lane = t - t_group;
       row = __shfl(lane_row, at_lane);
       const uint64_t others = __ballot(lane > at_lane && (t_group + lane >= t_end || lane_row != row));
@@ -247,7 +255,7 @@ __global__ __launch_bounds__(64 * G::WAVES, G::kWavesPerSimd) void exact_cache_k
       n = sees ? lane_n : 0;
       all_first = sees ? lane_first : 0;
       all_n = sees ? lane_n : INT32_MAX;
-      for (int off = kMaxTile / 2; off > 0; off >>= 1) {   // (a group is in the first 16 lanes)
+      for (int off = COLS / 2; off > 0; off >>= 1) {   // (a group is in the first COLS lanes)
         first = min(first, __shfl_xor(first, off));
         n = max(n, __shfl_xor(n, off));
         all_first = max(all_first, __shfl_xor(all_first, off));
@@ -257,10 +265,13 @@ __global__ __launch_bounds__(64 * G::WAVES, G::kWavesPerSimd) void exact_cache_k
       first = min(__builtin_amdgcn_readfirstlane(first), n);
       all_first = __builtin_amdgcn_readfirstlane(all_first);
       all_n = __builtin_amdgcn_readfirstlane(all_n);
-      const int f = __shfl(lane_first, token - t_group), c = __shfl(lane_n, token - t_group);
-      if (token >= t && token < t_last) {
-        my_first = f;
-        my_n = c;
+#pragma unroll
+      for (int y = 0; y < Y; ++y) {
+        const int f = __shfl(lane_first, token[y] - t_group), c = __shfl(lane_n, token[y] - t_group);
+        if (token[y] >= t && token[y] < t_last) {
+          my_first[y] = f;
+          my_n[y] = c;
+        }
       }
     } else {
       token_rows(a, t, first, n);
@@ -314,23 +325,29 @@ __global__ __launch_bounds__(64 * G::WAVES, G::kWavesPerSimd) void exact_cache_k
 
       // Q^T: the columns of step s that lane group g holds are those of K's pieces
       const float scale = a.scale_log2 * (kE4 && a.k_scale ? a.k_scale[kh] : 1.f);
-      u32x4 qo[D / 32];
-      {
-        const bool used = kColumns == kTokens ? token >= t && token < t_last : head < heads;
-        const uint16_t* qp = a.q + (int64_t)(kColumns == kTokens && used ? token : t) * a.q_st + (int64_t)(h0 + (used ? head : 0)) * a.q_sh;
-        const uint32_t flip = scale < 0.f ? 0x80008000u : 0u;   // scores of -q, so that the largest one has the largest weight
+      u32x4 qo[Y][D / 32];
+      const uint32_t flip = scale < 0.f ? 0x80008000u : 0u;   // scores of -q, so that the largest one has the largest weight
+#pragma unroll
+      for (int y = 0; y < Y; ++y) {
+        const bool used = kTokens ? token[y] >= t && token[y] < t_last : head[y] < heads;
+        const uint16_t* qp = a.q + (int64_t)(kTokens && used ? token[y] : t) * a.q_st + (int64_t)(h0 + (used ? head[y] : 0)) * a.q_sh;
 #pragma unroll
         for (int s = 0; s < D / 32; ++s) {
           const int col = kE4 ? 16 * (g + 4 * (s / 2)) + 8 * (s % 2) : 32 * s + 8 * g;
-          qo[s] = used ? ld16(qp + col) ^ flip : u32x4{0u, 0u, 0u, 0u};
+          qo[y][s] = used ? ld16(qp + col) ^ flip : u32x4{0u, 0u, 0u, 0u};
         }
       }
       const float factor = scale == 0.f ? 0x1p-126f : fabsf(scale);   // (a masked score stays -inf)
 
-      float m = -INFINITY, l = 0.f;
-      floatx4 o[CT];
+      float m[Y], l[Y];
+      floatx4 o[CT][Y];
 #pragma unroll
-      for (int c = 0; c < CT; ++c) o[c] = floatx4{0.f, 0.f, 0.f, 0.f};
+      for (int y = 0; y < Y; ++y) {
+        m[y] = -INFINITY;
+        l[y] = 0.f;
+#pragma unroll
+        for (int c = 0; c < CT; ++c) o[c][y] = floatx4{0.f, 0.f, 0.f, 0.f};
+      }
 
       if (mine > 0) {
         fetch_ids(0);
@@ -359,33 +376,38 @@ __global__ __launch_bounds__(64 * G::WAVES, G::kWavesPerSimd) void exact_cache_k
         const uint8_t* buf = buf0 + i % NB * G::TILE;
 
         constexpr int KB = KEYS / 16;
-        floatx4 s[KB];
+        floatx4 s[Y][KB];
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
-          s[b] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int y = 0; y < Y; ++y) s[y][b] = floatx4{0.f, 0.f, 0.f, 0.f};
           const int key = 16 * b + x;
 #pragma unroll
           for (int c = 0; c < CPR / 8; ++c) {
             const u32x4 v = ld16(buf + key * RB + 16 * ((4 * c + g) ^ swizzle<G>(key)));
             if (kE4) {
-              s[b] = mfma16x16x32(e4m3_to_bf16(v[0], v[1]), qo[2 * c], s[b]);
-              s[b] = mfma16x16x32(e4m3_to_bf16(v[2], v[3]), qo[2 * c + 1], s[b]);
+              const u32x4 lower = e4m3_to_bf16(v[0], v[1]), upper = e4m3_to_bf16(v[2], v[3]);
+#pragma unroll
+              for (int y = 0; y < Y; ++y) s[y][b] = mfma16x16x32(upper, qo[y][2 * c + 1], mfma16x16x32(lower, qo[y][2 * c], s[y][b]));
             } else {
-              s[b] = mfma16x16x32(v, qo[c], s[b]);
+#pragma unroll
+              for (int y = 0; y < Y; ++y) s[y][b] = mfma16x16x32(v, qo[y][c], s[y][b]);
             }
           }
         }
         const int row0 = lo + (wave + i * WAVES) * KEYS, left = hi - row0;   // keys of the tile
-        const bool mixed = kColumns == kTokens && (row0 < all_first || row0 + KEYS > all_n);   // some tokens see some of them
-        if (kColumns == kTokens) {
+        const bool mixed = kTokens && (row0 < all_first || row0 + KEYS > all_n);   // some tokens see some of them
+        if (kTokens) {
           if (mixed) {
 #pragma unroll
-            for (int b = 0; b < KB; ++b)
+            for (int y = 0; y < Y; ++y)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const int j = row0 + 16 * b + 4 * g + r;
-                if (j < my_first || j >= my_n) s[b][r] = -INFINITY;
-              }
+              for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  const int j = row0 + 16 * b + 4 * g + r;
+                  if (j < my_first[y] || j >= my_n[y]) s[y][b][r] = -INFINITY;
+                }
           }
         } else if (left < KEYS) {
           // rows past the last repeat it: no weight, and values of 0 (0 * inf is not)
@@ -393,61 +415,81 @@ __global__ __launch_bounds__(64 * G::WAVES, G::kWavesPerSimd) void exact_cache_k
           for (int b = 0; b < KB; ++b)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              if (16 * b + 4 * g + r >= left) s[b][r] = -INFINITY;
+              if (16 * b + 4 * g + r >= left) s[0][b][r] = -INFINITY;
           for (int j = left * CPR + lane; j < KEYS * CPR; j += 64) st16(const_cast<uint8_t*>(buf) + 16 * j, u32x4{0u, 0u, 0u, 0u});
           wait_reads();
         }
-        float top = -INFINITY;
+        u32x2 p[Y][KB], p2[Y][KB];   // the column's part of P; with 16 heads p2 has the rests
 #pragma unroll
-        for (int b = 0; b < KB; ++b)
+        for (int y = 0; y < Y; ++y) {
+          float top = -INFINITY;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) top = fmaxf(top, s[b][r]);
-        top = wave_max16x4(top) * factor;
-        if (__any(top > m + kRaise)) {
-          const float raised = fmaxf(m, top);
-          const float alpha = raised == -INFINITY ? 1.f : fast_exp2(m - raised);
-          m = raised;
-          l *= alpha;
+          for (int b = 0; b < KB; ++b)
 #pragma unroll
-          for (int c = 0; c < CT; ++c)
+            for (int r = 0; r < 4; ++r) top = fmaxf(top, s[y][b][r]);
+          top = wave_max16x4(top) * factor;
+          if (__any(top > m[y] + kRaise)) {
+            const float raised = fmaxf(m[y], top);
+            const float alpha = raised == -INFINITY ? 1.f : fast_exp2(m[y] - raised);
+            m[y] = raised;
+            l[y] *= alpha;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[c][r] *= alpha;
-        }
-        const float from = m == -INFINITY ? 0.f : m;   // (nothing but scores of -inf so far: weights of zero)
-        u32x2 p[KB], p2[KB];   // the column's part of P; with more than 8 heads p2 has the rests
+            for (int c = 0; c < CT; ++c)
 #pragma unroll
-        for (int b = 0; b < KB; ++b) {
-          float w[4];
+              for (int r = 0; r < 4; ++r) o[c][y][r] *= alpha;
+          }
+          const float from = m[y] == -INFINITY ? 0.f : m[y];   // (nothing but scores of -inf so far: weights of zero)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) l += w[r] = fast_exp2(fmaf(s[b][r], factor, -from));
-          p[b] = u32x2{upper_halves(w[0], w[1]), upper_halves(w[2], w[3])};
-          p2[b] = u32x2{rests(w[0], w[1], p[b][0]), rests(w[2], w[3], p[b][1])};
-          if (kColumns == kTwice && x >= 8) p[b] = p2[b];
+          for (int b = 0; b < KB; ++b) {
+            float w[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) l[y] += w[r] = fast_exp2(fmaf(s[y][b][r], factor, -from));
+            p[y][b] = u32x2{upper_halves(w[0], w[1]), upper_halves(w[2], w[3])};
+            p2[y][b] = u32x2{rests(w[0], w[1], p[y][b][0]), rests(w[2], w[3], p[y][b][1])};
+            if (kColumns == kTwice && x >= 8) p[y][b] = p2[y][b];
+          }
         }
         // V^T of 16 columns, as the A operand
         // e4m3: lane x of group g reads half a piece of key 4g + x/2 (x < 8) or 16 + 4g + x/2 - 4; bf16: of key 4g + x/4
         const int key = kE4 ? (x < 8 ? 0 : 12) + 4 * g + (x >> 1) : 4 * g + (x >> 2);
         const uint8_t* vr = buf + key * RB + 8 * (x & 1);
-        auto add = [&](floatx4 to, int c, const uint32_t* seen, bool both) {
+        auto add = [&](floatx4 (&to)[Y], int c, const uint32_t* seen, bool both) {
           if constexpr (kE4) {
             typedef int int2v __attribute__((ext_vector_type(2)));
             int2v v = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
                 (__attribute__((address_space(3))) int2v*)(vr + 16 * ((CPR / 2 + c) ^ swizzle<G>(key))));
             if (seen) v = int2v{(int)(v[0] & seen[0]), (int)(v[1] & seen[1])};
             const u32x4 vt = e4m3_to_bf16((uint32_t)v[0], (uint32_t)v[1]);
-            to = mfma16x16x32(vt, u32x4{p[0][0], p[0][1], p[1][0], p[1][1]}, to);
-            return both ? mfma16x16x32(vt, u32x4{p2[0][0], p2[0][1], p2[1][0], p2[1][1]}, to) : to;
+#pragma unroll
+            for (int y = 0; y < Y; ++y) {
+              to[y] = mfma16x16x32(vt, u32x4{p[y][0][0], p[y][0][1], p[y][1][0], p[y][1][1]}, to[y]);
+              if (both) to[y] = mfma16x16x32(vt, u32x4{p2[y][0][0], p2[y][0][1], p2[y][1][0], p2[y][1][1]}, to[y]);
+            }
           } else {
             u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                 (__attribute__((address_space(3))) short4v*)(vr + 16 * ((CPR / 2 + 2 * c + ((x >> 1) & 1)) ^ swizzle<G>(key)))));
             if (seen) v = u32x2{v[0] & seen[0], v[1] & seen[1]};
             const short4v vt = __builtin_bit_cast(short4v, v);
-            to = mfma16x16x16(vt, __builtin_bit_cast(short4v, p[0]), to);
-            return both ? mfma16x16x16(vt, __builtin_bit_cast(short4v, p2[0]), to) : to;
+#pragma unroll
+            for (int y = 0; y < Y; ++y) {
+              to[y] = mfma16x16x16(vt, __builtin_bit_cast(short4v, p[y][0]), to[y]);
+              if (both) to[y] = mfma16x16x16(vt, __builtin_bit_cast(short4v, p2[y][0]), to[y]);
+            }
           }
         };
-        if (kColumns == kTokens && mixed) {
-          // rows that a token does not see may hold anything, and 0 * NaN is not 0: a token at a time, its rows and its columns
+        bool apart = false;
+        if (kTokens && mixed) {
+          // rows that a token does not see may hold anything, and 0 * NaN is not 0: is there an infinity or NaN?
+          uint32_t bad = 0;
+          for (int i = lane; i < KEYS * CPR / 2; i += 64) {
+            const u32x4 v = ld16(buf + i / (CPR / 2) * RB + 16 * ((CPR / 2 + i % (CPR / 2)) ^ swizzle<G>(i / (CPR / 2))));
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              bad |= kE4 ? ((v[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u : ((v[e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+          }
+          apart = __any(bad != 0);
+        }
+        if (kTokens && apart) {   // a token at a time, its rows and its columns
           for (int u = t; u < t_last; ++u) {
             const int f = __shfl(lane_first, u - t_group), c1 = __shfl(lane_n, u - t_group);
             uint32_t seen[2];   // of keys 4g .. and 16 + 4g .. (a byte each), or of 4g, 4g + 1 and 4g + 2, 4g + 3 (a half each)
@@ -462,50 +504,57 @@ __global__ __launch_bounds__(64 * G::WAVES, G::kWavesPerSimd) void exact_cache_k
             }
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
-              const floatx4 more = add(floatx4{0.f, 0.f, 0.f, 0.f}, c, seen, true);
-              if (token == u) o[c] += more;
+              floatx4 more[Y] = {};
+              add(more, c, seen, true);
+#pragma unroll
+              for (int y = 0; y < Y; ++y)
+                if (token[y] == u) o[c][y] += more[y];
             }
           }
         } else {
 #pragma unroll
-          for (int c = 0; c < CT; ++c) o[c] = add(o[c], c, nullptr, kColumns != kTwice);
+          for (int c = 0; c < CT; ++c) add(o[c], c, nullptr, kColumns != kTwice);
         }
       }
 
       // the waves' parts together
-      l = wave_sum16x4(l);
-      if (g == 0) {
-        stats[wave][0][x] = m;
-        stats[wave][1][x] = l;
+#pragma unroll
+      for (int y = 0; y < Y; ++y) {
+        l[y] = wave_sum16x4(l[y]);
+        if (g == 0) {
+          stats[wave][0][16 * y + x] = m[y];
+          stats[wave][1][16 * y + x] = l[y];
+        }
       }
       __syncthreads();   // (and every wave has read its last tile)
       float* joined = reinterpret_cast<float*>(lds);
-      {
-        float top = -INFINITY;
-        for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stats[w][0][x]);
-        const float f = m == -INFINITY ? 0.f : fast_exp2(m - top);
-        // (a NaN among the scores is in l, and where m is -inf nothing but zeros and NaN are in o)
-        if (kColumns == kTokens || head < heads) {
 #pragma unroll
-          for (int c = 0; c < CT; ++c) *reinterpret_cast<floatx4*>(joined + (wave * 16 + x) * OS + 16 * c + 4 * g) = o[c] * f;
+      for (int y = 0; y < Y; ++y) {
+        float top = -INFINITY;
+        for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stats[w][0][16 * y + x]);
+        const float f = m[y] == -INFINITY ? 0.f : fast_exp2(m[y] - top);
+        // (a NaN among the scores is in l, and where m is -inf nothing but zeros and NaN are in o)
+        if (kTokens || head[y] < heads) {
+#pragma unroll
+          for (int c = 0; c < CT; ++c) *reinterpret_cast<floatx4*>(joined + (wave * COLS + 16 * y + x) * OS + 16 * c + 4 * g) = o[c][y] * f;
         }
       }
       __syncthreads();
       const int j_first = (t - t_group) * heads, j_count = (t_last - t) * heads;   // its columns (the tokens' ones)
-      for (int i = tid; i < (kColumns == kTokens ? j_count : heads) * (D / 4); i += 64 * WAVES) {
-        const int j = (kColumns == kTokens ? j_first : 0) + i / (D / 4), col = i % (D / 4) * 4;
-        const int u = kColumns == kTokens ? t_group + j / heads : t, h = h0 + (kColumns == kTokens ? j % heads : j);
+      for (int i = tid; i < (kTokens ? j_count : heads) * (D / 4); i += 64 * WAVES) {
+        const int j = (kTokens ? j_first : 0) + i / (D / 4), col = i % (D / 4) * 4;
+        const int u = kTokens ? t_group + j / heads : t, h = h0 + (kTokens ? j % heads : j);
         float top = -INFINITY, sum = 0.f;
         for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stats[w][0][j]);
         floatx4 v = floatx4{0.f, 0.f, 0.f, 0.f};
         for (int w = 0; w < WAVES; ++w) {
           const float mw = stats[w][0][j];
           sum += stats[w][1][j] * (mw == -INFINITY ? 0.f : fast_exp2(mw - top));
-          v += *reinterpret_cast<floatx4*>(joined + (w * 16 + j) * OS + col);
-          if (kColumns == kTwice) v += *reinterpret_cast<floatx4*>(joined + (w * 16 + j + 8) * OS + col);
+          v += *reinterpret_cast<floatx4*>(joined + (w * COLS + j) * OS + col);
+          if (kColumns == kTwice) v += *reinterpret_cast<floatx4*>(joined + (w * COLS + j + 8) * OS + col);
         }
         bool none = sum == 0.f;
-        if (kColumns == kTokens) {
+        if (kTokens) {
           int f, c;
           token_rows(a, u, f, c);
           none = none || c <= f;   // (its columns took part in what the others see)
@@ -524,7 +573,7 @@ __global__ __launch_bounds__(64 * G::WAVES, G::kWavesPerSimd) void exact_cache_k
         }
       }
     }
-    if constexpr (kColumns == kTokens) {
+    if constexpr (kTokens) {
       for (int skip = 0; skip < a.grouped; ++skip) heads_of_runs &= heads_of_runs - 1;
       if (!heads_of_runs) return;
       t = t_group + __ffs((int)heads_of_runs) - 1;
@@ -593,18 +642,24 @@ __global__ __launch_bounds__(256) void exact_join_kernel(ExactCacheParams a) {
 
 template <int D, bool kE4>
 void launch_exact_cache(const ExactCacheParams& p, hipStream_t st) {
-  const int group = p.grouped ? kMaxTile / p.G : 1, turns = p.grouped ? p.grouped : 1;
+  // groups of tokens: 32 columns take half as many reads of K and V, where there are two workgroups per CU all the same (4 x 512
+  // tokens on 8160 rows of 16 heads 555 -> 454 us; of 256 workgroups with them 61, of 512 without 53). With d = 256 their registers
+  // do not suffice (463 -> 817).
+  const int group32 = kMaxTile * 2 / p.G;
+  const bool more = D <= 128 && p.grouped && (int64_t)((p.T + group32 - 1) / group32) * p.KH >= 2 * kCus;
+  const int group = !p.grouped ? 1 : more ? group32 : kMaxTile / p.G, turns = p.grouped ? p.grouped : 1;
   const unsigned grid = (unsigned)((int64_t)(p.shares ? p.shares : (p.T + group - 1) / group) * turns * p.KH * p.tiles);
   const bool once = p.tiles == 1 && p.T < 2 * (int64_t)p.bt_count;   // a table row for every token, but for padding
   // whole tokens for at most a workgroup per CU: twice the waves (one token of 16 heads, 993 rows: 17.4 us with 4, 11.7 with 8)
   const bool wide = !p.shares && !p.grouped && (int64_t)p.T * p.KH * p.tiles <= kCus;
   using G = ExactGeo<D, kE4, false>;
   using W = ExactGeo<D, kE4, true>;
-  void (*const kernels[9])(ExactCacheParams) = {
+  void (*const kernels[10])(ExactCacheParams) = {
       exact_cache_kernel<G, false, kHeads>, exact_cache_kernel<G, false, kTwice>, exact_cache_kernel<G, true, kHeads>,
       exact_cache_kernel<G, true, kTwice>,  exact_cache_kernel<W, false, kHeads>, exact_cache_kernel<W, false, kTwice>,
-      exact_cache_kernel<W, true, kHeads>,  exact_cache_kernel<W, true, kTwice>,  exact_cache_kernel<G, false, kTokens>};
-  hipLaunchKernelGGL(kernels[p.grouped ? 8 : 4 * wide + 2 * once + (p.G <= 8)], dim3(grid), dim3(64 * (wide ? W::WAVES : G::WAVES)),
+      exact_cache_kernel<W, true, kHeads>,  exact_cache_kernel<W, true, kTwice>,  exact_cache_kernel<G, false, kTokens16>,
+      exact_cache_kernel<G, false, D <= 128 ? kTokens32 : kTokens16>};
+  hipLaunchKernelGGL(kernels[p.grouped ? 8 + more : 4 * wide + 2 * once + (p.G <= 8)], dim3(grid), dim3(64 * (wide ? W::WAVES : G::WAVES)),
                      0, st, p);
   if (p.shares)
     hipLaunchKernelGGL(exact_join_kernel<D>, dim3((unsigned)((int64_t)p.T * p.H)), dim3(256), 0, st, p);

@@ -502,3 +502,49 @@ def test_large_chunks(ec, kv_heads, G):
     check(o[some], lse[:, some], q[some], c, [requests[t] for t in some], [ctx[t] for t in some], 0.09)
     alone = ec.attention(q, c.cache, c.table, dev_i32(np.array(ctx)), 0.09, 3000, dev_i64(np.array(requests)), shares=0)
     assert (o.float() - alone[0].float()).abs().max() <= 2.0 ** -6 * alone[0].float().abs().max()
+
+
+@pytest.mark.parametrize('e4m3', [False, True])
+@pytest.mark.parametrize('kv_heads,G,d,block', [(128, 1, 128, 16), (64, 2, 64, 24), (43, 3, 128, 32), (26, 5, 64, 16), (18, 8, 128, 1),
+                                                (18, 7, 128, 16), (18, 8, 256, 16)])
+@pytest.mark.parametrize('window,turns', [(0, 1), (0, 4), (21, 16)])
+def test_groups_where_there_are_many(ec, monkeypatch, kv_heads, G, d, block, e4m3, window, turns):
+    """As above with two workgroups per CU (for groups of twice the tokens): chunks that end inside a group, single tokens, none."""
+    monkeypatch.setattr(ec, '_turns', lambda *a: turns)
+    n, lens = [300, 40, 17, 900, 33], [37, 40, 1, 5, 33]
+    c = Cache(G + d, n, kv_heads, d, block, e4m3)
+    requests, ctx = chunks(n, lens, (3, 0, 1, 2, 4))
+    ctx[7], ctx[60], ctx[-1] = 0, -4, 12
+    requests, ctx = requests + [2, 0, 2], ctx + [17, 300, 5]
+    assert -(-len(ctx) // (32 // G)) * kv_heads >= 512
+    q = query(G, len(ctx), kv_heads * G, d)
+    o, lse = ec.attention(q, c.cache, c.table, dev_i32(np.array(ctx)), d ** -0.5, max(n), dev_i64(np.array(requests)), window,
+                          c.k_scale, c.v_scale)
+    check(o, lse, q, c, requests, ctx, d ** -0.5, window)
+
+
+@pytest.mark.parametrize('e4m3', [False, True])
+def test_rows_that_a_token_of_many_does_not_see(ec, monkeypatch, e4m3):
+    """NaN behind a token's last row and before its window reach only the tokens that see them, in groups of 32 tokens."""
+    monkeypatch.setattr(ec, '_turns', lambda *a: 1)
+    n = [200]
+    c = Cache(42, n, 512, 64, 16, e4m3)
+    ctx = [170 + 7 * i % 31 for i in range(30)] + [0, 1]
+    table_rows, lengths = dev_i64(np.zeros(32)), dev_i32(np.array(ctx))
+    q = query(43, 32, 512, 64)
+    run = lambda window: ec.attention(q, c.cache, c.table, lengths, 0.1, 200, table_rows, window, c.k_scale, c.v_scale)
+    raw = c.cache.view(torch.uint8) if e4m3 else c.cache
+    bad = 0x7F if e4m3 else math.nan
+    clean = run(0), run(20)
+    check(*clean[0], q, c, [0] * 32, ctx, 0.1)
+    check(*clean[1], q, c, [0] * 32, ctx, 0.1, 20)
+    saved = raw.clone()
+    for at, window, sees in ((range(176, 200), 0, [x > 176 for x in ctx]), (range(160), 20, [0 < x < 180 for x in ctx])):
+        at = torch.tensor(at, device='cuda')
+        raw[c.table[0].long()[at // 16], :, at % 16] = bad
+        o, lse = run(window)
+        sees = torch.tensor(sees, device='cuda')
+        assert torch.isnan(o[sees]).all() and torch.isnan(lse[:, sees]).all()
+        seen_by_none = [i for i in range(32) if not sees[i]]
+        check(o[seen_by_none], lse[:, seen_by_none], q[seen_by_none], c, [0] * 32, [ctx[i] for i in seen_by_none], 0.1, window)
+        raw.copy_(saved)
