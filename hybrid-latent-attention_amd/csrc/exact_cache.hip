@@ -469,11 +469,11 @@ __global__ __launch_bounds__(64 * G::WAVES, G::kWavesPerSimd) void exact_cache_k
             u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                 (__attribute__((address_space(3))) short4v*)(vr + 16 * ((CPR / 2 + 2 * c + ((x >> 1) & 1)) ^ swizzle<G>(key)))));
             if (seen) v = u32x2{v[0] & seen[0], v[1] & seen[1]};
-            const short4v vt = __builtin_bit_cast(short4v, v);
 #pragma unroll
             for (int y = 0; y < Y; ++y) {
-              to[y] = mfma16x16x16(vt, __builtin_bit_cast(short4v, p[y][0]), to[y]);
-              if (both) to[y] = mfma16x16x16(vt, __builtin_bit_cast(short4v, p2[y][0]), to[y]);
+              // both parts of P as keys of one product, V twice
+              if (both) to[y] = mfma16x16x32(u32x4{v[0], v[1], v[0], v[1]}, u32x4{p[y][0][0], p[y][0][1], p2[y][0][0], p2[y][0][1]}, to[y]);
+              else to[y] = mfma16x16x16(__builtin_bit_cast(short4v, v), __builtin_bit_cast(short4v, p[y][0]), to[y]);
             }
           }
         };

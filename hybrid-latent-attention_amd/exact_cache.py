@@ -79,7 +79,8 @@ def row_shares(max_rows, groups, parts, cu_count=256):
 
 def _turns(tokens, heads, kv_heads, cu_count=256, per_request=1):
     """0, or the workgroups per group of ``16 // heads`` tokens (``heads`` query heads per KV head; the kernel takes ``32 // heads``
-    where groups are many) that go through rows together, where there is a group for every CU. Chunks on top of histories, us with groups / a workgroup per token: 4 x 512 tokens on 8160 rows of
+    where groups are many) that go through rows together, where there is a group for every CU. Chunks on top of histories, us with
+    groups / a workgroup per token: 4 x 512 tokens on 8160 rows of
     16 heads 454 / 5861, of 8 KV heads for 32 793 / 2939, a prompt of 4000 of 16 heads 269 / 3219, 8 x 64 on 4000 (8 KV heads for
     32) 117 / 397.
     A group of single tokens (which a step may have beside its chunks) has as many requests as tokens: with few tokens per request
