@@ -18,10 +18,11 @@
 //     scores have (16x16x32), and e4m3 values become bf16, exactly, on their way into the operands.
 // P goes into its product as two bf16 parts, upper half and rounded rest (2^-16 of a weight is left; one part alone would add about
 // two thirds of the output's own rounding to it: 0.0024 relative to the 64-bit result, now 0.0017). Up to 8 query heads have their
-// rests in the 8 columns that would be zero: the scores of a head are made twice, for free. More heads take a second product.
+// rests in the 8 columns that would be zero: the scores of a head are made twice, for free. With more heads, or
+// tokens, both parts are keys of one product of twice the keys, V twice in its operand (bf16), or of two products (e4m3).
 //
 // Large steps of many tokens per request (chunks) put the heads of 16 / G or 32 / G tokens in the columns: 4 x 512 tokens on
-// 8160 rows, 16 heads, 454 us, 292 TFLOP/s (matrix units 29 %, vector units 42 %, and the chain of the two between two waves).
+// 8160 rows, 16 heads, 398 us, 333 TFLOP/s (matrix units 23 %, vector units 53 %, LDS 17 %: two waves per SIMD, each a chain of them).
 //
 // Bound by HBM: 64 tokens of 4096 rows and 16 heads (2.1 GB) 320 us, 6.7 TB/s, the vector units at 15 %; a call is its bytes at
 // that rate and about 11 us (launch, lengths, table entries, first rows, joining waves, the second launch). Past the caches
@@ -643,8 +644,8 @@ __global__ __launch_bounds__(256) void exact_join_kernel(ExactCacheParams a) {
 template <int D, bool kE4>
 void launch_exact_cache(const ExactCacheParams& p, hipStream_t st) {
   // groups of tokens: 32 columns take half as many reads of K and V, where there are two workgroups per CU all the same (4 x 512
-  // tokens on 8160 rows of 16 heads 555 -> 454 us; of 256 workgroups with them 61, of 512 without 53). With d = 256 their registers
-  // do not suffice (463 -> 817).
+  // tokens on 8160 rows of 16 heads 555 -> 454 us, with P in two products; of 256 workgroups with them 61, of 512 without 53). With
+  // d = 256 the registers do not suffice for them (463 -> 817).
   const int group32 = kMaxTile * 2 / p.G;
   const bool more = D <= 128 && p.grouped && (int64_t)((p.T + group32 - 1) / group32) * p.KH >= 2 * kCus;
   const int group = !p.grouped ? 1 : more ? group32 : kMaxTile / p.G, turns = p.grouped ? p.grouped : 1;
@@ -789,7 +790,8 @@ extern "C" int hla_s6_exact_attention(const void* q, int32_t num_tokens, int32_t
   HLA_REQUIRE(grouped >= 0 && grouped <= kMaxTile && (!grouped || (shares == 0 && p.G <= kMaxTile / 2)), HLA_S6_EINVAL,
               "exact_attention: groups of tokens need shares 0, at most %d query heads per KV head and at most %d turns", kMaxTile / 2,
               kMaxTile);
-  HLA_REQUIRE((int64_t)max(grouped ? p.T + kMaxTile * kMaxTile : p.T, shares) * p.KH * p.tiles <= INT32_MAX / (grouped ? 2 : 1) && (int64_t)p.T * p.H <= INT32_MAX, HLA_S6_EINVAL,
+  HLA_REQUIRE((int64_t)max(grouped ? p.T + kMaxTile * kMaxTile : p.T, shares) * p.KH * p.tiles <= INT32_MAX / (grouped ? 2 : 1) &&
+                  (int64_t)p.T * p.H <= INT32_MAX, HLA_S6_EINVAL,
               "exact_attention: too many rows");
   if (shares) {
     const int64_t rows = (int64_t)2 * shares * p.H, need = rows * (head_dim + 1) + 2 * (int64_t)p.T;

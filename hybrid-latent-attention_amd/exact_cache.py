@@ -80,9 +80,9 @@ def row_shares(max_rows, groups, parts, cu_count=256):
 def _turns(tokens, heads, kv_heads, cu_count=256, per_request=1):
     """0, or the workgroups per group of ``16 // heads`` tokens (``heads`` query heads per KV head; the kernel takes ``32 // heads``
     where groups are many) that go through rows together, where there is a group for every CU. Chunks on top of histories, us with
-    groups / a workgroup per token: 4 x 512 tokens on 8160 rows of
-    16 heads 454 / 5861, of 8 KV heads for 32 793 / 2939, a prompt of 4000 of 16 heads 269 / 3219, 8 x 64 on 4000 (8 KV heads for
-    32) 117 / 397.
+    groups / a workgroup per token: 4 x 512 tokens on 8160 rows of 16 heads 398 / 5861, of 8 KV heads for 32 685 / 2939, a prompt
+    of 4000 of 16 heads 235 / 3219, 8 x 64 on 4000 (8 KV heads for 32) 103 / 397.
+
     A group of single tokens (which a step may have beside its chunks) has as many requests as tokens: with few tokens per request
     on average a workgroup for each; else 4, since most find nothing to do."""
     if heads > 8 or -(-tokens // (16 // heads)) * kv_heads < cu_count:
@@ -99,8 +99,8 @@ def attention(q, cache, block_table, ctx, scale, max_seq_len, token_requests=Non
     The rows of a token are those before it and its own, once ``store_rows`` has written it; tokens of one request (a chunk) have a
     ``ctx`` of their own each. ``block_table`` (int32) is per token, or per request with ``token_requests[t]`` (int64) naming the
     row of token ``t``. Tokens of a request that lie one behind the other go through its rows together in large steps of chunks:
-    ``max_query_len`` (a host number, the most tokens of a request) defaults to the tokens per row of the table. No entry of ``ctx`` should be above ``max_seq_len`` (a host number, which sets how rows are cut). Scores,
-    softmax statistics and sums are fp32; weights keep 16 bits in their product with V.
+    ``max_query_len`` (a host number, the most tokens of a request) defaults to the tokens per row of the table. No entry of ``ctx``
+    should be above ``max_seq_len`` (a host number, which sets how rows are cut). Scores, softmax statistics and sums are fp32; weights keep 16 bits in their product with V.
 
     The rows of all tokens are cut in ``shares`` equal parts per KV head (0: a workgroup takes all rows of a token; defaults to
     ``row_shares``); their partial results go through ``workspace`` (an ``S6Workspace`` of ``2 * shares * H * (d + 1) + 2 * T`` floats;
