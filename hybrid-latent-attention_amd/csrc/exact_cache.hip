@@ -560,7 +560,8 @@ __global__ __launch_bounds__(64 * G::WAVES, G::kWavesPerSimd) void exact_cache_k
           token_rows(a, u, f, c);
           none = none || c <= f;   // (its columns took part in what the others see)
         }
-        if (none) v = floatx4{0.f, 0.f, 0.f, 0.f};   // (weights of 0, of which a NaN in V made NaN)
+        // (weights of 0, of which a NaN in V made NaN: no weight at all gives 0, but a part may yet be joined to others)
+        if (none && whole) v = floatx4{0.f, 0.f, 0.f, 0.f};
         const float inv = none ? 0.f : (kE4 && a.v_scale ? a.v_scale[kh] : 1.f) / sum;
         const float lse = none ? -INFINITY : (top + log2f(sum)) * kLn2;
         if (!whole) {   // rows that began in an earlier share, or that go on in the next
@@ -618,7 +619,7 @@ __global__ __launch_bounds__(256) void exact_join_kernel(ExactCacheParams a) {
   top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   float w = 0.f;
   for (int s = tid; s < count; s += 256) {
-    // (a part with a NaN lse has a NaN weight; one with nothing but scores of -inf none)
+    // (a part with a NaN lse has a NaN weight; one with nothing but scores of -inf has a weight of 0, and its NaN, if V has any, stay)
     const float mine = weight[s];
     w += weight[s] = mine == -INFINITY ? 0.f : fast_exp2((mine - top) * kLog2e);
   }
@@ -635,6 +636,7 @@ __global__ __launch_bounds__(256) void exact_join_kernel(ExactCacheParams a) {
   if (tid >= PER) return;
   for (int i = 1; i < ROWS; ++i) v += sums[i][tid];
   const bool none = sum == 0.f;
+  if (none) v = floatx4{0.f, 0.f, 0.f, 0.f};
   const float inv = none ? 0.f : 1.f / sum;
   *reinterpret_cast<u32x2*>(a.out + (int64_t)t * a.o_st + (int64_t)h * a.o_sh + 4 * tid) =
       u32x2{pack2(v[0] * inv, v[1] * inv), pack2(v[2] * inv, v[3] * inv)};
