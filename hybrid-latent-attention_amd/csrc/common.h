@@ -194,6 +194,8 @@ __device__ __forceinline__ void plain_barrier() {
 namespace hla {
 int fail(int code, const char* fmt, ...);
 int check_launch(const char* what);
+// Whether a launch can have that many workgroups in a dimension: fewer than 2^32 threads
+inline bool launchable(int64_t workgroups, int threads) { return workgroups <= (int64_t)UINT32_MAX / threads; }
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 int khop_forward_mq(const void* q, int64_t q_st, int64_t q_sh, const void* k, const void* v, int64_t k_sn, int B,
                     int Lq, int N, int width, const uint8_t* mask, int64_t mask_sb, int64_t mask_st,

@@ -643,15 +643,23 @@ __global__ __launch_bounds__(256) void exact_join_kernel(ExactCacheParams a) {
   if (tid == 0) a.lse[(int64_t)h * a.T + t] = none ? -INFINITY : top + logf(sum);
 }
 
+// Groups of tokens: 32 columns take half as many reads of K and V, where there are two workgroups per CU all the same (4 x 512
+// tokens on 8160 rows of 16 heads 555 -> 454 us, with P in two products; of 256 workgroups with them 61, of 512 without 53). With
+// d = 256 the registers do not suffice for them (463 -> 817).
+bool groups_of_32(const ExactCacheParams& p, int dim) {
+  const int group = kMaxTile * 2 / p.G;
+  return dim <= 128 && p.grouped && ((int64_t)p.T + group - 1) / group * p.KH >= 2 * kCus;
+}
+
+int64_t exact_workgroups(const ExactCacheParams& p, int dim) {
+  const int group = !p.grouped ? 1 : (groups_of_32(p, dim) ? 2 : 1) * kMaxTile / p.G;
+  return (p.shares ? p.shares : ((int64_t)p.T + group - 1) / group) * (p.grouped ? p.grouped : 1) * p.KH * p.tiles;
+}
+
 template <int D, bool kE4>
 void launch_exact_cache(const ExactCacheParams& p, hipStream_t st) {
-  // groups of tokens: 32 columns take half as many reads of K and V, where there are two workgroups per CU all the same (4 x 512
-  // tokens on 8160 rows of 16 heads 555 -> 454 us, with P in two products; of 256 workgroups with them 61, of 512 without 53). With
-  // d = 256 the registers do not suffice for them (463 -> 817).
-  const int group32 = kMaxTile * 2 / p.G;
-  const bool more = D <= 128 && p.grouped && (int64_t)((p.T + group32 - 1) / group32) * p.KH >= 2 * kCus;
-  const int group = !p.grouped ? 1 : more ? group32 : kMaxTile / p.G, turns = p.grouped ? p.grouped : 1;
-  const unsigned grid = (unsigned)((int64_t)(p.shares ? p.shares : (p.T + group - 1) / group) * turns * p.KH * p.tiles);
+  const bool more = groups_of_32(p, D);
+  const unsigned grid = (unsigned)exact_workgroups(p, D);
   const bool once = p.tiles == 1 && p.T < 2 * (int64_t)p.bt_count;   // a table row for every token, but for padding
   // whole tokens for at most a workgroup per CU: twice the waves (one token of 16 heads, 993 rows: 17.4 us with 4, 11.7 with 8)
   const bool wide = !p.shares && !p.grouped && (int64_t)p.T * p.KH * p.tiles <= kCus;
@@ -792,9 +800,9 @@ extern "C" int hla_s6_exact_attention(const void* q, int32_t num_tokens, int32_t
   HLA_REQUIRE(grouped >= 0 && grouped <= kMaxTile && (!grouped || (shares == 0 && p.G <= kMaxTile / 2)), HLA_S6_EINVAL,
               "exact_attention: groups of tokens need shares 0, at most %d query heads per KV head and at most %d turns", kMaxTile / 2,
               kMaxTile);
-  HLA_REQUIRE((int64_t)max(grouped ? p.T + kMaxTile * kMaxTile : p.T, shares) * p.KH * p.tiles <= INT32_MAX / (grouped ? 2 : 1) &&
-                  (int64_t)p.T * p.H <= INT32_MAX, HLA_S6_EINVAL,
-              "exact_attention: too many rows");
+  // (KH * tiles is at most H, so that workgroups are counted in 64 bits; none of a grid has more than 256 threads but one of few)
+  HLA_REQUIRE((int64_t)p.T * p.H <= INT32_MAX && launchable(exact_workgroups(p, head_dim), 256) &&
+                  (!shares || launchable((int64_t)p.T * p.H, 256)), HLA_S6_EINVAL, "exact_attention: too many rows");
   if (shares) {
     const int64_t rows = (int64_t)2 * shares * p.H, need = rows * (head_dim + 1) + 2 * (int64_t)p.T;
     HLA_REQUIRE(workspace && workspace_floats >= need, HLA_S6_EWORKSPACE,
@@ -839,7 +847,7 @@ extern "C" int hla_s6_exact_store(const void* key, int64_t k_st, int64_t k_sh, c
                         num_tokens, kv_heads, head_dim, slots, k_scale, v_scale, static_cast<uint8_t*>(cache),
                         page_stride * es, head_stride * es, row_stride * es, block_size, num_blocks};
   const int64_t blocks = ((int64_t)num_tokens * kv_heads * (head_dim / 4) + 255) / 256;
-  HLA_REQUIRE(blocks <= INT32_MAX, HLA_S6_EINVAL, "exact_store: too many rows");
+  HLA_REQUIRE(launchable(blocks, 256), HLA_S6_EINVAL, "exact_store: too many rows");
   const hipStream_t st = as_stream(stream);
   if (e4m3) hipLaunchKernelGGL(exact_store_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, st, p);
   else hipLaunchKernelGGL(exact_store_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, st, p);

@@ -496,6 +496,7 @@ extern "C" int hla_s6_pool_release(int32_t* tables, int64_t t_st, int32_t num_re
   using namespace hla;
   HLA_POOL("pool_release");
   HLA_REQUIRE(count >= 0 && (count == 0 || requests), HLA_S6_EINVAL, "pool_release: bad list");
+  HLA_REQUIRE(launchable(count, 256), HLA_S6_EINVAL, "pool_release: list too long");
   if (count == 0 || num_reqs == 0) return HLA_S6_OK;
   hipLaunchKernelGGL(pool_release_kernel, dim3((unsigned)count), dim3(256), 0, as_stream(stream), p, requests, to);
   return check_launch("pool_release");
@@ -567,10 +568,11 @@ extern "C" int hla_s6_copy_pages(void* const* caches, int32_t num_caches, int64_
   a.source = source;
   a.target = target;
   a.count = count;
-  const int64_t pieces = (page_bytes + kPiece - 1) / kPiece;
+  const int64_t pieces = (page_bytes - 1) / kPiece + 1;
   a.per = count > 4096 ? 64 : 1;
-  const int64_t groups = (count + a.per - 1) / a.per;
-  HLA_REQUIRE(groups * pieces <= INT32_MAX, HLA_S6_EINVAL, "copy_pages: lists or pages too long");
+  const int64_t groups = (count - 1) / a.per + 1;
+  HLA_REQUIRE(pieces <= INT32_MAX && groups <= INT32_MAX && launchable(groups * pieces, 256), HLA_S6_EINVAL,
+              "copy_pages: lists or pages too long");
   a.pieces = (int)pieces;
   for (int c0 = 0; c0 < num_caches; c0 += kMaxCaches) {
     const int n = num_caches - c0 < kMaxCaches ? num_caches - c0 : kMaxCaches;
