@@ -13,7 +13,7 @@ import torch
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get('HLA_S6_LIBRARY') or os.path.join(HERE, 'libhla_s6.so')   # override: another build
-ABI_VERSION = 17
+ABI_VERSION = 18
 
 OK, EINVAL, EUNSUPPORTED, EWORKSPACE, ELAUNCH, EDEVICE = range(6)
 
@@ -97,7 +97,7 @@ SIGNATURES = {
     'hla_s6_select_rows': [P, I64, P, I64, P, I32, I32, I32, P, P, P, P, P, P, P, P],
     'hla_s6_move_rows': [P, I32, I32, I64, I64, I32, I64, P, I64, I32, P, P, I64, I32, I32, P],
     'hla_s6_exact_attention': [P, I32, I32, I32, I64, I64, P, I32, I32, I64, I64, I64, I32, I64, P, I64, I32, I32, P, P, I32,
-                               F32, P, P, I32, I32, P, I64, P, I64, I64, P, P],
+                               F32, P, P, I32, I32, P, I64, P, I64, I64, P, I32, P],
     'hla_s6_exact_store': [P, I64, I64, P, I64, I64, I32, I32, I32, P, P, P, P, I32, I64, I64, I64, I32, I64, P],
     'hla_s6_pool_release': [*POOL, P, P, I32, P],
     'hla_s6_pool_fork': [*POOL, P, P, I32, P, P],

@@ -59,6 +59,7 @@ struct ExactCacheParams {
   int T, H, KH, G, tiles;  // tiles: workgroups of query heads per KV head
   int shares;              // 0: a workgroup takes all rows of a token, or (grouped) of 16 / G or 32 / G tokens
   int grouped;             // workgroups among which the requests of a group are dealt; 0: a token by itself
+  bool shared;             // several tokens read the same rows
   float *ws_o, *ws_lse;    // [shares][2][H][D], [shares][2][H]
   int32_t* split;          // [T][2]: first and last share of a token's rows
   uint16_t* out;
@@ -660,7 +661,8 @@ template <int D, bool kE4>
 void launch_exact_cache(const ExactCacheParams& p, hipStream_t st) {
   const bool more = groups_of_32(p, D);
   const unsigned grid = (unsigned)exact_workgroups(p, D);
-  const bool once = p.tiles == 1 && p.T < 2 * (int64_t)p.bt_count;   // a table row for every token, but for padding
+  // past the caches where no other workgroup reads the rows (a chunk of 64 tokens on 8160 rows, 8 KV heads for 32: 128 us, past them 145)
+  const bool once = p.tiles == 1 && !p.shared;
   // whole tokens for at most a workgroup per CU: twice the waves (one token of 16 heads, 993 rows: 17.4 us with 4, 11.7 with 8)
   const bool wide = !p.shares && !p.grouped && (int64_t)p.T * p.KH * p.tiles <= kCus;
   using G = ExactGeo<D, kE4, false>;
@@ -753,7 +755,7 @@ extern "C" int hla_s6_exact_attention(const void* q, int32_t num_tokens, int32_t
                                       const int64_t* bt_rows, const int32_t* ctx, int32_t window, float scale,
                                       const float* k_scale, const float* v_scale, int32_t shares,
                                       int32_t grouped, float* workspace, int64_t workspace_floats, void* out, int64_t o_st, int64_t o_sh,
-                                      float* lse, void* stream) {
+                                      float* lse, int32_t shared_rows, void* stream) {
   using namespace hla;
   HLA_REQUIRE(num_tokens >= 0, HLA_S6_EINVAL, "exact_attention: negative token count");
   int rc = check_exact_cache("exact_attention", cache, e4m3, head_dim, kv_heads, page_stride, head_stride, row_stride,
@@ -797,6 +799,7 @@ extern "C" int hla_s6_exact_attention(const void* q, int32_t num_tokens, int32_t
   p.tiles = (p.G + kMaxTile - 1) / kMaxTile;
   p.shares = shares;
   p.grouped = grouped;
+  p.shared = shared_rows != 0;
   HLA_REQUIRE(grouped >= 0 && grouped <= kMaxTile && (!grouped || (shares == 0 && p.G <= kMaxTile / 2)), HLA_S6_EINVAL,
               "exact_attention: groups of tokens need shares 0, at most %d query heads per KV head and at most %d turns", kMaxTile / 2,
               kMaxTile);

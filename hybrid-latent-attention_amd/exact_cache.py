@@ -99,8 +99,10 @@ def attention(q, cache, block_table, ctx, scale, max_seq_len, token_requests=Non
     The rows of a token are those before it and its own, once ``store_rows`` has written it; tokens of one request (a chunk) have a
     ``ctx`` of their own each. ``block_table`` (int32) is per token, or per request with ``token_requests[t]`` (int64) naming the
     row of token ``t``. Tokens of a request that lie one behind the other go through its rows together in large steps of chunks:
-    ``max_query_len`` (a host number, the most tokens of a request) defaults to the tokens per row of the table. No entry of ``ctx``
-    should be above ``max_seq_len`` (a host number, which sets how rows are cut). Scores, softmax statistics and sums are fp32; weights keep 16 bits in their product with V.
+    ``max_query_len`` (a host number, the most tokens of a request) defaults to the tokens per row of the table; with a table that has
+    rows to spare (a pool's) the tokens would be taken for single ones, 15 times slower in large chunks: pass it. No entry of ``ctx``
+    should be above ``max_seq_len`` (a host number, which sets how rows are cut). Scores, softmax statistics and sums are fp32; weights
+    keep 16 bits in their product with V.
 
     The rows of all tokens are cut in ``shares`` equal parts per KV head (0: a workgroup takes all rows of a token; defaults to
     ``row_shares``); their partial results go through ``workspace`` (an ``S6Workspace`` of ``2 * shares * H * (d + 1) + 2 * T`` floats;
@@ -123,10 +125,11 @@ def attention(q, cache, block_table, ctx, scale, max_seq_len, token_requests=Non
     longest = min(int(max_seq_len), cols * block, window or cols * block)
     parts = kv_heads * -(-H // kv_heads // 16)
     cus = _lib.device_cus(dev.index)
-    turns = 0
+    turns, chunk = 0, 1
+    if token_requests is not None:
+        chunk = T // max(1, count) if max_query_len is None else int(max_query_len)
     if shares is None:
-        chunk = T // max(1, count) if max_query_len is None else max_query_len
-        turns = _turns(T, H // kv_heads, kv_heads, cus, T // max(1, count)) if token_requests is not None and chunk >= 4 else 0
+        turns = _turns(T, H // kv_heads, kv_heads, cus, T // max(1, count)) if chunk >= 4 else 0
         shares = 0 if turns else row_shares(longest, T * parts, parts, cus)
     else:
         shares = int(shares)
@@ -145,5 +148,5 @@ def attention(q, cache, block_table, ctx, scale, max_seq_len, token_requests=Non
     _call('hla_s6_exact_attention', dev, q.data_ptr(), T, H, d, token_stride, head_stride, cache.data_ptr(), int(e4m3), kv_heads,
           page, head, row, block, pages, block_table.data_ptr(), table_stride, cols, count, _lib.ptr(token_requests),
           ctx.data_ptr(), window, float(scale), _lib.ptr(k_scale), _lib.ptr(v_scale), shares, turns, _lib.ptr(ws),
-          0 if ws is None else ws.numel(), out.data_ptr(), H * d, d, lse.data_ptr())
+          0 if ws is None else ws.numel(), out.data_ptr(), H * d, d, lse.data_ptr(), int(chunk > 1))
     return out, lse

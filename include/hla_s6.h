@@ -24,7 +24,7 @@
 extern "C" {
 #endif
 
-#define HLA_S6_ABI_VERSION 17
+#define HLA_S6_ABI_VERSION 18
 
 #define HLA_S6_OK 0
 #define HLA_S6_EINVAL 1       /* bad shape, stride or argument            (Python: ValueError)   */
@@ -591,14 +591,16 @@ int hla_s6_move_rows(void *cache, int32_t width, int32_t compact, int64_t page_s
  * rows. shares 0: a workgroup takes all rows of a (token, KV head); else (at most 1024) the rows of all tokens together are cut in
  * that many equal shares per KV head, and the workspace holds 2 * shares * num_heads * (head_dim + 1) + 2 * num_tokens floats.
  * grouped > 0 (at most 16; shares 0, at most 8 query heads per KV head): groups of 16 / (num_heads / kv_heads) tokens, those that lie
- * one behind the other and read the same table row together; a group's table rows are dealt to `grouped` workgroups. */
+ * one behind the other and read the same table row together; a group's table rows are dealt to `grouped` workgroups. shared_rows
+ * != 0 says that several tokens read the same rows, which then do not stream past the caches (results are the same). */
 int hla_s6_exact_attention(const void *q, int32_t num_tokens, int32_t num_heads, int32_t head_dim, int64_t q_st,
                            int64_t q_sh, const void *cache, int32_t e4m3, int32_t kv_heads, int64_t page_stride,
                            int64_t head_stride, int64_t row_stride, int32_t block_size, int64_t num_blocks,
                            const int32_t *block_table, int64_t bt_stride, int32_t bt_cols, int32_t bt_count,
                            const int64_t *bt_rows, const int32_t *ctx, int32_t window, float scale,
                            const float *k_scale, const float *v_scale, int32_t shares, int32_t grouped,
-                           float *workspace, int64_t workspace_floats, void *out, int64_t o_st, int64_t o_sh, float *lse, void *stream);
+                           float *workspace, int64_t workspace_floats, void *out, int64_t o_st, int64_t o_sh, float *lse,
+                           int32_t shared_rows, void *stream);
 
 /* Row t of key / value (bf16 [num_tokens, kv_heads, head_dim]) into slot slots[t] (page * block_size + row; outside the cache:
  * skipped; the slots of a call differ). e4m3: x / scale, clamped to +-448, to the nearest, ties to even; NaN stays NaN. */

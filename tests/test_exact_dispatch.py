@@ -1,0 +1,32 @@
+"""CPU checks of how ``exact_cache.attention`` deals a step to workgroups, from host numbers alone; nothing is launched."""
+import pytest
+import torch
+
+
+@pytest.fixture
+def dealt(pkg, monkeypatch):
+    """``(shares, grouped, shared_rows)`` of a call with 256 CUs."""
+    ec = pkg.exact_cache
+    calls = []
+    monkeypatch.setattr(ec, '_same_device', lambda *a: None)
+    monkeypatch.setattr(ec, '_call', lambda name, device, *args: calls.append(args))
+    monkeypatch.setattr(ec._lib, 'device_cus', lambda index: 256)
+
+    def dealt(tokens, requests, kv_heads, group, longest, max_query_len=None, per_request=True, **more):
+        cache = torch.empty(4, kv_heads, 16, 128, dtype=torch.bfloat16)
+        q = torch.empty(tokens, kv_heads * group, 64, dtype=torch.bfloat16)
+        table = torch.empty(requests, -(-longest // 16), dtype=torch.int32)
+        ec.attention(q, cache, table, torch.zeros(tokens, dtype=torch.int32), 1.0, longest,
+                     torch.zeros(tokens, dtype=torch.int64) if per_request else None, max_query_len=max_query_len, **more)
+        args = calls.pop()
+        return args[24], args[25], args[32]
+
+    return dealt
+
+
+def test_who_reads_the_same_rows(dealt):
+    """A table with rows to spare says nothing about the tokens of a request where the caller does."""
+    assert dealt(64, 1, 8, 4, 8160, 64)[2] == 1 and dealt(64, 256, 8, 4, 8160, 64)[2] == 1
+    assert dealt(64, 1, 8, 4, 8160)[2] == 1 and dealt(64, 64, 8, 4, 8160)[2] == 0
+    assert dealt(64, 64, 8, 4, 8160, 1)[2] == 0 and dealt(130, 64, 8, 4, 8160, 1)[2] == 0      # (padding)
+    assert dealt(64, 64, 8, 4, 8160, per_request=False)[2] == 0 and dealt(64, 64, 8, 4, 8160, 64, per_request=False)[2] == 0
