@@ -84,7 +84,7 @@ def _turns(tokens, heads, kv_heads, cu_count=256, per_request=1):
     of 4000 of 16 heads 235 / 3219, 8 x 64 on 4000 (8 KV heads for 32) 103 / 397.
 
     A group of single tokens (which a step may have beside its chunks) has as many requests as tokens: with few tokens per request
-    on average a workgroup for each; else 4, since most find nothing to do."""
+    on average (``per_request``, at least) a workgroup for each; else 4, since most find nothing to do (a prompt of 4000 with 16: 260)."""
     if heads > 8 or -(-tokens // (16 // heads)) * kv_heads < cu_count:
         return 0
     return 16 // heads if per_request < 32 else min(4, 16 // heads)
@@ -129,7 +129,8 @@ def attention(q, cache, block_table, ctx, scale, max_seq_len, token_requests=Non
     if token_requests is not None:
         chunk = T // max(1, count) if max_query_len is None else int(max_query_len)
     if shares is None:
-        turns = _turns(T, H // kv_heads, kv_heads, cus, T // max(1, count)) if chunk >= 4 else 0
+        if chunk >= 4:
+            turns = _turns(T, H // kv_heads, kv_heads, cus, T // max(1, min(count, T - chunk + 1)))   # (most requests there can be)
         shares = 0 if turns else row_shares(longest, T * parts, parts, cus)
     else:
         shares = int(shares)

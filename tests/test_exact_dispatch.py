@@ -30,3 +30,10 @@ def test_who_reads_the_same_rows(dealt):
     assert dealt(64, 1, 8, 4, 8160)[2] == 1 and dealt(64, 64, 8, 4, 8160)[2] == 0
     assert dealt(64, 64, 8, 4, 8160, 1)[2] == 0 and dealt(130, 64, 8, 4, 8160, 1)[2] == 0      # (padding)
     assert dealt(64, 64, 8, 4, 8160, per_request=False)[2] == 0 and dealt(64, 64, 8, 4, 8160, 64, per_request=False)[2] == 0
+
+
+def test_requests_of_a_step(dealt):
+    """Nor how many requests there are: one that takes max_query_len of the tokens leaves few to others."""
+    assert dealt(4000, 1, 16, 1, 4000, 4000)[1] == 4 and dealt(4000, 256, 16, 1, 4000, 4000)[1] == 4
+    assert dealt(4016, 256, 16, 1, 4000, 4000)[1] == 4 and dealt(576, 65, 16, 1, 4000, 512)[1] == 16
+    assert dealt(256, 32, 16, 1, 4000, 8)[1] == 16 and dealt(256, 1000, 16, 1, 4000, 8)[1] == 16
