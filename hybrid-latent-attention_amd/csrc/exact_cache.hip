@@ -24,6 +24,8 @@
 // Large steps of many tokens per request (chunks) put the heads of 16 / G or 32 / G tokens in the columns: 4 x 512 tokens on
 // 8160 rows, 16 heads, 398 us, 333 TFLOP/s (matrix units 23 %, vector units 53 %, LDS 17 %: two waves per SIMD, each a chain of them).
 //
+// Single tokens beside chunks (exact_alone_kernel lists them) keep their shares, in a launch behind that of the groups.
+//
 // Bound by HBM: 64 tokens of 4096 rows and 16 heads (2.1 GB) 320 us, 6.7 TB/s, the vector units at 15 %; a call is its bytes at
 // that rate and about 11 us (launch, lengths, table entries, first rows, joining waves, the second launch). Past the caches
 // (kOnce) 7 % faster. Two workgroups of four waves per CU, a tile of each wave on its way: three waves, eight, or one workgroup
@@ -57,11 +59,12 @@ struct ExactCacheParams {
   float scale_log2;
   const float *k_scale, *v_scale;
   int T, H, KH, G, tiles;  // tiles: workgroups of query heads per KV head
-  int shares;              // 0: a workgroup takes all rows of a token, or (grouped) of 16 / G or 32 / G tokens
+  int shares;              // 0: a workgroup takes all rows of a token, or (grouped) of 16 / G or 32 / G tokens; beside groups: see alone
   int grouped;             // workgroups among which the requests of a group are dealt; 0: a token by itself
   bool shared;             // several tokens read the same rows
   float *ws_o, *ws_lse;    // [shares][2][H][D], [shares][2][H]
   int32_t* split;          // [T][2]: first and last share of a token's rows
+  int32_t* alone;          // null, or where shares take the tokens alone and groups the others: [1 + T], how many are alone, and which
   uint16_t* out;
   int64_t o_st, o_sh;
   float* lse;  // [H][T]
@@ -126,21 +129,48 @@ __device__ __forceinline__ void token_rows(const ExactCacheParams& a, int t, int
   first = a.window > 0 ? max(0, n - a.window) : 0;
 }
 
-// Steps of a token's rows
-__device__ __forceinline__ int token_steps(const ExactCacheParams& a, int t) {
+// Its row of the table
+__device__ __forceinline__ int64_t table_row(const ExactCacheParams& a, int t) {
+  return a.bt_rows ? min(max(a.bt_rows[t], (int64_t)0), (int64_t)a.bt_count - 1) : t;
+}
+
+// Whether a token has rows and its neighbours none of the same table row
+__device__ __forceinline__ bool is_alone(const ExactCacheParams& a, int t) {
   int first, n;
   token_rows(a, t, first, n);
+  if (n == 0) return false;
+  const int64_t row = table_row(a, t);
+  for (int i = max(t - 1, 0); i <= min(t + 1, a.T - 1); ++i) {
+    token_rows(a, i, first, n);
+    if (i != t && n > 0 && table_row(a, i) == row) return false;
+  }
+  return true;
+}
+
+// The tokens that shares take: all, or (kAlone) those alone
+template <bool kAlone>
+__device__ __forceinline__ int shared_tokens(const ExactCacheParams& a) { return kAlone ? a.alone[0] : a.T; }
+template <bool kAlone>
+__device__ __forceinline__ int shared_token(const ExactCacheParams& a, int i) { return kAlone ? a.alone[1 + i] : i; }
+
+// Steps of the rows of the i-th of them
+template <bool kAlone>
+__device__ __forceinline__ int token_steps(const ExactCacheParams& a, int i) {
+  int first, n;
+  token_rows(a, shared_token<kAlone>(a, i), first, n);
   return (n - first + kStep - 1) / kStep;
 }
 
 // Share k of the steps of all tokens, one token behind the other: a share is ceil(total / shares) of them, kMinSteps at least.
-// `left` steps of it (0: none) begin at step `at` of token t, whose first step is the `before`-th of all.
+// `left` steps of it (0: none) begin at step `at` of the t-th token, whose first step is the `before`-th of all.
+template <bool kAlone>
 __device__ __forceinline__ void find_share(const ExactCacheParams& a, int k, int threads, int64_t* sums, int64_t* found, int& t,
                                            int& at, int64_t& left, int64_t& before, int64_t& share) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int seg = (a.T + threads - 1) / threads, t0 = min(a.T, tid * seg), t1 = min(a.T, t0 + seg);
+  const int tokens = shared_tokens<kAlone>(a), seg = (tokens + threads - 1) / threads;
+  const int t0 = min(tokens, tid * seg), t1 = min(tokens, t0 + seg);
   int64_t mine = 0;
-  for (int i = t0; i < t1; ++i) mine += token_steps(a, i);
+  for (int i = t0; i < t1; ++i) mine += token_steps<kAlone>(a, i);
   int64_t x = mine;
   for (int off = 1; off < 64; off <<= 1) {
     const int64_t y = __shfl_up(x, off);
@@ -161,7 +191,7 @@ __device__ __forceinline__ void find_share(const ExactCacheParams& a, int k, int
   int64_t base = x - mine;
   if (begin >= base && begin < x)   // one thread's tokens hold it
     for (int i = t0; i < t1; ++i) {
-      const int steps = token_steps(a, i);
+      const int steps = token_steps<kAlone>(a, i);
       if (begin < base + steps) {
         found[0] = i;
         found[1] = base;
@@ -183,8 +213,9 @@ enum Columns {
   kTokens32, // the same with 32 columns
 };
 
-// kOnce: rows are read by one workgroup and stream past the caches
-template <class G, bool kOnce, Columns kColumns>
+// kOnce: rows are read by one workgroup and stream past the caches; kAlone: shares of the tokens alone, beside groups of the others
+// (a kernel of its own: told apart within one, every step in shares took 0.5 to 3 us longer)
+template <class G, bool kOnce, Columns kColumns, bool kAlone = false>
 __global__ __launch_bounds__(64 * G::WAVES, G::kWavesPerSimd) void exact_cache_kernel(ExactCacheParams a) {
   constexpr int D = G::D;
   constexpr bool kE4 = G::kE4;
@@ -219,20 +250,25 @@ __global__ __launch_bounds__(64 * G::WAVES, G::kWavesPerSimd) void exact_cache_k
     head[y] = kColumns == kTwice ? x & 7 : kTokens ? (16 * y + x) % a.G : x;
     token[y] = t_group + (kTokens ? (16 * y + x) / a.G : 0);
   }
-  auto table_row = [&](int i) { return a.bt_rows ? min(max(a.bt_rows[i], (int64_t)0), (int64_t)a.bt_count - 1) : i; };
 
-  // lane i: what token t_group + i reads and sees; a bit for every token that begins a run
+  // lane i: what token t_group + i reads and sees; a bit for every token that begins a run (tokens alone, where shares take them,
+  // are in none)
   int64_t lane_row = 0;
   int lane_first = 0, lane_n = 0;
   uint32_t heads_of_runs = 0;
   if constexpr (kTokens) {
     const int i = t_group + lane;
-    if (i < t_end) {
-      lane_row = table_row(i);
+    bool runs = i < t_end;
+    if (runs) {
+      lane_row = table_row(a, i);
       token_rows(a, i, lane_first, lane_n);
+      if (a.alone && is_alone(a, i)) {
+        lane_row = ~(int64_t)i;
+        runs = false;
+      }
     }
     const int64_t before = __shfl_up(lane_row, 1);
-    heads_of_runs = (uint32_t)__ballot(i < t_end && (lane == 0 || lane_row != before));
+    heads_of_runs = (uint32_t)__ballot(runs && (lane == 0 || lane_row != before));
     for (int skip = 0; skip < turn; ++skip) heads_of_runs &= heads_of_runs - 1;
     if (!heads_of_runs) return;
   }
@@ -240,13 +276,14 @@ __global__ __launch_bounds__(64 * G::WAVES, G::kWavesPerSimd) void exact_cache_k
   int t = kTokens ? t_group + __ffs((int)heads_of_runs) - 1 : t_group, at = 0;
   int64_t left_steps = INT32_MAX, before = 0, share = 1;
   if (a.shares) {
-    find_share(a, k, 64 * WAVES, sums, found, t, at, left_steps, before, share);
+    find_share<kAlone>(a, k, 64 * WAVES, sums, found, t, at, left_steps, before, share);
     if (left_steps <= 0) return;
   }
   for (;;) {   // the tokens of the share, or the requests of the group
     // tokens [t, t_last) of a request: rows [first, n) are seen by any of them, [all_first, all_n) by all that see any
     int first, n, t_last = t + 1, all_first, all_n, my_first[Y] = {}, my_n[Y] = {};
     int64_t row;
+    const int my_token = kAlone ? __builtin_amdgcn_readfirstlane(shared_token<kAlone>(a, t)) : t;   // (of one)
     if constexpr (kTokens) {
       const int at_lane = t - t_group;
       row = __shfl(lane_row, at_lane);
@@ -276,8 +313,8 @@ __global__ __launch_bounds__(64 * G::WAVES, G::kWavesPerSimd) void exact_cache_k
         }
       }
     } else {
-      token_rows(a, t, first, n);
-      row = table_row(t);
+      token_rows(a, my_token, first, n);
+      row = table_row(a, my_token);
       all_first = first;
       all_n = n;
     }
@@ -332,7 +369,7 @@ __global__ __launch_bounds__(64 * G::WAVES, G::kWavesPerSimd) void exact_cache_k
 #pragma unroll
       for (int y = 0; y < Y; ++y) {
         const bool used = kTokens ? token[y] >= t && token[y] < t_last : head[y] < heads;
-        const uint16_t* qp = a.q + (int64_t)(kTokens && used ? token[y] : t) * a.q_st + (int64_t)(h0 + (used ? head[y] : 0)) * a.q_sh;
+        const uint16_t* qp = a.q + (int64_t)(kTokens && used ? token[y] : my_token) * a.q_st + (int64_t)(h0 + (used ? head[y] : 0)) * a.q_sh;
 #pragma unroll
         for (int s = 0; s < D / 32; ++s) {
           const int col = kE4 ? 16 * (g + 4 * (s / 2)) + 8 * (s % 2) : 32 * s + 8 * g;
@@ -545,7 +582,7 @@ __global__ __launch_bounds__(64 * G::WAVES, G::kWavesPerSimd) void exact_cache_k
       const int j_first = (t - t_group) * heads, j_count = (t_last - t) * heads;   // its columns (the tokens' ones)
       for (int i = tid; i < (kTokens ? j_count : heads) * (D / 4); i += 64 * WAVES) {
         const int j = (kTokens ? j_first : 0) + i / (D / 4), col = i % (D / 4) * 4;
-        const int u = kTokens ? t_group + j / heads : t, h = h0 + (kTokens ? j % heads : j);
+        const int u = kTokens ? t_group + j / heads : my_token, h = h0 + (kTokens ? j % heads : j);
         float top = -INFINITY, sum = 0.f;
         for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stats[w][0][j]);
         floatx4 v = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -591,57 +628,83 @@ __global__ __launch_bounds__(64 * G::WAVES, G::kWavesPerSimd) void exact_cache_k
   }
 }
 
-// The parts of one (token, head) joined by their lse, where its rows lie in several shares; tokens without rows. One workgroup,
-// D / 4 threads per part.
-template <int D>
+// The tokens alone in a list, for shares beside groups
+__global__ __launch_bounds__(1024) void exact_alone_kernel(ExactCacheParams a) {
+  __shared__ int sums[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int count = 0;
+  for (int t0 = 0; t0 < a.T; t0 += 1024) {
+    const bool alone = t0 + tid < a.T && is_alone(a, t0 + tid);
+    const uint64_t mask = __ballot(alone);
+    if (lane == 0) sums[wave] = __popcll(mask);
+    __syncthreads();
+    int at = count;
+    for (int w = 0; w < 16; ++w) {
+      at += w < wave ? sums[w] : 0;
+      count += sums[w];
+    }
+    if (alone) a.alone[1 + at + __popcll(mask & ((1ull << lane) - 1))] = t0 + tid;
+    __syncthreads();
+  }
+  if (tid == 0) a.alone[0] = count;
+}
+
+// The parts of one (token, head) joined by their lse, where its rows lie in several shares; tokens without rows. One workgroup
+// for a token, or, of the tokens alone, for every gridDim.x / H-th; D / 4 threads per part.
+template <int D, bool kAlone>
 __global__ __launch_bounds__(256) void exact_join_kernel(ExactCacheParams a) {
   constexpr int PER = D / 4, ROWS = 256 / PER;
   __shared__ float weight[kMaxShares];
   __shared__ floatx4 sums[ROWS][PER];
   __shared__ float red[2][4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int t = blockIdx.x / a.H, h = blockIdx.x % a.H;
-  int first, n;
-  token_rows(a, t, first, n);
-  int k0 = 0, count = 0;
-  if (n > first) {
-    k0 = a.split[2 * t];
-    count = a.split[2 * t + 1] - k0 + 1;
-    if (count == 1) return;   // written by its workgroup
-  }
-  // part s: the rows' end of share k0 (s = 0), or their beginning in share k0 + s
-  const int64_t place = ((int64_t)2 * k0 + 1) * a.H + h;
-  auto where = [&](int s) { return place + (s ? (2 * (int64_t)s - 1) * a.H : 0); };
-  float top = -INFINITY;
-  for (int s = tid; s < count; s += 256) top = fmaxf(top, weight[s] = a.ws_lse[where(s)]);
-  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
-  if (lane == 0) red[0][wave] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-  float w = 0.f;
-  for (int s = tid; s < count; s += 256) {
-    // (a part with a NaN lse has a NaN weight; one with nothing but scores of -inf has a weight of 0, and its NaN, if V has any, stay)
-    const float mine = weight[s];
-    w += weight[s] = mine == -INFINITY ? 0.f : fast_exp2((mine - top) * kLog2e);
-  }
-  for (int off = 32; off > 0; off >>= 1) w += __shfl_xor(w, off);
-  if (lane == 0) red[1][wave] = w;
-  __syncthreads();
-  const float sum = red[1][0] + red[1][1] + red[1][2] + red[1][3];
-  floatx4 v = floatx4{0.f, 0.f, 0.f, 0.f};
+  const int h = blockIdx.x % a.H, tokens = shared_tokens<kAlone>(a);
+  int i = blockIdx.x / a.H;
+  if (i >= tokens) return;
+  do {
+    const int t = shared_token<kAlone>(a, i);
+    int first, n;
+    token_rows(a, t, first, n);
+    int k0 = 0, count = 0;
+    if (n > first) {
+      k0 = a.split[2 * i];
+      count = a.split[2 * i + 1] - k0 + 1;
+      if (count == 1) continue;   // written by its workgroup
+    }
+    // part s: the rows' end of share k0 (s = 0), or their beginning in share k0 + s
+    const int64_t place = ((int64_t)2 * k0 + 1) * a.H + h;
+    auto where = [&](int s) { return place + (s ? (2 * (int64_t)s - 1) * a.H : 0); };
+    float top = -INFINITY;
+    for (int s = tid; s < count; s += 256) top = fmaxf(top, weight[s] = a.ws_lse[where(s)]);
+    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+    if (lane == 0) red[0][wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    float w = 0.f;
+    for (int s = tid; s < count; s += 256) {
+      // (a part with a NaN lse has a NaN weight; one with nothing but scores of -inf has a weight of 0, and its NaN, if V has any, stay)
+      const float mine = weight[s];
+      w += weight[s] = mine == -INFINITY ? 0.f : fast_exp2((mine - top) * kLog2e);
+    }
+    for (int off = 32; off > 0; off >>= 1) w += __shfl_xor(w, off);
+    if (lane == 0) red[1][wave] = w;
+    __syncthreads();
+    const float sum = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+    floatx4 v = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int s = tid / PER; s < count; s += ROWS)
-    v += *reinterpret_cast<const floatx4*>(a.ws_o + where(s) * D + tid % PER * 4) * weight[s];
-  sums[tid / PER][tid % PER] = v;
-  __syncthreads();
-  if (tid >= PER) return;
-  for (int i = 1; i < ROWS; ++i) v += sums[i][tid];
-  const bool none = sum == 0.f;
-  if (none) v = floatx4{0.f, 0.f, 0.f, 0.f};
-  const float inv = none ? 0.f : 1.f / sum;
-  *reinterpret_cast<u32x2*>(a.out + (int64_t)t * a.o_st + (int64_t)h * a.o_sh + 4 * tid) =
-      u32x2{pack2(v[0] * inv, v[1] * inv), pack2(v[2] * inv, v[3] * inv)};
-  if (tid == 0) a.lse[(int64_t)h * a.T + t] = none ? -INFINITY : top + logf(sum);
+    for (int s = tid / PER; s < count; s += ROWS)
+      v += *reinterpret_cast<const floatx4*>(a.ws_o + where(s) * D + tid % PER * 4) * weight[s];
+    sums[tid / PER][tid % PER] = v;
+    __syncthreads();
+    if (tid >= PER) continue;   // (what is in LDS has been read before it is written again: barriers lie between)
+    for (int r = 1; r < ROWS; ++r) v += sums[r][tid];
+    const bool none = sum == 0.f;
+    if (none) v = floatx4{0.f, 0.f, 0.f, 0.f};
+    const float inv = none ? 0.f : 1.f / sum;
+    *reinterpret_cast<u32x2*>(a.out + (int64_t)t * a.o_st + (int64_t)h * a.o_sh + 4 * tid) =
+        u32x2{pack2(v[0] * inv, v[1] * inv), pack2(v[2] * inv, v[3] * inv)};
+    if (tid == 0) a.lse[(int64_t)h * a.T + t] = none ? -INFINITY : top + logf(sum);
+  } while (kAlone && (i += gridDim.x / a.H) < tokens);
 }
 
 // Groups of tokens: 32 columns take half as many reads of K and V, where there are two workgroups per CU all the same (4 x 512
@@ -655,6 +718,16 @@ bool groups_of_32(const ExactCacheParams& p, int dim) {
 int64_t exact_workgroups(const ExactCacheParams& p, int dim) {
   const int group = !p.grouped ? 1 : (groups_of_32(p, dim) ? 2 : 1) * kMaxTile / p.G;
   return (p.shares ? p.shares : ((int64_t)p.T + group - 1) / group) * (p.grouped ? p.grouped : 1) * p.KH * p.tiles;
+}
+
+// The two halves of a step with shares beside groups
+ExactCacheParams groups_of(ExactCacheParams p) {
+  p.shares = 0;
+  return p;
+}
+ExactCacheParams alone_of(ExactCacheParams p) {
+  p.grouped = 0;
+  return p;
 }
 
 template <int D, bool kE4>
@@ -675,7 +748,20 @@ void launch_exact_cache(const ExactCacheParams& p, hipStream_t st) {
   hipLaunchKernelGGL(kernels[p.grouped ? 8 + more : 4 * wide + 2 * once + (p.G <= 8)], dim3(grid), dim3(64 * (wide ? W::WAVES : G::WAVES)),
                      0, st, p);
   if (p.shares)
-    hipLaunchKernelGGL(exact_join_kernel<D>, dim3((unsigned)((int64_t)p.T * p.H)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((exact_join_kernel<D, false>), dim3((unsigned)((int64_t)p.T * p.H)), dim3(256), 0, st, p);
+}
+
+// Shares beside groups: the groups in a launch of their own, then the tokens alone
+template <int D, bool kE4>
+void launch_exact(const ExactCacheParams& p, hipStream_t st) {
+  if (!p.shares || !p.grouped) return launch_exact_cache<D, kE4>(p, st);
+  launch_exact_cache<D, kE4>(groups_of(p), st);
+  hipLaunchKernelGGL(exact_alone_kernel, dim3(1), dim3(1024), 0, st, p);
+  using G = ExactGeo<D, kE4, false>;   // (groups have at most 8 heads, and a table row of its own is read once)
+  hipLaunchKernelGGL((exact_cache_kernel<G, true, kTwice, true>), dim3((unsigned)exact_workgroups(alone_of(p), D)),
+                     dim3(64 * G::WAVES), 0, st, alone_of(p));
+  const int tokens = min(p.T, max(1, 4096 / p.H));
+  hipLaunchKernelGGL((exact_join_kernel<D, true>), dim3((unsigned)(tokens * p.H)), dim3(256), 0, st, p);
 }
 
 // ---- store -------------------------------------------------------------------------------------------------------
@@ -800,27 +886,30 @@ extern "C" int hla_s6_exact_attention(const void* q, int32_t num_tokens, int32_t
   p.shares = shares;
   p.grouped = grouped;
   p.shared = shared_rows != 0;
-  HLA_REQUIRE(grouped >= 0 && grouped <= kMaxTile && (!grouped || (shares == 0 && p.G <= kMaxTile / 2)), HLA_S6_EINVAL,
-              "exact_attention: groups of tokens need shares 0, at most %d query heads per KV head and at most %d turns", kMaxTile / 2,
-              kMaxTile);
+  HLA_REQUIRE(grouped >= 0 && grouped <= kMaxTile && (!grouped || ((shares == 0 || bt_rows) && p.G <= kMaxTile / 2)), HLA_S6_EINVAL,
+              "exact_attention: groups of tokens need table rows per request or shares 0, at most %d query heads per KV head and at "
+              "most %d turns", kMaxTile / 2, kMaxTile);
   // (KH * tiles is at most H, so that workgroups are counted in 64 bits; none of a grid has more than 256 threads but one of few)
-  HLA_REQUIRE((int64_t)p.T * p.H <= INT32_MAX && launchable(exact_workgroups(p, head_dim), 256) &&
-                  (!shares || launchable((int64_t)p.T * p.H, 256)), HLA_S6_EINVAL, "exact_attention: too many rows");
+  const bool both = shares && grouped;
+  HLA_REQUIRE((int64_t)p.T * p.H <= INT32_MAX && launchable(exact_workgroups(both ? groups_of(p) : p, head_dim), 256) &&
+                  (!both || launchable(exact_workgroups(alone_of(p), head_dim), 256)) &&
+                  (!shares || both || launchable((int64_t)p.T * p.H, 256)), HLA_S6_EINVAL, "exact_attention: too many rows");
   if (shares) {
-    const int64_t rows = (int64_t)2 * shares * p.H, need = rows * (head_dim + 1) + 2 * (int64_t)p.T;
+    const int64_t rows = (int64_t)2 * shares * p.H, need = rows * (head_dim + 1) + (both ? 3 * (int64_t)p.T + 1 : 2 * (int64_t)p.T);
     HLA_REQUIRE(workspace && workspace_floats >= need, HLA_S6_EWORKSPACE,
                 "exact_attention: workspace overflow: %lld floats, have %lld", (long long)need, (long long)workspace_floats);
     HLA_REQUIRE(aligned16(workspace), HLA_S6_EINVAL, "exact_attention: workspace must be 16-byte aligned");
     p.ws_o = workspace;
     p.ws_lse = workspace + rows * head_dim;
     p.split = reinterpret_cast<int32_t*>(p.ws_lse + rows);
+    if (both) p.alone = p.split + 2 * (int64_t)p.T;
   }
   p.out = static_cast<uint16_t*>(out);
   p.o_st = o_st;
   p.o_sh = o_sh;
   p.lse = lse;
   const hipStream_t st = as_stream(stream);
-#define HLA_EXACT(D) e4m3 ? launch_exact_cache<D, true>(p, st) : launch_exact_cache<D, false>(p, st)
+#define HLA_EXACT(D) e4m3 ? launch_exact<D, true>(p, st) : launch_exact<D, false>(p, st)
   switch (head_dim) {
     case 64: HLA_EXACT(64); break;
     case 128: HLA_EXACT(128); break;

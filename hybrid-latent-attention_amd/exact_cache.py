@@ -20,6 +20,11 @@ from .compact_cache import _call, _same_device, _table, _vector
 BF16, E4M3, F32, I32, I64 = torch.bfloat16, torch.float8_e4m3fn, torch.float32, torch.int32, torch.int64
 DIMS = (64, 128, 256)
 MAX_SHARES = 1024
+# Rows from which tokens alone, in a step with groups of tokens, are cut in shares. A workgroup streams a row in 20 ns, 4096 in 80 us; the
+# three launches more take 8 to 12. us with / without, 8 KV heads for 32: one token of 131,000 rows beside 512 tokens on 8160 rows
+# 405 / 2670, 16 tokens of 8160 beside 2048 tokens 730 / 950, 8 of 65,000 beside 512 tokens on 4000 440 / 2720; nothing but chunks
+# of 512 on 8160 rows 712 / 701.
+LONG_ROWS = 4096
 
 
 def _cache(cache, k_scale, v_scale):
@@ -74,6 +79,10 @@ def row_shares(max_rows, groups, parts, cu_count=256):
     (a call on the host takes 16 / 11). A function of constants and the row count only (graph-stable)."""
     if max_rows <= (1536 if 2 * groups >= cu_count else 1024) or groups >= 16 * cu_count:
         return 0
+    return _shares(parts, cu_count)
+
+
+def _shares(parts, cu_count):
     return max(1, min(MAX_SHARES, 2 * cu_count // parts))
 
 
@@ -88,6 +97,11 @@ def _turns(tokens, heads, kv_heads, cu_count=256, per_request=1):
     if heads > 8 or -(-tokens // (16 // heads)) * kv_heads < cu_count:
         return 0
     return 16 // heads if per_request < 32 else min(4, 16 // heads)
+
+
+def _most_alone(tokens, requests, max_query_len):
+    """How many tokens of a step can be the only ones of their request, where the longest has ``max_query_len`` (2 or more)."""
+    return max(0, min(tokens - max_query_len, (requests * max_query_len - tokens) // (max_query_len - 1)))
 
 
 def attention(q, cache, block_table, ctx, scale, max_seq_len, token_requests=None, window=0, k_scale=None, v_scale=None,
@@ -106,7 +120,8 @@ def attention(q, cache, block_table, ctx, scale, max_seq_len, token_requests=Non
 
     The rows of all tokens are cut in ``shares`` equal parts per KV head (0: a workgroup takes all rows of a token; defaults to
     ``row_shares``); their partial results go through ``workspace`` (an ``S6Workspace`` of ``2 * shares * H * (d + 1) + 2 * T`` floats;
-    defaults to a new buffer). Calls that share a workspace must not overlap."""
+    defaults to a new buffer). Calls that share a workspace must not overlap. Beside chunks, tokens that are the only ones of their
+    request are cut in shares where rows are long (``LONG_ROWS``); a workspace without room for that, ``T + 1`` floats more, is not used."""
     _same_device(cache, q, block_table, ctx, token_requests, k_scale, v_scale)
     kv_heads, d, e4m3, page, head, row, block, pages = _cache(cache, k_scale, v_scale)
     s6_ops._bf16('q', q)
@@ -131,15 +146,21 @@ def attention(q, cache, block_table, ctx, scale, max_seq_len, token_requests=Non
     if shares is None:
         if chunk >= 4:
             turns = _turns(T, H // kv_heads, kv_heads, cus, T // max(1, min(count, T - chunk + 1)))   # (most requests there can be)
-        shares = 0 if turns else row_shares(longest, T * parts, parts, cus)
+        if not turns:
+            shares = row_shares(longest, T * parts, parts, cus)
+        else:   # those of tokens alone
+            alone = count - 1 if max_query_len is None else _most_alone(T, count, chunk)
+            shares = _shares(parts, cus) if longest >= LONG_ROWS and alone else 0
     else:
         shares = int(shares)
     if not 0 <= shares <= MAX_SHARES:
         raise ValueError(f'shares must be 0 to {MAX_SHARES}, got {shares}')
     ws = None
     if shares:
-        need = 2 * shares * H * (d + 1) + 2 * T
-        ws = torch.empty(need, dtype=F32, device=dev) if workspace is None else workspace.ensure(dev)
+        need = 2 * shares * H * (d + 1) + (3 * T + 1 if turns else 2 * T)
+        ws = None if workspace is None else workspace.ensure(dev)
+        if ws is None or (turns and ws.numel() < need):
+            ws = torch.empty(need, dtype=F32, device=dev)
         if ws.numel() < need:
             raise RuntimeError(f'S6 workspace overflow: need {need} floats, have {ws.numel()}')
         _same_device(q, ws)   # (a workspace keeps the device of its first use)

@@ -37,3 +37,14 @@ def test_requests_of_a_step(dealt):
     assert dealt(4000, 1, 16, 1, 4000, 4000)[1] == 4 and dealt(4000, 256, 16, 1, 4000, 4000)[1] == 4
     assert dealt(4016, 256, 16, 1, 4000, 4000)[1] == 4 and dealt(576, 65, 16, 1, 4000, 512)[1] == 16
     assert dealt(256, 32, 16, 1, 4000, 8)[1] == 16 and dealt(256, 1000, 16, 1, 4000, 8)[1] == 16
+
+
+def test_tokens_alone_beside_chunks(dealt, pkg):
+    """Shares for tokens alone beside groups, where there can be any and rows are long."""
+    most = pkg.exact_cache._most_alone
+    assert most(2048, 4, 512) == 0 and most(2049, 5, 512) == 1 and most(513, 2, 512) == 1 and most(4000, 256, 4000) == 0
+    assert most(576, 65, 512) == 64 and most(576, 300, 512) == 64 and most(100, 4, 512) == 0 and most(12, 4, 8) == 2
+    assert dealt(513, 2, 8, 4, 131000, 512)[:2] == (64, 4) and dealt(4016, 17, 16, 1, 8160, 4000)[:2] == (32, 4)
+    assert dealt(513, 2, 8, 4, 4095, 512)[:2] == (0, 4) and dealt(2048, 4, 16, 1, 8160, 512)[:2] == (0, 4)
+    assert dealt(513, 2, 8, 4, 131000)[:2] == (64, 4) and dealt(513, 1, 8, 4, 131000)[:2] == (0, 4)
+    assert dealt(513, 2, 8, 4, 131000, 512, shares=3)[:2] == (3, 0) and dealt(64, 2, 8, 4, 131000, 63)[:2] == (64, 0)

@@ -2,9 +2,11 @@
 ``test_gpu_exact_cache``."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
+from s6util import dev_i32, dev_i64
 from test_gpu_exact_cache import Cache, attend, check, query
 
 pytestmark = pytest.mark.gpu
@@ -38,3 +40,125 @@ def test_rows_of_no_weight_whose_values_are_not_finite(ec, shares, bad):
         part = Cache.__new__(Cache)
         part.h, part.rows = 1, [c.rows[t][:, heads.start // 2:heads.stop // 2]]
         check(o[t:t + 1, heads].contiguous(), lse[heads, t:t + 1], q[t:t + 1, heads], part, [0], [c.rows[t].shape[0]], 128 ** -0.5)
+
+
+# ---- tokens alone beside chunks -----------------------------------------------------------------------------------------
+
+@pytest.fixture
+def in_shares(ec, monkeypatch):
+    """Tokens alone are cut in shares whatever the length of their rows; the ``(shares, grouped)`` of the calls."""
+    calls, call = [], ec._call
+
+    def record(name, device, *args):
+        calls.append(args[24:26])
+        return call(name, device, *args)
+
+    monkeypatch.setattr(ec, 'LONG_ROWS', 0)
+    monkeypatch.setattr(ec, '_call', record)
+    return calls
+
+
+def mixed_step(lens, order):
+    """Requests and lengths of a step: ``lens[r]`` tokens at the end of the ``n[r]`` rows of every request."""
+    n = [300, 40, 1700, 900, 33, 2500]
+    requests = sum(([r] * lens[r] for r in order), [])
+    ctx = sum(([n[r] - lens[r] + i + 1 for i in range(lens[r])] for r in order), [])
+    return n, requests, ctx
+
+
+@pytest.mark.parametrize('e4m3', [False, True])
+@pytest.mark.parametrize('kv_heads,G,d,block', [(2, 1, 128, 16), (128, 1, 128, 16), (1, 2, 64, 24), (43, 3, 128, 32), (1, 4, 256, 16),
+                                               (26, 5, 64, 16), (2, 8, 128, 1)])
+@pytest.mark.parametrize('window,turns', [(0, 4), (21, 2), (0, 16)])
+def test_tokens_alone_beside_chunks(ec, in_shares, monkeypatch, kv_heads, G, d, block, e4m3, window, turns):
+    """At both ends of a step, between chunks and one behind the other; a request that lies there twice; tokens without rows, of which
+    one hides a neighbour of the same request; a chunk whose last token lies in the next group."""
+    monkeypatch.setattr(ec, '_turns', lambda *a: turns)
+    n, requests, ctx = mixed_step([33, 40, 1, 5, 20, 1], (5, 0, 2, 1, 3, 4))
+    requests, ctx = requests + [2, 0, 5, 5, 5, 2, 3], ctx + [1000, 250, 2000, 0, 2100, 0, 850]
+    requests, ctx = requests + [4, 4, 1, 5], ctx + [0, 0, -3, 2222]
+    c = Cache(G + d, n, kv_heads, d, block, e4m3)
+    q = query(G, len(ctx), kv_heads * G, d)
+    o, lse = ec.attention(q, c.cache, c.table, dev_i32(np.array(ctx)), d ** -0.5, max(n), dev_i64(np.array(requests)), window,
+                          c.k_scale, c.v_scale, max_query_len=40)
+    assert in_shares == [(max(1, 512 // kv_heads), turns)]
+    check(o, lse, q, c, requests, ctx, d ** -0.5, window)
+
+
+@pytest.mark.parametrize('lens,order', [([1, 1, 1, 1, 1, 1], range(6)), ([64, 1, 64, 64, 32, 64], (0, 2, 3, 5, 4)),
+                                        ([1, 1, 1, 1, 1, 300], (0, 1, 2, 5, 3, 4))])
+def test_steps_of_one_kind(ec, in_shares, monkeypatch, lens, order):
+    """Nothing but tokens alone, nothing but chunks, and a replayed graph whose lengths make one of the other."""
+    monkeypatch.setattr(ec, '_turns', lambda *a: 3)
+    n, requests, ctx = mixed_step(lens, order)
+    c = Cache(90, n, 4, 128, 16)
+    q, table_rows, lengths = query(91, len(ctx), 8, 128), dev_i64(np.array(requests)), dev_i32(np.array(ctx))
+    ws = ec.s6_ops.S6Workspace(8, 128, 2 * 128 + 10)
+    call = lambda: ec.attention(q, c.cache, c.table, lengths, 0.1, max(n), table_rows, max_query_len=max(4, *lens), workspace=ws)
+    monkeypatch.setattr(ec, '_most_alone', lambda *a: 1)
+    check(*call(), q, c, requests, ctx, 0.1)
+    assert in_shares == [(128, 3)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o, lse = call()
+    for seed in (1, 2, 3):
+        rng = np.random.default_rng(seed)
+        now = np.where(rng.random(len(ctx)) < 0.5, 0, ctx)
+        rows = rng.integers(0, 6, len(ctx)) if seed == 3 else np.array(requests)
+        now = np.minimum(now, np.array(n)[rows])
+        lengths.copy_(dev_i32(now))
+        table_rows.copy_(dev_i64(rows))
+        graph.replay()
+        check(o, lse, q, c, rows, now.tolist(), 0.1)
+        eager = call()
+        torch.cuda.synchronize()
+        assert torch.equal(eager[0], o) and torch.equal(eager[1], lse)
+
+
+def test_many_tokens_alone(ec, in_shares, monkeypatch):
+    """More of them than are listed, or joined, at a time; a workspace that is too small for them is left alone."""
+    monkeypatch.setattr(ec, '_turns', lambda *a: 2)
+    rng = np.random.default_rng(5)
+    n = rng.integers(1, 400, 1500).tolist() + [700]
+    lens = [1] * 1500 + [600]
+    order = rng.permutation(1501).tolist()
+    requests = sum(([r] * lens[r] for r in order), [])
+    ctx = sum(([n[r] - lens[r] + i + 1 for i in range(lens[r])] for r in order), [])
+    c = Cache(92, n, 2, 64, 16)
+    q = query(93, len(ctx), 16, 64)
+    ws = ec.s6_ops.S6Workspace(16, 64, 10)
+    ws.ensure(q.device).fill_(math.nan)
+    o, lse = ec.attention(q, c.cache, c.table, dev_i32(np.array(ctx)), 0.125, max(n), dev_i64(np.array(requests)), max_query_len=600,
+                          workspace=ws)
+    assert in_shares == [(256, 2)] and torch.isnan(ws.buffer).all()
+    some = [t for t in range(len(ctx)) if requests[t] != 1500 or t % 20 == 0]
+    check(o[some], lse[:, some], q[some], c, [requests[t] for t in some], [ctx[t] for t in some], 0.125)
+
+
+def test_attend_exact_in_groups(pkg, ec, monkeypatch):
+    """A prompt, a chunk on a history and single tokens through the layer's call and a pool's tables, rows stored by it."""
+    calls, call = [], ec._call
+    monkeypatch.setattr(ec, '_call', lambda name, device, *args: (calls.append((name, *args[24:26])), call(name, device, *args))[1])
+    layer, ops = pkg.s6_layer, pkg.s6_ops
+    n, lens, block = [4200, 300, 700, 5000], [1, 300, 200, 1], 16
+    c = Cache(94, n, 16, 128, block)
+    pos = np.concatenate([np.arange(n[r] - lens[r], n[r]) for r in range(4)] + [[0, 0]])
+    T = len(pos)
+    table = torch.zeros(60, c.table.shape[1], dtype=torch.int32, device='cuda')
+    table[:4] = c.table
+    ctx = layer.StepContext(torch.as_tensor(pos, device='cuda'), dev_i32(np.concatenate(([0], np.cumsum(lens)))), dev_i32(np.array(n)),
+                            max(lens), T, {}, 0.09, ops.HIP_BACKENDS, max_seqlen_k=max(n))
+    k, v, q = (torch.randn(T, 16, 128, generator=torch.Generator('cuda').manual_seed(95 + i), device='cuda').to(torch.bfloat16)
+               for i in range(3))
+    t, requests = 0, []
+    for r in range(4):
+        c.rows[r][n[r] - lens[r]:] = torch.cat((k[t:t + lens[r]], v[t:t + lens[r]]), -1).double()
+        requests, t = requests + [r] * lens[r], t + lens[r]
+    o = layer.attend_exact(q, k, v, c.cache, table, ctx)
+    assert [x for x in calls if x[0] == 'hla_s6_exact_attention'] == [('hla_s6_exact_attention', 32, 16)]
+    assert (o[T - 2:] == 0).all()
+    lengths = (pos + 1).tolist()
+    _, lse = ec.attention(q[:T - 2], c.cache, c.table, dev_i32(np.array(lengths[:T - 2])), 0.09, max(n), dev_i64(np.array(requests)), shares=0)
+    some = [0, T - 3] + list(range(1, T - 3, 23))
+    check(o[some], lse[:, some], q[some], c, [requests[t] for t in some], [lengths[t] for t in some], 0.09)
