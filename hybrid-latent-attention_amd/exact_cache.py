@@ -71,13 +71,19 @@ def row_shares(max_rows, groups, parts, cu_count=256):
     """``shares`` of ``attention`` for rows of at most ``max_rows`` and ``groups`` (token, KV head) pairs over ``parts`` KV heads: two
     workgroups per CU together, which is what fits one at a time (32 tokens of 1000 to 8160 rows on 8 KV heads: 115 us with a half
     of them, 101, 102 with twice as many), or 0, a workgroup per group, where the second launch costs more than it evens out: on
-    short rows, and where the groups are many. GPU time in us with shares / a workgroup per group, 8 KV heads:
+    short rows, and where the groups are many and no row lasts longer than the others. GPU time in us with shares / a workgroup per group, 8 KV heads:
 
         tokens x rows   1 x 512     1 x 768     1 x 1024    4 x 1024    16 x 1024   16 x 1536   32 x 1536   64 x 1024
                         10.8 / 8.9  10.9 / 10.7 10.9 / 11.2 11.4 / 13.5 19.7 / 17.5 25.1 / 23.6 41.8 / 35.0 51.9 / 47.6
 
-    (a call on the host takes 16 / 11). A function of constants and the row count only (graph-stable)."""
-    if max_rows <= (1536 if 2 * groups >= cu_count else 1024) or groups >= 16 * cu_count:
+    (a call on the host takes 16 / 11), and with 256 tokens, 16 KV heads:
+
+        rows            256 x 2000  256 x 4000   256 x 8160   1000 to 8160  one of 16000, else 1000  of 32000   of 131000
+                        626 / 632   1284 / 1264  2594 / 2573  1459 / 1468   365 / 505                397 / 676  500 / 1735
+
+    (512 tokens of 100 to 2000 rows: 815 / 728). A place takes ``groups / (2 * cu_count)`` of them one behind the other, with 512 rows
+    on average as many as the longest may have. A function of constants and the row count only (graph-stable)."""
+    if max_rows <= (1536 if 2 * groups >= cu_count else 1024) or (groups >= 16 * cu_count and 256 * groups >= max_rows * cu_count):
         return 0
     return _shares(parts, cu_count)
 

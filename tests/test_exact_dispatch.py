@@ -48,3 +48,10 @@ def test_tokens_alone_beside_chunks(dealt, pkg):
     assert dealt(513, 2, 8, 4, 4095, 512)[:2] == (0, 4) and dealt(2048, 4, 16, 1, 8160, 512)[:2] == (0, 4)
     assert dealt(513, 2, 8, 4, 131000)[:2] == (64, 4) and dealt(513, 1, 8, 4, 131000)[:2] == (0, 4)
     assert dealt(513, 2, 8, 4, 131000, 512, shares=3)[:2] == (3, 0) and dealt(64, 2, 8, 4, 131000, 63)[:2] == (64, 0)
+
+
+def test_a_long_row_among_many_groups(dealt):
+    """Many groups take a workgroup each only as long as none of them takes much longer than the others together."""
+    assert dealt(256, 256, 16, 1, 131000, 1)[0] == 32 and dealt(256, 256, 16, 1, 8160, 1)[0] == 32
+    assert dealt(256, 256, 16, 1, 4096, 1)[0] == 0 and dealt(256, 256, 16, 1, 4097, 1)[0] == 32
+    assert dealt(512, 512, 16, 1, 8192, 1)[0] == 0 and dealt(512, 512, 16, 1, 131000, 1)[0] == 32

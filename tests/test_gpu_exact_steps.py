@@ -162,3 +162,14 @@ def test_attend_exact_in_groups(pkg, ec, monkeypatch):
     _, lse = ec.attention(q[:T - 2], c.cache, c.table, dev_i32(np.array(lengths[:T - 2])), 0.09, max(n), dev_i64(np.array(requests)), shares=0)
     some = [0, T - 3] + list(range(1, T - 3, 23))
     check(o[some], lse[:, some], q[some], c, [requests[t] for t in some], [lengths[t] for t in some], 0.09)
+
+
+def test_a_long_row_among_many_tokens(ec):
+    """By the rule in shares, of which some end inside one of several short rows."""
+    n = np.random.default_rng(6).integers(0, 300, 300).tolist()
+    n[200] = 20000
+    c = Cache(96, n, 16, 64, 16)
+    q = query(97, 300, 16, 64)
+    assert ec.row_shares(20000, 300 * 16, 16) == 32
+    o, lse = attend(ec, q, c, n)
+    check(o, lse, q, c, range(300), n, 0.125)
