@@ -202,16 +202,22 @@ class StepContext:
                 self._plans[(s, key[1])] = plan
         return self._plans[key]
 
+    @staticmethod
+    def _address(table):
+        """What tells the tables of a step apart. (Who keeps results by it keeps the table too: the next one to be made could lie
+        where a table lay that is gone.)"""
+        return table.data_ptr(), tuple(table.shape), table.stride()
+
     def slots(self, table, block_size):
         """Commit slot of every token for a per-request block table (``slot_mapping``), once per table per step."""
-        key = (table.data_ptr(), int(block_size))
+        key = (*self._address(table), int(block_size))
         if key not in self._slots:
-            self._slots[key] = slot_mapping(self, table, block_size)
-        return self._slots[key]
+            self._slots[key] = table, slot_mapping(self, table, block_size)
+        return self._slots[key][1]
 
     def block_table(self, table):
         """Per-token gather of a per-request block table, done once per distinct tensor per step."""
-        key = table.data_ptr()
+        key = self._address(table)
         if key not in self._block_tables:
             if table.dtype != torch.int32 or table.stride(-1) != 1:
                 raise ValueError('block tables must be int32 with a unit last stride')
@@ -219,8 +225,8 @@ class StepContext:
             out = torch.empty(T, cols, dtype=torch.int32, device=table.device)
             _lib.call('hla_s6_gather_block_table', _lib.ptr(table), table.stride(0), table.shape[0], cols,
                       _lib.ptr(self.token_requests), T, _lib.ptr(out), out.stride(0), _lib.stream(table.device))
-            self._block_tables[key] = out
-        return self._block_tables[key]
+            self._block_tables[key] = table, out
+        return self._block_tables[key][1]
 
     def latent_query(self, sl, loop, q_pre_rope):
         A, _, width = sl.readers(loop)

@@ -173,3 +173,21 @@ def test_a_long_row_among_many_tokens(ec):
     assert ec.row_shares(20000, 300 * 16, 16) == 32
     o, lse = attend(ec, q, c, n)
     check(o, lse, q, c, range(300), n, 0.125)
+
+
+def test_two_pools_in_a_step(pkg):
+    """Layers on pools of their own, whose rows of the step are gathered anew for every call."""
+    layer, ops = pkg.s6_layer, pkg.s6_ops
+    g = torch.Generator(device='cuda').manual_seed(98)
+    n = [40, 25, 1]
+    ctx = layer.StepContext(torch.tensor([39, 24, 0], device='cuda'), dev_i32(np.arange(4)), dev_i32(np.array(n)), 1, 3, {}, 0.1,
+                            ops.HIP_BACKENDS, max_seqlen_k=40)
+    live = torch.tensor([5, 2, 0], device='cuda')
+    for tables in (torch.arange(18, dtype=torch.int32, device='cuda').view(6, 3), torch.arange(17, -1, -1, dtype=torch.int32, device='cuda').view(6, 3)):
+        cache = torch.randn(18, 2, 16, 128, generator=g, device='cuda').to(torch.bfloat16)
+        q, k, v = (torch.randn(3, 2, 64, generator=g, device='cuda').to(torch.bfloat16) for _ in range(3))
+        want = cache.clone()
+        for t, r in enumerate(live.tolist()):
+            want[tables[r, (n[t] - 1) // 16].long(), :, (n[t] - 1) % 16] = torch.cat((k[t], v[t]), -1)
+        layer.attend_exact(q, k, v, cache, tables[live], ctx)
+        assert torch.equal(cache, want)
