@@ -222,9 +222,12 @@ class StepContext:
             if table.dtype != torch.int32 or table.stride(-1) != 1:
                 raise ValueError('block tables must be int32 with a unit last stride')
             T, cols = self.token_requests.shape[0], table.shape[1]
+            requests = self.token_requests
+            if table.shape[0] < self.query_start_loc.shape[0] - 1:
+                requests = requests.clamp(max=table.shape[0] - 1)
             out = torch.empty(T, cols, dtype=torch.int32, device=table.device)
             _lib.call('hla_s6_gather_block_table', _lib.ptr(table), table.stride(0), table.shape[0], cols,
-                      _lib.ptr(self.token_requests), T, _lib.ptr(out), out.stride(0), _lib.stream(table.device))
+                      _lib.ptr(requests), T, _lib.ptr(out), out.stride(0), _lib.stream(table.device))
             self._block_tables[key] = table, out
         return self._block_tables[key][1]
 
@@ -510,9 +513,12 @@ def slot_mapping(ctx, block_table, block_size):
     T = ctx.token_requests.shape[0]
     slots = torch.empty(T, dtype=torch.int64, device=block_table.device)
     pos = s6_ops._int('positions', ctx.positions, torch.int64)
+    rows, valid = block_table.shape[0], ctx.valid
+    if rows < ctx.query_start_loc.shape[0] - 1:   # (requests without a row have no slots)
+        valid = valid & (ctx.token_requests < rows)
     _lib.call('hla_s6_slot_mapping', _lib.ptr(block_table), block_table.stride(0), block_table.shape[1],
               _lib.ptr(ctx.token_requests),
-              _lib.ptr(ctx.valid), _lib.ptr(pos), T, int(block_size), _lib.ptr(slots), _lib.stream(block_table.device))
+              _lib.ptr(valid), _lib.ptr(pos), T, int(block_size), _lib.ptr(slots), _lib.stream(block_table.device))
     return slots
 
 
