@@ -406,6 +406,8 @@ def attend_exact(q_rope, k_rope, v, cache, block_table, ctx, k_scale=None, v_sca
     zero. A step without metadata (profiling) has neither rows nor cache writes and returns zeros."""
     if not ctx.md_present:
         return torch.zeros_like(q_rope)
+    compact_cache._same_device(cache, q_rope, block_table)
+    compact_cache._table(block_table, 1)
     if k_rope is not None:
         exact_cache.store_rows(k_rope, v, ctx.slots(block_table, cache.shape[2]), cache, k_scale, v_scale)
     rows = block_table.shape[1] * cache.shape[2]

@@ -191,3 +191,20 @@ def test_two_pools_in_a_step(pkg):
             want[tables[r, (n[t] - 1) // 16].long(), :, (n[t] - 1) % 16] = torch.cat((k[t], v[t]), -1)
         layer.attend_exact(q, k, v, cache, tables[live], ctx)
         assert torch.equal(cache, want)
+
+
+def test_attend_exact_refuses_tables_before_it_stores(pkg):
+    layer, ops = pkg.s6_layer, pkg.s6_ops
+    ctx = layer.StepContext(torch.tensor([3, 4], device='cuda'), dev_i32(np.arange(3)), dev_i32(np.array([4, 5])), 1, 2, {}, 0.1,
+                            ops.HIP_BACKENDS, max_seqlen_k=5)
+    cache = query(99, 4, 2 * 16, 128).view(4, 2, 16, 128)
+    before, rows = cache.clone(), query(100, 2, 2, 64)
+    table = torch.arange(4, dtype=torch.int32, device='cuda').view(2, 2)
+    for bad, error in ((table.long(), ValueError), (table.t(), ValueError), (table[0], ValueError), (table[:0], ValueError),
+                       (table.cpu(), RuntimeError)):
+        with pytest.raises(error):
+            layer.attend_exact(rows, rows, rows, cache, bad, ctx)
+        assert torch.equal(cache, before)
+    o = layer.attend_exact(rows, rows, rows, cache, table[:1], ctx)       # the second request has no row: it stores nothing
+    before[0, :, 3] = torch.cat((rows[0], rows[0]), -1)
+    assert torch.equal(cache, before) and torch.isfinite(o).all()
