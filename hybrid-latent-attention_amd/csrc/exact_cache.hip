@@ -1,4 +1,4 @@
-// Attention over a whole exact (per-head K / V) paged cache, one new token per row, and the store into it.
+// Attention of new tokens, single ones and chunks, over a whole exact (per-head K / V) paged cache, and the store into it.
 //
 // A cache page holds `block` rows of every KV head, [K | V] of 2d values in bf16 or e4m3; G query heads read one KV head.
 //   o[t, h] = sum_j softmax_j(scale q[t, h] . K[j]) V[j], j over the rows [max(0, n - window), n) of n = ctx[t].
@@ -22,7 +22,8 @@
 // tokens, both parts are keys of one product of twice the keys, V twice in its operand (bf16), or of two products (e4m3).
 //
 // Large steps of many tokens per request (chunks) put the heads of 16 / G or 32 / G tokens in the columns: 4 x 512 tokens on
-// 8160 rows, 16 heads, 398 us, 333 TFLOP/s (matrix units 23 %, vector units 53 %, LDS 17 %: two waves per SIMD, each a chain of them).
+// 8160 rows, 16 heads, 370 to 410 us, 320 to 360 TFLOP/s (matrix units 23 %, vector units 53 %, LDS 17 %: two waves per SIMD, each a
+// chain of them, on 16 keys at a time; K and V cross the caches once per group).
 //
 // Single tokens beside chunks (exact_alone_kernel lists them) keep their shares, in a launch behind that of the groups.
 //
@@ -766,7 +767,8 @@ void launch_exact(const ExactCacheParams& p, hipStream_t st) {
 
 // ---- store -------------------------------------------------------------------------------------------------------
 // Rows into slots, a thread per 8 values (16 bytes in); e4m3: x / scale, clamped to +-448, to the nearest, ties to even. Bound by
-// HBM; stores past the caches (8192 tokens of 16 heads, 134 MB both ways: 31.6 -> 26.7 us, 5.0 TB/s, as a large copy).
+// HBM: 8192 tokens of 16 heads, 134 MB both ways, 23.8 us, 5.6 TB/s (a large copy 5.1: some rows are in the last cache), with stores
+// past the caches; with plain ones 30.
 struct ExactStoreParams {
   const uint16_t *key, *value;
   int64_t k_st, k_sh, v_st, v_sh;

@@ -252,8 +252,9 @@ __global__ __launch_bounds__(kPoolThreads) void pool_extend_kernel(ExtendParams 
 }
 
 // from = write_from[r]: any column may be shared, and lists have an entry per table entry. In three launches: a workgroup per
-// request finds what it asks for (`source` has the shared pages), one plans, and a workgroup per request fills its columns. (One
-// workgroup for all three: 243 us for the 32,640 pages of 64 requests of 8160 rows, 59 where none was shared.)
+// request finds what it asks for (`source` has the shared pages), one plans, and a workgroup per request fills its columns: 27 us for
+// the 32,640 shared pages of 64 requests of 8160 rows, 19 of them in the one that hands the new ones out (bound by the instructions of
+// its one workgroup), 10 where none is shared. (One workgroup for all three: 243, and 59.)
 struct Columns {   // columns [c0, c1) have rows to write, those from `held` on no page yet
   int length, want, held, c0, c1;
   bool fits;

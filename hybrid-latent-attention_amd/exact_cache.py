@@ -1,8 +1,8 @@
 """Whole exact caches on MI355X: attention of new tokens over all rows of a paged per-head K / V cache, and the store into it.
 
 The S6 path reads exact K / V in a window of a few rows. Layers and loops that keep their exact cache, and the teacher that a
-latent model is measured against, attend to all of it: ``attention`` does, for single tokens, with any number of query heads per
-KV head, and ``store_rows`` writes the rows of new tokens.
+latent model is measured against, attend to all of it: ``attention`` does, for single tokens and chunks, with any number of query
+heads per KV head, and ``store_rows`` writes the rows of new tokens.
 
 A cache is ``[num_blocks, KV heads, block, 2d]`` (K then V, the layout of the exact window; any strides, the last one 1), ``d`` 64,
 128 or 256, in bf16 or in ``torch.float8_e4m3fn``. The values of an e4m3 cache count times a scale per KV head (``k_scale``,
@@ -71,7 +71,8 @@ def row_shares(max_rows, groups, parts, cu_count=256):
     """``shares`` of ``attention`` for rows of at most ``max_rows`` and ``groups`` (token, KV head) pairs over ``parts`` KV heads: two
     workgroups per CU together, which is what fits one at a time (32 tokens of 1000 to 8160 rows on 8 KV heads: 115 us with a half
     of them, 101, 102 with twice as many), or 0, a workgroup per group, where the second launch costs more than it evens out: on
-    short rows, and where the groups are many and no row lasts longer than the others. GPU time in us with shares / a workgroup per group, 8 KV heads:
+    short rows, and where the groups are many and no row lasts longer than the others. GPU time in us with shares / a workgroup per
+    group, 8 KV heads:
 
         tokens x rows   1 x 512     1 x 768     1 x 1024    4 x 1024    16 x 1024   16 x 1536   32 x 1536   64 x 1024
                         10.8 / 8.9  10.9 / 10.7 10.9 / 11.2 11.4 / 13.5 19.7 / 17.5 25.1 / 23.6 41.8 / 35.0 51.9 / 47.6
@@ -95,8 +96,8 @@ def _shares(parts, cu_count):
 def _turns(tokens, heads, kv_heads, cu_count=256, per_request=1):
     """0, or the workgroups per group of ``16 // heads`` tokens (``heads`` query heads per KV head; the kernel takes ``32 // heads``
     where groups are many) that go through rows together, where there is a group for every CU. Chunks on top of histories, us with
-    groups / a workgroup per token: 4 x 512 tokens on 8160 rows of 16 heads 398 / 5861, of 8 KV heads for 32 685 / 2939, a prompt
-    of 4000 of 16 heads 235 / 3219, 8 x 64 on 4000 (8 KV heads for 32) 103 / 397.
+    groups / a workgroup per token: 4 x 512 tokens on 8160 rows of 16 heads 398 / 5861, of 8 KV heads for 32 685 / 2939 (in e4m3 591
+    with groups), a prompt of 4000 of 16 heads 235 / 3219, 8 x 64 on 4000 (8 KV heads for 32) 103 / 397.
 
     A group of single tokens (which a step may have beside its chunks) has as many requests as tokens: with few tokens per request
     on average (``per_request``, at least) a workgroup for each; else 4, since most find nothing to do (a prompt of 4000 with 16: 260)."""

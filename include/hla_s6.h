@@ -590,11 +590,11 @@ int hla_s6_move_rows(void *cache, int32_t width, int32_t compact, int64_t page_s
  * bt_rows[t] : t of the table, clamped into its bt_count rows; page ids are clamped into the cache; at most bt_cols * block_size
  * rows. shares 0: a workgroup takes all rows of a (token, KV head); else (at most 1024) the rows of all tokens together are cut in
  * that many equal shares per KV head, and the workspace holds 2 * shares * num_heads * (head_dim + 1) + 2 * num_tokens floats.
- * grouped > 0 (at most 16; at most 8 query heads per KV head): groups of 16 / (num_heads / kv_heads) tokens, those that lie
- * one behind the other and read the same table row together; a group's table rows are dealt to `grouped` workgroups. With shares > 0
- * too (and bt_rows) the shares take the tokens alone, which have rows and no neighbour with rows of their table row, the groups the
- * others; the workspace then holds num_tokens + 1 floats more. shared_rows
- * != 0 says that several tokens read the same rows, which then do not stream past the caches (results are the same). */
+ * grouped > 0 (at most 16; at most 8 query heads per KV head): groups of 16 / (num_heads / kv_heads) tokens, or of twice as many
+ * where the step is large; those that lie one behind the other and read the same table row go through it together; a group's table
+ * rows are dealt to `grouped` workgroups. With shares > 0 too (and bt_rows) the shares take the tokens alone, which have rows
+ * and no neighbour with rows of their table row, the groups the others; the workspace then holds num_tokens + 1 floats more.
+ * shared_rows != 0 says that several tokens read the same rows, which then do not stream past the caches (results are the same). */
 int hla_s6_exact_attention(const void *q, int32_t num_tokens, int32_t num_heads, int32_t head_dim, int64_t q_st,
                            int64_t q_sh, const void *cache, int32_t e4m3, int32_t kv_heads, int64_t page_stride,
                            int64_t head_stride, int64_t row_stride, int32_t block_size, int64_t num_blocks,
